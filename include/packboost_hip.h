@@ -142,6 +142,13 @@ const int32_t* pb_era_offsets_dev(const pb_ctx* ctx);
 int pb_round_begin(pb_ctx* ctx, const float* preds_dev, const float* y_dev, float* grad_dev,
                    uint16_t* nid_dev, uint16_t* tnode_dev, void* stream);
 
+/* Gradients of another objective: with grad_dev != NULL (float32, as many entries as the rows) every
+ * later pb_round_begin and pb_grow_round takes the round's gradients from there, when its kernels run,
+ * instead of forming preds - y; NULL returns to the squared loss. The hessian stays 1 a row. grad_dev is
+ * not the buffers' own grad_dev, which the round writes. No counterpart in the reference, whose one
+ * objective is the squared loss (booster.py:2149-2154). */
+int pb_set_gradients(pb_ctx* ctx, const float* grad_dev);
+
 /* Kernel 1 — histogram build. Replaces the per-feature histogram + scan of
  * find_best_splits_batched_cpu (frontier_cpu.cpp:261-321) and the histogram part of
  * cuda_find_best_splits_kernel (frontier_cuda.cu:441-498). For every active node u,
@@ -536,6 +543,94 @@ int pb_best_thresholds(const pb_candidate* cand_dev, int32_t M, int32_t K, int32
  * [M][K * T] scratch. */
 int pb_pick_sequential(const pb_candidate* cand_dev, int32_t M, int32_t K, int32_t T, int32_t* band_dev,
                        pb_candidate* out_dev, void* stream);
+
+/* ---- choices and preferences ----------------------------------------------------------- */
+/* Objectives beside the squared loss, on ragged sets of candidate rows (no counterpart in the
+ * reference). Set g holds rows [offsets[g], offsets[g + 1]); sets may be empty. A row's logit is its score
+ * plus, with a position bias, table[bucket of its position], and -inf where its mask is 0: what a masked
+ * row holds is not used, NaN included. Its log-probability is the logit less the set's lse, the log
+ * of the sum of exponentials (-inf for a set without probability). A step is a set with a chosen row,
+ * given by its index within the set; a step whose index lies outside the set, whose row is masked or whose
+ * set has no probability is left out: log-probability 0, no loss, no gradient.
+ *
+ * pb_sets holds the device copy of the offsets and how their work is laid out; it may serve calls on
+ * any stream of its device at once (each with a workspace of its own) and must outlive them. */
+typedef struct pb_sets pb_sets;
+int pb_sets_create(const int64_t* offsets_host, int64_t num_sets, pb_sets** out);
+int pb_sets_destroy(pb_sets* sets);
+
+#define PB_F32 0
+#define PB_BF16 1
+#define PB_F16 2
+
+/* Scores of the rows of a pb_sets. num_buckets 0: no position bias. Else table_dev float32
+ * [num_buckets] (at most 256), positions_dev int32 [rows] and buckets_dev uint8 [2 (reach + 1)], every
+ * entry below num_buckets: a row at position q takes bucket buckets_dev[min(|q|, reach)] for q <= 0 and
+ * buckets_dev[reach + 1 + min(q, reach)] for q > 0. */
+typedef struct {
+    const void* scores_dev;       /* score_type [rows], element i at i * score_stride */
+    const uint8_t* mask_dev;      /* NULL, or [rows]: 0 leaves a row out */
+    const int32_t* positions_dev;
+    const float* table_dev;
+    const uint8_t* buckets_dev;
+    int64_t score_stride;
+    int32_t score_type;           /* PB_F32, PB_BF16, PB_F16 */
+    int32_t num_buckets;
+    int32_t reach;
+    int32_t reserved;
+} pb_choice_scores;
+
+/* Bytes of the workspace (16-byte aligned) of a call on these sets; -1: bad argument. */
+int64_t pb_choice_work_bytes(const pb_sets* sets, int32_t num_buckets);
+
+/* chosen_dev NULL: log_probs_dev float32 [rows], every row's (-inf where masked). Else (int32
+ * [num_sets]) log_probs_dev float32 [num_sets], the steps'. lse_dev: float32 [num_sets]. */
+int pb_choice_log_probs(const pb_sets* sets, const pb_choice_scores* scores, const int32_t* chosen_dev,
+                        float* log_probs_dev, float* lse_dev, void* work_dev, int64_t work_bytes, void* stream);
+
+/* Gradients of the scores (score_type [rows], stride 1, 0 where masked) and of the bias table (float32
+ * [num_buckets]) from grad_dev, that of the rows' (chosen_dev NULL) or the steps' log-probabilities;
+ * masked rows' entries are not used. lse_dev: pb_choice_log_probs' for the same scores. */
+int pb_choice_log_probs_backward(const pb_sets* sets, const pb_choice_scores* scores, const int32_t* chosen_dev,
+                                 const float* grad_dev, const float* lse_dev, void* grad_scores_dev,
+                                 float* grad_table_dev, void* work_dev, int64_t work_bytes, void* stream);
+
+/* Inputs of the clipped policy loss, float32 [num_sets] each. */
+typedef struct {
+    const float* advantages_dev;
+    const float* old_log_probs_dev;
+    const float* ref_log_probs_dev;  /* NULL: no KL term */
+    const float* weights_dev;        /* NULL: 1 */
+    float ratio_min, ratio_max;      /* the ratio's bounds, e.g. 0.8 and 1.2 */
+    float kl_weight, scale;
+} pb_policy_terms;
+
+/* With r = exp(log p - old), A the advantage and d = ref - log p, summed over the steps:
+ *   loss = scale * w * (kl_weight * kl - min(r A, clip(r, ratio_min, ratio_max) A)), kl = e^d - d - 1.
+ * stats_dev float32 [3]: the loss, scale * sum of w * kl, scale * sum of w over steps whose bound holds
+ * (r A above the clipped product). log_probs_dev: the steps', as pb_choice_log_probs gives them. The
+ * gradients are the loss's, laid out as in pb_choice_log_probs_backward. One pass over the scores
+ * (sets of more than 2048 rows are read twice). */
+int pb_policy_loss(const pb_sets* sets, const pb_choice_scores* scores, const pb_policy_terms* terms,
+                   const int32_t* chosen_dev, float* stats_dev, float* log_probs_dev, void* grad_scores_dev,
+                   float* grad_table_dev, void* work_dev, int64_t work_bytes, void* stream);
+
+/* Pairs of values (winner, loser), by index in [0, num_values). seq_offsets_host (int64 [num_values + 1],
+ * or NULL): the values are sums over runs of consecutive steps, run k [seq_offsets[k], seq_offsets[k + 1]).
+ * PB_ERR_RANGE if an index is out of range. Sharing and lifetime as for pb_sets. */
+typedef struct pb_pairs pb_pairs;
+int pb_pairs_create(const int64_t* winners_host, const int64_t* losers_host, int64_t num_pairs, int64_t num_values,
+                    const int64_t* seq_offsets_host, pb_pairs** out);
+int pb_pairs_destroy(pb_pairs* pairs);
+int64_t pb_preference_work_bytes(const pb_pairs* pairs);
+
+/* Paired log ratios: z = beta (a_winner - a_loser), a = values - ref (ref_dev NULL: 0), summed over each
+ * run's steps where the pairs have runs; loss_dev[0] = scale * sum of w (-(1 - e) log s(z) - e log s(-z))
+ * with s the sigmoid, e label_smoothing and w weights_dev [num_pairs] (NULL: 1). grad_dev: the loss's
+ * gradient, one entry per value (per step); margins_dev [num_pairs]: z. All float32. */
+int pb_preference_loss(const pb_pairs* pairs, const float* values_dev, const float* ref_dev, const float* weights_dev,
+                       float beta, float label_smoothing, float scale, float* loss_dev, float* grad_dev,
+                       float* margins_dev, void* work_dev, int64_t work_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -39,7 +39,10 @@ EXPORTED_SYMBOLS = (
     "pb_rowlist_partition_noalloc", "pb_transpose_bins", "pb_forest_takes_rows",
     "pb_forest_predict_rows", "pb_bin_rows", "pb_quantile_work_bytes", "pb_column_quantiles",
     "pb_era_corr_work_elems", "pb_era_corr_rows", "pb_fold_tree",
-    "pb_rowlist_facts_get",
+    "pb_rowlist_facts_get", "pb_set_gradients",
+    "pb_sets_create", "pb_sets_destroy", "pb_choice_work_bytes", "pb_choice_log_probs",
+    "pb_choice_log_probs_backward", "pb_policy_loss", "pb_pairs_create", "pb_pairs_destroy",
+    "pb_preference_work_bytes", "pb_preference_loss",
 )
 
 
@@ -72,6 +75,26 @@ class PbFitBuffers(ctypes.Structure):
         ("hist_cnt_dev", ctypes.c_void_p), ("hist_grad_dev", ctypes.c_void_p),
         ("values_dev", ctypes.c_void_p), ("pack_size", ctypes.c_int32),
         ("learning_rate", ctypes.c_float), ("params", PbSplitParams),
+    ]
+
+
+PB_F32, PB_BF16, PB_F16 = 0, 1, 2
+
+
+class PbChoiceScores(ctypes.Structure):
+    _fields_ = [
+        ("scores_dev", ctypes.c_void_p), ("mask_dev", ctypes.c_void_p), ("positions_dev", ctypes.c_void_p),
+        ("table_dev", ctypes.c_void_p), ("buckets_dev", ctypes.c_void_p), ("score_stride", ctypes.c_int64),
+        ("score_type", ctypes.c_int32), ("num_buckets", ctypes.c_int32), ("reach", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+class PbPolicyTerms(ctypes.Structure):
+    _fields_ = [
+        ("advantages_dev", ctypes.c_void_p), ("old_log_probs_dev", ctypes.c_void_p),
+        ("ref_log_probs_dev", ctypes.c_void_p), ("weights_dev", ctypes.c_void_p), ("ratio_min", ctypes.c_float),
+        ("ratio_max", ctypes.c_float), ("kl_weight", ctypes.c_float), ("scale", ctypes.c_float),
     ]
 
 
@@ -157,6 +180,18 @@ _SIGNATURES = {
     "pb_best_thresholds": (ctypes.c_int, [_VP, _I32, _I32, _I32, _VP, _VP, _VP, _VP, _VP, _VP]),
     "pb_pick_sequential": (ctypes.c_int, [_VP, _I32, _I32, _I32, _VP, _VP, _VP]),
     "pb_set_segment_mode": (ctypes.c_int, [_VP, _I32, _I32]),
+    "pb_set_gradients": (ctypes.c_int, [_VP, _VP]),
+    "pb_sets_create": (ctypes.c_int, [_VP, _I64, ctypes.POINTER(_VP)]),
+    "pb_sets_destroy": (ctypes.c_int, [_VP]),
+    "pb_choice_work_bytes": (_I64, [_VP, _I32]),
+    "pb_choice_log_probs": (ctypes.c_int, [_VP, ctypes.POINTER(PbChoiceScores)] + [_VP] * 4 + [_I64, _VP]),
+    "pb_choice_log_probs_backward": (ctypes.c_int, [_VP, ctypes.POINTER(PbChoiceScores)] + [_VP] * 6 + [_I64, _VP]),
+    "pb_policy_loss": (ctypes.c_int, [_VP, ctypes.POINTER(PbChoiceScores), ctypes.POINTER(PbPolicyTerms)] + [_VP] * 6 +
+                       [_I64, _VP]),
+    "pb_pairs_create": (ctypes.c_int, [_VP, _VP, _I64, _I64, _VP, ctypes.POINTER(_VP)]),
+    "pb_pairs_destroy": (ctypes.c_int, [_VP]),
+    "pb_preference_work_bytes": (_I64, [_VP]),
+    "pb_preference_loss": (ctypes.c_int, [_VP] * 4 + [_F32] * 3 + [_VP] * 4 + [_I64, _VP]),
     "pb_rowlist_noalloc_max_segments": (ctypes.c_int64, []),
     "pb_rowlist_partition_noalloc": (ctypes.c_int, [_VP, _I64, _I64, _I32, _VP, _I64, _VP, _VP, _I32, _I32,
                                                     _VP, _VP, _VP, _VP, _I64, _VP, _VP, _VP, _VP]),

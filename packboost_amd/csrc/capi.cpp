@@ -73,6 +73,7 @@ struct pb_ctx {
     int32_t* seg[2];            // [E][segw] segment starts of the rows in sb[i]
     pb::SegState ss;            // partition shape and workspace
     int32_t profile;  // 0 off, 1 every phase, 2 the histogram only
+    const float* given_grad;  // pb_set_gradients: the round's gradients, else preds - y
     int32_t bin_layout;  // bins_dev of pb_hist_build / pb_partition: 0 uint8, 1 nibble
     std::vector<hipEvent_t> ev_free;
     std::vector<std::pair<int32_t, std::array<hipEvent_t, 5>>> ev_pending;
@@ -150,6 +151,11 @@ void free_ctx(pb_ctx* c) {
 }
 
 }  // namespace
+
+namespace pb {
+int api_fail(int code, const char* msg) { return fail(code, msg); }
+int api_hip_fail(hipError_t e, const char* where) { return hip_fail(e, where); }
+}  // namespace pb
 
 extern "C" {
 
@@ -344,13 +350,19 @@ int32_t pb_max_nodes(const pb_ctx* c, int32_t depth) {
 
 const int32_t* pb_era_offsets_dev(const pb_ctx* c) { return c ? c->era_off_dev : nullptr; }
 
+int pb_set_gradients(pb_ctx* c, const float* grad) {
+    if (!c) return fail(PB_ERR_INVALID, "pb_set_gradients: null context");
+    c->given_grad = grad;
+    return PB_OK;
+}
+
 int pb_round_begin(pb_ctx* c, const float* preds, const float* y, float* grad, uint16_t* nid,
                    uint16_t* tnode, void* stream) {
     if (!c || !preds || !y || !grad || !nid || !tnode)
         return fail(PB_ERR_INVALID, "pb_round_begin: null argument");
     const int64_t N = c->d.num_rows;
     const int32_t root_active = (N >= 2 * (int64_t)c->d.min_samples_leaf) ? 1 : 0;
-    PB_HIP(pb::launch_round_begin(preds, y, grad, nid, tnode, N, c->rows_padded, root_active,
+    PB_HIP(pb::launch_round_begin(preds, y, c->given_grad, grad, nid, tnode, N, c->rows_padded, root_active,
                                   c->era_off_dev, c->d.num_eras, c->win_sum, c->sh_era, c->st,
                                   c->ids[0], (hipStream_t)stream),
            "round_begin launch");

@@ -1,0 +1,345 @@
+// C-ABI host layer of the choice and preference operators: their layouts (built on the host, kept on
+// the device), argument checks, workspaces.
+#include <algorithm>
+#include <memory>
+#include <new>
+#include <string>
+#include <vector>
+
+#include "pb_internal.h"
+
+struct pb_sets {
+    pb::SetLayout s;
+    int32_t device;
+    char* arena;  // offsets, items and split list
+};
+
+struct pb_pairs {
+    pb::PairLayout p;
+    int32_t device;
+    pb_sets* lists;
+    pb_sets* seqs;
+    int32_t* arena;  // winners, losers, entries
+};
+
+namespace {
+
+using pb::SetItem;
+
+void free_sets(pb_sets* s) {
+    if (!s) return;
+    if (s->arena) (void)hipFree(s->arena);
+    delete s;
+}
+
+void free_pairs(pb_pairs* p) {
+    if (!p) return;
+    free_sets(p->lists);
+    free_sets(p->seqs);
+    if (p->arena) (void)hipFree(p->arena);
+    delete p;
+}
+
+// Lanes to a set of a tile: about 4 rows a lane on average and at most 32 in the tile's largest set,
+// whose lanes the others' would wait for.
+int32_t team_of(int64_t rows, int64_t sets, int64_t largest) {
+    int32_t t = 0;
+    while (t < 6 && (((int64_t)4 << t) * sets < rows || ((int64_t)32 << t) < largest)) ++t;
+    return t;
+}
+
+int lay_out(const int64_t* off, int64_t num_sets, std::vector<SetItem>& items, std::vector<int32_t>& split) {
+    SetItem tile{};
+    int64_t largest = 0;
+    auto flush = [&] {
+        if (tile.sets == 0) return;
+        tile.team = team_of(tile.rows, tile.sets, largest);
+        items.push_back(tile);
+        tile = SetItem{};
+        largest = 0;
+    };
+    for (int64_t g = 0; g < num_sets; ++g) {
+        const int64_t size = off[g + 1] - off[g];
+        if (size > pb::kSetShort) {
+            flush();
+            const int64_t parts = (size + pb::kSetTileRows - 1) / pb::kSetTileRows;
+            const int64_t each = (size + parts - 1) / parts;
+            for (int64_t p = 0; p < parts; ++p) {
+                SetItem im{};
+                im.row0 = off[g] + p * each;
+                im.rows = (int32_t)std::min(each, off[g + 1] - im.row0);
+                im.set0 = (int32_t)g;
+                im.sets = 1;
+                im.part = (int32_t)p;
+                im.parts = (int32_t)parts;
+                if (parts > 1) split.push_back((int32_t)items.size());
+                items.push_back(im);
+            }
+            continue;
+        }
+        if (tile.rows + size > pb::kSetTileRows || tile.sets == pb::kSetTileSets) flush();
+        if (tile.sets == 0) {
+            tile.row0 = off[g];
+            tile.set0 = (int32_t)g;
+        }
+        tile.rows += (int32_t)size;
+        ++tile.sets;
+        largest = std::max(largest, size);
+    }
+    flush();
+    return 0;
+}
+
+size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+
+int sets_create(const int64_t* off, int64_t num_sets, pb_sets** out) {
+    if (num_sets < 0 || num_sets >= INT32_MAX) return pb::api_fail(PB_ERR_UNSUPPORTED, "pb_sets_create: num_sets must lie in [0, 2^31 - 1)");
+    if (off[0] != 0) return pb::api_fail(PB_ERR_INVALID, "pb_sets_create: offsets must start at 0");
+    for (int64_t g = 0; g < num_sets; ++g)
+        if (off[g + 1] < off[g]) return pb::api_fail(PB_ERR_INVALID, "pb_sets_create: offsets must not decrease");
+    if (off[num_sets] > ((int64_t)1 << 40)) return pb::api_fail(PB_ERR_UNSUPPORTED, "pb_sets_create: more than 2^40 rows");
+    std::vector<SetItem> items;
+    std::vector<int32_t> split;
+    lay_out(off, num_sets, items, split);
+    const size_t b_off = round256(sizeof(int64_t) * (size_t)(num_sets + 1));
+    const size_t b_items = round256(sizeof(SetItem) * items.size());
+    const size_t b_split = round256(sizeof(int32_t) * split.size());
+    std::vector<char> host(b_off + b_items + b_split);
+    std::copy_n(off, num_sets + 1, reinterpret_cast<int64_t*>(host.data()));
+    std::copy(items.begin(), items.end(), reinterpret_cast<SetItem*>(host.data() + b_off));
+    std::copy(split.begin(), split.end(), reinterpret_cast<int32_t*>(host.data() + b_off + b_items));
+    pb_sets* h = new pb_sets();
+    hipError_t e = hipGetDevice(&h->device);
+    if (e == hipSuccess) e = hipMalloc(&h->arena, host.size());
+    if (e == hipSuccess) e = hipMemcpy(h->arena, host.data(), host.size(), hipMemcpyHostToDevice);
+    if (e != hipSuccess) {
+        free_sets(h);
+        return pb::api_hip_fail(e, "pb_sets_create");
+    }
+    h->s.off = reinterpret_cast<int64_t*>(h->arena);
+    h->s.items = reinterpret_cast<SetItem*>(h->arena + b_off);
+    h->s.split = reinterpret_cast<int32_t*>(h->arena + b_off + b_items);
+    h->s.num_items = (int32_t)items.size();
+    h->s.num_split = (int32_t)split.size();
+    h->s.num_sets = num_sets;
+    h->s.rows = off[num_sets];
+    *out = h;
+    return PB_OK;
+}
+
+int pairs_create(const int64_t* winners, const int64_t* losers, int64_t num_pairs, int64_t num_values,
+                 const int64_t* seq_off, pb_pairs** out) {
+    if (num_values >= INT32_MAX || num_pairs >= ((int64_t)1 << 30))
+        return pb::api_fail(PB_ERR_UNSUPPORTED, "pb_pairs_create: at most 2^30 pairs and 2^31 - 2 values");
+    std::vector<int64_t> off((size_t)num_values + 1, 0);
+    for (int64_t p = 0; p < num_pairs; ++p) {
+        if (winners[p] < 0 || winners[p] >= num_values || losers[p] < 0 || losers[p] >= num_values)
+            return pb::api_fail(PB_ERR_RANGE, "pb_pairs_create: a pair names a value out of range");
+        ++off[(size_t)winners[p] + 1];
+        ++off[(size_t)losers[p] + 1];
+    }
+    for (int64_t v = 0; v < num_values; ++v) off[(size_t)v + 1] += off[(size_t)v];
+    // [winners | losers | entries], the entries of a value in the order of its pairs
+    std::vector<int32_t> host((size_t)num_pairs * 4);
+    std::vector<int64_t> next(off.begin(), off.end() - 1);
+    int32_t* entries = host.data() + 2 * num_pairs;
+    for (int64_t p = 0; p < num_pairs; ++p) {
+        host[(size_t)p] = (int32_t)winners[p];
+        host[(size_t)(num_pairs + p)] = (int32_t)losers[p];
+        entries[next[(size_t)winners[p]]++] = (int32_t)(p * 2);
+        entries[next[(size_t)losers[p]]++] = (int32_t)(p * 2 + 1);
+    }
+    std::unique_ptr<pb_pairs, void (*)(pb_pairs*)> h(new pb_pairs(), free_pairs);
+    int rc = sets_create(off.data(), num_values, &h->lists);
+    if (rc == PB_OK && seq_off) rc = sets_create(seq_off, num_values, &h->seqs);
+    if (rc == PB_OK) {
+        hipError_t e = hipGetDevice(&h->device);
+        if (e == hipSuccess) e = hipMalloc(&h->arena, std::max<size_t>(256, host.size() * 4));
+        if (e == hipSuccess && !host.empty()) e = hipMemcpy(h->arena, host.data(), host.size() * 4, hipMemcpyHostToDevice);
+        if (e != hipSuccess) rc = pb::api_hip_fail(e, "pb_pairs_create");
+    }
+    if (rc != PB_OK) return rc;
+    h->p.winners = h->arena;
+    h->p.losers = h->arena + num_pairs;
+    h->p.entries = h->arena + 2 * num_pairs;
+    h->p.num_pairs = num_pairs;
+    h->p.lists = h->lists->s;
+    h->p.has_seqs = h->seqs != nullptr;
+    if (h->seqs) h->p.seqs = h->seqs->s;
+    *out = h.release();
+    return PB_OK;
+}
+
+// Checks what every choice call takes and fills the arguments it shares.
+int choice_args(const char* who, const pb_sets* s, const pb_choice_scores* in, void* work, int64_t work_bytes,
+                pb::ChoiceArgs& a) {
+    const auto bad = [&](int code, const char* what) {
+        return pb::api_fail(code, (std::string(who) + ": " + what).c_str());
+    };
+    if (!s || !in) return bad(PB_ERR_INVALID, "null argument");
+    if (s->s.rows > 0 && !in->scores_dev) return bad(PB_ERR_INVALID, "null scores");
+    if (in->score_type != PB_F32 && in->score_type != PB_BF16 && in->score_type != PB_F16)
+        return bad(PB_ERR_UNSUPPORTED, "scores must be float32, bfloat16 or float16");
+    if (in->num_buckets < 0 || in->num_buckets > pb::kMaxBuckets)
+        return bad(PB_ERR_UNSUPPORTED, "at most 256 position buckets");
+    if (in->num_buckets > 0 && (!in->table_dev || !in->buckets_dev || (s->s.rows > 0 && !in->positions_dev)))
+        return bad(PB_ERR_INVALID, "a position bias needs its table, buckets and positions");
+    if (in->num_buckets > 0 && in->reach < 0) return bad(PB_ERR_INVALID, "reach must not be negative");
+    if (!work || work_bytes < pb_choice_work_bytes(s, in->num_buckets)) return bad(PB_ERR_INVALID, "workspace too small");
+    if (reinterpret_cast<uintptr_t>(work) & 15) return bad(PB_ERR_INVALID, "workspace must be 16-byte aligned");
+    a.num_buckets = in->num_buckets;
+    a.scores = in->scores_dev;
+    a.stride = in->score_stride;
+    a.mask = in->mask_dev;
+    a.positions = in->positions_dev;
+    a.table = in->num_buckets > 0 ? in->table_dev : nullptr;
+    a.buckets = in->buckets_dev;
+    a.reach = in->reach;
+    a.sums = static_cast<double*>(work);
+    a.parts = reinterpret_cast<float2*>(a.sums + (int64_t)pb::choice_grid(s->s) * (3 + in->num_buckets));
+    return PB_OK;
+}
+
+int launch(const char* who, int mode, const pb_sets* s, const pb::ChoiceArgs& a, int32_t type, void* stream) {
+    const hipError_t e = pb::launch_choice(mode, s->s, a, type, (hipStream_t)stream);
+    return e == hipSuccess ? PB_OK : pb::api_hip_fail(e, who);
+}
+
+// A table of sets without any set has no work to launch: its sums are zeros.
+int clear(const char* who, float* out, int64_t n, void* stream) {
+    const hipError_t e = pb::launch_zero(out, n, (hipStream_t)stream);
+    return e == hipSuccess ? PB_OK : pb::api_hip_fail(e, who);
+}
+
+}  // namespace
+
+extern "C" {
+
+int pb_sets_create(const int64_t* offsets_host, int64_t num_sets, pb_sets** out) {
+    if (!out) return pb::api_fail(PB_ERR_INVALID, "pb_sets_create: null output");
+    *out = nullptr;
+    if (!offsets_host) return pb::api_fail(PB_ERR_INVALID, "pb_sets_create: null offsets");
+    try {
+        return sets_create(offsets_host, num_sets, out);
+    } catch (const std::bad_alloc&) {
+        return pb::api_fail(PB_ERR_NOMEM, "pb_sets_create: out of host memory");
+    }
+}
+
+int pb_sets_destroy(pb_sets* sets) {
+    free_sets(sets);
+    return PB_OK;
+}
+
+int64_t pb_choice_work_bytes(const pb_sets* s, int32_t num_buckets) {
+    if (!s || num_buckets < 0 || num_buckets > pb::kMaxBuckets) return -1;
+    return 16 + 8 * ((int64_t)pb::choice_grid(s->s) * (3 + num_buckets) + s->s.num_items);
+}
+
+int pb_choice_log_probs(const pb_sets* s, const pb_choice_scores* in, const int32_t* chosen_dev, float* log_probs_dev,
+                        float* lse_dev, void* work_dev, int64_t work_bytes, void* stream) {
+    pb::ChoiceArgs a{};
+    const int rc = choice_args("pb_choice_log_probs", s, in, work_dev, work_bytes, a);
+    if (rc != PB_OK) return rc;
+    if (s->s.num_sets == 0) return PB_OK;
+    if (!lse_dev || ((chosen_dev || s->s.rows > 0) && !log_probs_dev))
+        return pb::api_fail(PB_ERR_INVALID, "pb_choice_log_probs: null output");
+    a.chosen = chosen_dev;
+    a.log_probs = log_probs_dev;
+    a.lse_out = lse_dev;
+    return launch("pb_choice_log_probs", chosen_dev ? pb::kSteps : pb::kRows, s, a, in->score_type, stream);
+}
+
+int pb_choice_log_probs_backward(const pb_sets* s, const pb_choice_scores* in, const int32_t* chosen_dev,
+                                 const float* grad_dev, const float* lse_dev, void* grad_scores_dev,
+                                 float* grad_table_dev, void* work_dev, int64_t work_bytes, void* stream) {
+    pb::ChoiceArgs a{};
+    const int rc = choice_args("pb_choice_log_probs_backward", s, in, work_dev, work_bytes, a);
+    if (rc != PB_OK) return rc;
+    if (in->num_buckets > 0 && !grad_table_dev)
+        return pb::api_fail(PB_ERR_INVALID, "pb_choice_log_probs_backward: null table gradient");
+    if (s->s.num_sets == 0) return clear("pb_choice_log_probs_backward", grad_table_dev, in->num_buckets, stream);
+    if (!lse_dev || ((chosen_dev || s->s.rows > 0) && !grad_dev) || (s->s.rows > 0 && !grad_scores_dev))
+        return pb::api_fail(PB_ERR_INVALID, "pb_choice_log_probs_backward: null argument");
+    a.chosen = chosen_dev;
+    a.grad = grad_dev;
+    a.lse = lse_dev;
+    a.grad_scores = grad_scores_dev;
+    a.grad_table = grad_table_dev;
+    return launch("pb_choice_log_probs_backward", chosen_dev ? pb::kStepsBack : pb::kRowsBack, s, a, in->score_type, stream);
+}
+
+int pb_policy_loss(const pb_sets* s, const pb_choice_scores* in, const pb_policy_terms* t, const int32_t* chosen_dev,
+                   float* stats_dev, float* log_probs_dev, void* grad_scores_dev, float* grad_table_dev, void* work_dev,
+                   int64_t work_bytes, void* stream) {
+    pb::ChoiceArgs a{};
+    const int rc = choice_args("pb_policy_loss", s, in, work_dev, work_bytes, a);
+    if (rc != PB_OK) return rc;
+    if (!t || !stats_dev || (in->num_buckets > 0 && !grad_table_dev))
+        return pb::api_fail(PB_ERR_INVALID, "pb_policy_loss: null argument");
+    if (s->s.num_sets == 0) {
+        const int rz = clear("pb_policy_loss", stats_dev, 3, stream);
+        return rz != PB_OK ? rz : clear("pb_policy_loss", grad_table_dev, in->num_buckets, stream);
+    }
+    if (!chosen_dev || !log_probs_dev || !t->advantages_dev || !t->old_log_probs_dev || (s->s.rows > 0 && !grad_scores_dev))
+        return pb::api_fail(PB_ERR_INVALID, "pb_policy_loss: null argument");
+    a.chosen = chosen_dev;
+    a.advantages = t->advantages_dev;
+    a.old = t->old_log_probs_dev;
+    a.ref = t->ref_log_probs_dev;
+    a.weights = t->weights_dev;
+    a.ratio_min = t->ratio_min;
+    a.ratio_max = t->ratio_max;
+    a.kl_weight = t->kl_weight;
+    a.scale = t->scale;
+    a.stats = stats_dev;
+    a.log_probs = log_probs_dev;
+    a.grad_scores = grad_scores_dev;
+    a.grad_table = grad_table_dev;
+    return launch("pb_policy_loss", pb::kPolicy, s, a, in->score_type, stream);
+}
+
+int pb_pairs_create(const int64_t* winners_host, const int64_t* losers_host, int64_t num_pairs, int64_t num_values,
+                    const int64_t* seq_offsets_host, pb_pairs** out) {
+    if (!out) return pb::api_fail(PB_ERR_INVALID, "pb_pairs_create: null output");
+    *out = nullptr;
+    if (num_pairs < 0 || num_values < 0 || (num_pairs > 0 && (!winners_host || !losers_host)))
+        return pb::api_fail(PB_ERR_INVALID, "pb_pairs_create: bad shape or null pairs");
+    try {
+        return pairs_create(winners_host, losers_host, num_pairs, num_values, seq_offsets_host, out);
+    } catch (const std::bad_alloc&) {
+        return pb::api_fail(PB_ERR_NOMEM, "pb_pairs_create: out of host memory");
+    }
+}
+
+int pb_pairs_destroy(pb_pairs* pairs) {
+    free_pairs(pairs);
+    return PB_OK;
+}
+
+int64_t pb_preference_work_bytes(const pb_pairs* p) { return p ? pb::preference_work_bytes(p->p) : -1; }
+
+int pb_preference_loss(const pb_pairs* p, const float* values_dev, const float* ref_dev, const float* weights_dev,
+                       float beta, float label_smoothing, float scale, float* loss_dev, float* grad_dev,
+                       float* margins_dev, void* work_dev, int64_t work_bytes, void* stream) {
+    if (!p || !loss_dev) return pb::api_fail(PB_ERR_INVALID, "pb_preference_loss: null argument");
+    const int64_t n = p->p.has_seqs ? p->p.seqs.rows : p->p.lists.num_sets;
+    if (n > 0 && (!values_dev || !grad_dev)) return pb::api_fail(PB_ERR_INVALID, "pb_preference_loss: null argument");
+    if (p->p.num_pairs > 0 && !margins_dev) return pb::api_fail(PB_ERR_INVALID, "pb_preference_loss: null margins");
+    if (!work_dev || work_bytes < pb::preference_work_bytes(p->p))
+        return pb::api_fail(PB_ERR_INVALID, "pb_preference_loss: workspace too small");
+    if (reinterpret_cast<uintptr_t>(work_dev) & 15)
+        return pb::api_fail(PB_ERR_INVALID, "pb_preference_loss: workspace must be 16-byte aligned");
+    pb::PairArgs a{};
+    a.weights = weights_dev;
+    a.beta = beta;
+    a.smoothing = label_smoothing;
+    a.scale = scale;
+    a.margins = margins_dev;
+    a.loss = loss_dev;
+    const hipError_t e = pb::launch_preference(p->p, a, values_dev, ref_dev, grad_dev, static_cast<char*>(work_dev),
+                                               (hipStream_t)stream);
+    return e == hipSuccess ? PB_OK : pb::api_hip_fail(e, "pb_preference_loss");
+}
+
+}  // extern "C"

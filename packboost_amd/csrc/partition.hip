@@ -164,8 +164,9 @@ __global__ __launch_bounds__(kBlock) void partition_kernel(const uint8_t* __rest
 // reduction tree, so the sums do not depend on scheduling), which bounds the eras' fixed-point
 // scales. The first thread also resets the frontier of the round. VEC: the 4 rows of a thread
 // move as one 16-byte (grad, preds, y) and 8-byte (node ids, tree nodes) access (the host checks
-// the alignment; rows_padded is a multiple of 16).
-template <bool VEC>
+// the alignment; rows_padded is a multiple of 16). GIVEN: `preds` holds the gradients themselves (of
+// an objective other than the squared loss) and y is not read.
+template <bool VEC, bool GIVEN>
 __global__ __launch_bounds__(kBlock) void round_begin_kernel(const float* __restrict__ preds,
                                                          const float* __restrict__ y,
                                                          float* __restrict__ grad,
@@ -193,8 +194,8 @@ __global__ __launch_bounds__(kBlock) void round_begin_kernel(const float* __rest
                 ushort4 nv = make_ushort4(PB_INACTIVE, PB_INACTIVE, PB_INACTIVE, PB_INACTIVE);
                 if (r0 + 3 < N) {
                     const float4 p = *reinterpret_cast<const float4*>(preds + r0);
-                    const float4 t = *reinterpret_cast<const float4*>(y + r0);
-                    gv = make_float4(p.x - t.x, p.y - t.y, p.z - t.z, p.w - t.w);
+                    const float4 t = GIVEN ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : *reinterpret_cast<const float4*>(y + r0);
+                    gv = GIVEN ? p : make_float4(p.x - t.x, p.y - t.y, p.z - t.z, p.w - t.w);
                     s = s + fabsf(gv.x);
                     s = s + fabsf(gv.y);
                     s = s + fabsf(gv.z);
@@ -206,7 +207,7 @@ __global__ __launch_bounds__(kBlock) void round_begin_kernel(const float* __rest
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         if (r0 + j < N) {
-                            g4[j] = preds[r0 + j] - y[r0 + j];
+                            g4[j] = GIVEN ? preds[r0 + j] : preds[r0 + j] - y[r0 + j];
                             s = s + fabsf(g4[j]);
                             n4[j] = n_root;
                         }
@@ -223,7 +224,7 @@ __global__ __launch_bounds__(kBlock) void round_begin_kernel(const float* __rest
                 if (r >= rows_padded) break;
                 float g = 0.0f;
                 if (r < N) {
-                    g = preds[r] - y[r];
+                    g = GIVEN ? preds[r] : preds[r] - y[r];
                     s = s + fabsf(g);
                 }
                 grad[r] = g;
@@ -360,19 +361,18 @@ hipError_t launch_frontier_set(Frontier* st, int32_t depth, int32_t num_active, 
     return hipGetLastError();
 }
 
-hipError_t launch_round_begin(const float* preds, const float* y, float* grad, uint16_t* nid,
+hipError_t launch_round_begin(const float* preds, const float* y, const float* given, float* grad, uint16_t* nid,
                               uint16_t* tnode, int64_t N, int64_t rows_padded, int32_t root_active,
                               const int32_t* era_off, int32_t E, float* win_sum, int32_t* sh_era,
                               Frontier* st, int32_t* cur_ids, hipStream_t s) {
     const int grid = grid_for(rows_padded, kGradWinRows, 1024);
-    const bool vec = (rows_padded % 16 == 0) && aligned(preds, 16) && aligned(y, 16) && aligned(grad, 16) &&
+    const float* src = given ? given : preds;
+    const bool vec = (rows_padded % 16 == 0) && aligned(src, 16) && (given || aligned(y, 16)) && aligned(grad, 16) &&
                      aligned(nid, 8) && aligned(tnode, 8);
-    if (vec)
-        hipLaunchKernelGGL(round_begin_kernel<true>, dim3(grid), dim3(kBlock), 0, s, preds, y, grad, nid,
-                           tnode, N, rows_padded, root_active, win_sum, st, cur_ids);
-    else
-        hipLaunchKernelGGL(round_begin_kernel<false>, dim3(grid), dim3(kBlock), 0, s, preds, y, grad, nid,
-                           tnode, N, rows_padded, root_active, win_sum, st, cur_ids);
+    const auto kernel = given ? (vec ? round_begin_kernel<true, true> : round_begin_kernel<false, true>)
+                              : (vec ? round_begin_kernel<true, false> : round_begin_kernel<false, false>);
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(kBlock), 0, s, src, y, grad, nid, tnode, N, rows_padded, root_active,
+                       win_sum, st, cur_ids);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     constexpr int kEras = kBlock / kWave;

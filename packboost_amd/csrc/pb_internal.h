@@ -371,7 +371,8 @@ hipError_t launch_partition_end(const uint8_t* bins, int64_t ld, int32_t nibble,
                                 float* preds, int64_t N, pb_round_header* header, hipStream_t s);
 // Also writes win_sum [ceil(rows_padded / kGradWinRows)] (sum of |grad| per window) and
 // sh_era [E] (era_grad_scale of each era, eras at era_off [E+1]).
-hipError_t launch_round_begin(const float* preds, const float* y, float* grad, uint16_t* nid,
+// given != nullptr: the gradients are read from there instead of formed as preds - y
+hipError_t launch_round_begin(const float* preds, const float* y, const float* given, float* grad, uint16_t* nid,
                               uint16_t* tnode, int64_t N, int64_t rows_padded, int32_t root_active,
                               const int32_t* era_off, int32_t E, float* win_sum, int32_t* sh_era,
                               Frontier* st, int32_t* cur_ids, hipStream_t s);
@@ -486,5 +487,97 @@ hipError_t launch_predict_bins(const uint8_t* bins, int64_t N, int64_t ld, int32
                                const int32_t* left, const int32_t* right, const float* value,
                                const uint8_t* is_leaf, int32_t num_nodes, float* out,
                                hipStream_t s);
+
+// ---- choices and preferences (choice.hip) ----
+// A table of ragged sets laid out for workgroups: items in row order, each a tile of consecutive short
+// sets (parts 0; at most kSetTileRows rows and kSetTileSets sets, lanes of 1 << team to a set) or part
+// `part` of the `parts` of one set of more than kSetShort rows. The items of a set in several parts are
+// consecutive and listed in `split`.
+constexpr int kSetTileRows = 2048;
+constexpr int kSetTileSets = 1024;
+constexpr int kSetShort = 512;
+struct SetItem {
+    int64_t row0;
+    int32_t rows;
+    int32_t set0;
+    int32_t sets;
+    int32_t team;
+    int32_t part;
+    int32_t parts;
+};
+static_assert(sizeof(SetItem) == 32, "an item is 32 bytes");
+struct SetLayout {
+    const int64_t* off;    // [num_sets + 1]
+    const SetItem* items;  // [num_items]
+    const int32_t* split;  // [num_split]
+    int32_t num_items;
+    int32_t num_split;
+    int64_t num_sets;
+    int64_t rows;
+};
+struct PairLayout {
+    const int32_t* winners;  // [num_pairs]
+    const int32_t* losers;
+    const int32_t* entries;  // [2 num_pairs] by value: pair * 2 + (1 where it is the loser)
+    int64_t num_pairs;
+    SetLayout lists;         // the entries of each value (or sequence)
+    SetLayout seqs;          // the steps of each sequence
+    bool has_seqs;
+};
+enum ChoiceMode { kRows, kSteps, kRowsBack, kStepsBack, kPolicy };
+constexpr int kMaxBuckets = 256;
+constexpr int kChoiceGrid = 2048;  // workgroups of a pass over the items: 8 per compute unit
+constexpr int kPairGrid = 1024;
+struct ChoiceArgs {
+    const int64_t* off;
+    const SetItem* items;
+    int32_t num_items;
+    int32_t num_buckets;
+    const void* scores;
+    int64_t stride;
+    const uint8_t* mask;
+    const int32_t* positions;
+    const float* table;
+    const uint8_t* buckets;  // [2 (reach + 1)]: of distances at or before the reference, then after it
+    int32_t reach;
+    const int32_t* chosen;
+    const float* lse;   // backward
+    const float* grad;  // backward: of the rows' or the steps' log-probabilities
+    const float* advantages;
+    const float* old;
+    const float* ref;
+    const float* weights;
+    float ratio_min, ratio_max, kl_weight, scale;
+    float* log_probs;
+    float* lse_out;
+    void* grad_scores;
+    float* grad_table;
+    float* stats;   // policy: loss, kl, clipped weight
+    float2* parts;  // [num_items] maximum and sum of the parts of split sets
+    double* sums;   // [choice_grid][3 (policy) + num_buckets (gradient)]
+};
+struct PairArgs {
+    const int32_t* winners;
+    const int32_t* losers;
+    int64_t num_pairs;
+    const float* values;
+    const float* ref;
+    const float* weights;
+    float beta, smoothing, scale;
+    float* margins;
+    float* slopes;
+    float* loss;
+    double* sums;
+};
+int32_t choice_grid(const SetLayout& s);
+hipError_t launch_zero(float* out, int64_t n, hipStream_t stream);
+hipError_t launch_choice(int mode, const SetLayout& s, ChoiceArgs a, int32_t type, hipStream_t stream);
+hipError_t launch_preference(const PairLayout& p, PairArgs a, const float* values, const float* ref, float* grad,
+                             char* work, hipStream_t stream);
+int64_t preference_work_bytes(const PairLayout& p);
+
+// Sets the calling thread's error message (pb_last_error) and returns the code (capi.cpp).
+int api_fail(int code, const char* msg);
+int api_hip_fail(hipError_t e, const char* where);
 
 }  // namespace pb
