@@ -8,11 +8,13 @@ from .booster import PackBoost, Tree, TreeBuilder, TreeNode
 from .choices import (ChoiceSets, PolicyLoss, PositionBias, PositionBuckets, PreferenceLoss, PreferencePairs,
                       choice_log_probs, choice_log_probs_backward, policy_loss, preference_loss)
 from .config import PackBoostConfig
+from .objectives import ChoicePreferenceObjective, Objective, PolicyObjective, PreferenceObjective
 from .predictor import PackBoostPredictor, load_bundle, save_bundle
 from .wrapper import PackBoostRegressor
 
 __all__ = ["PackBoost", "PackBoostConfig", "PackBoostPredictor", "PackBoostRegressor", "Tree",
            "TreeNode", "TreeBuilder", "load_bundle", "save_bundle",
            "ChoiceSets", "PositionBias", "PositionBuckets", "PreferencePairs", "PolicyLoss", "PreferenceLoss",
-           "choice_log_probs", "choice_log_probs_backward", "policy_loss", "preference_loss"]
+           "choice_log_probs", "choice_log_probs_backward", "policy_loss", "preference_loss",
+           "Objective", "PreferenceObjective", "ChoicePreferenceObjective", "PolicyObjective"]
 __version__ = "0.1.0"

@@ -30,6 +30,7 @@ from .data import (BinningResult, apply_bins, apply_bins_device, detect_prebinne
                    quantile_bin_device)
 from .engine import (DeviceFit, column_major_bins, depth_log_from_round, empty_columns, features_adjacent,
                      padded_rows, subset_size, transpose_rows, tree_arrays_from_log)
+from .objectives import Objective
 
 
 # ------------------------------------------------------------------ tree structures
@@ -202,7 +203,7 @@ def _require_backend(device: torch.device) -> None:
 
 # ------------------------------------------------------------------ booster
 class PackBoost:
-    """Pack-parallel gradient booster with DES scoring (squared loss)."""
+    """Pack-parallel gradient booster with DES scoring (squared loss, or a fit's objective)."""
 
     NONFINITE_POLICIES = ("raise", "truncate")
 
@@ -280,10 +281,17 @@ class PackBoost:
     def fit(self, X, y, era: Iterable[int] | None, *, num_rounds: int,
             feature_names: Sequence[str] | None = None,
             eval_sets: Sequence[tuple] | None = None,
-            round_callback: Callable[[int, dict[str, float]], None] | None = None) -> "PackBoost":
-        """Squared-loss boosting with pack-synchronous growth and DES (booster.py:375-656)."""
+            round_callback: Callable[[int, dict[str, float]], None] | None = None,
+            objective: Objective | None = None) -> "PackBoost":
+        """Boosting with pack-synchronous growth and DES (booster.py:375-656), of the squared loss or of
+        an `objective` (objectives.py). With one, y serves the correlation metrics alone and may be
+        None, and the round metrics hold train_loss, the objective's loss before the round."""
         _require_backend(self._device)
         cfg = self.config
+        if objective is not None and not isinstance(objective, Objective):
+            raise TypeError("objective must be a packboost_amd Objective")
+        if y is None and objective is not None:
+            y = np.zeros(int(X.shape[0]), dtype=np.float32)
         y_np = np.asarray(y.detach().cpu().numpy() if isinstance(y, torch.Tensor) else y,
                           dtype=np.float32)
         if y_np.ndim != 1:
@@ -330,7 +338,20 @@ class PackBoost:
         self._tree_weight = None
         self._trained_pack_size = None
 
-        fitter = DeviceFit(bins_fm, N, y_dev, offsets, cfg)
+        try:
+            if objective is not None:
+                objective.bind(perm, N, device)
+            return self._fit_rounds(DeviceFit(bins_fm, N, y_dev, offsets, cfg, objective=objective), bins_fm, N, F,
+                                    offsets, device, num_rounds, eval_sets, round_callback)
+        finally:
+            if objective is not None:
+                torch.cuda.synchronize(device)
+                objective.release()
+
+    def _fit_rounds(self, fitter: DeviceFit, bins_fm: torch.Tensor, N: int, F: int, offsets: np.ndarray,
+                    device: torch.device, num_rounds: int, eval_sets, round_callback) -> "PackBoost":
+        cfg = self.config
+        E = int(len(offsets) - 1)
         self._fitter = fitter
         k = subset_size(cfg, F)
         era_off_dev = torch.from_numpy(np.asarray(offsets, dtype=np.int32)).to(device)
@@ -393,6 +414,8 @@ class PackBoost:
                     "trees_per_second": (cfg.pack_size / round_time) if round_time > 0 else float("inf"),
                     "round_seconds": round_time,
                 }
+                if log.loss is not None:
+                    metrics["train_loss"] = log.loss
                 metrics.update(eval_corr)
                 self._round_metrics.append(metrics)
                 if round_callback is not None:
@@ -407,6 +430,8 @@ class PackBoost:
         finally:
             torch.cuda.synchronize(device)
         if truncated:
+            if fitter.objective is not None:
+                fitter.objective.rewind(len(self._rounds))
             # the device has run the non-finite round (and the one enqueued after it) on
             # `fitter.preds`: the kept rounds' training predictions come from their trees
             self._train_preds = (self._predict_device(bins_fm, N, device) if self._rounds

@@ -4,7 +4,7 @@
 per-row frontier ids, histogram planes, decision log) and runs one boosting round as a
 sequence of asynchronous kernel launches on the caller's stream:
 
-    round_begin                         grad = preds - y, every row in the root
+    round_begin                         grad = preds - y (or an objective's), every row in the root
     for depth in 0..D-1:
         hist_build -> des_score -> decide -> partition
     round_end                           preds += lr * pack_sum
@@ -75,6 +75,7 @@ class RoundLog:
     decisions: np.ndarray     # DECISION_DTYPE [2^D - 1], depth d at offset 2^d - 1
     root_grad: float          # float32 sum of grad over all rows (root value numerator)
     depths_drawn: int         # feature subsets the reference would have drawn
+    loss: float | None = None  # the objective's loss before the round (fits with an objective)
     phase_ms: np.ndarray | None = None  # float64 [4][D] GPU ms of hist / score / decide /
                                         # partition per depth (timed rounds only: rounds()
                                         # with phase_times or phase_every)
@@ -119,8 +120,10 @@ class DeviceFit:
     def __init__(self, bins_fm: torch.Tensor, num_rows: int, y: torch.Tensor,
                  era_offsets: np.ndarray, cfg: PackBoostConfig, *,
                  stream: torch.cuda.Stream | None = None, bin_layout: str = "auto",
-                 fit_mode: str | None = None) -> None:
-        """bin_layout: "u8" (the histogram reads bins_fm), "nibble" (a two-rows-per-byte copy,
+                 fit_mode: str | None = None, objective=None) -> None:
+        """objective: a bound objectives.Objective whose gradients the rounds take instead of preds - y.
+
+        bin_layout: "u8" (the histogram reads bins_fm), "nibble" (a two-rows-per-byte copy,
         pb_pack_bins4, max_bins <= 16) or "auto" (nibble whenever max_bins <= 16).
 
         fit_mode: "planes" (histogram planes in HBM, then the scorer), "segments" (from a
@@ -252,6 +255,9 @@ class DeviceFit:
         b.learning_rate = self.lr
         b.params = self.params
         self._bufs = b
+        self.objective = objective
+        self._given = None  # the enqueued round's gradients
+        self._loss_host = torch.zeros(2, dtype=torch.float32).pin_memory() if objective is not None else None
         # a root below 2*min_samples_leaf never splits: the per-phase path sets its value
         self._root_splittable = self.N >= 2 * int(cfg.min_samples_leaf)
 
@@ -269,6 +275,16 @@ class DeviceFit:
             pass
 
     # ------------------------------------------------------------------ rounds
+    def _set_gradients(self, slot: int) -> None:
+        """Enqueues the objective's gradients at the current predictions for the round to come, and its
+        loss into host slot `slot`."""
+        if self.objective is None:
+            return
+        with torch.cuda.stream(self.stream):
+            loss, self._given = self.objective.gradient(self.preds[: self.N])
+            _hip.check(self.lib.pb_set_gradients(self.ctx, self._given.data_ptr()), "pb_set_gradients")
+            self._loss_host[slot: slot + 1].copy_(loss.reshape(1), non_blocking=True)
+
     def draw_subsets(self, rng: torch.Generator) -> tuple[np.ndarray, list]:
         """Draws the subsets of every depth, keeping the generator state before each draw."""
         states = []
@@ -290,6 +306,7 @@ class DeviceFit:
         lib, ctx, s = self.lib, self.ctx, _hip.stream_ptr(self.stream)
         chk = _hip.check
         self.feats_host.numpy()[...] = subsets
+        self._set_gradients(0)
         with torch.cuda.stream(self.stream):
             self.feats_dev.copy_(self.feats_host, non_blocking=True)
         chk(lib.pb_round_begin(ctx, self.preds.data_ptr(), self.y.data_ptr(), self.grad.data_ptr(),
@@ -335,6 +352,7 @@ class DeviceFit:
         log_dev = self._log_dev[slot]
         dec_ptr = log_dev.data_ptr()
         hdr_ptr = dec_ptr + self._n_dec * _hip.DECISION_DTYPE.itemsize
+        self._set_gradients(slot)
         with torch.cuda.stream(self.stream):
             self._feats_slot_dev[slot].copy_(fh, non_blocking=True)
             _hip.check(self.lib.pb_grow_round(self.ctx, ctypes.byref(self._bufs),
@@ -358,6 +376,7 @@ class DeviceFit:
         log_dev = self._log_dev[slot]
         dec_ptr = log_dev.data_ptr()
         sp = _hip.stream_ptr(self.stream)
+        self._set_gradients(slot)
         with torch.cuda.stream(self.stream):
             self._win_dev[slot].copy_(wh, non_blocking=True)
             _hip.check(self.lib.pb_select_subsets(
@@ -383,7 +402,11 @@ class DeviceFit:
         u = np.asarray(hdr["u_active"], dtype=np.int32)
         drawn = int(np.count_nonzero(u[: self.D] > 0))
         return RoundLog(u_active=u[: self.D + 1].copy(), tree_size=int(hdr["tree_size"]),
-                        decisions=dec, root_grad=float(dec[0]["node_grad"]), depths_drawn=drawn)
+                        decisions=dec, root_grad=float(dec[0]["node_grad"]), depths_drawn=drawn,
+                        loss=self._loss(slot))
+
+    def _loss(self, slot: int) -> float | None:
+        return None if self._loss_host is None else float(self._loss_host[slot])
 
     def read_phase_ms(self) -> tuple[np.ndarray, np.ndarray]:
         """GPU ms and launch counts [4][D] (hist, score, decide, partition per depth) of the
@@ -499,7 +522,7 @@ class DeviceFit:
         else:
             root_grad = float(self.root_grad_dev.cpu()[0])
         return RoundLog(u_active=u[: self.D + 1].copy(), tree_size=int(ts.value), decisions=dec,
-                        root_grad=root_grad, depths_drawn=drawn)
+                        root_grad=root_grad, depths_drawn=drawn, loss=self._loss(0))
 
     def run_round(self, rng: torch.Generator, events: list | None = None) -> RoundLog:
         """One round, synchronously. With `events` (or a root that cannot split) the round
