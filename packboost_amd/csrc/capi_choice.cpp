@@ -48,13 +48,18 @@ int32_t team_of(int64_t rows, int64_t sets, int64_t largest) {
     return t;
 }
 
-int lay_out(const int64_t* off, int64_t num_sets, std::vector<SetItem>& items, std::vector<int32_t>& split) {
+struct Layout {
+    std::vector<SetItem> tiles, whole, parts;
+    std::vector<int32_t> split;  // the first part of each split set, within `parts`
+};
+
+void lay_out(const int64_t* off, int64_t num_sets, Layout& out) {
     SetItem tile{};
     int64_t largest = 0;
     auto flush = [&] {
         if (tile.sets == 0) return;
         tile.team = team_of(tile.rows, tile.sets, largest);
-        items.push_back(tile);
+        out.tiles.push_back(tile);
         tile = SetItem{};
         largest = 0;
     };
@@ -62,22 +67,30 @@ int lay_out(const int64_t* off, int64_t num_sets, std::vector<SetItem>& items, s
         const int64_t size = off[g + 1] - off[g];
         if (size > pb::kSetShort) {
             flush();
-            const int64_t parts = (size + pb::kSetTileRows - 1) / pb::kSetTileRows;
-            const int64_t each = (size + parts - 1) / parts;
-            for (int64_t p = 0; p < parts; ++p) {
-                SetItem im{};
-                im.row0 = off[g] + p * each;
+            SetItem im{};
+            im.row0 = off[g];
+            im.rows = (int32_t)std::min<int64_t>(size, pb::kSetWideRows);
+            im.set0 = (int32_t)g;
+            im.sets = 1;
+            im.parts = 1;
+            if ((off[g] & 7) + size <= pb::kSetWideRows) {
+                out.whole.push_back(im);
+                continue;
+            }
+            const int64_t most = pb::kSetWideRows - 8;
+            const int64_t want = (size + most - 1) / most;
+            const int64_t each = ((size + want - 1) / want + 7) / 8 * 8;  // at most `most`, itself a multiple of 8
+            im.parts = (int32_t)((size + each - 1) / each);
+            out.split.push_back((int32_t)out.parts.size());
+            for (im.part = 0; im.part < im.parts; ++im.part) {
+                im.row0 = off[g] + im.part * each;
                 im.rows = (int32_t)std::min(each, off[g + 1] - im.row0);
-                im.set0 = (int32_t)g;
-                im.sets = 1;
-                im.part = (int32_t)p;
-                im.parts = (int32_t)parts;
-                if (parts > 1) split.push_back((int32_t)items.size());
-                items.push_back(im);
+                out.parts.push_back(im);
             }
             continue;
         }
-        if (tile.rows + size > pb::kSetTileRows || tile.sets == pb::kSetTileSets) flush();
+        if (tile.sets > 0 && ((tile.row0 & 7) + tile.rows + size > pb::kSetTileRows || tile.sets == pb::kSetTileSets))
+            flush();
         if (tile.sets == 0) {
             tile.row0 = off[g];
             tile.set0 = (int32_t)g;
@@ -87,7 +100,6 @@ int lay_out(const int64_t* off, int64_t num_sets, std::vector<SetItem>& items, s
         largest = std::max(largest, size);
     }
     flush();
-    return 0;
 }
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
@@ -98,9 +110,14 @@ int sets_create(const int64_t* off, int64_t num_sets, pb_sets** out) {
     for (int64_t g = 0; g < num_sets; ++g)
         if (off[g + 1] < off[g]) return pb::api_fail(PB_ERR_INVALID, "pb_sets_create: offsets must not decrease");
     if (off[num_sets] > ((int64_t)1 << 40)) return pb::api_fail(PB_ERR_UNSUPPORTED, "pb_sets_create: more than 2^40 rows");
-    std::vector<SetItem> items;
-    std::vector<int32_t> split;
-    lay_out(off, num_sets, items, split);
+    Layout lay;
+    lay_out(off, num_sets, lay);
+    const size_t tiles = lay.tiles.size(), whole = lay.whole.size();
+    std::vector<SetItem>& items = lay.tiles;  // the tiles, the whole sets, the parts
+    items.insert(items.end(), lay.whole.begin(), lay.whole.end());
+    items.insert(items.end(), lay.parts.begin(), lay.parts.end());
+    for (int32_t& first : lay.split) first += (int32_t)whole;
+    const std::vector<int32_t>& split = lay.split;
     const size_t b_off = round256(sizeof(int64_t) * (size_t)(num_sets + 1));
     const size_t b_items = round256(sizeof(SetItem) * items.size());
     const size_t b_split = round256(sizeof(int32_t) * split.size());
@@ -117,9 +134,12 @@ int sets_create(const int64_t* off, int64_t num_sets, pb_sets** out) {
         return pb::api_hip_fail(e, "pb_sets_create");
     }
     h->s.off = reinterpret_cast<int64_t*>(h->arena);
-    h->s.items = reinterpret_cast<SetItem*>(h->arena + b_off);
+    h->s.tiles = reinterpret_cast<SetItem*>(h->arena + b_off);
+    h->s.wide = h->s.tiles + tiles;
     h->s.split = reinterpret_cast<int32_t*>(h->arena + b_off + b_items);
-    h->s.num_items = (int32_t)items.size();
+    h->s.num_tiles = (int32_t)tiles;
+    h->s.num_wide = (int32_t)(items.size() - tiles);
+    h->s.num_whole = (int32_t)whole;
     h->s.num_split = (int32_t)split.size();
     h->s.num_sets = num_sets;
     h->s.rows = off[num_sets];
@@ -233,7 +253,7 @@ int pb_sets_destroy(pb_sets* sets) {
 
 int64_t pb_choice_work_bytes(const pb_sets* s, int32_t num_buckets) {
     if (!s || num_buckets < 0 || num_buckets > pb::kMaxBuckets) return -1;
-    return 16 + 8 * ((int64_t)pb::choice_grid(s->s) * (3 + num_buckets) + s->s.num_items);
+    return 16 + 8 * ((int64_t)pb::choice_grid(s->s) * (3 + num_buckets) + s->s.num_wide);
 }
 
 int pb_choice_log_probs(const pb_sets* s, const pb_choice_scores* in, const int32_t* chosen_dev, float* log_probs_dev,

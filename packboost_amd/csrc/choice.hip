@@ -6,78 +6,283 @@
 // lse = m + log s and log p_i = (x_i - m) - log s; a set without probability (empty, all masked) has
 // s = 0 and lse = -inf. The gradient of a step's log p_c is [i = c] - p_i, of all rows' d_i - p_i sum d.
 //
-// Work is laid out once per table of sets (set_items): a workgroup takes an item at a time, either a
-// tile of consecutive short sets, staged in LDS and reduced by teams of lanes, or one long set or a
-// part of it, kept in registers. Parts of a set are reduced by an extra pass (part_kernel) before.
-// Every sum has a fixed order (teams, workgroups, then items), so results do not change from run to
-// run. Maxima, sums of exponentials and log-probabilities are float32; losses and the table's gradient
-// are joined in double, each rounded once when it is written.
+// Work is laid out once per table of sets. A wavefront takes a tile of consecutive short sets, 8 rows a
+// lane, and reduces them by a segmented scan over the lanes, whose cost does not depend on how the rows
+// fall into sets; a workgroup takes one longer set, or a part of it, in registers. Parts of a set are
+// reduced by a pass before (part_kernel). Every sum has a fixed order (lanes, waves, workgroups), so
+// results do not change from run to run. Maxima, sums of exponentials and log-probabilities are float32;
+// losses and the table's gradient are joined in double, each rounded once when it is written.
+#include <algorithm>
+
 #include "pb_internal.h"
 
 namespace pb {
 namespace {
 
-constexpr int kPer = kSetTileRows / kBlock;  // rows per thread
 constexpr int kWaves = kBlock / kWave;
-constexpr float kNegInf = -__builtin_huge_valf();
-constexpr int kBins = 1024;  // LDS words of the table's gradient: buckets x copies
+constexpr float kInf = __builtin_huge_valf();
+constexpr int kRun = 8;                                     // consecutive rows of a lane
+constexpr int kWideRuns = kSetWideRows / (kRun * kBlock);   // runs of a thread of a longer set
+constexpr int kTileRounds = kSetTileSets / kWave;           // sets of a tile per lane
+constexpr int kBins = 256;     // LDS words of the table's gradient per wave: buckets x copies
+constexpr int kLookup = 2048;  // bytes of the position lookup kept in LDS
+static_assert(kSetTileRows == kRun * kWave, "a lane holds one run of a tile");
 
-__device__ __forceinline__ float bf16_value(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
+// e^x for x up to about 0 (any x below 88 is right): 2^t at t = x log2(e), whose rounding and
+// log2(e)'s own are made up for by a factor 1 + r log(2). Within 2 units in the last place; results below
+// 2^-126 are 0. NaN stays NaN.
+__device__ __forceinline__ float exp_of(float x) {
+    constexpr float kL = 1.44269502162933349609375f;       // log2(e) rounded to float,
+    constexpr float kLow = 1.92596299112661746887e-8f;     // and what is missing
+    constexpr float kLn2 = 0.69314718055994530942f;
+    x = x < -200.0f ? -200.0f : x;
+    const float t = x * kL;
+    const float r = fmaf(x, kLow, fmaf(x, kL, -t));
+    const float y = __builtin_amdgcn_exp2f(t);
+    return fmaf(y, r * kLn2, y);
+}
 
-__device__ __forceinline__ uint16_t bf16_bits(float f) {  // to nearest, ties to even; NaN stays NaN
-    const uint32_t u = __float_as_uint(f);
-    if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((u >> 16) | 0x40u);
-    return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
+__device__ __forceinline__ float bf16_value(uint32_t b) { return __uint_as_float(b << 16); }
+
+__device__ __forceinline__ float f16_value(uint32_t b) {
+    const uint16_t u = (uint16_t)b;
+    _Float16 h;
+    __builtin_memcpy(&h, &u, 2);
+    return (float)h;
+}
+
+template <int TYPE>
+__device__ __forceinline__ float half_value(uint32_t b) {
+    return TYPE == PB_BF16 ? bf16_value(b) : f16_value(b);
+}
+
+// Two values rounded to nearest, ties to even, as the halves of a word.
+template <int TYPE>
+__device__ __forceinline__ uint32_t half_pair(float lo, float hi) {
+    uint32_t w;
+    if (TYPE == PB_BF16) {
+        const __bf16 h[2] = {(__bf16)lo, (__bf16)hi};
+        __builtin_memcpy(&w, h, 4);
+    } else {
+        const _Float16 h[2] = {(_Float16)lo, (_Float16)hi};
+        __builtin_memcpy(&w, h, 4);
+    }
+    return w;
 }
 
 template <int TYPE>
 __device__ __forceinline__ float load_score(const void* p, int64_t i) {
-    if (TYPE == PB_BF16) return bf16_value(static_cast<const uint16_t*>(p)[i]);
-    if (TYPE == PB_F16) return (float)static_cast<const _Float16*>(p)[i];
-    return static_cast<const float*>(p)[i];
+    if (TYPE == PB_F32) return static_cast<const float*>(p)[i];
+    return half_value<TYPE>(static_cast<const uint16_t*>(p)[i]);
 }
 
 template <int TYPE>
 __device__ __forceinline__ void store_score(void* p, int64_t i, float v) {
-    if (TYPE == PB_BF16)
-        static_cast<uint16_t*>(p)[i] = bf16_bits(v);
-    else if (TYPE == PB_F16)
-        static_cast<_Float16*>(p)[i] = (_Float16)v;
-    else
+    if (TYPE == PB_F32)
         static_cast<float*>(p)[i] = v;
+    else
+        static_cast<uint16_t*>(p)[i] = (uint16_t)half_pair<TYPE>(v, 0.0f);
 }
 
-__device__ __forceinline__ int bucket_of(const ChoiceArgs& a, int64_t row) {
-    const int32_t q = a.positions[row];
+// The rows of an item as its lanes count them: from row q0, a multiple of kRun, on; [lo, hi) are the
+// item's, and all below `end` lie in the table.
+struct Span {
+    int64_t q0;
+    int lo, hi, end;
+};
+
+__device__ __forceinline__ Span span_of(const ChoiceArgs& a, const SetItem& im) {
+    Span s;
+    s.q0 = im.row0 & ~(int64_t)(kRun - 1);
+    s.lo = (int)(im.row0 - s.q0);
+    s.hi = s.lo + im.rows;
+    s.end = (int)min(a.rows - s.q0, (int64_t)1 << 30);
+    return s;
+}
+
+// Runs of kRun rows from row i of a span on: as 16-byte accesses where the addresses are aligned
+// (a.vec) and all lie in the table, else row by row within [lo, hi).
+template <int TYPE>
+__device__ __forceinline__ void load_scores(const ChoiceArgs& a, const Span& s, int i, float (&x)[kRun]) {
+    if (a.vec && i + kRun <= s.end) {
+        if (TYPE == PB_F32) {
+            const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(a.scores) + s.q0 + i);
+            const float4 t = p[0], u = p[1];
+            x[0] = t.x, x[1] = t.y, x[2] = t.z, x[3] = t.w;
+            x[4] = u.x, x[5] = u.y, x[6] = u.z, x[7] = u.w;
+        } else {
+            const uint4 t = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.scores) + s.q0 + i);
+            x[0] = half_value<TYPE>(t.x & 0xffffu), x[1] = half_value<TYPE>(t.x >> 16);
+            x[2] = half_value<TYPE>(t.y & 0xffffu), x[3] = half_value<TYPE>(t.y >> 16);
+            x[4] = half_value<TYPE>(t.z & 0xffffu), x[5] = half_value<TYPE>(t.z >> 16);
+            x[6] = half_value<TYPE>(t.w & 0xffffu), x[7] = half_value<TYPE>(t.w >> 16);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < kRun; ++k)
+            x[k] = i + k >= s.lo && i + k < s.hi ? load_score<TYPE>(a.scores, (s.q0 + i + k) * a.stride) : 0.0f;
+    }
+}
+
+__device__ __forceinline__ void load_floats(const ChoiceArgs& a, const Span& s, int i, const float* p, float (&x)[kRun]) {
+    if (a.vec && i + kRun <= s.end) {
+        const float4* v = reinterpret_cast<const float4*>(p + s.q0 + i);
+        const float4 t = v[0], u = v[1];
+        x[0] = t.x, x[1] = t.y, x[2] = t.z, x[3] = t.w;
+        x[4] = u.x, x[5] = u.y, x[6] = u.z, x[7] = u.w;
+    } else {
+#pragma unroll
+        for (int k = 0; k < kRun; ++k) x[k] = i + k >= s.lo && i + k < s.hi ? p[s.q0 + i + k] : 0.0f;
+    }
+}
+
+__device__ __forceinline__ bool inside(const Span& s, int i) { return i >= s.lo && i + kRun <= s.hi; }
+
+// A run's values out, those in [lo, hi) alone.
+template <int TYPE>
+__device__ __forceinline__ void store_run(const ChoiceArgs& a, const Span& s, int i, void* p, const float (&x)[kRun]) {
+    if (a.vec && inside(s, i)) {
+        if (TYPE == PB_F32) {
+            float4* v = reinterpret_cast<float4*>(static_cast<float*>(p) + s.q0 + i);
+            v[0] = make_float4(x[0], x[1], x[2], x[3]);
+            v[1] = make_float4(x[4], x[5], x[6], x[7]);
+        } else {
+            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + s.q0 + i) =
+                make_uint4(half_pair<TYPE>(x[0], x[1]), half_pair<TYPE>(x[2], x[3]), half_pair<TYPE>(x[4], x[5]),
+                           half_pair<TYPE>(x[6], x[7]));
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < kRun; ++k)
+            if (i + k >= s.lo && i + k < s.hi) store_score<TYPE>(p, s.q0 + i + k, x[k]);
+    }
+}
+
+// The position bias in LDS: the table, and the lookup of its buckets where that is short.
+struct BiasShared {
+    float table[kMaxBuckets];
+    uint8_t lookup[kLookup];
+};
+
+__device__ __forceinline__ uint32_t bucket_of(const ChoiceArgs& a, const BiasShared& b, int32_t q) {
     const uint32_t d = q < 0 ? 0u - (uint32_t)q : (uint32_t)q;
-    return a.buckets[min(d, (uint32_t)a.reach) + (q > 0 ? (uint32_t)a.reach + 1u : 0u)];
+    const uint32_t i = min(d, (uint32_t)a.reach) + (q > 0 ? (uint32_t)a.reach + 1u : 0u);
+    return a.reach < kLookup / 2 ? b.lookup[i] : a.buckets[i];
 }
 
+__device__ __forceinline__ void stage_bias(const ChoiceArgs& a, BiasShared& b) {
+    for (int i = (int)threadIdx.x; i < a.num_buckets; i += kBlock) b.table[i] = a.table[i];
+    if (a.reach < kLookup / 2)
+        for (int i = (int)threadIdx.x; i < 2 * (a.reach + 1); i += kBlock) b.lookup[i] = a.buckets[i];
+    __syncthreads();
+}
+
+// Buckets of a run's rows, a byte each.
+struct Buckets {
+    uint32_t w[2];
+    __device__ __forceinline__ int at(int k) const { return (int)(w[k >> 2] >> (8 * (k & 3)) & 0xffu); }
+};
+
+// A run's logits: -inf outside [lo, hi) and where masked (`hidden`, a bit a row).
 template <int TYPE, bool MASK, bool BIAS>
-__device__ __forceinline__ float load_logit(const ChoiceArgs& a, int64_t row) {
+__device__ __forceinline__ void load_logits(const ChoiceArgs& a, const BiasShared* bias, const Span& s, int i,
+                                            float (&x)[kRun], uint32_t& hidden, Buckets& buckets) {
+    const bool vec = a.vec && i + kRun <= s.end;
+    load_scores<TYPE>(a, s, i, x);
+    hidden = 0;
+    buckets.w[0] = buckets.w[1] = 0;
+    if (MASK) {
+        if (vec) {
+            const uint2 m = *reinterpret_cast<const uint2*>(a.mask + s.q0 + i);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                hidden |= (m.x >> (8 * k) & 0xffu) == 0 ? 1u << k : 0u;
+                hidden |= (m.y >> (8 * k) & 0xffu) == 0 ? 16u << k : 0u;
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < kRun; ++k)
+                if (i + k >= s.lo && i + k < s.hi && !a.mask[s.q0 + i + k]) hidden |= 1u << k;
+        }
+    }
+    if (BIAS) {
+        int32_t pos[kRun];
+        if (vec) {
+            const int4* p = reinterpret_cast<const int4*>(a.positions + s.q0 + i);
+            const int4 t = p[0], u = p[1];
+            pos[0] = t.x, pos[1] = t.y, pos[2] = t.z, pos[3] = t.w;
+            pos[4] = u.x, pos[5] = u.y, pos[6] = u.z, pos[7] = u.w;
+        } else {
+#pragma unroll
+            for (int k = 0; k < kRun; ++k) pos[k] = i + k >= s.lo && i + k < s.hi ? a.positions[s.q0 + i + k] : 0;
+        }
+#pragma unroll
+        for (int k = 0; k < kRun; ++k) {
+            const uint32_t b = bucket_of(a, *bias, pos[k]);
+            buckets.w[k >> 2] |= b << (8 * (k & 3));
+            x[k] += bias->table[b];
+        }
+    }
+    if (MASK) {
+#pragma unroll
+        for (int k = 0; k < kRun; ++k)
+            if (hidden >> k & 1u) x[k] = -kInf;
+    }
+    if (!inside(s, i)) {
+#pragma unroll
+        for (int k = 0; k < kRun; ++k)
+            if (i + k < s.lo || i + k >= s.hi) x[k] = -kInf;
+    }
+}
+
+// One logit.
+template <int TYPE, bool BIAS>
+__device__ __forceinline__ float one_logit(const ChoiceArgs& a, const BiasShared* bias, int64_t row) {
     float x = load_score<TYPE>(a.scores, row * a.stride);
-    if (BIAS) x += a.table[bucket_of(a, row)];
-    if (MASK && !a.mask[row]) x = kNegInf;
+    if (BIAS) x += bias->table[bucket_of(a, *bias, a.positions[row])];
     return x;
 }
 
-__device__ __forceinline__ float nan_max(float a, float b) { return b > a ? b : a; }  // a NaN b is passed over
-
-__device__ float block_max(float v, float* sh) {
+// Gradients of a run: 0 where masked, and outside [lo, hi) (nothing is added there).
+template <bool MASK>
+__device__ __forceinline__ void clear_hidden(const Span& s, int i, uint32_t hidden, float (&g)[kRun]) {
+    if (MASK) {
 #pragma unroll
-    for (int m = kWave / 2; m >= 1; m >>= 1) v = nan_max(v, __shfl_xor(v, m));
-    __syncthreads();
-    if ((threadIdx.x & (kWave - 1)) == 0) sh[threadIdx.x / kWave] = v;
-    __syncthreads();
-    float t = sh[0];
-    for (int w = 1; w < kWaves; ++w) t = nan_max(t, sh[w]);
-    return t;
+        for (int k = 0; k < kRun; ++k)
+            if (hidden >> k & 1u) g[k] = 0.0f;
+    }
+    if (!inside(s, i)) {
+#pragma unroll
+        for (int k = 0; k < kRun; ++k)
+            if (i + k < s.lo || i + k >= s.hi) g[k] = 0.0f;
+    }
+}
+
+__device__ __forceinline__ float over(float a, float b) { return b > a ? b : a; }  // a NaN b is passed over
+
+// LDS written by lanes of this wave is read by others of it: the wave's LDS accesses keep their order,
+// the compiler must too.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+template <class F>
+__device__ __forceinline__ F wave_sum(F v) {
+#pragma unroll
+    for (int m = kWave / 2; m >= 1; m >>= 1) v += __shfl_xor(v, m);
+    return v;
+}
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int m = kWave / 2; m >= 1; m >>= 1) v = over(v, __shfl_xor(v, m));
+    return v;
 }
 
 template <class F>
 __device__ F block_sum(F v, F* sh) {
-#pragma unroll
-    for (int m = kWave / 2; m >= 1; m >>= 1) v += __shfl_xor(v, m);
+    v = wave_sum(v);
     __syncthreads();
     if ((threadIdx.x & (kWave - 1)) == 0) sh[threadIdx.x / kWave] = v;
     __syncthreads();
@@ -86,320 +291,653 @@ __device__ F block_sum(F v, F* sh) {
     return t;
 }
 
-// What a step's log-probability gives and takes.
-struct Step {
-    bool counts;  // the chosen row lies in the set, is on offer, and the set has probability
-    float lp;
-    float coef;   // gradient of the loss with respect to lp
+// (maximum, sum of exponentials) of a set from those of its parts. A part without probability has sum 0
+// and any maximum.
+struct Soft {
+    float top, sum;
 };
 
-// Where the step's choice lies: the row in the set, or -1 for a step that is left out.
-template <bool MASK>
-__device__ __forceinline__ int64_t chosen_row(const ChoiceArgs& a, int64_t g, int64_t r0, int64_t size) {
-    const int32_t c = a.chosen[g];
-    if (c < 0 || c >= size) return -1;
-    if (MASK && !a.mask[r0 + c]) return -1;
-    return c;
+// The workgroup's from its waves' (every lane of a wave holds the wave's).
+__device__ __forceinline__ Soft block_soft(Soft w, Soft* sh) {
+    __syncthreads();
+    if ((threadIdx.x & (kWave - 1)) == 0) sh[threadIdx.x / kWave] = w;
+    __syncthreads();
+    Soft t{-kInf, 0.0f};
+    for (int i = 0; i < kWaves; ++i) t.top = over(t.top, sh[i].sum != 0.0f ? sh[i].top : -kInf);
+    if (t.top == -kInf) t.top = 0.0f;
+    for (int i = 0; i < kWaves; ++i) t.sum += sh[i].sum != 0.0f ? sh[i].sum * exp_of(sh[i].top - t.top) : 0.0f;
+    return t;
+}
+
+// A wave's from its lanes' (one part each, or none).
+__device__ __forceinline__ Soft wave_soft(Soft l) {
+    Soft w;
+    w.top = wave_max(l.sum != 0.0f ? l.top : -kInf);
+    if (w.top == -kInf) w.top = 0.0f;
+    w.sum = wave_sum(l.sum != 0.0f ? l.sum * exp_of(l.top - w.top) : 0.0f);
+    return w;
+}
+
+// A lane's from parts first, first + step, ... of a set.
+__device__ __forceinline__ Soft join_parts(const float2* parts, int n, int first, int step) {
+    Soft l{-kInf, 0.0f};
+    for (int j = first; j < n; j += step) l.top = over(l.top, parts[j].y != 0.0f ? parts[j].x : -kInf);
+    if (l.top == -kInf) l.top = 0.0f;
+    for (int j = first; j < n; j += step) l.sum += parts[j].y != 0.0f ? parts[j].y * exp_of(parts[j].x - l.top) : 0.0f;
+    return l;
+}
+
+// Sums and maxima over runs of rows that may start and end in any lane of a wave. `heads` holds a bit for
+// each row of the lane that starts a set, `tails` for each that ends one. A lane's value since its last
+// head is carried on by a scan of the lanes that stops at heads: 4 steps in rows of 16 lanes, 2 between
+// them.
+struct Segments {
+    uint32_t heads, tails;
+    bool from1, from2, from4, from8, from15, from31;  // the scan's steps that stay within the set
+
+    __device__ __forceinline__ void start(uint32_t h, int lane, int first, int last) {  // rows first .. last - 1 of the lane
+        heads = h;
+        const unsigned long long m = __ballot(h != 0);
+        const unsigned long long next = __ballot((h & 1u) != 0);
+        tails = h >> 1 | ((lane < kWave - 1 && (next >> (lane + 1) & 1ull)) ? 1u << (kRun - 1) : 0u);
+        if (last >= 1 && last <= kRun) tails |= 1u << (last - 1);
+        const uint32_t from = first <= 0 ? 0xffu : first >= kRun ? 0u : 0xffu << first;
+        const uint32_t upto = last <= 0 ? 0u : last >= kRun ? 0xffu : (1u << last) - 1u;
+        tails &= from & upto;
+        const unsigned long long below = m & (~0ull >> (kWave - 1 - lane));
+        const int head = below ? kWave - 1 - __clzll((long long)below) : 0;  // the last lane up to this one with a head
+        const int in_row = lane & 15;
+        from1 = in_row >= 1 && lane - 1 >= head;
+        from2 = in_row >= 2 && lane - 2 >= head;
+        from4 = in_row >= 4 && lane - 4 >= head;
+        from8 = in_row >= 8 && lane - 8 >= head;
+        from15 = (lane & 16) != 0 && (lane & ~15) - 1 >= head;
+        from31 = lane >= 32 && 31 >= head;
+    }
+};
+
+template <int CTRL>
+__device__ __forceinline__ float lane_move(float v) {  // lanes without a source keep their own
+    const int i = __float_as_int(v);
+    return __int_as_float(__builtin_amdgcn_update_dpp(i, i, CTRL, 0xf, 0xf, false));
+}
+
+struct TakeMax {
+    static constexpr float kNone = -__builtin_huge_valf();
+    static __device__ __forceinline__ float of(float a, float b) { return over(a, b); }
+};
+struct TakeSum {
+    static constexpr float kNone = 0.0f;
+    static __device__ __forceinline__ float of(float a, float b) { return a + b; }
+};
+
+// out[id[k] - 1] = the reduction of x over the set that row k ends; `before`: the lane's rows up to its
+// first head belong to a set that began in a lane below.
+template <class OP>
+__device__ __forceinline__ void segment_reduce(const Segments& seg, const float (&x)[kRun], const int (&id)[kRun],
+                                               int lane, float* out) {
+    float v = OP::of(OP::kNone, x[0]);
+#pragma unroll
+    for (int k = 1; k < kRun; ++k) v = OP::of(seg.heads >> k & 1u ? OP::kNone : v, x[k]);
+    float t;
+    t = lane_move<0x111>(v), v = seg.from1 ? OP::of(t, v) : v;    // row_shr:1
+    t = lane_move<0x112>(v), v = seg.from2 ? OP::of(t, v) : v;    // row_shr:2
+    t = lane_move<0x114>(v), v = seg.from4 ? OP::of(t, v) : v;    // row_shr:4
+    t = lane_move<0x118>(v), v = seg.from8 ? OP::of(t, v) : v;    // row_shr:8
+    t = lane_move<0x142>(v), v = seg.from15 ? OP::of(t, v) : v;   // row_bcast:15
+    t = lane_move<0x143>(v), v = seg.from31 ? OP::of(t, v) : v;   // row_bcast:31
+    t = __shfl_up(v, 1);
+    v = lane > 0 ? t : OP::kNone;
+#pragma unroll
+    for (int k = 0; k < kRun; ++k) {
+        v = OP::of(seg.heads >> k & 1u ? OP::kNone : v, x[k]);
+        if (seg.tails >> k & 1u) out[id[k] - 1] = v;
+    }
 }
 
 // The clipped loss of a step and its slope: surrogate min(rA, clip(r) A) with r = exp(lp - old), and
 // kl = e^d - d - 1 with d = ref - lp. A NaN ratio takes no bound, so it stays visible.
-__device__ __forceinline__ void policy_step(const ChoiceArgs& a, int64_t g, Step& st, bool tally, double (&sum)[3]) {
-    const float w = (a.weights ? a.weights[g] : 1.0f) * a.scale;
-    const float adv = a.advantages[g];
-    const float ratio = expf(st.lp - a.old[g]);
-    const float free = ratio * adv;
-    const float held = fminf(fmaxf(ratio, a.ratio_min), a.ratio_max) * adv;
+struct PolicyIn {
+    float adv, old, ref, w;
+};
+
+__device__ __forceinline__ PolicyIn load_policy(const ChoiceArgs& a, int64_t g) {
+    return PolicyIn{a.advantages[g], a.old[g], a.ref ? a.ref[g] : 0.0f, a.weights ? a.weights[g] : 1.0f};
+}
+
+__device__ __forceinline__ float policy_step(const ChoiceArgs& a, const PolicyIn& in, float lp, bool tally, double (&sum)[3]) {
+    const float w = in.w * a.scale;
+    const float ratio = expf(lp - in.old);
+    const float free = ratio * in.adv;
+    const float held = fminf(fmaxf(ratio, a.ratio_min), a.ratio_max) * in.adv;
     const bool clipped = free > held;
     float kl = 0.0f, slope = clipped ? 0.0f : -free;
     if (a.ref) {
-        const float d = a.ref[g] - st.lp;
+        const float d = in.ref - lp;
         const float e = expf(d);
         kl = e - d - 1.0f;
         slope += a.kl_weight * (1.0f - e);
     }
-    st.coef = w * slope;
     if (tally) {
         sum[0] += (double)(w * (a.kl_weight * kl - (clipped ? held : free)));
         sum[1] += (double)(w * kl);
         sum[2] += clipped ? (double)w : 0.0;
     }
+    return w * slope;
 }
 
-// The maximum and the sum of exponentials of a part of a set, or (listwise backward) the sum of its
-// rows' gradients.
-template <int MODE, int TYPE, bool MASK, bool BIAS>
-__global__ __launch_bounds__(kBlock) void part_kernel(ChoiceArgs a, const int32_t* __restrict__ list) {
-    __shared__ float sh[kWaves];
-    const int32_t it = list[blockIdx.x];
-    const SetItem im = a.items[it];
-    float v[kPer], top = kNegInf, sum = 0.0f;
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-        const int i = k * kBlock + (int)threadIdx.x;
-        const int64_t row = im.row0 + i;
-        if (MODE == kRowsBack) {
-            if (i < im.rows && (!MASK || a.mask[row])) sum += a.grad[row];
-        } else {
-            v[k] = i < im.rows ? load_logit<TYPE, MASK, BIAS>(a, row) : kNegInf;
-            top = nan_max(top, v[k]);
-        }
-    }
-    if (MODE != kRowsBack) {
-        top = block_max(top, sh);
-        if (top == kNegInf) top = 0.0f;
-#pragma unroll
-        for (int k = 0; k < kPer; ++k) sum += expf(v[k] - top);
-    }
-    sum = block_sum(sum, sh);
-    if (threadIdx.x == 0) a.parts[it] = make_float2(top, sum);
-}
+// The table's gradient as a wave gathers it: bins of whole numbers in units of 2^(e - 30), 2^e above
+// every gradient so far, so that their sums do not depend on the order of the atomics; what the rounding
+// takes is below 2^-31 * 2^e a row. A larger gradient empties the bins into `sum` (lane l holds
+// buckets l, l + 64, ...) and raises e. Copies of the bins keep lanes that meet in a bucket apart.
+struct TableSum {
+    unsigned long long* bins;  // [kBins] of this wave
+    int* bad;                  // [num_buckets]: a gradient that is not finite
+    int copies, e;
+    float limit;               // 2^e, 0 before the first gradient
+    double sum[kMaxBuckets / kWave];
 
-// One item at a time per workgroup; see the head of the file.
-template <int MODE, int TYPE, bool MASK, bool BIAS>
-__global__ __launch_bounds__(kBlock) void choice_kernel(ChoiceArgs a) {
-    constexpr bool GRAD = MODE == kRowsBack || MODE == kStepsBack || MODE == kPolicy;
-    constexpr bool STEPS = MODE != kRows && MODE != kRowsBack;
-    constexpr bool TABLE = BIAS && GRAD;
-    __shared__ float xs[kSetTileRows];
-    __shared__ float dsum[MODE == kRowsBack ? kSetTileRows : 1];
-    __shared__ float shf[kWaves];
-    __shared__ double shd[kWaves];
-    __shared__ unsigned long long bins[TABLE ? kBins : 1];
-    __shared__ double table_sum[TABLE ? kMaxBuckets : 1];
-    __shared__ int table_nan[TABLE ? kMaxBuckets : 1];
-    const int tid = (int)threadIdx.x;
-    // copies of the table's bins, so that lanes that meet in a bucket rarely meet in a word
-    int copies = 1;
-    if (TABLE) {
-        while (copies < 32 && copies * 2 * a.num_buckets <= kBins) copies *= 2;
-        for (int i = tid; i < copies * a.num_buckets; i += kBlock) bins[i] = 0;
-        for (int b = tid; b < a.num_buckets; b += kBlock) {
-            table_sum[b] = 0.0;
-            table_nan[b] = 0;
-        }
+    __device__ void start(const ChoiceArgs& a, unsigned long long* b, int* flags) {
+        bins = b;
+        bad = flags;
+        copies = 1;
+        while (copies * 2 * a.num_buckets <= kBins && copies < 32) copies *= 2;
+        e = 0;
+        limit = 0.0f;
+        const int lane = (int)threadIdx.x & (kWave - 1);
+        for (int i = lane; i < kBins; i += kWave) bins[i] = 0;
+#pragma unroll
+        for (int k = 0; k < kMaxBuckets / kWave; ++k) sum[k] = 0.0;
+        wave_sync();
     }
-    double tally[3] = {0.0, 0.0, 0.0};
-    for (int it = (int)blockIdx.x; it < a.num_items; it += (int)gridDim.x) {
-        const SetItem im = a.items[it];
-        float v[kPer];
-        uint32_t hidden = 0;
-        int bucket[kPer];
+
+    __device__ void empty(const ChoiceArgs& a) {
+        wave_sync();
+        const int lane = (int)threadIdx.x & (kWave - 1);
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) {
-            const int i = k * kBlock + tid;
-            v[k] = kNegInf;
-            bucket[k] = 0;
-            if (i < im.rows) {
-                const int64_t row = im.row0 + i;
-                float x = load_score<TYPE>(a.scores, row * a.stride);
-                if (BIAS) {
-                    bucket[k] = bucket_of(a, row);
-                    x += a.table[bucket[k]];
-                }
-                if (MASK && !a.mask[row]) {
-                    x = kNegInf;
-                    hidden |= 1u << k;
-                }
-                v[k] = x;
-            }
-        }
-        if (im.parts == 0) {
-            __syncthreads();  // the last item's tile has been read
-#pragma unroll
-            for (int k = 0; k < kPer; ++k) {
-                const int i = k * kBlock + tid;
-                if (i < im.rows) {
-                    xs[i] = v[k];
-                    if (MODE == kRowsBack) dsum[i] = (hidden >> k) & 1u ? 0.0f : a.grad[im.row0 + i];
-                }
-            }
-            __syncthreads();
-            const int L = 1 << im.team, lane = tid & (L - 1);
-            for (int s = tid >> im.team; s < im.sets; s += kBlock >> im.team) {
-                const int64_t g = (int64_t)im.set0 + s;
-                const int64_t r0 = a.off[g];
-                const int b = (int)(r0 - im.row0), e = (int)(a.off[g + 1] - im.row0);
-                float top = 0.0f, sum = 0.0f, lse = 0.0f;
-                if (MODE == kRows || MODE == kSteps || MODE == kPolicy) {
-                    top = kNegInf;
-                    for (int i = b + lane; i < e; i += L) top = nan_max(top, xs[i]);
-                    for (int m = 1; m < L; m <<= 1) top = nan_max(top, __shfl_xor(top, m));
-                    if (top == kNegInf) top = 0.0f;
-                    for (int i = b + lane; i < e; i += L) sum += expf(xs[i] - top);
-                    for (int m = 1; m < L; m <<= 1) sum += __shfl_xor(sum, m);
-                    lse = top + logf(sum);
-                    if (lane == 0 && MODE != kPolicy) a.lse_out[g] = lse;
-                } else {
-                    lse = a.lse[g];
-                }
-                if (MODE == kRows) {
-                    const float ls = logf(sum);
-                    for (int i = b + lane; i < e; i += L) xs[i] = xs[i] == kNegInf ? kNegInf : (xs[i] - top) - ls;
-                }
-                if (MODE == kRowsBack) {
-                    float d = 0.0f;
-                    for (int i = b + lane; i < e; i += L) d += dsum[i];
-                    for (int m = 1; m < L; m <<= 1) d += __shfl_xor(d, m);
-                    for (int i = b + lane; i < e; i += L)
-                        xs[i] = dsum[i] - (xs[i] == kNegInf ? 0.0f : expf(xs[i] - lse) * d);
-                }
-                if (STEPS) {
-                    const int64_t c = chosen_row<MASK>(a, g, r0, e - b);
-                    Step st;
-                    st.counts = c >= 0 && (MODE == kStepsBack ? lse != kNegInf : sum != 0.0f);
-                    st.lp = st.counts && MODE != kStepsBack ? (xs[b + c] - top) - logf(sum) : 0.0f;
-                    st.coef = 0.0f;
-                    if (MODE == kStepsBack && st.counts) st.coef = a.grad[g];
-                    if (MODE == kPolicy && st.counts) policy_step(a, g, st, lane == 0, tally);
-                    if (MODE != kStepsBack && lane == 0) a.log_probs[g] = st.lp;
-                    if (GRAD) {
-                        const float shift = MODE == kStepsBack ? lse : top;
-                        const float f = MODE == kStepsBack ? st.coef : st.coef / sum;
-                        for (int i = b + lane; i < e; i += L) {
-                            const float p = xs[i] == kNegInf ? 0.0f : expf(xs[i] - shift);
-                            xs[i] = st.counts ? (i - b == c ? st.coef : 0.0f) - f * p : 0.0f;
-                        }
-                    }
-                }
-            }
-            __syncthreads();
-#pragma unroll
-            for (int k = 0; k < kPer; ++k) {
-                const int i = k * kBlock + tid;
-                if (i < im.rows) v[k] = xs[i];
-            }
-        } else {
-            const int64_t g = im.set0;
-            const int64_t r0 = a.off[g], size = a.off[g + 1] - r0;
-            float top = 0.0f, sum = 0.0f, lse = 0.0f, d = 0.0f, dv[kPer];
-            if (MODE == kRowsBack) {
-#pragma unroll
-                for (int k = 0; k < kPer; ++k) {
-                    const int i = k * kBlock + tid;
-                    dv[k] = i < im.rows && !((hidden >> k) & 1u) ? a.grad[im.row0 + i] : 0.0f;
-                }
-            }
-            if (MODE == kStepsBack) {
-                lse = a.lse[g];
-            } else if (im.parts > 1) {
-                const float2* parts = a.parts + (it - im.part);
-                top = kNegInf;
-                for (int j = tid; j < im.parts; j += kBlock) top = nan_max(top, parts[j].y != 0.0f ? parts[j].x : kNegInf);
-                top = block_max(top, shf);
-                if (top == kNegInf) top = 0.0f;
-                for (int j = tid; j < im.parts; j += kBlock)
-                    sum += MODE == kRowsBack ? parts[j].y : parts[j].y != 0.0f ? parts[j].y * expf(parts[j].x - top) : 0.0f;
-                sum = block_sum(sum, shf);
-                if (MODE == kRowsBack) d = sum;
-            } else if (MODE == kRowsBack) {
-#pragma unroll
-                for (int k = 0; k < kPer; ++k) d += dv[k];
-                d = block_sum(d, shf);
-            } else {
-                top = kNegInf;
-#pragma unroll
-                for (int k = 0; k < kPer; ++k) top = nan_max(top, v[k]);
-                top = block_max(top, shf);
-                if (top == kNegInf) top = 0.0f;
-#pragma unroll
-                for (int k = 0; k < kPer; ++k) sum += expf(v[k] - top);
-                sum = block_sum(sum, shf);
-            }
-            const bool first = im.part == 0 && tid == 0;
-            if (MODE == kRowsBack) {
-                lse = a.lse[g];
-#pragma unroll
-                for (int k = 0; k < kPer; ++k) v[k] = dv[k] - (v[k] == kNegInf ? 0.0f : expf(v[k] - lse) * d);
-            }
-            const float ls = logf(sum);
-            if ((MODE == kRows || MODE == kSteps) && first) a.lse_out[g] = top + ls;
-            if (MODE == kRows) {
-#pragma unroll
-                for (int k = 0; k < kPer; ++k) v[k] = v[k] == kNegInf ? kNegInf : (v[k] - top) - ls;
-            }
-            if (STEPS) {
-                const int64_t c = chosen_row<MASK>(a, g, r0, size);
-                Step st;
-                st.counts = c >= 0 && (MODE == kStepsBack ? lse != kNegInf : sum != 0.0f);
-                st.lp = st.counts && MODE != kStepsBack ? (load_logit<TYPE, MASK, BIAS>(a, r0 + c) - top) - ls : 0.0f;
-                st.coef = 0.0f;
-                if (MODE == kStepsBack && st.counts) st.coef = a.grad[g];
-                if (MODE == kPolicy && st.counts) policy_step(a, g, st, first, tally);
-                if (MODE != kStepsBack && first) a.log_probs[g] = st.lp;
-                if (GRAD) {
-                    const float shift = MODE == kStepsBack ? lse : top;
-                    const float f = MODE == kStepsBack ? st.coef : st.coef / sum;
-                    const int64_t at = r0 + c - im.row0;  // the chosen row, as this part counts
-#pragma unroll
-                    for (int k = 0; k < kPer; ++k) {
-                        const float p = v[k] == kNegInf ? 0.0f : expf(v[k] - shift);
-                        v[k] = st.counts ? (k * kBlock + tid == at ? st.coef : 0.0f) - f * p : 0.0f;
-                    }
-                }
-            }
-        }
-        if (MODE == kRows) {
-#pragma unroll
-            for (int k = 0; k < kPer; ++k) {
-                const int i = k * kBlock + tid;
-                if (i < im.rows) a.log_probs[im.row0 + i] = v[k];
-            }
-        }
-        if (GRAD) {
-#pragma unroll
-            for (int k = 0; k < kPer; ++k) {
-                const int i = k * kBlock + tid;
-                if ((hidden >> k) & 1u) v[k] = 0.0f;
-                if (i < im.rows) store_score<TYPE>(a.grad_scores, im.row0 + i, v[k]);
-            }
-        }
-        if (TABLE) {
-            // The item's gradients as whole numbers of 2^(e - 30), 2^e above the largest of them: their
-            // sums do not depend on the order of the atomics, and what the rounding takes is below
-            // 2^-31 of the largest a row. Gradients that are not finite make their bucket NaN.
-            float big = 0.0f;
-#pragma unroll
-            for (int k = 0; k < kPer; ++k) {
-                const int i = k * kBlock + tid;
-                const float m = fabsf(v[k]);
-                if (i < im.rows && m < __builtin_huge_valf()) big = fmaxf(big, m);
-            }
-            big = block_max(big, shf);
-            int e = 0;
-            (void)frexpf(big, &e);
-            const int own_copy = tid & (copies - 1);
-#pragma unroll
-            for (int k = 0; k < kPer; ++k) {
-                const int i = k * kBlock + tid;
-                if (i < im.rows && v[k] != 0.0f) {
-                    if (fabsf(v[k]) < __builtin_huge_valf())
-                        atomicAdd(&bins[bucket[k] * copies + own_copy],
-                                  (unsigned long long)(long long)__float2int_rn(ldexpf(v[k], 30 - e)));
-                    else
-                        table_nan[bucket[k]] = 1;
-                }
-            }
-            __syncthreads();
-            for (int b = tid; b < a.num_buckets; b += kBlock) {
+        for (int k = 0; k < kMaxBuckets / kWave; ++k) {
+            const int b = k * kWave + lane;
+            if (b < a.num_buckets) {
                 long long t = 0;
                 for (int c = 0; c < copies; ++c) {
                     t += (long long)bins[b * copies + c];
                     bins[b * copies + c] = 0;
                 }
-                table_sum[b] += ldexp((double)t, e - 30);
+                sum[k] += ldexp((double)t, e - 30);
             }
-            __syncthreads();
+        }
+        wave_sync();
+    }
+
+    // raises e above every lane's `big`, finite; the whole wave
+    __device__ __forceinline__ void make_room(const ChoiceArgs& a, float big) {
+        if (__any(big >= limit && big > 0.0f)) {
+            empty(a);
+            (void)frexpf(wave_max(big), &e);
+            limit = ldexpf(1.0f, e);
         }
     }
-    const int cols = (MODE == kPolicy ? 3 : 0) + (TABLE ? a.num_buckets : 0);
-    double* mine = a.sums + (int64_t)blockIdx.x * cols;
+
+    __device__ __forceinline__ void put(float v, int bucket) {
+        if (fabsf(v) < kInf)
+            atomicAdd(&bins[bucket * copies + ((int)threadIdx.x & (copies - 1))],
+                      (unsigned long long)(long long)__float2int_rn(ldexpf(v, 30 - e)));
+        else
+            bad[bucket] = 1;
+    }
+
+    __device__ __forceinline__ void add(const ChoiceArgs& a, const float (&g)[kRun], const Buckets& buckets) {
+        float big = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kRun; ++k) {
+            const float m = fabsf(g[k]);
+            if (m < kInf) big = fmaxf(big, m);
+        }
+        make_room(a, big);
+#pragma unroll
+        for (int k = 0; k < kRun; ++k)
+            if (g[k] != 0.0f) put(g[k], buckets.at(k));
+    }
+};
+
+// The maximum and the sum of exponentials of a part of a set, or (listwise backward) the sum of its
+// rows' gradients.
+template <int MODE, int TYPE, bool MASK, bool BIAS>
+__global__ __launch_bounds__(kBlock) void part_kernel(ChoiceArgs a, int first) {
+    __shared__ Soft sh[kWaves];
+    __shared__ float shf[kWaves];
+    __shared__ BiasShared bias;
+    const int it = first + (int)blockIdx.x;
+    const Span s = span_of(a, a.wide[it]);
+    if (BIAS && MODE != kRowsBack) stage_bias(a, bias);
+    float v[kWideRuns][kRun];
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kWideRuns; ++j) {
+        const int i = kRun * (j * kBlock + (int)threadIdx.x);
+#pragma unroll
+        for (int k = 0; k < kRun; ++k) v[j][k] = MODE == kRowsBack ? 0.0f : -kInf;
+        if (i < s.hi) {
+            if (MODE == kRowsBack) {
+                load_floats(a, s, i, a.grad, v[j]);
+                uint32_t hidden = 0;
+                if (MASK)
+#pragma unroll
+                    for (int k = 0; k < kRun; ++k)
+                        if (i + k >= s.lo && i + k < s.hi && !a.mask[s.q0 + i + k]) hidden |= 1u << k;
+                clear_hidden<MASK>(s, i, hidden, v[j]);
+            } else {
+                uint32_t hidden;
+                Buckets buckets;
+                load_logits<TYPE, MASK, BIAS>(a, &bias, s, i, v[j], hidden, buckets);
+            }
+        }
+    }
+    if (MODE == kRowsBack) {
+#pragma unroll
+        for (int j = 0; j < kWideRuns; ++j)
+#pragma unroll
+            for (int k = 0; k < kRun; ++k) sum += v[j][k];
+        sum = block_sum(sum, shf);
+        if (threadIdx.x == 0) a.parts[it] = make_float2(0.0f, sum);
+        return;
+    }
+    float top = -kInf;
+#pragma unroll
+    for (int j = 0; j < kWideRuns; ++j)
+#pragma unroll
+        for (int k = 0; k < kRun; ++k) top = over(top, v[j][k]);
+    top = wave_max(top);
+    if (top == -kInf) top = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kWideRuns; ++j)
+#pragma unroll
+        for (int k = 0; k < kRun; ++k) sum += exp_of(v[j][k] - top);
+    const Soft t = block_soft(Soft{top, wave_sum(sum)}, sh);
+    if (threadIdx.x == 0) a.parts[it] = make_float2(t.top, t.sum);
+}
+
+// What a wave keeps of its tile in LDS.
+struct TileShared {
+    float x[kSetTileRows];          // logits, then what the chosen rows' gradients are more than the others'
+    float shift[kSetTileSets];      // per set: maximum, or lse
+    float factor[kSetTileSets];     // sum of exponentials, then what the rows' are multiplied by
+    uint16_t head[kSetTileRows];    // the set that starts at a row, from 1; 0: none
+    uint16_t begin[kSetTileSets + 4];
+};
+
+__device__ __forceinline__ void write_run(float* p, const float (&x)[kRun]) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+}
+
+__device__ __forceinline__ void read_run(const float* p, float (&x)[kRun]) {
+    const float4 t = reinterpret_cast<const float4*>(p)[0], u = reinterpret_cast<const float4*>(p)[1];
+    x[0] = t.x, x[1] = t.y, x[2] = t.z, x[3] = t.w;
+    x[4] = u.x, x[5] = u.y, x[6] = u.z, x[7] = u.w;
+}
+
+// One tile of short sets by one wave.
+template <int MODE, int TYPE, bool MASK, bool BIAS>
+__device__ __forceinline__ void tile_pass(const ChoiceArgs& a, const SetItem& im, TileShared& sh, const BiasShared* bias,
+                                          TableSum& table, double (&tally)[3]) {
+    constexpr bool GRAD = MODE == kRowsBack || MODE == kStepsBack || MODE == kPolicy;
+    constexpr bool STEPS = MODE != kRows && MODE != kRowsBack;
+    constexpr bool SOFT = MODE == kRows || MODE == kSteps || MODE == kPolicy;
+    const int lane = (int)threadIdx.x & (kWave - 1);
+    const Span sp = span_of(a, im);
+    const int i0 = kRun * lane;
+    // everything the tile reads is asked for before anything is waited for
+    float x[kRun], d[kRun];
+    uint32_t hidden = 0;
+    Buckets buckets{{0, 0}};
+#pragma unroll
+    for (int k = 0; k < kRun; ++k) x[k] = -kInf, d[k] = 0.0f;
+    if (i0 < sp.hi) {
+        load_logits<TYPE, MASK, BIAS>(a, bias, sp, i0, x, hidden, buckets);
+        if (MODE == kRowsBack) {
+            load_floats(a, sp, i0, a.grad, d);
+            clear_hidden<MASK>(sp, i0, hidden, d);
+        }
+    }
+    int32_t begin[kTileRounds], chosen[kTileRounds];
+    float given[kTileRounds], lse[kTileRounds];
+    PolicyIn pol[kTileRounds];
+#pragma unroll
+    for (int r = 0; r < kTileRounds; ++r) {
+        const int s = r * kWave + lane;
+        const int64_t g = (int64_t)im.set0 + s;
+        chosen[r] = -1;
+        given[r] = lse[r] = 0.0f;
+        if (s < im.sets) {
+            begin[r] = (int)(a.off[g] - sp.q0);
+            if (STEPS) chosen[r] = a.chosen[g];
+            if (MODE == kStepsBack) given[r] = a.grad[g];
+            if (!SOFT) lse[r] = a.lse[g];
+            if (MODE == kPolicy) pol[r] = load_policy(a, g);
+        }
+    }
+    wave_sync();  // the last tile's values have been read
+    *reinterpret_cast<uint4*>(&sh.head[i0]) = make_uint4(0, 0, 0, 0);
+    if (STEPS) write_run(&sh.x[i0], x);
+#pragma unroll
+    for (int r = 0; r < kTileRounds; ++r) {
+        const int s = r * kWave + lane;
+        if (s < im.sets) {
+            sh.begin[s] = (uint16_t)begin[r];
+            if (!SOFT) sh.shift[s] = lse[r];
+        }
+    }
+    if (lane == 0) sh.begin[im.sets] = (uint16_t)sp.hi;
+    wave_sync();
+    // which set each row is of, and the chosen rows' logits (a choice outside its set is none)
+    int end[kTileRounds];
+    float picked[kTileRounds];
+#pragma unroll
+    for (int r = 0; r < kTileRounds; ++r) {
+        const int s = r * kWave + lane;
+        if (s < im.sets) {
+            end[r] = sh.begin[s + 1];
+            if (end[r] > begin[r]) sh.head[begin[r]] = (uint16_t)(s + 1);
+            if (STEPS) {
+                if (chosen[r] >= end[r] - begin[r]) chosen[r] = -1;
+                picked[r] = chosen[r] >= 0 ? sh.x[begin[r] + chosen[r]] : -kInf;
+            }
+        }
+    }
+    wave_sync();
+    int id[kRun];
+    Segments seg;
+    {
+        const uint4 w = *reinterpret_cast<const uint4*>(&sh.head[i0]);
+        const int raw[kRun] = {(int)(w.x & 0xffffu), (int)(w.x >> 16), (int)(w.y & 0xffffu), (int)(w.y >> 16),
+                               (int)(w.z & 0xffffu), (int)(w.z >> 16), (int)(w.w & 0xffffu), (int)(w.w >> 16)};
+        uint32_t heads = 0;
+        int last = 0;
+#pragma unroll
+        for (int k = 0; k < kRun; ++k) {
+            heads |= raw[k] ? 1u << k : 0u;
+            last = raw[k] ? raw[k] : last;
+        }
+        // the set that the rows before the lane's first head are of: the last head's below
+        const unsigned long long below = __ballot(heads != 0) & ((1ull << lane) - 1ull);
+        const int from = below ? kWave - 1 - __clzll((long long)below) : lane;
+        const int carried = __shfl(last, from);
+        int now = below ? carried : 1;
+#pragma unroll
+        for (int k = 0; k < kRun; ++k) {
+            now = raw[k] ? raw[k] : now;
+            id[k] = now;
+        }
+        if (SOFT || MODE == kRowsBack) seg.start(heads, lane, sp.lo - i0, sp.hi - i0);
+    }
+    float v[kRun];
+    if (SOFT) {
+        segment_reduce<TakeMax>(seg, x, id, lane, sh.shift);
+        wave_sync();
+#pragma unroll
+        for (int k = 0; k < kRun; ++k) {
+            const float t = sh.shift[id[k] - 1];
+            v[k] = exp_of(x[k] - (t == -kInf ? 0.0f : t));
+        }
+        segment_reduce<TakeSum>(seg, v, id, lane, sh.factor);
+        wave_sync();
+    }
+    if (MODE == kRowsBack) {
+        segment_reduce<TakeSum>(seg, d, id, lane, sh.factor);
+        wave_sync();
+    }
+    // a lane to a set: log-probabilities, losses, slopes
+    float coef[kTileRounds];
+    if (SOFT || STEPS) {
+#pragma unroll
+        for (int r = 0; r < kTileRounds; ++r) {
+            const int s = r * kWave + lane;
+            coef[r] = 0.0f;
+            if (s < im.sets) {
+                const int64_t g = (int64_t)im.set0 + s;
+                const bool empty = end[r] == begin[r];
+                float top = SOFT ? (empty ? 0.0f : sh.shift[s]) : lse[r];
+                if (SOFT && top == -kInf) top = 0.0f;
+                const float sum = SOFT && !empty ? sh.factor[s] : 0.0f;
+                const float ls = SOFT ? logf(sum) : 0.0f;
+                if (MODE == kRows || MODE == kSteps) a.lse_out[g] = top + ls;
+                if (MODE == kRows) {
+                    sh.shift[s] = top;
+                    sh.factor[s] = ls;
+                }
+                if (STEPS) {
+                    // left out: a choice outside the set or masked, a set without probability. A masked row's
+                    // logit is -inf, as one of that score is: the mask says which.
+                    bool counts = chosen[r] >= 0 && (SOFT ? sum != 0.0f : top != -kInf);
+                    if (MASK && counts && picked[r] == -kInf) counts = a.mask[sp.q0 + begin[r] + chosen[r]] != 0;
+                    const float lp = SOFT && counts ? (picked[r] - top) - ls : 0.0f;
+                    if (SOFT) a.log_probs[g] = lp;
+                    if (MODE == kStepsBack && counts) coef[r] = given[r];
+                    if (MODE == kPolicy && counts) coef[r] = policy_step(a, pol[r], lp, true, tally);
+                    if (GRAD) sh.factor[s] = counts ? (SOFT ? -coef[r] / sum : -coef[r]) : 0.0f;
+                    if (!counts) chosen[r] = -1;
+                }
+            }
+        }
+    }
+    if (MODE == kSteps) return;
+    if (STEPS) {  // the chosen rows' own part
+        const float none[kRun] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+        write_run(&sh.x[i0], none);
+        wave_sync();
+#pragma unroll
+        for (int r = 0; r < kTileRounds; ++r)
+            if (r * kWave + lane < im.sets && chosen[r] >= 0) sh.x[begin[r] + chosen[r]] = coef[r];
+    }
+    wave_sync();
+    if (MODE == kRows) {
+#pragma unroll
+        for (int k = 0; k < kRun; ++k)
+            v[k] = x[k] == -kInf ? -kInf : (x[k] - sh.shift[id[k] - 1]) - sh.factor[id[k] - 1];
+    }
+    if (MODE == kRowsBack) {
+#pragma unroll
+        for (int k = 0; k < kRun; ++k)
+            v[k] = d[k] - (x[k] == -kInf ? 0.0f : exp_of(x[k] - sh.shift[id[k] - 1]) * sh.factor[id[k] - 1]);
+    }
+    if (STEPS) {
+        float own[kRun];
+        read_run(&sh.x[i0], own);
+#pragma unroll
+        for (int k = 0; k < kRun; ++k) {
+            const float f = sh.factor[id[k] - 1];
+            const float e = SOFT ? v[k] : exp_of(x[k] - sh.shift[id[k] - 1]);
+            v[k] = (f == 0.0f ? 0.0f : f * e) + own[k];
+        }
+    }
+    if (GRAD) clear_hidden<MASK>(sp, i0, hidden, v);
+    if (i0 < sp.hi) {
+        if (MODE == kRows)
+            store_run<PB_F32>(a, sp, i0, a.log_probs, v);
+        else
+            store_run<TYPE>(a, sp, i0, a.grad_scores, v);
+    }
+    if (BIAS && GRAD) table.add(a, v, buckets);
+}
+
+// One set of more than kSetShort rows, or a part of it, by a workgroup.
+template <int MODE, int TYPE, bool MASK, bool BIAS>
+__device__ __forceinline__ void wide_pass(const ChoiceArgs& a, const SetItem& im, int32_t index, Soft* shs, float* shf,
+                                          const BiasShared* bias, TableSum& table, double (&tally)[3]) {
+    constexpr bool GRAD = MODE == kRowsBack || MODE == kStepsBack || MODE == kPolicy;
+    constexpr bool STEPS = MODE != kRows && MODE != kRowsBack;
+    constexpr bool SOFT = MODE == kRows || MODE == kSteps || MODE == kPolicy;
+    const int tid = (int)threadIdx.x;
+    const Span sp = span_of(a, im);
+    const int64_t g = im.set0;
+    const bool first = im.part == 0 && tid == 0;
+    float v[kWideRuns][kRun], d[kWideRuns][kRun];
+    uint32_t hidden[kWideRuns];
+    Buckets buckets[kWideRuns];
+#pragma unroll
+    for (int j = 0; j < kWideRuns; ++j) {
+        const int i = kRun * (j * kBlock + tid);
+        hidden[j] = 0;
+        buckets[j].w[0] = buckets[j].w[1] = 0;
+#pragma unroll
+        for (int k = 0; k < kRun; ++k) v[j][k] = -kInf, d[j][k] = 0.0f;
+        if (i < sp.hi) {
+            load_logits<TYPE, MASK, BIAS>(a, bias, sp, i, v[j], hidden[j], buckets[j]);
+            if (MODE == kRowsBack) {
+                load_floats(a, sp, i, a.grad, d[j]);
+                clear_hidden<MASK>(sp, i, hidden[j], d[j]);
+            }
+        }
+    }
+    const float lse = SOFT ? 0.0f : a.lse[g];
+    const int32_t c = STEPS ? a.chosen[g] : -1;
+    const int live = (sp.hi + kRun * kBlock - 1) / (kRun * kBlock);  // runs that hold rows
+    Soft t{0.0f, 0.0f};
+    float own = 1.0f;  // what the wave's exponentials are relative to, over the set's maximum
+    if (SOFT) {
+        Soft w;
+        if (im.parts > 1) {
+            t = block_soft(wave_soft(join_parts(a.parts + (index - im.part), im.parts, tid, kBlock)), shs);
+            w.top = t.top;
+        } else {
+            w.top = -kInf;
+#pragma unroll
+            for (int j = 0; j < kWideRuns; ++j)
+#pragma unroll
+                for (int k = 0; k < kRun; ++k) w.top = over(w.top, v[j][k]);
+            w.top = wave_max(w.top);
+            if (w.top == -kInf) w.top = 0.0f;
+        }
+        w.sum = 0.0f;
+        if (im.parts == 1 || GRAD) {
+#pragma unroll
+            for (int j = 0; j < kWideRuns; ++j)
+                if (j < live)
+#pragma unroll
+                    for (int k = 0; k < kRun; ++k) {
+                        const float e = exp_of(v[j][k] - w.top);
+                        w.sum += e;
+                        if (GRAD) v[j][k] = e;
+                    }
+        }
+        if (im.parts == 1) {
+            w.sum = wave_sum(w.sum);
+            t = block_soft(w, shs);
+            if (GRAD) own = w.sum != 0.0f ? exp_of(w.top - t.top) : 0.0f;
+        }
+    }
+    const float ls = SOFT ? logf(t.sum) : 0.0f;
+    if ((MODE == kRows || MODE == kSteps) && first) a.lse_out[g] = t.top + ls;
+    if (MODE == kRows) {
+#pragma unroll
+        for (int j = 0; j < kWideRuns; ++j)
+#pragma unroll
+            for (int k = 0; k < kRun; ++k) v[j][k] = v[j][k] == -kInf ? -kInf : (v[j][k] - t.top) - ls;
+    }
+    if (MODE == kRowsBack) {
+        float total = 0.0f;
+        if (im.parts > 1) {
+            const float2* parts = a.parts + (index - im.part);
+            for (int j = tid; j < im.parts; j += kBlock) total += parts[j].y;
+        } else {
+#pragma unroll
+            for (int j = 0; j < kWideRuns; ++j)
+#pragma unroll
+                for (int k = 0; k < kRun; ++k) total += d[j][k];
+        }
+        total = block_sum(total, shf);
+#pragma unroll
+        for (int j = 0; j < kWideRuns; ++j)
+            if (j < live)
+#pragma unroll
+                for (int k = 0; k < kRun; ++k)
+                    v[j][k] = d[j][k] - (v[j][k] == -kInf ? 0.0f : exp_of(v[j][k] - lse) * total);
+    }
+    int at = -kRun;  // the chosen row, as the span counts
+    float extra = 0.0f;
+    if (STEPS) {
+        const int64_t r0 = a.off[g], size = a.off[g + 1] - r0;
+        bool counts = c >= 0 && c < size && (SOFT ? t.sum != 0.0f : lse != -kInf);
+        if (MASK && counts) counts = a.mask[r0 + c] != 0;
+        const float xc = counts ? one_logit<TYPE, BIAS>(a, bias, r0 + c) : 0.0f;
+        const float lp = SOFT && counts ? (xc - t.top) - ls : 0.0f;
+        if (SOFT && first) a.log_probs[g] = lp;
+        if (GRAD) {
+            float coef = 0.0f;
+            if (MODE == kStepsBack && counts) coef = a.grad[g];
+            if (MODE == kPolicy && counts) coef = policy_step(a, load_policy(a, g), lp, first, tally);
+            const float f = counts ? (SOFT ? -coef / t.sum : -coef) : 0.0f;
+            const float fw = f * own;
+            const int64_t row = r0 + c - sp.q0;
+            if (counts && row >= sp.lo && row < sp.hi) {
+                at = (int)row;
+                extra = coef;
+            }
+#pragma unroll
+            for (int j = 0; j < kWideRuns; ++j)
+                if (j < live)
+#pragma unroll
+                    for (int k = 0; k < kRun; ++k) {
+                        const float e = SOFT ? v[j][k] : exp_of(v[j][k] - lse);
+                        v[j][k] = f == 0.0f ? 0.0f : fw * e;
+                    }
+        }
+    }
+    if (MODE == kSteps) return;
+#pragma unroll
+    for (int j = 0; j < kWideRuns; ++j) {
+        const int i = kRun * (j * kBlock + tid);
+        if (MODE == kRows) {
+            if (i < sp.hi) store_run<PB_F32>(a, sp, i, a.log_probs, v[j]);
+        } else {
+            clear_hidden<MASK>(sp, i, hidden[j], v[j]);
+            if (STEPS && at >= i && at < i + kRun) {
+#pragma unroll
+                for (int k = 0; k < kRun; ++k)
+                    if (at - i == k) v[j][k] += extra;
+            }
+            if (i < sp.hi) store_run<TYPE>(a, sp, i, a.grad_scores, v[j]);
+            if (BIAS && j < live) table.add(a, v[j], buckets[j]);
+        }
+    }
+}
+
+// The steps of the sets in parts, from the parts' maxima and sums: a wave to a set.
+template <int TYPE, bool MASK, bool BIAS>
+__global__ __launch_bounds__(kBlock) void split_steps_kernel(ChoiceArgs a, const int32_t* __restrict__ firsts, int n) {
+    __shared__ BiasShared bias;
+    if (BIAS) stage_bias(a, bias);
+    const int lane = (int)threadIdx.x & (kWave - 1), k = (int)blockIdx.x * kWaves + (int)threadIdx.x / kWave;
+    if (k >= n) return;
+    const SetItem im = a.wide[firsts[k]];
+    const int64_t g = im.set0, r0 = a.off[g], size = a.off[g + 1] - r0;
+    const int32_t c = a.chosen[g];
+    const Soft t = wave_soft(join_parts(a.parts + firsts[k], im.parts, lane, kWave));
+    bool counts = c >= 0 && c < size && t.sum != 0.0f;
+    if (MASK && counts) counts = a.mask[r0 + c] != 0;
+    const float ls = logf(t.sum);
+    if (lane == 0) {
+        a.lse_out[g] = t.top + ls;
+        a.log_probs[g] = counts ? (one_logit<TYPE, BIAS>(a, &bias, r0 + c) - t.top) - ls : 0.0f;
+    }
+}
+
+// What a workgroup leaves behind of the loss's sums and the table's gradient: in its row of a.sums
+// (workgroup `block` of the call's), or as the result where it is the only one.
+template <int MODE, bool TABLE>
+__device__ __forceinline__ void leave_sums(const ChoiceArgs& a, int block, double (&tally)[3], TableSum& table,
+                                           unsigned long long (*bins)[kBins], const int* bad, double* shd) {
+    const int tid = (int)threadIdx.x, wave = tid / kWave, lane = tid & (kWave - 1);
+    const int head = MODE == kPolicy ? 3 : 0;
+    const int cols = head + (TABLE ? a.num_buckets : 0);
+    double* mine = a.sums + (int64_t)block * cols;
     if (MODE == kPolicy) {
 #pragma unroll
         for (int j = 0; j < 3; ++j) {
             const double t = block_sum(tally[j], shd);
             if (tid == 0) {
-                if (gridDim.x == 1)
+                if (a.blocks == 1)
                     a.stats[j] = (float)t;
                 else
                     mine[j] = t;
@@ -407,14 +945,70 @@ __global__ __launch_bounds__(kBlock) void choice_kernel(ChoiceArgs a) {
         }
     }
     if (TABLE) {
+        table.empty(a);
+        double* own = reinterpret_cast<double*>(bins[wave]);
+#pragma unroll
+        for (int k = 0; k < kMaxBuckets / kWave; ++k) own[k * kWave + lane] = table.sum[k];
+        __syncthreads();
         for (int b = tid; b < a.num_buckets; b += kBlock) {
-            const double t = table_nan[b] ? __longlong_as_double(0x7ff8000000000000ll) : table_sum[b];
-            if (gridDim.x == 1)
+            double t = 0.0;
+            for (int w = 0; w < kWaves; ++w) t += reinterpret_cast<const double*>(bins[w])[b];
+            if (bad[b]) t = __longlong_as_double(0x7ff8000000000000ll);
+            if (a.blocks == 1)
                 a.grad_table[b] = (float)t;
             else
-                mine[(MODE == kPolicy ? 3 : 0) + b] = t;
+                mine[head + b] = t;
         }
     }
+}
+
+template <int MODE, bool BIAS>
+constexpr bool kTable = BIAS && (MODE == kRowsBack || MODE == kStepsBack || MODE == kPolicy);
+
+// The tiles, one a wave at a time.
+template <int MODE, int TYPE, bool MASK, bool BIAS>
+__global__ __launch_bounds__(kBlock) void tile_kernel(ChoiceArgs a) {
+    constexpr bool TABLE = kTable<MODE, BIAS>;
+    __shared__ TileShared tiles[kWaves];
+    __shared__ BiasShared bias;
+    __shared__ unsigned long long bins[TABLE ? kWaves : 1][kBins];
+    __shared__ int bad[kMaxBuckets];
+    __shared__ double shd[kWaves];
+    const int tid = (int)threadIdx.x, wave = tid / kWave;
+    TableSum table;
+    if (TABLE) {
+        for (int b = tid; b < kMaxBuckets; b += kBlock) bad[b] = 0;
+        table.start(a, bins[wave], bad);
+    }
+    if (BIAS) stage_bias(a, bias);
+    double tally[3] = {0.0, 0.0, 0.0};
+    for (int it = (int)blockIdx.x * kWaves + wave; it < a.num_tiles; it += (int)gridDim.x * kWaves)
+        tile_pass<MODE, TYPE, MASK, BIAS>(a, a.tiles[it], tiles[wave], &bias, table, tally);
+    leave_sums<MODE, TABLE>(a, (int)blockIdx.x, tally, table, bins, bad, shd);
+}
+
+// The longer sets and their parts, one a workgroup at a time.
+template <int MODE, int TYPE, bool MASK, bool BIAS>
+__global__ __launch_bounds__(kBlock) void wide_kernel(ChoiceArgs a) {
+    constexpr bool TABLE = kTable<MODE, BIAS>;
+    __shared__ BiasShared bias;
+    __shared__ unsigned long long bins[TABLE ? kWaves : 1][kBins];
+    __shared__ int bad[kMaxBuckets];
+    __shared__ Soft shs[kWaves];
+    __shared__ float shf[kWaves];
+    __shared__ double shd[kWaves];
+    const int tid = (int)threadIdx.x, wave = tid / kWave;
+    TableSum table;
+    if (TABLE) {
+        for (int b = tid; b < kMaxBuckets; b += kBlock) bad[b] = 0;
+        table.start(a, bins[wave], bad);
+    }
+    if (BIAS) stage_bias(a, bias);
+    double tally[3] = {0.0, 0.0, 0.0};
+    const int n = MODE == kSteps ? a.num_whole : a.num_wide;
+    for (int it = (int)blockIdx.x; it < n; it += (int)gridDim.x)
+        wide_pass<MODE, TYPE, MASK, BIAS>(a, a.wide[it], it, shs, shf, &bias, table, tally);
+    leave_sums<MODE, TABLE>(a, a.blocks - (int)gridDim.x + (int)blockIdx.x, tally, table, bins, bad, shd);
 }
 
 // out[j] = sum over the workgroups' sums [n][cols] of column j, in a fixed order; the first `head`
@@ -435,8 +1029,10 @@ __global__ __launch_bounds__(kBlock) void join_kernel(const double* __restrict__
 // pairs that a value is in (list entry: pair * 2 + (1 where it is the loser)).
 struct SumArgs {
     const int64_t* off;
-    const SetItem* items;
-    int32_t num_items;
+    const SetItem* tiles;
+    const SetItem* wide;
+    int32_t num_tiles;
+    int32_t num_wide;
     const float* values;
     const float* ref;
     const int32_t* entries;
@@ -457,23 +1053,12 @@ __device__ __forceinline__ double sum_term(const SumArgs& a, int64_t i) {
 
 template <bool PAIRS>
 __global__ __launch_bounds__(kBlock) void set_sum_kernel(SumArgs a) {
-    __shared__ double xs[kSetTileRows];
+    constexpr int kPer = kSetTileRows / kWave;
+    __shared__ double xs[kWaves][kSetTileRows];
     __shared__ double sh[kWaves];
-    const int tid = (int)threadIdx.x;
-    const SetItem im = a.items[blockIdx.x];
-    if (im.parts == 0) {
-        for (int i = tid; i < im.rows; i += kBlock) xs[i] = sum_term<PAIRS>(a, im.row0 + i);
-        __syncthreads();
-        const int L = 1 << im.team, lane = tid & (L - 1);
-        for (int s = tid >> im.team; s < im.sets; s += kBlock >> im.team) {
-            const int64_t g = (int64_t)im.set0 + s;
-            const int b = (int)(a.off[g] - im.row0), e = (int)(a.off[g + 1] - im.row0);
-            double t = 0.0;
-            for (int i = b + lane; i < e; i += L) t += xs[i];
-            for (int m = 1; m < L; m <<= 1) t += __shfl_xor(t, m);
-            if (lane == 0) a.out[g] = (float)t;
-        }
-    } else {
+    const int tid = (int)threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+    if ((int)blockIdx.x < a.num_wide) {
+        const SetItem im = a.wide[blockIdx.x];
         double t = 0.0;
         for (int i = tid; i < im.rows; i += kBlock) t += sum_term<PAIRS>(a, im.row0 + i);
         t = block_sum(t, sh);
@@ -483,15 +1068,36 @@ __global__ __launch_bounds__(kBlock) void set_sum_kernel(SumArgs a) {
             else
                 a.parts[blockIdx.x] = t;
         }
+        return;
+    }
+    const int it = ((int)blockIdx.x - a.num_wide) * kWaves + wave;
+    if (it >= a.num_tiles) return;
+    const SetItem im = a.tiles[it];
+    double v[kPer];
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+        const int i = k * kWave + lane;
+        v[k] = i < im.rows ? sum_term<PAIRS>(a, im.row0 + i) : 0.0;
+    }
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) xs[wave][k * kWave + lane] = v[k];
+    wave_sync();
+    const int L = 1 << im.team, sub = lane & (L - 1);
+    for (int s = lane >> im.team; s < im.sets; s += kWave >> im.team) {
+        const int64_t g = (int64_t)im.set0 + s;
+        const int b = (int)(a.off[g] - im.row0), e = (int)(a.off[g + 1] - im.row0);
+        double t = 0.0;
+        for (int i = b + sub; i < e; i += L) t += xs[wave][i];
+        for (int m = 1; m < L; m <<= 1) t += __shfl_xor(t, m);
+        if (sub == 0) a.out[g] = (float)t;
     }
 }
 
 // The sets that were summed in parts.
-__global__ __launch_bounds__(kBlock) void set_join_kernel(SumArgs a, const int32_t* __restrict__ list, int32_t n) {
+__global__ __launch_bounds__(kBlock) void set_join_kernel(SumArgs a, const int32_t* __restrict__ list) {
     __shared__ double sh[kWaves];
     const int32_t it = list[blockIdx.x];
-    const SetItem im = a.items[it];
-    if (im.part != 0) return;  // the whole workgroup
+    const SetItem im = a.wide[it];
     double t = 0.0;
     for (int j = (int)threadIdx.x; j < im.parts; j += kBlock) t += a.parts[it + j];
     t = block_sum(t, sh);
@@ -528,60 +1134,92 @@ __global__ __launch_bounds__(kBlock) void pair_kernel(PairArgs a) {
 }
 
 // out[i] = per_set[set of i]
-__global__ __launch_bounds__(kBlock) void spread_kernel(const int64_t* __restrict__ off, const SetItem* __restrict__ items,
-                                                        const float* __restrict__ per_set, float* __restrict__ out) {
-    const int tid = (int)threadIdx.x;
-    const SetItem im = items[blockIdx.x];
-    if (im.parts == 0) {
-        const int L = 1 << im.team, lane = tid & (L - 1);
-        for (int s = tid >> im.team; s < im.sets; s += kBlock >> im.team) {
-            const int64_t g = (int64_t)im.set0 + s;
-            const float v = per_set[g];
-            for (int64_t i = off[g] + lane; i < off[g + 1]; i += L) out[i] = v;
-        }
-    } else {
+__global__ __launch_bounds__(kBlock) void spread_kernel(SumArgs a, const float* __restrict__ per_set) {
+    const int tid = (int)threadIdx.x, lane = tid & (kWave - 1);
+    if ((int)blockIdx.x < a.num_wide) {
+        const SetItem im = a.wide[blockIdx.x];
         const float v = per_set[im.set0];
-        for (int i = tid; i < im.rows; i += kBlock) out[im.row0 + i] = v;
+        for (int i = tid; i < im.rows; i += kBlock) a.out[im.row0 + i] = v;
+        return;
+    }
+    const int it = ((int)blockIdx.x - a.num_wide) * kWaves + tid / kWave;
+    if (it >= a.num_tiles) return;
+    const SetItem im = a.tiles[it];
+    const int L = 1 << im.team, sub = lane & (L - 1);
+    for (int s = lane >> im.team; s < im.sets; s += kWave >> im.team) {
+        const int64_t g = (int64_t)im.set0 + s;
+        const float v = per_set[g];
+        const int64_t e = a.off[g + 1];
+        for (int64_t i = a.off[g] + sub; i < e; i += L) a.out[i] = v;
     }
 }
 
+int tile_groups(const SetLayout& s) { return (s.num_tiles + kWaves - 1) / kWaves; }
+
+int tile_blocks(const SetLayout& s) { return std::min(tile_groups(s), kChoiceGrid); }
+
+int wide_blocks(const SetLayout& s) { return std::min(s.num_wide, kChoiceGrid); }
+
 template <int MODE, int TYPE, bool MASK, bool BIAS>
-hipError_t launch_choice_as(const SetLayout& s, const ChoiceArgs& a, int32_t grid, hipStream_t stream) {
-    if (MODE != kStepsBack && s.num_split > 0) {
-        hipLaunchKernelGGL((part_kernel<MODE, TYPE, MASK, BIAS>), dim3(s.num_split), dim3(kBlock), 0, stream, a, s.split);
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
+hipError_t launch_choice_as(const SetLayout& s, const ChoiceArgs& a, hipStream_t stream) {
+    hipError_t e = hipSuccess;
+    const int parts = s.num_wide - s.num_whole;
+    if (MODE != kStepsBack && parts > 0) {
+        hipLaunchKernelGGL((part_kernel<MODE, TYPE, MASK, BIAS>), dim3(parts), dim3(kBlock), 0, stream, a, s.num_whole);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
     }
-    hipLaunchKernelGGL((choice_kernel<MODE, TYPE, MASK, BIAS>), dim3(grid), dim3(kBlock), 0, stream, a);
-    return hipGetLastError();
+    if (s.num_tiles > 0) {
+        hipLaunchKernelGGL((tile_kernel<MODE, TYPE, MASK, BIAS>), dim3(tile_blocks(s)), dim3(kBlock), 0, stream, a);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
+    const int wide = MODE == kSteps ? s.num_whole : s.num_wide;
+    if (wide > 0) {
+        hipLaunchKernelGGL((wide_kernel<MODE, TYPE, MASK, BIAS>), dim3(std::min(wide, wide_blocks(s))), dim3(kBlock), 0,
+                           stream, a);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
+    if (MODE == kSteps && s.num_split > 0) {
+        hipLaunchKernelGGL((split_steps_kernel<TYPE, MASK, BIAS>), dim3((s.num_split + kWaves - 1) / kWaves), dim3(kBlock), 0,
+                           stream, a, s.split, s.num_split);
+        e = hipGetLastError();
+    }
+    return e;
 }
 
 template <int MODE, int TYPE>
-hipError_t launch_choice_typed(const SetLayout& s, const ChoiceArgs& a, int32_t grid, hipStream_t stream) {
+hipError_t launch_choice_typed(const SetLayout& s, const ChoiceArgs& a, hipStream_t stream) {
     if (a.mask)
-        return a.table ? launch_choice_as<MODE, TYPE, true, true>(s, a, grid, stream)
-                       : launch_choice_as<MODE, TYPE, true, false>(s, a, grid, stream);
-    return a.table ? launch_choice_as<MODE, TYPE, false, true>(s, a, grid, stream)
-                   : launch_choice_as<MODE, TYPE, false, false>(s, a, grid, stream);
+        return a.table ? launch_choice_as<MODE, TYPE, true, true>(s, a, stream)
+                       : launch_choice_as<MODE, TYPE, true, false>(s, a, stream);
+    return a.table ? launch_choice_as<MODE, TYPE, false, true>(s, a, stream)
+                   : launch_choice_as<MODE, TYPE, false, false>(s, a, stream);
 }
 
 template <int MODE>
-hipError_t launch_choice_mode(const SetLayout& s, const ChoiceArgs& a, int32_t type, int32_t grid, hipStream_t stream) {
-    if (type == PB_BF16) return launch_choice_typed<MODE, PB_BF16>(s, a, grid, stream);
-    if (type == PB_F16) return launch_choice_typed<MODE, PB_F16>(s, a, grid, stream);
-    return launch_choice_typed<MODE, PB_F32>(s, a, grid, stream);
+hipError_t launch_choice_mode(const SetLayout& s, const ChoiceArgs& a, int32_t type, hipStream_t stream) {
+    if (type == PB_BF16) return launch_choice_typed<MODE, PB_BF16>(s, a, stream);
+    if (type == PB_F16) return launch_choice_typed<MODE, PB_F16>(s, a, stream);
+    return launch_choice_typed<MODE, PB_F32>(s, a, stream);
+}
+
+SumArgs sum_args(const SetLayout& s) {
+    SumArgs a{};
+    a.off = s.off;
+    a.tiles = s.tiles;
+    a.wide = s.wide;
+    a.num_tiles = s.num_tiles;
+    a.num_wide = s.num_wide;
+    return a;
 }
 
 template <bool PAIRS>
-hipError_t launch_set_sum(const SetLayout& s, SumArgs a, hipStream_t stream) {
-    if (s.num_items == 0) return hipSuccess;
-    a.off = s.off;
-    a.items = s.items;
-    a.num_items = s.num_items;
-    hipLaunchKernelGGL(set_sum_kernel<PAIRS>, dim3(s.num_items), dim3(kBlock), 0, stream, a);
+hipError_t launch_set_sum(const SetLayout& s, const SumArgs& a, hipStream_t stream) {
+    const int grid = s.num_wide + tile_groups(s);
+    if (grid == 0) return hipSuccess;
+    hipLaunchKernelGGL(set_sum_kernel<PAIRS>, dim3(grid), dim3(kBlock), 0, stream, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || s.num_split == 0) return e;
-    hipLaunchKernelGGL(set_join_kernel, dim3(s.num_split), dim3(kBlock), 0, stream, a, s.split, s.num_split);
+    hipLaunchKernelGGL(set_join_kernel, dim3(s.num_split), dim3(kBlock), 0, stream, a, s.split);
     return hipGetLastError();
 }
 
@@ -598,23 +1236,31 @@ hipError_t launch_zero(float* out, int64_t n, hipStream_t stream) {
     return hipGetLastError();
 }
 
-int32_t choice_grid(const SetLayout& s) { return s.num_items < kChoiceGrid ? s.num_items : kChoiceGrid; }
+int32_t choice_grid(const SetLayout& s) { return tile_blocks(s) + wide_blocks(s); }
 
 hipError_t launch_choice(int mode, const SetLayout& s, ChoiceArgs a, int32_t type, hipStream_t stream) {
     a.off = s.off;
-    a.items = s.items;
-    a.num_items = s.num_items;
-    const int32_t grid = choice_grid(s);
+    a.tiles = s.tiles;
+    a.wide = s.wide;
+    a.num_tiles = s.num_tiles;
+    a.num_wide = s.num_wide;
+    a.num_whole = s.num_whole;
+    a.blocks = choice_grid(s);
+    a.rows = s.rows;
+    // runs of eight rows in accesses of 16 bytes, 8 of the mask
+    const auto at = [](const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; };
+    a.vec = a.stride == 1 && at(a.scores, 16) && at(a.grad_scores, 16) && at(a.mask, 8) && at(a.positions, 16) &&
+            (mode != kRows || at(a.log_probs, 16)) && (mode != kRowsBack || at(a.grad, 16));
     hipError_t e = hipSuccess;
-    if (mode == kRows) e = launch_choice_mode<kRows>(s, a, type, grid, stream);
-    if (mode == kSteps) e = launch_choice_mode<kSteps>(s, a, type, grid, stream);
-    if (mode == kRowsBack) e = launch_choice_mode<kRowsBack>(s, a, type, grid, stream);
-    if (mode == kStepsBack) e = launch_choice_mode<kStepsBack>(s, a, type, grid, stream);
-    if (mode == kPolicy) e = launch_choice_mode<kPolicy>(s, a, type, grid, stream);
+    if (mode == kRows) e = launch_choice_mode<kRows>(s, a, type, stream);
+    if (mode == kSteps) e = launch_choice_mode<kSteps>(s, a, type, stream);
+    if (mode == kRowsBack) e = launch_choice_mode<kRowsBack>(s, a, type, stream);
+    if (mode == kStepsBack) e = launch_choice_mode<kStepsBack>(s, a, type, stream);
+    if (mode == kPolicy) e = launch_choice_mode<kPolicy>(s, a, type, stream);
     const int32_t head = mode == kPolicy ? 3 : 0;
     const int32_t cols = head + (a.table && mode != kRows && mode != kSteps ? a.num_buckets : 0);
-    if (e != hipSuccess || cols == 0 || grid == 1) return e;
-    hipLaunchKernelGGL(join_kernel, dim3(cols), dim3(kBlock), 0, stream, a.sums, grid, cols, head, a.stats, a.grad_table);
+    if (e != hipSuccess || cols == 0 || a.blocks == 1) return e;
+    hipLaunchKernelGGL(join_kernel, dim3(cols), dim3(kBlock), 0, stream, a.sums, a.blocks, cols, head, a.stats, a.grad_table);
     return hipGetLastError();
 }
 
@@ -625,14 +1271,14 @@ hipError_t launch_preference(const PairLayout& p, PairArgs a, const float* value
     a.num_pairs = p.num_pairs;
     a.sums = reinterpret_cast<double*>(work);
     double* parts = a.sums + kPairGrid;
-    a.slopes = reinterpret_cast<float*>(parts + p.lists.num_items + p.seqs.num_items);
+    a.slopes = reinterpret_cast<float*>(parts + p.lists.num_wide + p.seqs.num_wide);
     float* seq_sum = a.slopes + p.num_pairs;
     float* seq_grad = seq_sum + p.seqs.num_sets;
     const bool seqs = p.has_seqs;
     hipError_t e = hipSuccess;
-    SumArgs sa{};
-    sa.parts = parts;
     if (seqs) {
+        SumArgs sa = sum_args(p.seqs);
+        sa.parts = parts;
         sa.values = values;
         sa.ref = ref;
         sa.out = seq_sum;
@@ -651,21 +1297,24 @@ hipError_t launch_preference(const PairLayout& p, PairArgs a, const float* value
         hipLaunchKernelGGL(join_kernel, dim3(1), dim3(kBlock), 0, stream, a.sums, grid, 1, 1, a.loss, nullptr);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
-    sa.parts = parts + p.seqs.num_items;
+    SumArgs sa = sum_args(p.lists);
+    sa.parts = parts + p.seqs.num_wide;
     sa.entries = p.entries;
     sa.slopes = a.slopes;
     sa.out = seqs ? seq_grad : grad;
     if ((e = launch_set_sum<true>(p.lists, sa, stream)) != hipSuccess) return e;
-    if (seqs && p.seqs.num_items > 0) {
-        hipLaunchKernelGGL(spread_kernel, dim3(p.seqs.num_items), dim3(kBlock), 0, stream, p.seqs.off, p.seqs.items,
-                           seq_grad, grad);
+    const int grid_steps = p.seqs.num_wide + tile_groups(p.seqs);
+    if (seqs && grid_steps > 0) {
+        SumArgs sp = sum_args(p.seqs);
+        sp.out = grad;
+        hipLaunchKernelGGL(spread_kernel, dim3(grid_steps), dim3(kBlock), 0, stream, sp, seq_grad);
         e = hipGetLastError();
     }
     return e;
 }
 
 int64_t preference_work_bytes(const PairLayout& p) {
-    return 8 * ((int64_t)kPairGrid + p.lists.num_items + p.seqs.num_items) + 4 * (p.num_pairs + 2 * p.seqs.num_sets);
+    return 8 * ((int64_t)kPairGrid + p.lists.num_wide + p.seqs.num_wide) + 4 * (p.num_pairs + 2 * p.seqs.num_sets);
 }
 
 }  // namespace pb

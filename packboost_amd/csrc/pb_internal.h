@@ -489,13 +489,16 @@ hipError_t launch_predict_bins(const uint8_t* bins, int64_t N, int64_t ld, int32
                                hipStream_t s);
 
 // ---- choices and preferences (choice.hip) ----
-// A table of ragged sets laid out for workgroups: items in row order, each a tile of consecutive short
-// sets (parts 0; at most kSetTileRows rows and kSetTileSets sets, lanes of 1 << team to a set) or part
-// `part` of the `parts` of one set of more than kSetShort rows. The items of a set in several parts are
-// consecutive and listed in `split`.
-constexpr int kSetTileRows = 2048;
-constexpr int kSetTileSets = 1024;
-constexpr int kSetShort = 512;
+// A table of ragged sets laid out for wavefronts and workgroups. Tiles, for a wave each, in row order: runs
+// of consecutive sets of at most kSetShort rows, at most kSetTileSets of them; their rows, counted from the
+// multiple of 8 at or before the first, are at most kSetTileRows; `team`: lanes of 1 << team to a set, where
+// a wave's lanes are shared out by sets. Wide items, for a workgroup each: longer sets of at most
+// kSetWideRows rows counted the same way, then the parts (part `part` of `parts`) of those that are longer,
+// a set's consecutive; `split` names the first of each.
+constexpr int kSetTileRows = 512;
+constexpr int kSetTileSets = 256;
+constexpr int kSetShort = kSetTileRows - 8;
+constexpr int kSetWideRows = 8192;
 struct SetItem {
     int64_t row0;
     int32_t rows;
@@ -508,9 +511,12 @@ struct SetItem {
 static_assert(sizeof(SetItem) == 32, "an item is 32 bytes");
 struct SetLayout {
     const int64_t* off;    // [num_sets + 1]
-    const SetItem* items;  // [num_items]
-    const int32_t* split;  // [num_split]
-    int32_t num_items;
+    const SetItem* tiles;  // [num_tiles]
+    const SetItem* wide;   // [num_wide], of which the first num_whole are whole sets
+    const int32_t* split;  // [num_split], indices of wide items
+    int32_t num_tiles;
+    int32_t num_wide;
+    int32_t num_whole;
     int32_t num_split;
     int64_t num_sets;
     int64_t rows;
@@ -526,13 +532,19 @@ struct PairLayout {
 };
 enum ChoiceMode { kRows, kSteps, kRowsBack, kStepsBack, kPolicy };
 constexpr int kMaxBuckets = 256;
-constexpr int kChoiceGrid = 2048;  // workgroups of a pass over the items: 8 per compute unit
+constexpr int kChoiceGrid = 2048;  // workgroups of a pass over the tiles, and over the wide items, at most
 constexpr int kPairGrid = 1024;
 struct ChoiceArgs {
     const int64_t* off;
-    const SetItem* items;
-    int32_t num_items;
+    const SetItem* tiles;
+    const SetItem* wide;
+    int32_t num_tiles;
+    int32_t num_wide;
+    int32_t num_whole;
+    int32_t blocks;  // workgroups that leave sums: the tiles', then the wide items'
     int32_t num_buckets;
+    int64_t rows;
+    bool vec;  // runs of eight rows can be read and written in accesses of 16 bytes
     const void* scores;
     int64_t stride;
     const uint8_t* mask;
@@ -553,7 +565,7 @@ struct ChoiceArgs {
     void* grad_scores;
     float* grad_table;
     float* stats;   // policy: loss, kl, clipped weight
-    float2* parts;  // [num_items] maximum and sum of the parts of split sets
+    float2* parts;  // [num_wide] maximum and sum of the parts of split sets
     double* sums;   // [choice_grid][3 (policy) + num_buckets (gradient)]
 };
 struct PairArgs {
