@@ -580,8 +580,12 @@ typedef struct {
     int32_t reserved;
 } pb_choice_scores;
 
-/* Bytes of the workspace (16-byte aligned) of a call on these sets; -1: bad argument. */
-int64_t pb_choice_work_bytes(const pb_sets* sets, int32_t num_buckets);
+/* Bytes of the workspace (16-byte aligned; none where this is 0) of a call on these sets: op PB_LOG_PROBS
+ * (pb_choice_log_probs), PB_BACKWARD or PB_POLICY; -1: bad argument. */
+#define PB_LOG_PROBS 0
+#define PB_BACKWARD 1
+#define PB_POLICY 2
+int64_t pb_choice_work_bytes(const pb_sets* sets, int32_t op, int32_t num_buckets);
 
 /* chosen_dev NULL: log_probs_dev float32 [rows], every row's (-inf where masked). Else (int32
  * [num_sets]) log_probs_dev float32 [num_sets], the steps'. lse_dev: float32 [num_sets]. */

@@ -20,6 +20,7 @@ type), everything else is float32.
 from __future__ import annotations
 
 import ctypes
+from contextlib import nullcontext
 from typing import NamedTuple
 
 import numpy as np
@@ -108,13 +109,13 @@ class ChoiceSets(_Handle):
         with torch.cuda.device(self.device):
             _hip.check(_hip.load().pb_sets_create(off.ctypes.data, self.num_sets, ctypes.byref(h)), "pb_sets_create")
         self._handle = h
-        self._work: dict[int, int] = {}
+        self._work: dict[tuple[int, int], int] = {}
 
-    def _work_bytes(self, num_buckets: int) -> int:
-        n = self._work.get(num_buckets)
+    def _workspace(self, op: int, num_buckets: int) -> tuple[torch.Tensor | None, int]:
+        n = self._work.get((op, num_buckets))
         if n is None:
-            n = self._work[num_buckets] = int(_hip.load().pb_choice_work_bytes(self._open(), num_buckets))
-        return n
+            n = self._work[op, num_buckets] = int(_hip.load().pb_choice_work_bytes(self._open(), op, num_buckets))
+        return (_empty(n, self.device, torch.uint8), n) if n else (None, 0)
 
 
 class PositionBuckets:
@@ -260,6 +261,14 @@ def _scores(scores, sets: ChoiceSets, mask, bias) -> tuple[_hip.PbChoiceScores, 
     return c, keep
 
 
+_HERE = nullcontext()
+
+
+def _on(device: torch.device):
+    """torch.cuda.device(device), for nothing where that is the current one."""
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
 def _empty(n: int, like: torch.device, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     return torch.empty(n, dtype=dtype, device=like)
 
@@ -275,13 +284,12 @@ def choice_log_probs(scores: torch.Tensor, sets: ChoiceSets, *, chosen: torch.Te
     dev = sets.device
     if chosen is not None:
         chosen = _column("chosen", chosen, sets.num_sets, dev, torch.int32)
-    with torch.cuda.device(dev):
+    with _on(dev):
         out = _empty(sets.num_rows if chosen is None else sets.num_sets, dev)
         lse = _empty(sets.num_sets, dev)
-        size = sets._work_bytes(c.num_buckets)
-        work = _empty(size, dev, torch.uint8)
+        work, size = sets._workspace(_hip.PB_LOG_PROBS, c.num_buckets)
         _hip.check(_hip.load().pb_choice_log_probs(
-            sets._open(), c, _hip.ptr(chosen), out.data_ptr(), lse.data_ptr(), work.data_ptr(), size,
+            sets._open(), c, _hip.ptr(chosen), out.data_ptr(), lse.data_ptr(), _hip.ptr(work), size,
             _hip.stream_ptr()), "pb_choice_log_probs")
     return out, lse
 
@@ -298,14 +306,13 @@ def choice_log_probs_backward(grad: torch.Tensor, scores: torch.Tensor, lse: tor
     lse = _column("lse", lse, sets.num_sets, dev, torch.float32)
     if chosen is not None:
         chosen = _column("chosen", chosen, sets.num_sets, dev, torch.int32)
-    with torch.cuda.device(dev):
+    with _on(dev):
         gs = _empty(sets.num_rows, dev, scores.dtype)
         gt = _empty(c.num_buckets, dev) if bias is not None else None
-        size = sets._work_bytes(c.num_buckets)
-        work = _empty(size, dev, torch.uint8)
+        work, size = sets._workspace(_hip.PB_BACKWARD, c.num_buckets)
         _hip.check(_hip.load().pb_choice_log_probs_backward(
             sets._open(), c, _hip.ptr(chosen), grad.data_ptr(), lse.data_ptr(), gs.data_ptr(), _hip.ptr(gt),
-            work.data_ptr(), size, _hip.stream_ptr()), "pb_choice_log_probs_backward")
+            _hip.ptr(work), size, _hip.stream_ptr()), "pb_choice_log_probs_backward")
     return gs, gt
 
 
@@ -345,15 +352,14 @@ def policy_loss(scores: torch.Tensor, sets: ChoiceSets, chosen: torch.Tensor, ad
     low, high = _finite("clip[0]", clip[0], 0.0), _finite("clip[1]", clip[1], 0.0)
     t.ratio_min, t.ratio_max = 1.0 - low, 1.0 + high
     t.kl_weight, t.scale = _finite("kl_weight", kl_weight), _finite("scale", scale)
-    with torch.cuda.device(dev):
+    with _on(dev):
         stats, lp = _empty(3, dev), _empty(g, dev)
         gs = _empty(sets.num_rows, dev, scores.dtype)
         gt = _empty(c.num_buckets, dev) if bias is not None else None
-        size = sets._work_bytes(c.num_buckets)
-        work = _empty(size, dev, torch.uint8)
+        work, size = sets._workspace(_hip.PB_POLICY, c.num_buckets)
         _hip.check(_hip.load().pb_policy_loss(
             sets._open(), c, t, chosen.data_ptr(), stats.data_ptr(), lp.data_ptr(), gs.data_ptr(), _hip.ptr(gt),
-            work.data_ptr(), size, _hip.stream_ptr()), "pb_policy_loss")
+            _hip.ptr(work), size, _hip.stream_ptr()), "pb_policy_loss")
     return PolicyLoss(stats[0], gs, gt, lp, stats[1], stats[2])
 
 
@@ -381,7 +387,7 @@ def preference_loss(values: torch.Tensor, pairs: PreferencePairs, *, ref_values:
     beta, scale = _finite("beta", beta), _finite("scale", scale)
     if not 0.0 <= label_smoothing <= 1.0:
         raise ValueError(f"label_smoothing must lie in [0, 1], got {label_smoothing}")
-    with torch.cuda.device(dev):
+    with _on(dev):
         loss, grad, margins = _empty(1, dev), _empty(n, dev), _empty(pairs.num_pairs, dev)
         work = _empty(max(16, pairs._work_bytes), dev, torch.uint8)
         _hip.check(_hip.load().pb_preference_loss(

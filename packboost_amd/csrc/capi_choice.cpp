@@ -190,9 +190,20 @@ int pairs_create(const int64_t* winners, const int64_t* losers, int64_t num_pair
     return PB_OK;
 }
 
+// Sums that a workgroup leaves (none where there is one workgroup, which writes the results itself).
+int64_t sum_cols(const pb_sets* s, int32_t op, int32_t num_buckets) {
+    if (op == PB_LOG_PROBS || pb::choice_grid(s->s) <= 1) return 0;
+    return (op == PB_POLICY ? 3 : 0) + num_buckets;
+}
+
+int64_t work_need(const pb_sets* s, int32_t op, int32_t num_buckets) {
+    const int64_t parts = s->s.num_wide > s->s.num_whole ? s->s.num_wide : 0;
+    return 8 * (sum_cols(s, op, num_buckets) * pb::choice_grid(s->s) + parts);
+}
+
 // Checks what every choice call takes and fills the arguments it shares.
-int choice_args(const char* who, const pb_sets* s, const pb_choice_scores* in, void* work, int64_t work_bytes,
-                pb::ChoiceArgs& a) {
+int choice_args(const char* who, int32_t op, const pb_sets* s, const pb_choice_scores* in, void* work,
+                int64_t work_bytes, pb::ChoiceArgs& a) {
     const auto bad = [&](int code, const char* what) {
         return pb::api_fail(code, (std::string(who) + ": " + what).c_str());
     };
@@ -205,7 +216,8 @@ int choice_args(const char* who, const pb_sets* s, const pb_choice_scores* in, v
     if (in->num_buckets > 0 && (!in->table_dev || !in->buckets_dev || (s->s.rows > 0 && !in->positions_dev)))
         return bad(PB_ERR_INVALID, "a position bias needs its table, buckets and positions");
     if (in->num_buckets > 0 && in->reach < 0) return bad(PB_ERR_INVALID, "reach must not be negative");
-    if (!work || work_bytes < pb_choice_work_bytes(s, in->num_buckets)) return bad(PB_ERR_INVALID, "workspace too small");
+    const int64_t sums = sum_cols(s, op, in->num_buckets) * pb::choice_grid(s->s), need = work_need(s, op, in->num_buckets);
+    if (need > 0 && (!work || work_bytes < need)) return bad(PB_ERR_INVALID, "workspace too small");
     if (reinterpret_cast<uintptr_t>(work) & 15) return bad(PB_ERR_INVALID, "workspace must be 16-byte aligned");
     a.num_buckets = in->num_buckets;
     a.scores = in->scores_dev;
@@ -216,7 +228,7 @@ int choice_args(const char* who, const pb_sets* s, const pb_choice_scores* in, v
     a.buckets = in->buckets_dev;
     a.reach = in->reach;
     a.sums = static_cast<double*>(work);
-    a.parts = reinterpret_cast<float2*>(a.sums + (int64_t)pb::choice_grid(s->s) * (3 + in->num_buckets));
+    a.parts = reinterpret_cast<float2*>(a.sums + sums);
     return PB_OK;
 }
 
@@ -251,15 +263,15 @@ int pb_sets_destroy(pb_sets* sets) {
     return PB_OK;
 }
 
-int64_t pb_choice_work_bytes(const pb_sets* s, int32_t num_buckets) {
-    if (!s || num_buckets < 0 || num_buckets > pb::kMaxBuckets) return -1;
-    return 16 + 8 * ((int64_t)pb::choice_grid(s->s) * (3 + num_buckets) + s->s.num_wide);
+int64_t pb_choice_work_bytes(const pb_sets* s, int32_t op, int32_t num_buckets) {
+    if (!s || op < PB_LOG_PROBS || op > PB_POLICY || num_buckets < 0 || num_buckets > pb::kMaxBuckets) return -1;
+    return work_need(s, op, num_buckets);
 }
 
 int pb_choice_log_probs(const pb_sets* s, const pb_choice_scores* in, const int32_t* chosen_dev, float* log_probs_dev,
                         float* lse_dev, void* work_dev, int64_t work_bytes, void* stream) {
     pb::ChoiceArgs a{};
-    const int rc = choice_args("pb_choice_log_probs", s, in, work_dev, work_bytes, a);
+    const int rc = choice_args("pb_choice_log_probs", PB_LOG_PROBS, s, in, work_dev, work_bytes, a);
     if (rc != PB_OK) return rc;
     if (s->s.num_sets == 0) return PB_OK;
     if (!lse_dev || ((chosen_dev || s->s.rows > 0) && !log_probs_dev))
@@ -274,7 +286,7 @@ int pb_choice_log_probs_backward(const pb_sets* s, const pb_choice_scores* in, c
                                  const float* grad_dev, const float* lse_dev, void* grad_scores_dev,
                                  float* grad_table_dev, void* work_dev, int64_t work_bytes, void* stream) {
     pb::ChoiceArgs a{};
-    const int rc = choice_args("pb_choice_log_probs_backward", s, in, work_dev, work_bytes, a);
+    const int rc = choice_args("pb_choice_log_probs_backward", PB_BACKWARD, s, in, work_dev, work_bytes, a);
     if (rc != PB_OK) return rc;
     if (in->num_buckets > 0 && !grad_table_dev)
         return pb::api_fail(PB_ERR_INVALID, "pb_choice_log_probs_backward: null table gradient");
@@ -293,7 +305,7 @@ int pb_policy_loss(const pb_sets* s, const pb_choice_scores* in, const pb_policy
                    float* stats_dev, float* log_probs_dev, void* grad_scores_dev, float* grad_table_dev, void* work_dev,
                    int64_t work_bytes, void* stream) {
     pb::ChoiceArgs a{};
-    const int rc = choice_args("pb_policy_loss", s, in, work_dev, work_bytes, a);
+    const int rc = choice_args("pb_policy_loss", PB_POLICY, s, in, work_dev, work_bytes, a);
     if (rc != PB_OK) return rc;
     if (!t || !stats_dev || (in->num_buckets > 0 && !grad_table_dev))
         return pb::api_fail(PB_ERR_INVALID, "pb_policy_loss: null argument");

@@ -24,6 +24,7 @@ constexpr float kInf = __builtin_huge_valf();
 constexpr int kRun = 8;                                     // consecutive rows of a lane
 constexpr int kWideRuns = kSetWideRows / (kRun * kBlock);   // runs of a thread of a longer set
 constexpr int kTileRounds = kSetTileSets / kWave;           // sets of a tile per lane
+constexpr int kPairs = 4;                                   // pairs a thread has in flight
 constexpr int kBins = 256;     // LDS words of the table's gradient per wave: buckets x copies
 constexpr int kLookup = 2048;  // bytes of the position lookup kept in LDS
 static_assert(kSetTileRows == kRun * kWave, "a lane holds one run of a tile");
@@ -1039,7 +1040,18 @@ struct SumArgs {
     const float* slopes;
     float* out;
     double* parts;
+    const double* sums;  // the pairs' workgroups' losses [num_sums], joined by a workgroup more
+    int32_t num_sums;
+    float* loss;
 };
+
+// loss[0] = the sum of the workgroups' sums, in a fixed order.
+__device__ void join_loss(const SumArgs& a, double* sh) {
+    double t = 0.0;
+    for (int i = (int)threadIdx.x; i < a.num_sums; i += kBlock) t += a.sums[i];
+    t = block_sum(t, sh);
+    if (threadIdx.x == 0) a.loss[0] = (float)t;
+}
 
 template <bool PAIRS>
 __device__ __forceinline__ double sum_term(const SumArgs& a, int64_t i) {
@@ -1071,6 +1083,10 @@ __global__ __launch_bounds__(kBlock) void set_sum_kernel(SumArgs a) {
         return;
     }
     const int it = ((int)blockIdx.x - a.num_wide) * kWaves + wave;
+    if (it - wave >= a.num_tiles) {
+        if (PAIRS) join_loss(a, sh);
+        return;
+    }
     if (it >= a.num_tiles) return;
     const SetItem im = a.tiles[it];
     double v[kPer];
@@ -1110,19 +1126,37 @@ __global__ __launch_bounds__(kBlock) void set_join_kernel(SumArgs a, const int32
 __global__ __launch_bounds__(kBlock) void pair_kernel(PairArgs a) {
     __shared__ double sh[kWaves];
     double sum = 0.0;
-    for (int64_t p = (int64_t)blockIdx.x * kBlock + threadIdx.x; p < a.num_pairs; p += (int64_t)gridDim.x * kBlock) {
-        const int32_t w = a.winners[p], l = a.losers[p];
-        double d = (double)a.values[w] - (double)a.values[l];
-        if (a.ref) d -= (double)a.ref[w] - (double)a.ref[l];
-        const float z = (float)((double)a.beta * d);
-        const float weight = (a.weights ? a.weights[p] : 1.0f) * a.scale;
-        const float t = expf(-fabsf(z)), soft = log1pf(t);
-        const float e = a.smoothing;
-        const float up = z > 0.0f ? 1.0f / (1.0f + t) : t / (1.0f + t);    // sigmoid(z)
-        const float down = z > 0.0f ? t / (1.0f + t) : 1.0f / (1.0f + t);  // sigmoid(-z)
-        a.margins[p] = z;
-        a.slopes[p] = a.beta * weight * (e * up - (1.0f - e) * down);
-        sum += (double)(weight * ((1.0f - e) * (soft + fmaxf(-z, 0.0f)) + e * (soft + fmaxf(z, 0.0f))));
+    const int64_t stride = (int64_t)gridDim.x * kBlock;
+    for (int64_t p0 = (int64_t)blockIdx.x * kBlock + threadIdx.x; p0 < a.num_pairs; p0 += stride * kPairs) {
+        int32_t w[kPairs], l[kPairs];
+        float weight[kPairs];
+        double d[kPairs];
+#pragma unroll
+        for (int k = 0; k < kPairs; ++k) {  // past the end: the last pair again, unused
+            const int64_t p = min(p0 + k * stride, a.num_pairs - 1);
+            w[k] = a.winners[p];
+            l[k] = a.losers[p];
+            weight[k] = a.weights ? a.weights[p] : 1.0f;
+        }
+#pragma unroll
+        for (int k = 0; k < kPairs; ++k) {
+            d[k] = (double)a.values[w[k]] - (double)a.values[l[k]];
+            if (a.ref) d[k] -= (double)a.ref[w[k]] - (double)a.ref[l[k]];
+        }
+#pragma unroll
+        for (int k = 0; k < kPairs; ++k) {
+            const int64_t p = p0 + k * stride;
+            if (p >= a.num_pairs) break;
+            const float z = (float)((double)a.beta * d[k]);
+            const float ws = weight[k] * a.scale;
+            const float t = expf(-fabsf(z)), soft = log1pf(t);
+            const float e = a.smoothing;
+            const float up = z > 0.0f ? 1.0f / (1.0f + t) : t / (1.0f + t);    // sigmoid(z)
+            const float down = z > 0.0f ? t / (1.0f + t) : 1.0f / (1.0f + t);  // sigmoid(-z)
+            a.margins[p] = z;
+            a.slopes[p] = a.beta * ws * (e * up - (1.0f - e) * down);
+            sum += (double)(ws * ((1.0f - e) * (soft + fmaxf(-z, 0.0f)) + e * (soft + fmaxf(z, 0.0f))));
+        }
     }
     sum = block_sum(sum, sh);
     if (threadIdx.x == 0) {
@@ -1133,22 +1167,38 @@ __global__ __launch_bounds__(kBlock) void pair_kernel(PairArgs a) {
     }
 }
 
-// out[i] = per_set[set of i]
-__global__ __launch_bounds__(kBlock) void spread_kernel(SumArgs a, const float* __restrict__ per_set) {
+// The pairs' slopes summed over a sequence's list (a team of L lanes, this one `sub`).
+__device__ __forceinline__ float list_slope(const SumArgs& a, const int64_t* list_off, int64_t g, int sub, int L) {
+    double t = 0.0;
+    const int64_t e = list_off[g + 1];
+    for (int64_t i = list_off[g] + sub; i < e; i += L) t += sum_term<true>(a, i);
+    for (int m = 1; m < L; m <<= 1) t += __shfl_xor(t, m);
+    return (float)t;
+}
+
+// out[i] = the slope of step i's sequence: per_set[sequence], or (per_set NULL) the sum over the sequence's
+// list of pairs, where no list is long.
+__global__ __launch_bounds__(kBlock) void spread_kernel(SumArgs a, const float* __restrict__ per_set,
+                                                        const int64_t* __restrict__ list_off) {
+    __shared__ double sh[kWaves];
     const int tid = (int)threadIdx.x, lane = tid & (kWave - 1);
     if ((int)blockIdx.x < a.num_wide) {
         const SetItem im = a.wide[blockIdx.x];
-        const float v = per_set[im.set0];
+        const float v = per_set ? per_set[im.set0] : list_slope(a, list_off, im.set0, lane, kWave);
         for (int i = tid; i < im.rows; i += kBlock) a.out[im.row0 + i] = v;
         return;
     }
-    const int it = ((int)blockIdx.x - a.num_wide) * kWaves + tid / kWave;
+    const int first = ((int)blockIdx.x - a.num_wide) * kWaves, it = first + tid / kWave;
+    if (first >= a.num_tiles) {
+        join_loss(a, sh);
+        return;
+    }
     if (it >= a.num_tiles) return;
     const SetItem im = a.tiles[it];
     const int L = 1 << im.team, sub = lane & (L - 1);
     for (int s = lane >> im.team; s < im.sets; s += kWave >> im.team) {
         const int64_t g = (int64_t)im.set0 + s;
-        const float v = per_set[g];
+        const float v = per_set ? per_set[g] : list_slope(a, list_off, g, sub, L);
         const int64_t e = a.off[g + 1];
         for (int64_t i = a.off[g] + sub; i < e; i += L) a.out[i] = v;
     }
@@ -1214,7 +1264,7 @@ SumArgs sum_args(const SetLayout& s) {
 
 template <bool PAIRS>
 hipError_t launch_set_sum(const SetLayout& s, const SumArgs& a, hipStream_t stream) {
-    const int grid = s.num_wide + tile_groups(s);
+    const int grid = s.num_wide + tile_groups(s) + (PAIRS && a.num_sums > 0 ? 1 : 0);
     if (grid == 0) return hipSuccess;
     hipLaunchKernelGGL(set_sum_kernel<PAIRS>, dim3(grid), dim3(kBlock), 0, stream, a);
     hipError_t e = hipGetLastError();
@@ -1293,21 +1343,30 @@ hipError_t launch_preference(const PairLayout& p, PairArgs a, const float* value
     const int grid = (int)(want < 1 ? 1 : want > kPairGrid ? kPairGrid : want);
     hipLaunchKernelGGL(pair_kernel, dim3(grid), dim3(kBlock), 0, stream, a);
     if ((e = hipGetLastError()) != hipSuccess) return e;
-    if (grid > 1) {
-        hipLaunchKernelGGL(join_kernel, dim3(1), dim3(kBlock), 0, stream, a.sums, grid, 1, 1, a.loss, nullptr);
-        if ((e = hipGetLastError()) != hipSuccess) return e;
-    }
+    // the losses of several workgroups are joined by the next launch
+    const int num_sums = grid > 1 ? grid : 0;
     SumArgs sa = sum_args(p.lists);
     sa.parts = parts + p.seqs.num_wide;
     sa.entries = p.entries;
     sa.slopes = a.slopes;
     sa.out = seqs ? seq_grad : grad;
-    if ((e = launch_set_sum<true>(p.lists, sa, stream)) != hipSuccess) return e;
-    const int grid_steps = p.seqs.num_wide + tile_groups(p.seqs);
-    if (seqs && grid_steps > 0) {
-        SumArgs sp = sum_args(p.seqs);
-        sp.out = grad;
-        hipLaunchKernelGGL(spread_kernel, dim3(grid_steps), dim3(kBlock), 0, stream, sp, seq_grad);
+    sa.sums = a.sums;
+    sa.num_sums = num_sums;
+    sa.loss = a.loss;
+    // Sequences whose lists are all short are summed where their steps are written
+    const bool direct = seqs && p.lists.num_wide == 0;
+    if (!direct && (e = launch_set_sum<true>(p.lists, sa, stream)) != hipSuccess) return e;
+    if (!seqs) return e;
+    SumArgs sp = sum_args(p.seqs);
+    sp.entries = p.entries;
+    sp.slopes = a.slopes;
+    sp.out = grad;
+    sp.sums = a.sums;
+    sp.num_sums = num_sums;
+    sp.loss = a.loss;
+    const int steps = p.seqs.num_wide + tile_groups(p.seqs) + (direct && num_sums > 0 ? 1 : 0);
+    if (steps > 0) {
+        hipLaunchKernelGGL(spread_kernel, dim3(steps), dim3(kBlock), 0, stream, sp, direct ? nullptr : seq_grad, p.lists.off);
         e = hipGetLastError();
     }
     return e;

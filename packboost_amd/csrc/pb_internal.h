@@ -533,7 +533,7 @@ struct PairLayout {
 enum ChoiceMode { kRows, kSteps, kRowsBack, kStepsBack, kPolicy };
 constexpr int kMaxBuckets = 256;
 constexpr int kChoiceGrid = 2048;  // workgroups of a pass over the tiles, and over the wide items, at most
-constexpr int kPairGrid = 1024;
+constexpr int kPairGrid = 2048;
 struct ChoiceArgs {
     const int64_t* off;
     const SetItem* tiles;
