@@ -49,7 +49,7 @@ int32_t team_of(int64_t rows, int64_t sets, int64_t largest) {
 }
 
 struct Layout {
-    std::vector<SetItem> tiles, whole, parts;
+    std::vector<SetItem> tiles, mid, whole, parts;
     std::vector<int32_t> split;  // the first part of each split set, within `parts`
 };
 
@@ -73,6 +73,10 @@ void lay_out(const int64_t* off, int64_t num_sets, Layout& out) {
             im.set0 = (int32_t)g;
             im.sets = 1;
             im.parts = 1;
+            if ((off[g] & 7) + size <= pb::kSetMidRows) {
+                out.mid.push_back(im);
+                continue;
+            }
             if ((off[g] & 7) + size <= pb::kSetWideRows) {
                 out.whole.push_back(im);
                 continue;
@@ -112,11 +116,12 @@ int sets_create(const int64_t* off, int64_t num_sets, pb_sets** out) {
     if (off[num_sets] > ((int64_t)1 << 40)) return pb::api_fail(PB_ERR_UNSUPPORTED, "pb_sets_create: more than 2^40 rows");
     Layout lay;
     lay_out(off, num_sets, lay);
-    const size_t tiles = lay.tiles.size(), whole = lay.whole.size();
-    std::vector<SetItem>& items = lay.tiles;  // the tiles, the whole sets, the parts
+    const size_t tiles = lay.tiles.size(), mid = lay.mid.size(), whole = lay.whole.size();
+    std::vector<SetItem>& items = lay.tiles;  // the tiles, the wide items
+    items.insert(items.end(), lay.mid.begin(), lay.mid.end());
     items.insert(items.end(), lay.whole.begin(), lay.whole.end());
     items.insert(items.end(), lay.parts.begin(), lay.parts.end());
-    for (int32_t& first : lay.split) first += (int32_t)whole;
+    for (int32_t& first : lay.split) first += (int32_t)(mid + whole);
     const std::vector<int32_t>& split = lay.split;
     const size_t b_off = round256(sizeof(int64_t) * (size_t)(num_sets + 1));
     const size_t b_items = round256(sizeof(SetItem) * items.size());
@@ -138,7 +143,8 @@ int sets_create(const int64_t* off, int64_t num_sets, pb_sets** out) {
     h->s.wide = h->s.tiles + tiles;
     h->s.split = reinterpret_cast<int32_t*>(h->arena + b_off + b_items);
     h->s.num_tiles = (int32_t)tiles;
-    h->s.num_wide = (int32_t)(items.size() - tiles);
+    h->s.num_mid = (int32_t)mid;
+    h->s.num_wide = (int32_t)(items.size() - tiles - mid);
     h->s.num_whole = (int32_t)whole;
     h->s.num_split = (int32_t)split.size();
     h->s.num_sets = num_sets;
@@ -197,7 +203,7 @@ int64_t sum_cols(const pb_sets* s, int32_t op, int32_t num_buckets) {
 }
 
 int64_t work_need(const pb_sets* s, int32_t op, int32_t num_buckets) {
-    const int64_t parts = s->s.num_wide > s->s.num_whole ? s->s.num_wide : 0;
+    const int64_t parts = s->s.num_wide > s->s.num_whole ? s->s.num_mid + s->s.num_wide : 0;
     return 8 * (sum_cols(s, op, num_buckets) * pb::choice_grid(s->s) + parts);
 }
 

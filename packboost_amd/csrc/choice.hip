@@ -24,6 +24,7 @@ constexpr float kInf = __builtin_huge_valf();
 constexpr int kRun = 8;                                     // consecutive rows of a lane
 constexpr int kWideRuns = kSetWideRows / (kRun * kBlock);   // runs of a thread of a longer set
 constexpr int kTileRounds = kSetTileSets / kWave;           // sets of a tile per lane
+constexpr int kTileAhead = 2;                               // and of those, asked for with the rows
 constexpr int kPairs = 4;                                   // pairs a thread has in flight
 constexpr int kBins = 256;     // LDS words of the table's gradient per wave: buckets x copies
 constexpr int kLookup = 2048;  // bytes of the position lookup kept in LDS
@@ -101,48 +102,64 @@ __device__ __forceinline__ Span span_of(const ChoiceArgs& a, const SetItem& im) 
     return s;
 }
 
-// Runs of kRun rows from row i of a span on: as 16-byte accesses where the addresses are aligned
-// (a.vec) and all lie in the table, else row by row within [lo, hi).
+// The rows of a lane's run from row i on that lie outside [lo, hi), a bit each.
+__device__ __forceinline__ uint32_t outside(const Span& s, int i) {
+    uint32_t b = 0;
+    if (i < s.lo) b |= (1u << min(s.lo - i, kRun)) - 1u;
+    if (i + kRun > s.hi) b |= 0xffu << max(s.hi - i, 0);
+    return b & 0xffu;
+}
+
+// Whether a run goes in accesses of 16 bytes: the addresses are aligned (a.vec) and all its rows lie in the
+// table. Else it goes row by row, in a rolled loop, within [lo, hi).
+__device__ __forceinline__ bool whole_run(const ChoiceArgs& a, const Span& s, int i) { return a.vec && i + kRun <= s.end; }
+
+__device__ __forceinline__ void put_row(float (&x)[kRun], int k, float v) {
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) x[j] = j == k ? v : x[j];
+}
+
 template <int TYPE>
 __device__ __forceinline__ void load_scores(const ChoiceArgs& a, const Span& s, int i, float (&x)[kRun]) {
-    if (a.vec && i + kRun <= s.end) {
-        if (TYPE == PB_F32) {
-            const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(a.scores) + s.q0 + i);
-            const float4 t = p[0], u = p[1];
-            x[0] = t.x, x[1] = t.y, x[2] = t.z, x[3] = t.w;
-            x[4] = u.x, x[5] = u.y, x[6] = u.z, x[7] = u.w;
-        } else {
-            const uint4 t = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.scores) + s.q0 + i);
-            x[0] = half_value<TYPE>(t.x & 0xffffu), x[1] = half_value<TYPE>(t.x >> 16);
-            x[2] = half_value<TYPE>(t.y & 0xffffu), x[3] = half_value<TYPE>(t.y >> 16);
-            x[4] = half_value<TYPE>(t.z & 0xffffu), x[5] = half_value<TYPE>(t.z >> 16);
-            x[6] = half_value<TYPE>(t.w & 0xffffu), x[7] = half_value<TYPE>(t.w >> 16);
-        }
+    if (TYPE == PB_F32) {
+        const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(a.scores) + s.q0 + i);
+        const float4 t = p[0], u = p[1];
+        x[0] = t.x, x[1] = t.y, x[2] = t.z, x[3] = t.w;
+        x[4] = u.x, x[5] = u.y, x[6] = u.z, x[7] = u.w;
     } else {
-#pragma unroll
-        for (int k = 0; k < kRun; ++k)
-            x[k] = i + k >= s.lo && i + k < s.hi ? load_score<TYPE>(a.scores, (s.q0 + i + k) * a.stride) : 0.0f;
+        const uint4 t = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.scores) + s.q0 + i);
+        x[0] = half_value<TYPE>(t.x & 0xffffu), x[1] = half_value<TYPE>(t.x >> 16);
+        x[2] = half_value<TYPE>(t.y & 0xffffu), x[3] = half_value<TYPE>(t.y >> 16);
+        x[4] = half_value<TYPE>(t.z & 0xffffu), x[5] = half_value<TYPE>(t.z >> 16);
+        x[6] = half_value<TYPE>(t.w & 0xffffu), x[7] = half_value<TYPE>(t.w >> 16);
     }
 }
 
-__device__ __forceinline__ void load_floats(const ChoiceArgs& a, const Span& s, int i, const float* p, float (&x)[kRun]) {
-    if (a.vec && i + kRun <= s.end) {
+// A run of the rows' gradients, 0 where `off` has a bit.
+__device__ __forceinline__ void load_floats(const ChoiceArgs& a, const Span& s, int i, const float* p, uint32_t off,
+                                            float (&x)[kRun]) {
+    if (whole_run(a, s, i)) {
         const float4* v = reinterpret_cast<const float4*>(p + s.q0 + i);
         const float4 t = v[0], u = v[1];
         x[0] = t.x, x[1] = t.y, x[2] = t.z, x[3] = t.w;
         x[4] = u.x, x[5] = u.y, x[6] = u.z, x[7] = u.w;
     } else {
+        const uint32_t out = outside(s, i);
+#pragma unroll 1
+        for (int k = 0; k < kRun; ++k)
+            if (!(out >> k & 1u)) put_row(x, k, p[s.q0 + i + k]);
+    }
+    if (off) {
 #pragma unroll
-        for (int k = 0; k < kRun; ++k) x[k] = i + k >= s.lo && i + k < s.hi ? p[s.q0 + i + k] : 0.0f;
+        for (int k = 0; k < kRun; ++k) x[k] = off >> k & 1u ? 0.0f : x[k];
     }
 }
-
-__device__ __forceinline__ bool inside(const Span& s, int i) { return i >= s.lo && i + kRun <= s.hi; }
 
 // A run's values out, those in [lo, hi) alone.
 template <int TYPE>
 __device__ __forceinline__ void store_run(const ChoiceArgs& a, const Span& s, int i, void* p, const float (&x)[kRun]) {
-    if (a.vec && inside(s, i)) {
+    const uint32_t out = outside(s, i);
+    if (a.vec && out == 0) {
         if (TYPE == PB_F32) {
             float4* v = reinterpret_cast<float4*>(static_cast<float*>(p) + s.q0 + i);
             v[0] = make_float4(x[0], x[1], x[2], x[3]);
@@ -155,7 +172,7 @@ __device__ __forceinline__ void store_run(const ChoiceArgs& a, const Span& s, in
     } else {
 #pragma unroll
         for (int k = 0; k < kRun; ++k)
-            if (i + k >= s.lo && i + k < s.hi) store_score<TYPE>(p, s.q0 + i + k, x[k]);
+            if (!(out >> k & 1u)) store_score<TYPE>(p, s.q0 + i + k, x[k]);
     }
 }
 
@@ -184,55 +201,55 @@ struct Buckets {
     __device__ __forceinline__ int at(int k) const { return (int)(w[k >> 2] >> (8 * (k & 3)) & 0xffu); }
 };
 
-// A run's logits: -inf outside [lo, hi) and where masked (`hidden`, a bit a row).
+// A run's logits: -inf where `off` has a bit, outside [lo, hi) and where masked.
 template <int TYPE, bool MASK, bool BIAS>
 __device__ __forceinline__ void load_logits(const ChoiceArgs& a, const BiasShared* bias, const Span& s, int i,
-                                            float (&x)[kRun], uint32_t& hidden, Buckets& buckets) {
-    const bool vec = a.vec && i + kRun <= s.end;
-    load_scores<TYPE>(a, s, i, x);
-    hidden = 0;
+                                            float (&x)[kRun], uint32_t& off, Buckets& buckets) {
+    off = outside(s, i);
     buckets.w[0] = buckets.w[1] = 0;
-    if (MASK) {
-        if (vec) {
+    if (whole_run(a, s, i)) {
+        load_scores<TYPE>(a, s, i, x);
+        if (MASK) {
             const uint2 m = *reinterpret_cast<const uint2*>(a.mask + s.q0 + i);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                hidden |= (m.x >> (8 * k) & 0xffu) == 0 ? 1u << k : 0u;
-                hidden |= (m.y >> (8 * k) & 0xffu) == 0 ? 16u << k : 0u;
+                off |= (m.x >> (8 * k) & 0xffu) == 0 ? 1u << k : 0u;
+                off |= (m.y >> (8 * k) & 0xffu) == 0 ? 16u << k : 0u;
             }
-        } else {
-#pragma unroll
-            for (int k = 0; k < kRun; ++k)
-                if (i + k >= s.lo && i + k < s.hi && !a.mask[s.q0 + i + k]) hidden |= 1u << k;
         }
-    }
-    if (BIAS) {
-        int32_t pos[kRun];
-        if (vec) {
+        if (BIAS) {
             const int4* p = reinterpret_cast<const int4*>(a.positions + s.q0 + i);
             const int4 t = p[0], u = p[1];
-            pos[0] = t.x, pos[1] = t.y, pos[2] = t.z, pos[3] = t.w;
-            pos[4] = u.x, pos[5] = u.y, pos[6] = u.z, pos[7] = u.w;
-        } else {
+            const int32_t pos[kRun] = {t.x, t.y, t.z, t.w, u.x, u.y, u.z, u.w};
 #pragma unroll
-            for (int k = 0; k < kRun; ++k) pos[k] = i + k >= s.lo && i + k < s.hi ? a.positions[s.q0 + i + k] : 0;
+            for (int k = 0; k < kRun; ++k) {
+                const uint32_t b = bucket_of(a, *bias, pos[k]);
+                buckets.w[k >> 2] |= b << (8 * (k & 3));
+                x[k] += bias->table[b];
+            }
         }
-#pragma unroll
+    } else {
+        const uint32_t out = off;
+#pragma unroll 1
         for (int k = 0; k < kRun; ++k) {
-            const uint32_t b = bucket_of(a, *bias, pos[k]);
-            buckets.w[k >> 2] |= b << (8 * (k & 3));
-            x[k] += bias->table[b];
+            if (out >> k & 1u) continue;
+            const int64_t row = s.q0 + i + k;
+            float v = load_score<TYPE>(a.scores, row * a.stride);
+            if (BIAS) {
+                const uint32_t b = bucket_of(a, *bias, a.positions[row]);
+                if (k < 4)
+                    buckets.w[0] |= b << (8 * k);
+                else
+                    buckets.w[1] |= b << (8 * (k - 4));
+                v += bias->table[b];
+            }
+            if (MASK && !a.mask[row]) off |= 1u << k;
+            put_row(x, k, v);
         }
     }
-    if (MASK) {
+    if (off) {
 #pragma unroll
-        for (int k = 0; k < kRun; ++k)
-            if (hidden >> k & 1u) x[k] = -kInf;
-    }
-    if (!inside(s, i)) {
-#pragma unroll
-        for (int k = 0; k < kRun; ++k)
-            if (i + k < s.lo || i + k >= s.hi) x[k] = -kInf;
+        for (int k = 0; k < kRun; ++k) x[k] = off >> k & 1u ? -kInf : x[k];
     }
 }
 
@@ -242,21 +259,6 @@ __device__ __forceinline__ float one_logit(const ChoiceArgs& a, const BiasShared
     float x = load_score<TYPE>(a.scores, row * a.stride);
     if (BIAS) x += bias->table[bucket_of(a, *bias, a.positions[row])];
     return x;
-}
-
-// Gradients of a run: 0 where masked, and outside [lo, hi) (nothing is added there).
-template <bool MASK>
-__device__ __forceinline__ void clear_hidden(const Span& s, int i, uint32_t hidden, float (&g)[kRun]) {
-    if (MASK) {
-#pragma unroll
-        for (int k = 0; k < kRun; ++k)
-            if (hidden >> k & 1u) g[k] = 0.0f;
-    }
-    if (!inside(s, i)) {
-#pragma unroll
-        for (int k = 0; k < kRun; ++k)
-            if (i + k < s.lo || i + k >= s.hi) g[k] = 0.0f;
-    }
 }
 
 __device__ __forceinline__ float over(float a, float b) { return b > a ? b : a; }  // a NaN b is passed over
@@ -328,32 +330,30 @@ __device__ __forceinline__ Soft join_parts(const float2* parts, int n, int first
     return l;
 }
 
-// Sums and maxima over runs of rows that may start and end in any lane of a wave. `heads` holds a bit for
-// each row of the lane that starts a set, `tails` for each that ends one. A lane's value since its last
-// head is carried on by a scan of the lanes that stops at heads: 4 steps in rows of 16 lanes, 2 between
-// them.
+// Sums and maxima over runs of rows that may start and end in any lane of a wave: a bit in `heads` where
+// a row starts a set, in `tails` where it ends one. A lane's value since its last head is carried on by a
+// scan of the lanes that stops at heads: 4 steps in rows of 16 lanes, 2 between them.
 struct Segments {
     uint32_t heads, tails;
-    bool from1, from2, from4, from8, from15, from31;  // the scan's steps that stay within the set
+    uint32_t steps;  // a bit for each step of the scan that stays within the lane's set
 
-    __device__ __forceinline__ void start(uint32_t h, int lane, int first, int last) {  // rows first .. last - 1 of the lane
-        heads = h;
-        const unsigned long long m = __ballot(h != 0);
-        const unsigned long long next = __ballot((h & 1u) != 0);
-        tails = h >> 1 | ((lane < kWave - 1 && (next >> (lane + 1) & 1ull)) ? 1u << (kRun - 1) : 0u);
+    // raw: the sets that start at the lane's rows, 0 for none; rows first .. last - 1 of the lane count
+    __device__ __forceinline__ void start(const int (&raw)[kRun], int lane, int first, int last) {
+        heads = 0;
+#pragma unroll
+        for (int k = 0; k < kRun; ++k) heads |= raw[k] ? 1u << k : 0u;
+        const unsigned long long m = __ballot(heads != 0);
+        const unsigned long long next = __ballot((heads & 1u) != 0) >> 1;
+        tails = heads >> 1 | (uint32_t)(next >> lane & 1ull) << (kRun - 1);
         if (last >= 1 && last <= kRun) tails |= 1u << (last - 1);
         const uint32_t from = first <= 0 ? 0xffu : first >= kRun ? 0u : 0xffu << first;
         const uint32_t upto = last <= 0 ? 0u : last >= kRun ? 0xffu : (1u << last) - 1u;
         tails &= from & upto;
         const unsigned long long below = m & (~0ull >> (kWave - 1 - lane));
-        const int head = below ? kWave - 1 - __clzll((long long)below) : 0;  // the last lane up to this one with a head
-        const int in_row = lane & 15;
-        from1 = in_row >= 1 && lane - 1 >= head;
-        from2 = in_row >= 2 && lane - 2 >= head;
-        from4 = in_row >= 4 && lane - 4 >= head;
-        from8 = in_row >= 8 && lane - 8 >= head;
-        from15 = (lane & 16) != 0 && (lane & ~15) - 1 >= head;
-        from31 = lane >= 32 && 31 >= head;
+        const int at = below ? kWave - 1 - __clzll((long long)below) : 0;  // the last lane up to this one with a head
+        const int room = min(lane - at, lane & 15);  // lanes down to it, in the row of 16
+        steps = (room >= 1 ? 1u : 0u) | (room >= 2 ? 2u : 0u) | (room >= 4 ? 4u : 0u) | (room >= 8 ? 8u : 0u) |
+                ((lane & 16) != 0 && (lane & ~15) - 1 >= at ? 16u : 0u) | (lane >= 32 && 31 >= at ? 32u : 0u);
     }
 };
 
@@ -365,7 +365,7 @@ __device__ __forceinline__ float lane_move(float v) {  // lanes without a source
 
 struct TakeMax {
     static constexpr float kNone = -__builtin_huge_valf();
-    static __device__ __forceinline__ float of(float a, float b) { return over(a, b); }
+    static __device__ __forceinline__ float of(float a, float b) { return fmaxf(a, b); }  // passes a NaN over
 };
 struct TakeSum {
     static constexpr float kNone = 0.0f;
@@ -381,12 +381,12 @@ __device__ __forceinline__ void segment_reduce(const Segments& seg, const float 
 #pragma unroll
     for (int k = 1; k < kRun; ++k) v = OP::of(seg.heads >> k & 1u ? OP::kNone : v, x[k]);
     float t;
-    t = lane_move<0x111>(v), v = seg.from1 ? OP::of(t, v) : v;    // row_shr:1
-    t = lane_move<0x112>(v), v = seg.from2 ? OP::of(t, v) : v;    // row_shr:2
-    t = lane_move<0x114>(v), v = seg.from4 ? OP::of(t, v) : v;    // row_shr:4
-    t = lane_move<0x118>(v), v = seg.from8 ? OP::of(t, v) : v;    // row_shr:8
-    t = lane_move<0x142>(v), v = seg.from15 ? OP::of(t, v) : v;   // row_bcast:15
-    t = lane_move<0x143>(v), v = seg.from31 ? OP::of(t, v) : v;   // row_bcast:31
+    t = lane_move<0x111>(v), v = (seg.steps & 1u) ? OP::of(t, v) : v;    // row_shr:1
+    t = lane_move<0x112>(v), v = (seg.steps & 2u) ? OP::of(t, v) : v;    // row_shr:2
+    t = lane_move<0x114>(v), v = (seg.steps & 4u) ? OP::of(t, v) : v;    // row_shr:4
+    t = lane_move<0x118>(v), v = (seg.steps & 8u) ? OP::of(t, v) : v;    // row_shr:8
+    t = lane_move<0x142>(v), v = (seg.steps & 16u) ? OP::of(t, v) : v;   // row_bcast:15
+    t = lane_move<0x143>(v), v = (seg.steps & 32u) ? OP::of(t, v) : v;   // row_bcast:31
     t = __shfl_up(v, 1);
     v = lane > 0 ? t : OP::kNone;
 #pragma unroll
@@ -427,16 +427,16 @@ __device__ __forceinline__ float policy_step(const ChoiceArgs& a, const PolicyIn
     return w * slope;
 }
 
-// The table's gradient as a wave gathers it: bins of whole numbers in units of 2^(e - 30), 2^e above
-// every gradient so far, so that their sums do not depend on the order of the atomics; what the rounding
-// takes is below 2^-31 * 2^e a row. A larger gradient empties the bins into `sum` (lane l holds
-// buckets l, l + 64, ...) and raises e. Copies of the bins keep lanes that meet in a bucket apart.
+// The table's gradient as a wave gathers it: bins of whole numbers in units of 2^(e - 38), 2^e above
+// every gradient so far, so that their sums do not depend on the order of the atomics. A gradient is
+// rounded to 2^(e - 30) (what that takes is below 2^-31 * 2^e a row); a larger one raises e and halves what
+// the bins hold so often, to the nearest. Copies of the bins keep lanes that meet in a bucket apart. 2^25
+// rows of a wave fit.
 struct TableSum {
     unsigned long long* bins;  // [kBins] of this wave
     int* bad;                  // [num_buckets]: a gradient that is not finite
     int copies, e;
     float limit;               // 2^e, 0 before the first gradient
-    double sum[kMaxBuckets / kWave];
 
     __device__ void start(const ChoiceArgs& a, unsigned long long* b, int* flags) {
         bins = b;
@@ -445,59 +445,54 @@ struct TableSum {
         while (copies * 2 * a.num_buckets <= kBins && copies < 32) copies *= 2;
         e = 0;
         limit = 0.0f;
-        const int lane = (int)threadIdx.x & (kWave - 1);
-        for (int i = lane; i < kBins; i += kWave) bins[i] = 0;
-#pragma unroll
-        for (int k = 0; k < kMaxBuckets / kWave; ++k) sum[k] = 0.0;
-        wave_sync();
-    }
-
-    __device__ void empty(const ChoiceArgs& a) {
-        wave_sync();
-        const int lane = (int)threadIdx.x & (kWave - 1);
-#pragma unroll
-        for (int k = 0; k < kMaxBuckets / kWave; ++k) {
-            const int b = k * kWave + lane;
-            if (b < a.num_buckets) {
-                long long t = 0;
-                for (int c = 0; c < copies; ++c) {
-                    t += (long long)bins[b * copies + c];
-                    bins[b * copies + c] = 0;
-                }
-                sum[k] += ldexp((double)t, e - 30);
-            }
-        }
+        for (int i = (int)threadIdx.x & (kWave - 1); i < kBins; i += kWave) bins[i] = 0;
         wave_sync();
     }
 
     // raises e above every lane's `big`, finite; the whole wave
-    __device__ __forceinline__ void make_room(const ChoiceArgs& a, float big) {
+    __device__ __forceinline__ void make_room(float big) {
         if (__any(big >= limit && big > 0.0f)) {
-            empty(a);
-            (void)frexpf(wave_max(big), &e);
-            limit = ldexpf(1.0f, e);
+            int now;
+            (void)frexpf(wave_max(big), &now);
+            const int by = limit > 0.0f ? min(now - e, 62) : 62;
+            wave_sync();
+#pragma unroll 1
+            for (int i = (int)threadIdx.x & (kWave - 1); i < kBins; i += kWave) {
+                const long long t = (long long)bins[i];
+                bins[i] = (unsigned long long)((t + (1ll << (by - 1))) >> by);
+            }
+            wave_sync();
+            e = now;
+            limit = ldexpf(1.0f, now);
         }
     }
 
-    __device__ __forceinline__ void put(float v, int bucket) {
-        if (fabsf(v) < kInf)
-            atomicAdd(&bins[bucket * copies + ((int)threadIdx.x & (copies - 1))],
-                      (unsigned long long)(long long)__float2int_rn(ldexpf(v, 30 - e)));
-        else
-            bad[bucket] = 1;
-    }
-
-    __device__ __forceinline__ void add(const ChoiceArgs& a, const float (&g)[kRun], const Buckets& buckets) {
+    __device__ __forceinline__ void add(const float (&g)[kRun], const Buckets& buckets) {
         float big = 0.0f;
 #pragma unroll
         for (int k = 0; k < kRun; ++k) {
             const float m = fabsf(g[k]);
-            if (m < kInf) big = fmaxf(big, m);
+            big = m < kInf ? fmaxf(big, m) : big;
         }
-        make_room(a, big);
+        make_room(big);
+        const int mine = (int)threadIdx.x & (copies - 1);
 #pragma unroll
-        for (int k = 0; k < kRun; ++k)
-            if (g[k] != 0.0f) put(g[k], buckets.at(k));
+        for (int k = 0; k < kRun; ++k) {
+            if (g[k] == 0.0f) continue;
+            const int b = buckets.at(k);
+            if (fabsf(g[k]) < kInf) {
+                const long long t = (long long)__float2int_rn(ldexpf(g[k], 30 - e)) << 8;
+                atomicAdd(&bins[b * copies + mine], (unsigned long long)t);
+            } else {
+                bad[b] = 1;
+            }
+        }
+    }
+
+    __device__ __forceinline__ double value(int b) const {  // of bucket b
+        long long t = 0;
+        for (int c = 0; c < copies; ++c) t += (long long)bins[b * copies + c];
+        return ldexp((double)t, e - 38);
     }
 };
 
@@ -520,17 +515,17 @@ __global__ __launch_bounds__(kBlock) void part_kernel(ChoiceArgs a, int first) {
         for (int k = 0; k < kRun; ++k) v[j][k] = MODE == kRowsBack ? 0.0f : -kInf;
         if (i < s.hi) {
             if (MODE == kRowsBack) {
-                load_floats(a, s, i, a.grad, v[j]);
-                uint32_t hidden = 0;
-                if (MASK)
-#pragma unroll
+                uint32_t off = outside(s, i);
+                if (MASK) {
+                    const uint32_t out = off;
                     for (int k = 0; k < kRun; ++k)
-                        if (i + k >= s.lo && i + k < s.hi && !a.mask[s.q0 + i + k]) hidden |= 1u << k;
-                clear_hidden<MASK>(s, i, hidden, v[j]);
+                        if (!(out >> k & 1u) && !a.mask[s.q0 + i + k]) off |= 1u << k;
+                }
+                load_floats(a, s, i, a.grad, off, v[j]);
             } else {
-                uint32_t hidden;
+                uint32_t off;
                 Buckets buckets;
-                load_logits<TYPE, MASK, BIAS>(a, &bias, s, i, v[j], hidden, buckets);
+                load_logits<TYPE, MASK, BIAS>(a, &bias, s, i, v[j], off, buckets);
             }
         }
     }
@@ -547,7 +542,7 @@ __global__ __launch_bounds__(kBlock) void part_kernel(ChoiceArgs a, int first) {
 #pragma unroll
     for (int j = 0; j < kWideRuns; ++j)
 #pragma unroll
-        for (int k = 0; k < kRun; ++k) top = over(top, v[j][k]);
+        for (int k = 0; k < kRun; ++k) top = fmaxf(top, v[j][k]);
     top = wave_max(top);
     if (top == -kInf) top = 0.0f;
 #pragma unroll
@@ -562,8 +557,10 @@ __global__ __launch_bounds__(kBlock) void part_kernel(ChoiceArgs a, int first) {
 struct TileShared {
     float x[kSetTileRows];          // logits, then what the chosen rows' gradients are more than the others'
     float shift[kSetTileSets];      // per set: maximum, or lse
-    float factor[kSetTileSets];     // sum of exponentials, then what the rows' are multiplied by
-    uint16_t head[kSetTileRows];    // the set that starts at a row, from 1; 0: none
+    union {
+        uint16_t head[kSetTileRows];  // the set that starts at a row, from 1; 0: none
+        float factor[kSetTileSets];   // later: sum of exponentials, then what the rows' are multiplied by
+    };
     uint16_t begin[kSetTileSets + 4];
 };
 
@@ -590,20 +587,17 @@ __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, const SetItem& im
     const int i0 = kRun * lane;
     // everything the tile reads is asked for before anything is waited for
     float x[kRun], d[kRun];
-    uint32_t hidden = 0;
+    uint32_t off = 0xffu;
     Buckets buckets{{0, 0}};
 #pragma unroll
     for (int k = 0; k < kRun; ++k) x[k] = -kInf, d[k] = 0.0f;
     if (i0 < sp.hi) {
-        load_logits<TYPE, MASK, BIAS>(a, bias, sp, i0, x, hidden, buckets);
-        if (MODE == kRowsBack) {
-            load_floats(a, sp, i0, a.grad, d);
-            clear_hidden<MASK>(sp, i0, hidden, d);
-        }
+        load_logits<TYPE, MASK, BIAS>(a, bias, sp, i0, x, off, buckets);
+        if (MODE == kRowsBack) load_floats(a, sp, i0, a.grad, off, d);
     }
     int32_t begin[kTileRounds], chosen[kTileRounds];
     float given[kTileRounds], lse[kTileRounds];
-    PolicyIn pol[kTileRounds];
+    PolicyIn pol[kTileAhead];
 #pragma unroll
     for (int r = 0; r < kTileRounds; ++r) {
         const int s = r * kWave + lane;
@@ -615,7 +609,7 @@ __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, const SetItem& im
             if (STEPS) chosen[r] = a.chosen[g];
             if (MODE == kStepsBack) given[r] = a.grad[g];
             if (!SOFT) lse[r] = a.lse[g];
-            if (MODE == kPolicy) pol[r] = load_policy(a, g);
+            if (MODE == kPolicy && r < kTileAhead) pol[r < kTileAhead ? r : 0] = load_policy(a, g);
         }
     }
     wave_sync();  // the last tile's values have been read
@@ -653,15 +647,11 @@ __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, const SetItem& im
         const uint4 w = *reinterpret_cast<const uint4*>(&sh.head[i0]);
         const int raw[kRun] = {(int)(w.x & 0xffffu), (int)(w.x >> 16), (int)(w.y & 0xffffu), (int)(w.y >> 16),
                                (int)(w.z & 0xffffu), (int)(w.z >> 16), (int)(w.w & 0xffffu), (int)(w.w >> 16)};
-        uint32_t heads = 0;
         int last = 0;
 #pragma unroll
-        for (int k = 0; k < kRun; ++k) {
-            heads |= raw[k] ? 1u << k : 0u;
-            last = raw[k] ? raw[k] : last;
-        }
+        for (int k = 0; k < kRun; ++k) last = raw[k] ? raw[k] : last;
         // the set that the rows before the lane's first head are of: the last head's below
-        const unsigned long long below = __ballot(heads != 0) & ((1ull << lane) - 1ull);
+        const unsigned long long below = __ballot(last != 0) & ((1ull << lane) - 1ull);
         const int from = below ? kWave - 1 - __clzll((long long)below) : lane;
         const int carried = __shfl(last, from);
         int now = below ? carried : 1;
@@ -670,7 +660,7 @@ __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, const SetItem& im
             now = raw[k] ? raw[k] : now;
             id[k] = now;
         }
-        if (SOFT || MODE == kRowsBack) seg.start(heads, lane, sp.lo - i0, sp.hi - i0);
+        if (SOFT || MODE == kRowsBack) seg.start(raw, lane, sp.lo - i0, sp.hi - i0);
     }
     float v[kRun];
     if (SOFT) {
@@ -715,8 +705,9 @@ __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, const SetItem& im
                     const float lp = SOFT && counts ? (picked[r] - top) - ls : 0.0f;
                     if (SOFT) a.log_probs[g] = lp;
                     if (MODE == kStepsBack && counts) coef[r] = given[r];
-                    if (MODE == kPolicy && counts) coef[r] = policy_step(a, pol[r], lp, true, tally);
-                    if (GRAD) sh.factor[s] = counts ? (SOFT ? -coef[r] / sum : -coef[r]) : 0.0f;
+                    if (MODE == kPolicy && counts) 
+                        coef[r] = policy_step(a, r < kTileAhead ? pol[r < kTileAhead ? r : 0] : load_policy(a, g), lp, true, tally);
+                    if (GRAD) sh.factor[s] = counts ? (SOFT ? -coef[r] * __builtin_amdgcn_rcpf(sum) : -coef[r]) : 0.0f;
                     if (!counts) chosen[r] = -1;
                 }
             }
@@ -752,66 +743,70 @@ __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, const SetItem& im
             v[k] = (f == 0.0f ? 0.0f : f * e) + own[k];
         }
     }
-    if (GRAD) clear_hidden<MASK>(sp, i0, hidden, v);
+    if (GRAD && off) {
+#pragma unroll
+        for (int k = 0; k < kRun; ++k) v[k] = off >> k & 1u ? 0.0f : v[k];
+    }
     if (i0 < sp.hi) {
         if (MODE == kRows)
             store_run<PB_F32>(a, sp, i0, a.log_probs, v);
         else
             store_run<TYPE>(a, sp, i0, a.grad_scores, v);
     }
-    if (BIAS && GRAD) table.add(a, v, buckets);
+    if (BIAS && GRAD) table.add(v, buckets);
 }
 
-// One set of more than kSetShort rows, or a part of it, by a workgroup.
-template <int MODE, int TYPE, bool MASK, bool BIAS>
+// One set of more than kSetShort rows by a wave (THREADS 64), or a longer one or a part of it by a
+// workgroup. A wave passes over runs beyond its rows.
+template <int MODE, int TYPE, bool MASK, bool BIAS, int THREADS>
 __device__ __forceinline__ void wide_pass(const ChoiceArgs& a, const SetItem& im, int32_t index, Soft* shs, float* shf,
                                           const BiasShared* bias, TableSum& table, double (&tally)[3]) {
     constexpr bool GRAD = MODE == kRowsBack || MODE == kStepsBack || MODE == kPolicy;
     constexpr bool STEPS = MODE != kRows && MODE != kRowsBack;
     constexpr bool SOFT = MODE == kRows || MODE == kSteps || MODE == kPolicy;
-    const int tid = (int)threadIdx.x;
+    constexpr bool ALONE = THREADS == kWave;
+    const int tid = (int)threadIdx.x & (THREADS - 1);
+    const int wave0 = __builtin_amdgcn_readfirstlane(tid & ~(kWave - 1));  // the wave's first thread
     const Span sp = span_of(a, im);
     const int64_t g = im.set0;
     const bool first = im.part == 0 && tid == 0;
     float v[kWideRuns][kRun], d[kWideRuns][kRun];
-    uint32_t hidden[kWideRuns];
+    uint32_t off[kWideRuns];
     Buckets buckets[kWideRuns];
 #pragma unroll
     for (int j = 0; j < kWideRuns; ++j) {
-        const int i = kRun * (j * kBlock + tid);
-        hidden[j] = 0;
+        const int i = kRun * (j * THREADS + tid);
+        off[j] = 0xffu;
         buckets[j].w[0] = buckets[j].w[1] = 0;
 #pragma unroll
         for (int k = 0; k < kRun; ++k) v[j][k] = -kInf, d[j][k] = 0.0f;
-        if (i < sp.hi) {
-            load_logits<TYPE, MASK, BIAS>(a, bias, sp, i, v[j], hidden[j], buckets[j]);
-            if (MODE == kRowsBack) {
-                load_floats(a, sp, i, a.grad, d[j]);
-                clear_hidden<MASK>(sp, i, hidden[j], d[j]);
-            }
+        if (kRun * (j * THREADS + wave0) < sp.hi && i < sp.hi) {
+            load_logits<TYPE, MASK, BIAS>(a, bias, sp, i, v[j], off[j], buckets[j]);
+            if (MODE == kRowsBack) load_floats(a, sp, i, a.grad, off[j], d[j]);
         }
     }
     const float lse = SOFT ? 0.0f : a.lse[g];
     const int32_t c = STEPS ? a.chosen[g] : -1;
-    const int live = (sp.hi + kRun * kBlock - 1) / (kRun * kBlock);  // runs that hold rows
+    const int live = sp.hi <= kRun * wave0 ? 0 : (sp.hi - kRun * wave0 + kRun * THREADS - 1) / (kRun * THREADS);  // the wave's runs
     Soft t{0.0f, 0.0f};
     float own = 1.0f;  // what the wave's exponentials are relative to, over the set's maximum
     if (SOFT) {
         Soft w;
-        if (im.parts > 1) {
-            t = block_soft(wave_soft(join_parts(a.parts + (index - im.part), im.parts, tid, kBlock)), shs);
+        if (!ALONE && im.parts > 1) {
+            t = block_soft(wave_soft(join_parts(a.parts + (index - im.part), im.parts, tid, THREADS)), shs);
             w.top = t.top;
         } else {
             w.top = -kInf;
 #pragma unroll
             for (int j = 0; j < kWideRuns; ++j)
+                if (j < live)
 #pragma unroll
-                for (int k = 0; k < kRun; ++k) w.top = over(w.top, v[j][k]);
+                    for (int k = 0; k < kRun; ++k) w.top = fmaxf(w.top, v[j][k]);
             w.top = wave_max(w.top);
             if (w.top == -kInf) w.top = 0.0f;
         }
         w.sum = 0.0f;
-        if (im.parts == 1 || GRAD) {
+        if (ALONE || im.parts == 1 || GRAD) {
 #pragma unroll
             for (int j = 0; j < kWideRuns; ++j)
                 if (j < live)
@@ -822,10 +817,10 @@ __device__ __forceinline__ void wide_pass(const ChoiceArgs& a, const SetItem& im
                         if (GRAD) v[j][k] = e;
                     }
         }
-        if (im.parts == 1) {
+        if (ALONE || im.parts == 1) {
             w.sum = wave_sum(w.sum);
-            t = block_soft(w, shs);
-            if (GRAD) own = w.sum != 0.0f ? exp_of(w.top - t.top) : 0.0f;
+            t = ALONE ? w : block_soft(w, shs);
+            if (GRAD && !ALONE) own = w.sum != 0.0f ? exp_of(w.top - t.top) : 0.0f;
         }
     }
     const float ls = SOFT ? logf(t.sum) : 0.0f;
@@ -833,21 +828,22 @@ __device__ __forceinline__ void wide_pass(const ChoiceArgs& a, const SetItem& im
     if (MODE == kRows) {
 #pragma unroll
         for (int j = 0; j < kWideRuns; ++j)
+            if (j < live)
 #pragma unroll
-            for (int k = 0; k < kRun; ++k) v[j][k] = v[j][k] == -kInf ? -kInf : (v[j][k] - t.top) - ls;
+                for (int k = 0; k < kRun; ++k) v[j][k] = v[j][k] == -kInf ? -kInf : (v[j][k] - t.top) - ls;
     }
     if (MODE == kRowsBack) {
         float total = 0.0f;
-        if (im.parts > 1) {
+        if (!ALONE && im.parts > 1) {
             const float2* parts = a.parts + (index - im.part);
-            for (int j = tid; j < im.parts; j += kBlock) total += parts[j].y;
+            for (int j = tid; j < im.parts; j += THREADS) total += parts[j].y;
         } else {
 #pragma unroll
             for (int j = 0; j < kWideRuns; ++j)
 #pragma unroll
                 for (int k = 0; k < kRun; ++k) total += d[j][k];
         }
-        total = block_sum(total, shf);
+        total = ALONE ? wave_sum(total) : block_sum(total, shf);
 #pragma unroll
         for (int j = 0; j < kWideRuns; ++j)
             if (j < live)
@@ -868,7 +864,7 @@ __device__ __forceinline__ void wide_pass(const ChoiceArgs& a, const SetItem& im
             float coef = 0.0f;
             if (MODE == kStepsBack && counts) coef = a.grad[g];
             if (MODE == kPolicy && counts) coef = policy_step(a, load_policy(a, g), lp, first, tally);
-            const float f = counts ? (SOFT ? -coef / t.sum : -coef) : 0.0f;
+            const float f = counts ? (SOFT ? -coef * __builtin_amdgcn_rcpf(t.sum) : -coef) : 0.0f;
             const float fw = f * own;
             const int64_t row = r0 + c - sp.q0;
             if (counts && row >= sp.lo && row < sp.hi) {
@@ -888,18 +884,22 @@ __device__ __forceinline__ void wide_pass(const ChoiceArgs& a, const SetItem& im
     if (MODE == kSteps) return;
 #pragma unroll
     for (int j = 0; j < kWideRuns; ++j) {
-        const int i = kRun * (j * kBlock + tid);
+        if (j >= live) break;
+        const int i = kRun * (j * THREADS + tid);
         if (MODE == kRows) {
             if (i < sp.hi) store_run<PB_F32>(a, sp, i, a.log_probs, v[j]);
         } else {
-            clear_hidden<MASK>(sp, i, hidden[j], v[j]);
+            if (off[j]) {
+#pragma unroll
+                for (int k = 0; k < kRun; ++k) v[j][k] = off[j] >> k & 1u ? 0.0f : v[j][k];
+            }
             if (STEPS && at >= i && at < i + kRun) {
 #pragma unroll
                 for (int k = 0; k < kRun; ++k)
                     if (at - i == k) v[j][k] += extra;
             }
             if (i < sp.hi) store_run<TYPE>(a, sp, i, a.grad_scores, v[j]);
-            if (BIAS && j < live) table.add(a, v[j], buckets[j]);
+            if (BIAS) table.add(v[j], buckets[j]);
         }
     }
 }
@@ -946,10 +946,17 @@ __device__ __forceinline__ void leave_sums(const ChoiceArgs& a, int block, doubl
         }
     }
     if (TABLE) {
-        table.empty(a);
+        // each wave's values in the place of its bins: bucket b's are all read before slot b is written,
+        // since a lane's bucket lies at or after the lane's slot and the wave takes 64 at a time
         double* own = reinterpret_cast<double*>(bins[wave]);
-#pragma unroll
-        for (int k = 0; k < kMaxBuckets / kWave; ++k) own[k * kWave + lane] = table.sum[k];
+        wave_sync();
+#pragma unroll 1
+        for (int b0 = 0; b0 < a.num_buckets; b0 += kWave) {
+            const double t = b0 + lane < a.num_buckets ? table.value(b0 + lane) : 0.0;
+            wave_sync();
+            if (b0 + lane < a.num_buckets) own[b0 + lane] = t;
+            wave_sync();
+        }
         __syncthreads();
         for (int b = tid; b < a.num_buckets; b += kBlock) {
             double t = 0.0;
@@ -983,14 +990,16 @@ __global__ __launch_bounds__(kBlock) void tile_kernel(ChoiceArgs a) {
     }
     if (BIAS) stage_bias(a, bias);
     double tally[3] = {0.0, 0.0, 0.0};
-    for (int it = (int)blockIdx.x * kWaves + wave; it < a.num_tiles; it += (int)gridDim.x * kWaves)
+    for (int it = __builtin_amdgcn_readfirstlane((int)blockIdx.x * kWaves + wave); it < a.num_tiles;
+         it += (int)gridDim.x * kWaves)
         tile_pass<MODE, TYPE, MASK, BIAS>(a, a.tiles[it], tiles[wave], &bias, table, tally);
     leave_sums<MODE, TABLE>(a, (int)blockIdx.x, tally, table, bins, bad, shd);
 }
 
-// The longer sets and their parts, one a workgroup at a time.
+// The longer sets: workgroups [0, mid_blocks) take those for a wave, the others those for a workgroup and
+// the parts, one at a time.
 template <int MODE, int TYPE, bool MASK, bool BIAS>
-__global__ __launch_bounds__(kBlock) void wide_kernel(ChoiceArgs a) {
+__global__ __launch_bounds__(kBlock) void wide_kernel(ChoiceArgs a, int mid_blocks) {
     constexpr bool TABLE = kTable<MODE, BIAS>;
     __shared__ BiasShared bias;
     __shared__ unsigned long long bins[TABLE ? kWaves : 1][kBins];
@@ -1006,9 +1015,14 @@ __global__ __launch_bounds__(kBlock) void wide_kernel(ChoiceArgs a) {
     }
     if (BIAS) stage_bias(a, bias);
     double tally[3] = {0.0, 0.0, 0.0};
-    const int n = MODE == kSteps ? a.num_whole : a.num_wide;
-    for (int it = (int)blockIdx.x; it < n; it += (int)gridDim.x)
-        wide_pass<MODE, TYPE, MASK, BIAS>(a, a.wide[it], it, shs, shf, &bias, table, tally);
+    if ((int)blockIdx.x < mid_blocks) {
+        for (int it = __builtin_amdgcn_readfirstlane((int)blockIdx.x * kWaves + wave); it < a.num_mid; it += mid_blocks * kWaves)
+            wide_pass<MODE, TYPE, MASK, BIAS, kWave>(a, a.wide[it], it, shs, shf, &bias, table, tally);
+    } else {
+        const int n = a.num_mid + (MODE == kSteps ? a.num_whole : a.num_wide);
+        for (int it = a.num_mid + (int)blockIdx.x - mid_blocks; it < n; it += (int)gridDim.x - mid_blocks)
+            wide_pass<MODE, TYPE, MASK, BIAS, kBlock>(a, a.wide[it], it, shs, shf, &bias, table, tally);
+    }
     leave_sums<MODE, TABLE>(a, a.blocks - (int)gridDim.x + (int)blockIdx.x, tally, table, bins, bad, shd);
 }
 
@@ -1208,24 +1222,26 @@ int tile_groups(const SetLayout& s) { return (s.num_tiles + kWaves - 1) / kWaves
 
 int tile_blocks(const SetLayout& s) { return std::min(tile_groups(s), kChoiceGrid); }
 
-int wide_blocks(const SetLayout& s) { return std::min(s.num_wide, kChoiceGrid); }
+int mid_blocks(const SetLayout& s) { return std::min((s.num_mid + kWaves - 1) / kWaves, kChoiceGrid); }
+
+int wide_blocks(int wide) { return std::min(wide, kChoiceGrid); }
 
 template <int MODE, int TYPE, bool MASK, bool BIAS>
 hipError_t launch_choice_as(const SetLayout& s, const ChoiceArgs& a, hipStream_t stream) {
     hipError_t e = hipSuccess;
     const int parts = s.num_wide - s.num_whole;
     if (MODE != kStepsBack && parts > 0) {
-        hipLaunchKernelGGL((part_kernel<MODE, TYPE, MASK, BIAS>), dim3(parts), dim3(kBlock), 0, stream, a, s.num_whole);
+        hipLaunchKernelGGL((part_kernel<MODE, TYPE, MASK, BIAS>), dim3(parts), dim3(kBlock), 0, stream, a,
+                           s.num_mid + s.num_whole);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
     if (s.num_tiles > 0) {
         hipLaunchKernelGGL((tile_kernel<MODE, TYPE, MASK, BIAS>), dim3(tile_blocks(s)), dim3(kBlock), 0, stream, a);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
-    const int wide = MODE == kSteps ? s.num_whole : s.num_wide;
+    const int wide = mid_blocks(s) + wide_blocks(MODE == kSteps ? s.num_whole : s.num_wide);
     if (wide > 0) {
-        hipLaunchKernelGGL((wide_kernel<MODE, TYPE, MASK, BIAS>), dim3(std::min(wide, wide_blocks(s))), dim3(kBlock), 0,
-                           stream, a);
+        hipLaunchKernelGGL((wide_kernel<MODE, TYPE, MASK, BIAS>), dim3(wide), dim3(kBlock), 0, stream, a, mid_blocks(s));
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
     if (MODE == kSteps && s.num_split > 0) {
@@ -1252,19 +1268,22 @@ hipError_t launch_choice_mode(const SetLayout& s, const ChoiceArgs& a, int32_t t
     return launch_choice_typed<MODE, PB_F32>(s, a, stream);
 }
 
+// Items a workgroup each of the sums
+int long_items(const SetLayout& s) { return s.num_mid + s.num_wide; }
+
 SumArgs sum_args(const SetLayout& s) {
     SumArgs a{};
     a.off = s.off;
     a.tiles = s.tiles;
     a.wide = s.wide;
     a.num_tiles = s.num_tiles;
-    a.num_wide = s.num_wide;
+    a.num_wide = s.num_mid + s.num_wide;
     return a;
 }
 
 template <bool PAIRS>
 hipError_t launch_set_sum(const SetLayout& s, const SumArgs& a, hipStream_t stream) {
-    const int grid = s.num_wide + tile_groups(s) + (PAIRS && a.num_sums > 0 ? 1 : 0);
+    const int grid = long_items(s) + tile_groups(s) + (PAIRS && a.num_sums > 0 ? 1 : 0);
     if (grid == 0) return hipSuccess;
     hipLaunchKernelGGL(set_sum_kernel<PAIRS>, dim3(grid), dim3(kBlock), 0, stream, a);
     hipError_t e = hipGetLastError();
@@ -1286,7 +1305,7 @@ hipError_t launch_zero(float* out, int64_t n, hipStream_t stream) {
     return hipGetLastError();
 }
 
-int32_t choice_grid(const SetLayout& s) { return tile_blocks(s) + wide_blocks(s); }
+int32_t choice_grid(const SetLayout& s) { return tile_blocks(s) + mid_blocks(s) + wide_blocks(s.num_wide); }
 
 hipError_t launch_choice(int mode, const SetLayout& s, ChoiceArgs a, int32_t type, hipStream_t stream) {
     a.off = s.off;
@@ -1294,6 +1313,7 @@ hipError_t launch_choice(int mode, const SetLayout& s, ChoiceArgs a, int32_t typ
     a.wide = s.wide;
     a.num_tiles = s.num_tiles;
     a.num_wide = s.num_wide;
+    a.num_mid = s.num_mid;
     a.num_whole = s.num_whole;
     a.blocks = choice_grid(s);
     a.rows = s.rows;
@@ -1321,7 +1341,7 @@ hipError_t launch_preference(const PairLayout& p, PairArgs a, const float* value
     a.num_pairs = p.num_pairs;
     a.sums = reinterpret_cast<double*>(work);
     double* parts = a.sums + kPairGrid;
-    a.slopes = reinterpret_cast<float*>(parts + p.lists.num_wide + p.seqs.num_wide);
+    a.slopes = reinterpret_cast<float*>(parts + long_items(p.lists) + long_items(p.seqs));
     float* seq_sum = a.slopes + p.num_pairs;
     float* seq_grad = seq_sum + p.seqs.num_sets;
     const bool seqs = p.has_seqs;
@@ -1346,7 +1366,7 @@ hipError_t launch_preference(const PairLayout& p, PairArgs a, const float* value
     // the losses of several workgroups are joined by the next launch
     const int num_sums = grid > 1 ? grid : 0;
     SumArgs sa = sum_args(p.lists);
-    sa.parts = parts + p.seqs.num_wide;
+    sa.parts = parts + long_items(p.seqs);
     sa.entries = p.entries;
     sa.slopes = a.slopes;
     sa.out = seqs ? seq_grad : grad;
@@ -1354,7 +1374,7 @@ hipError_t launch_preference(const PairLayout& p, PairArgs a, const float* value
     sa.num_sums = num_sums;
     sa.loss = a.loss;
     // Sequences whose lists are all short are summed where their steps are written
-    const bool direct = seqs && p.lists.num_wide == 0;
+    const bool direct = seqs && long_items(p.lists) == 0;
     if (!direct && (e = launch_set_sum<true>(p.lists, sa, stream)) != hipSuccess) return e;
     if (!seqs) return e;
     SumArgs sp = sum_args(p.seqs);
@@ -1364,7 +1384,7 @@ hipError_t launch_preference(const PairLayout& p, PairArgs a, const float* value
     sp.sums = a.sums;
     sp.num_sums = num_sums;
     sp.loss = a.loss;
-    const int steps = p.seqs.num_wide + tile_groups(p.seqs) + (direct && num_sums > 0 ? 1 : 0);
+    const int steps = long_items(p.seqs) + tile_groups(p.seqs) + (direct && num_sums > 0 ? 1 : 0);
     if (steps > 0) {
         hipLaunchKernelGGL(spread_kernel, dim3(steps), dim3(kBlock), 0, stream, sp, direct ? nullptr : seq_grad, p.lists.off);
         e = hipGetLastError();
@@ -1373,7 +1393,7 @@ hipError_t launch_preference(const PairLayout& p, PairArgs a, const float* value
 }
 
 int64_t preference_work_bytes(const PairLayout& p) {
-    return 8 * ((int64_t)kPairGrid + p.lists.num_wide + p.seqs.num_wide) + 4 * (p.num_pairs + 2 * p.seqs.num_sets);
+    return 8 * ((int64_t)kPairGrid + long_items(p.lists) + long_items(p.seqs)) + 4 * (p.num_pairs + 2 * p.seqs.num_sets);
 }
 
 }  // namespace pb

@@ -492,12 +492,13 @@ hipError_t launch_predict_bins(const uint8_t* bins, int64_t N, int64_t ld, int32
 // A table of ragged sets laid out for wavefronts and workgroups. Tiles, for a wave each, in row order: runs
 // of consecutive sets of at most kSetShort rows, at most kSetTileSets of them; their rows, counted from the
 // multiple of 8 at or before the first, are at most kSetTileRows; `team`: lanes of 1 << team to a set, where
-// a wave's lanes are shared out by sets. Wide items, for a workgroup each: longer sets of at most
-// kSetWideRows rows counted the same way, then the parts (part `part` of `parts`) of those that are longer,
-// a set's consecutive; `split` names the first of each.
+// a wave's lanes are shared out by sets. Wide items: first longer sets of at most kSetMidRows rows counted
+// the same way, for a wave each; then, for a workgroup each, sets of at most kSetWideRows rows and the parts
+// (part `part` of `parts`) of those that are longer, a set's consecutive; `split` names the first of each.
 constexpr int kSetTileRows = 512;
-constexpr int kSetTileSets = 256;
+constexpr int kSetTileSets = 128;
 constexpr int kSetShort = kSetTileRows - 8;
+constexpr int kSetMidRows = 2048;
 constexpr int kSetWideRows = 8192;
 struct SetItem {
     int64_t row0;
@@ -512,9 +513,10 @@ static_assert(sizeof(SetItem) == 32, "an item is 32 bytes");
 struct SetLayout {
     const int64_t* off;    // [num_sets + 1]
     const SetItem* tiles;  // [num_tiles]
-    const SetItem* wide;   // [num_wide], of which the first num_whole are whole sets
+    const SetItem* wide;   // [num_mid + num_wide], of the last num_wide the first num_whole whole sets
     const int32_t* split;  // [num_split], indices of wide items
     int32_t num_tiles;
+    int32_t num_mid;
     int32_t num_wide;
     int32_t num_whole;
     int32_t num_split;
@@ -539,6 +541,7 @@ struct ChoiceArgs {
     const SetItem* tiles;
     const SetItem* wide;
     int32_t num_tiles;
+    int32_t num_mid;
     int32_t num_wide;
     int32_t num_whole;
     int32_t blocks;  // workgroups that leave sums: the tiles', then the wide items'
@@ -565,7 +568,7 @@ struct ChoiceArgs {
     void* grad_scores;
     float* grad_table;
     float* stats;   // policy: loss, kl, clipped weight
-    float2* parts;  // [num_wide] maximum and sum of the parts of split sets
+    float2* parts;  // [num_mid + num_wide] maximum and sum of the parts of split sets
     double* sums;   // [choice_grid][3 (policy) + num_buckets (gradient)]
 };
 struct PairArgs {
