@@ -63,9 +63,12 @@ void lay_out(const int64_t* off, int64_t num_sets, Layout& out) {
         tile = SetItem{};
         largest = 0;
     };
+    int64_t many = 0;
+    for (int64_t g = 0; g < num_sets; ++g) many += off[g + 1] - off[g] > pb::kSetLean;
+    const int64_t most_short = many >= pb::kSetMany ? pb::kSetLean : pb::kSetShort;
     for (int64_t g = 0; g < num_sets; ++g) {
         const int64_t size = off[g + 1] - off[g];
-        if (size > pb::kSetShort) {
+        if (size > most_short) {
             flush();
             SetItem im{};
             im.row0 = off[g];

@@ -21,27 +21,37 @@ namespace {
 
 constexpr int kWaves = kBlock / kWave;
 constexpr float kInf = __builtin_huge_valf();
+// The maximum of no row: below every logit but -inf, whose exponential over it is 0, and finite.
+constexpr float kLowest = -3.402823466e38f;
 constexpr int kRun = 8;                                     // consecutive rows of a lane
 constexpr int kWideRuns = kSetWideRows / (kRun * kBlock);   // runs of a thread of a longer set
 constexpr int kTileRounds = kSetTileSets / kWave;           // sets of a tile per lane
 constexpr int kTileAhead = 2;                               // and of those, asked for with the rows
+// Values from which on they are laid beside their references first: two arrays of them pass a quarter of an
+// XCD's 4 MB L2, and every pair's four reads miss it more and more.
+constexpr int64_t kBothFrom = 1 << 17;
+constexpr int kJoin = 8;
 constexpr int kPairs = 4;                                   // pairs a thread has in flight
 constexpr int kBins = 256;     // LDS words of the table's gradient per wave: buckets x copies
 constexpr int kLookup = 2048;  // bytes of the position lookup kept in LDS
 static_assert(kSetTileRows == kRun * kWave, "a lane holds one run of a tile");
 
-// e^x for x up to about 0 (any x below 88 is right): 2^t at t = x log2(e), whose rounding and
-// log2(e)'s own are made up for by a factor 1 + r log(2). Within 2 units in the last place; results below
-// 2^-126 are 0. NaN stays NaN.
-__device__ __forceinline__ float exp_of(float x) {
-    constexpr float kL = 1.44269502162933349609375f;       // log2(e) rounded to float,
-    constexpr float kLow = 1.92596299112661746887e-8f;     // and what is missing
-    constexpr float kLn2 = 0.69314718055994530942f;
-    x = x < -200.0f ? -200.0f : x;
-    const float t = x * kL;
-    const float r = fmaf(x, kLow, fmaf(x, kL, -t));
-    const float y = __builtin_amdgcn_exp2f(t);
-    return fmaf(y, r * kLn2, y);
+// e^x of a difference to a set's maximum or lse: 2^(x log2(e)) in two instructions. The product's rounding
+// and log2(e)'s own move the result by at most |x| 2^-23 of itself, as a unit in the last place of x does.
+// Results below 2^-126 are 0; e^-inf is 0 and NaN stays NaN.
+__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * 1.44269502162933349609375f); }
+
+// Maxima that pass a NaN over (fmaxf first quiets operands that the compiler cannot see through).
+__device__ __forceinline__ float max2(float a, float b) {
+    float r;
+    asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
 }
 
 __device__ __forceinline__ float bf16_value(uint32_t b) { return __uint_as_float(b << 16); }
@@ -261,8 +271,6 @@ __device__ __forceinline__ float one_logit(const ChoiceArgs& a, const BiasShared
     return x;
 }
 
-__device__ __forceinline__ float over(float a, float b) { return b > a ? b : a; }  // a NaN b is passed over
-
 // LDS written by lanes of this wave is read by others of it: the wave's LDS accesses keep their order,
 // the compiler must too.
 __device__ __forceinline__ void wave_sync() {
@@ -279,7 +287,7 @@ __device__ __forceinline__ F wave_sum(F v) {
 
 __device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
-    for (int m = kWave / 2; m >= 1; m >>= 1) v = over(v, __shfl_xor(v, m));
+    for (int m = kWave / 2; m >= 1; m >>= 1) v = max2(v, __shfl_xor(v, m));
     return v;
 }
 
@@ -295,7 +303,7 @@ __device__ F block_sum(F v, F* sh) {
 }
 
 // (maximum, sum of exponentials) of a set from those of its parts. A part without probability has sum 0
-// and any maximum.
+// and the lowest maximum.
 struct Soft {
     float top, sum;
 };
@@ -305,28 +313,26 @@ __device__ __forceinline__ Soft block_soft(Soft w, Soft* sh) {
     __syncthreads();
     if ((threadIdx.x & (kWave - 1)) == 0) sh[threadIdx.x / kWave] = w;
     __syncthreads();
-    Soft t{-kInf, 0.0f};
-    for (int i = 0; i < kWaves; ++i) t.top = over(t.top, sh[i].sum != 0.0f ? sh[i].top : -kInf);
-    if (t.top == -kInf) t.top = 0.0f;
-    for (int i = 0; i < kWaves; ++i) t.sum += sh[i].sum != 0.0f ? sh[i].sum * exp_of(sh[i].top - t.top) : 0.0f;
+    Soft t = sh[0];
+    for (int i = 1; i < kWaves; ++i) t.top = fmaxf(t.top, sh[i].top);
+    t.sum = 0.0f;
+    for (int i = 0; i < kWaves; ++i) t.sum += sh[i].sum * exp_of(sh[i].top - t.top);
     return t;
 }
 
 // A wave's from its lanes' (one part each, or none).
 __device__ __forceinline__ Soft wave_soft(Soft l) {
     Soft w;
-    w.top = wave_max(l.sum != 0.0f ? l.top : -kInf);
-    if (w.top == -kInf) w.top = 0.0f;
-    w.sum = wave_sum(l.sum != 0.0f ? l.sum * exp_of(l.top - w.top) : 0.0f);
+    w.top = wave_max(l.top);
+    w.sum = wave_sum(l.sum * exp_of(l.top - w.top));
     return w;
 }
 
 // A lane's from parts first, first + step, ... of a set.
 __device__ __forceinline__ Soft join_parts(const float2* parts, int n, int first, int step) {
-    Soft l{-kInf, 0.0f};
-    for (int j = first; j < n; j += step) l.top = over(l.top, parts[j].y != 0.0f ? parts[j].x : -kInf);
-    if (l.top == -kInf) l.top = 0.0f;
-    for (int j = first; j < n; j += step) l.sum += parts[j].y != 0.0f ? parts[j].y * exp_of(parts[j].x - l.top) : 0.0f;
+    Soft l{kLowest, 0.0f};
+    for (int j = first; j < n; j += step) l.top = fmaxf(l.top, parts[j].x);
+    for (int j = first; j < n; j += step) l.sum += parts[j].y * exp_of(parts[j].x - l.top);
     return l;
 }
 
@@ -364,8 +370,8 @@ __device__ __forceinline__ float lane_move(float v) {  // lanes without a source
 }
 
 struct TakeMax {
-    static constexpr float kNone = -__builtin_huge_valf();
-    static __device__ __forceinline__ float of(float a, float b) { return fmaxf(a, b); }  // passes a NaN over
+    static constexpr float kNone = kLowest;
+    static __device__ __forceinline__ float of(float a, float b) { return max2(a, b); }
 };
 struct TakeSum {
     static constexpr float kNone = 0.0f;
@@ -538,13 +544,12 @@ __global__ __launch_bounds__(kBlock) void part_kernel(ChoiceArgs a, int first) {
         if (threadIdx.x == 0) a.parts[it] = make_float2(0.0f, sum);
         return;
     }
-    float top = -kInf;
+    float top = kLowest;
 #pragma unroll
     for (int j = 0; j < kWideRuns; ++j)
 #pragma unroll
-        for (int k = 0; k < kRun; ++k) top = fmaxf(top, v[j][k]);
+        for (int k = 0; k < kRun; k += 2) top = max3(top, v[j][k], v[j][k + 1]);
     top = wave_max(top);
-    if (top == -kInf) top = 0.0f;
 #pragma unroll
     for (int j = 0; j < kWideRuns; ++j)
 #pragma unroll
@@ -668,8 +673,7 @@ __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, const SetItem& im
         wave_sync();
 #pragma unroll
         for (int k = 0; k < kRun; ++k) {
-            const float t = sh.shift[id[k] - 1];
-            v[k] = exp_of(x[k] - (t == -kInf ? 0.0f : t));
+            v[k] = exp_of(x[k] - sh.shift[id[k] - 1]);
         }
         segment_reduce<TakeSum>(seg, v, id, lane, sh.factor);
         wave_sync();
@@ -688,8 +692,7 @@ __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, const SetItem& im
             if (s < im.sets) {
                 const int64_t g = (int64_t)im.set0 + s;
                 const bool empty = end[r] == begin[r];
-                float top = SOFT ? (empty ? 0.0f : sh.shift[s]) : lse[r];
-                if (SOFT && top == -kInf) top = 0.0f;
+                const float top = SOFT ? (empty ? 0.0f : sh.shift[s]) : lse[r];
                 const float sum = SOFT && !empty ? sh.factor[s] : 0.0f;
                 const float ls = SOFT ? logf(sum) : 0.0f;
                 if (MODE == kRows || MODE == kSteps) a.lse_out[g] = top + ls;
@@ -785,8 +788,19 @@ __device__ __forceinline__ void wide_pass(const ChoiceArgs& a, const SetItem& im
             if (MODE == kRowsBack) load_floats(a, sp, i, a.grad, off[j], d[j]);
         }
     }
+    // what the set has beside its rows, asked for with them
     const float lse = SOFT ? 0.0f : a.lse[g];
+    const int64_t r0 = STEPS ? a.off[g] : 0, size = STEPS ? a.off[g + 1] - r0 : 0;
     const int32_t c = STEPS ? a.chosen[g] : -1;
+    const float given = MODE == kStepsBack ? a.grad[g] : 0.0f;
+    PolicyIn pol{0.0f, 0.0f, 0.0f, 0.0f};
+    if (MODE == kPolicy) pol = load_policy(a, g);
+    bool counts = STEPS && c >= 0 && c < size;
+    float xc = 0.0f;
+    if (STEPS && counts) {
+        if (MASK) counts = a.mask[r0 + c] != 0;
+        if (SOFT) xc = one_logit<TYPE, BIAS>(a, bias, r0 + c);
+    }
     const int live = sp.hi <= kRun * wave0 ? 0 : (sp.hi - kRun * wave0 + kRun * THREADS - 1) / (kRun * THREADS);  // the wave's runs
     Soft t{0.0f, 0.0f};
     float own = 1.0f;  // what the wave's exponentials are relative to, over the set's maximum
@@ -796,14 +810,13 @@ __device__ __forceinline__ void wide_pass(const ChoiceArgs& a, const SetItem& im
             t = block_soft(wave_soft(join_parts(a.parts + (index - im.part), im.parts, tid, THREADS)), shs);
             w.top = t.top;
         } else {
-            w.top = -kInf;
+            w.top = kLowest;
 #pragma unroll
             for (int j = 0; j < kWideRuns; ++j)
                 if (j < live)
 #pragma unroll
-                    for (int k = 0; k < kRun; ++k) w.top = fmaxf(w.top, v[j][k]);
+                    for (int k = 0; k < kRun; k += 2) w.top = max3(w.top, v[j][k], v[j][k + 1]);
             w.top = wave_max(w.top);
-            if (w.top == -kInf) w.top = 0.0f;
         }
         w.sum = 0.0f;
         if (ALONE || im.parts == 1 || GRAD) {
@@ -820,7 +833,7 @@ __device__ __forceinline__ void wide_pass(const ChoiceArgs& a, const SetItem& im
         if (ALONE || im.parts == 1) {
             w.sum = wave_sum(w.sum);
             t = ALONE ? w : block_soft(w, shs);
-            if (GRAD && !ALONE) own = w.sum != 0.0f ? exp_of(w.top - t.top) : 0.0f;
+            if (GRAD && !ALONE) own = exp_of(w.top - t.top);
         }
     }
     const float ls = SOFT ? logf(t.sum) : 0.0f;
@@ -854,16 +867,13 @@ __device__ __forceinline__ void wide_pass(const ChoiceArgs& a, const SetItem& im
     int at = -kRun;  // the chosen row, as the span counts
     float extra = 0.0f;
     if (STEPS) {
-        const int64_t r0 = a.off[g], size = a.off[g + 1] - r0;
-        bool counts = c >= 0 && c < size && (SOFT ? t.sum != 0.0f : lse != -kInf);
-        if (MASK && counts) counts = a.mask[r0 + c] != 0;
-        const float xc = counts ? one_logit<TYPE, BIAS>(a, bias, r0 + c) : 0.0f;
+        counts = counts && (SOFT ? t.sum != 0.0f : lse != -kInf);
         const float lp = SOFT && counts ? (xc - t.top) - ls : 0.0f;
         if (SOFT && first) a.log_probs[g] = lp;
         if (GRAD) {
             float coef = 0.0f;
-            if (MODE == kStepsBack && counts) coef = a.grad[g];
-            if (MODE == kPolicy && counts) coef = policy_step(a, load_policy(a, g), lp, first, tally);
+            if (MODE == kStepsBack && counts) coef = given;
+            if (MODE == kPolicy && counts) coef = policy_step(a, pol, lp, first, tally);
             const float f = counts ? (SOFT ? -coef * __builtin_amdgcn_rcpf(t.sum) : -coef) : 0.0f;
             const float fw = f * own;
             const int64_t row = r0 + c - sp.q0;
@@ -884,22 +894,23 @@ __device__ __forceinline__ void wide_pass(const ChoiceArgs& a, const SetItem& im
     if (MODE == kSteps) return;
 #pragma unroll
     for (int j = 0; j < kWideRuns; ++j) {
-        if (j >= live) break;
-        const int i = kRun * (j * THREADS + tid);
-        if (MODE == kRows) {
-            if (i < sp.hi) store_run<PB_F32>(a, sp, i, a.log_probs, v[j]);
-        } else {
-            if (off[j]) {
+        if (j < live) {
+            const int i = kRun * (j * THREADS + tid);
+            if (MODE == kRows) {
+                if (i < sp.hi) store_run<PB_F32>(a, sp, i, a.log_probs, v[j]);
+            } else {
+                if (off[j]) {
 #pragma unroll
-                for (int k = 0; k < kRun; ++k) v[j][k] = off[j] >> k & 1u ? 0.0f : v[j][k];
-            }
-            if (STEPS && at >= i && at < i + kRun) {
+                    for (int k = 0; k < kRun; ++k) v[j][k] = off[j] >> k & 1u ? 0.0f : v[j][k];
+                }
+                if (STEPS && at >= i && at < i + kRun) {
 #pragma unroll
-                for (int k = 0; k < kRun; ++k)
-                    if (at - i == k) v[j][k] += extra;
+                    for (int k = 0; k < kRun; ++k)
+                        if (at - i == k) v[j][k] += extra;
+                }
+                if (i < sp.hi) store_run<TYPE>(a, sp, i, a.grad_scores, v[j]);
+                if (BIAS) table.add(v[j], buckets[j]);
             }
-            if (i < sp.hi) store_run<TYPE>(a, sp, i, a.grad_scores, v[j]);
-            if (BIAS) table.add(v[j], buckets[j]);
         }
     }
 }
@@ -973,9 +984,13 @@ __device__ __forceinline__ void leave_sums(const ChoiceArgs& a, int block, doubl
 template <int MODE, bool BIAS>
 constexpr bool kTable = BIAS && (MODE == kRowsBack || MODE == kStepsBack || MODE == kPolicy);
 
+// Waves per SIMD that a kernel's registers leave room for: as many as go without spilling.
+template <int MODE, bool BIAS>
+constexpr int kTileWaves = MODE == kPolicy ? 4 : 5;
+
 // The tiles, one a wave at a time.
 template <int MODE, int TYPE, bool MASK, bool BIAS>
-__global__ __launch_bounds__(kBlock) void tile_kernel(ChoiceArgs a) {
+__global__ __launch_bounds__(kBlock, (kTileWaves<MODE, BIAS>)) void tile_kernel(ChoiceArgs a) {
     constexpr bool TABLE = kTable<MODE, BIAS>;
     __shared__ TileShared tiles[kWaves];
     __shared__ BiasShared bias;
@@ -1034,7 +1049,16 @@ __global__ __launch_bounds__(kBlock) void join_kernel(const double* __restrict__
     __shared__ double sh[kWaves];
     const int j = (int)blockIdx.x;
     double t = 0.0;
-    for (int i = (int)threadIdx.x; i < n; i += kBlock) t += sums[(int64_t)i * cols + j];
+    for (int i0 = 0; i0 < n; i0 += kBlock * kJoin) {  // kJoin loads in flight
+        double v[kJoin];
+#pragma unroll
+        for (int k = 0; k < kJoin; ++k) {
+            const int i = i0 + k * kBlock + (int)threadIdx.x;
+            v[k] = i < n ? sums[(int64_t)i * cols + j] : 0.0;
+        }
+#pragma unroll
+        for (int k = 0; k < kJoin; ++k) t += v[k];
+    }
     t = block_sum(t, sh);
     if (threadIdx.x == 0) (j < head ? stats[j] : table[j - head]) = (float)t;
 }
@@ -1070,7 +1094,7 @@ __device__ void join_loss(const SumArgs& a, double* sh) {
 template <bool PAIRS>
 __device__ __forceinline__ double sum_term(const SumArgs& a, int64_t i) {
     if (PAIRS) {
-        const int32_t e = a.entries[i];
+        const int32_t e = __builtin_nontemporal_load(a.entries + i);
         const float c = a.slopes[e >> 1];
         return (double)(e & 1 ? -c : c);
     }
@@ -1148,14 +1172,22 @@ __global__ __launch_bounds__(kBlock) void pair_kernel(PairArgs a) {
 #pragma unroll
         for (int k = 0; k < kPairs; ++k) {  // past the end: the last pair again, unused
             const int64_t p = min(p0 + k * stride, a.num_pairs - 1);
-            w[k] = a.winners[p];
-            l[k] = a.losers[p];
-            weight[k] = a.weights ? a.weights[p] : 1.0f;
+            w[k] = __builtin_nontemporal_load(a.winners + p);
+            l[k] = __builtin_nontemporal_load(a.losers + p);
+            weight[k] = a.weights ? __builtin_nontemporal_load(a.weights + p) : 1.0f;
         }
+        if (a.both) {
 #pragma unroll
-        for (int k = 0; k < kPairs; ++k) {
-            d[k] = (double)a.values[w[k]] - (double)a.values[l[k]];
-            if (a.ref) d[k] -= (double)a.ref[w[k]] - (double)a.ref[l[k]];
+            for (int k = 0; k < kPairs; ++k) {
+                const float2 t = a.both[w[k]], u = a.both[l[k]];
+                d[k] = ((double)t.x - (double)u.x) - ((double)t.y - (double)u.y);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < kPairs; ++k) {
+                d[k] = (double)a.values[w[k]] - (double)a.values[l[k]];
+                if (a.ref) d[k] -= (double)a.ref[w[k]] - (double)a.ref[l[k]];
+            }
         }
 #pragma unroll
         for (int k = 0; k < kPairs; ++k) {
@@ -1167,7 +1199,7 @@ __global__ __launch_bounds__(kBlock) void pair_kernel(PairArgs a) {
             const float e = a.smoothing;
             const float up = z > 0.0f ? 1.0f / (1.0f + t) : t / (1.0f + t);    // sigmoid(z)
             const float down = z > 0.0f ? t / (1.0f + t) : 1.0f / (1.0f + t);  // sigmoid(-z)
-            a.margins[p] = z;
+            __builtin_nontemporal_store(z, a.margins + p);
             a.slopes[p] = a.beta * ws * (e * up - (1.0f - e) * down);
             sum += (double)(ws * ((1.0f - e) * (soft + fmaxf(-z, 0.0f)) + e * (soft + fmaxf(z, 0.0f))));
         }
@@ -1179,6 +1211,13 @@ __global__ __launch_bounds__(kBlock) void pair_kernel(PairArgs a) {
         else
             a.sums[blockIdx.x] = sum;
     }
+}
+
+// Values beside their references, so that a pair finds both in one access.
+__global__ __launch_bounds__(kBlock) void both_kernel(const float* __restrict__ values, const float* __restrict__ ref,
+                                                      int64_t n, float2* __restrict__ both) {
+    const int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+    if (i < n) both[i] = make_float2(values[i], ref[i]);
 }
 
 // The pairs' slopes summed over a sequence's list (a team of L lanes, this one `sub`).
@@ -1358,6 +1397,14 @@ hipError_t launch_preference(const PairLayout& p, PairArgs a, const float* value
     } else {
         a.values = values;
         a.ref = ref;
+        if (ref && p.lists.num_sets >= kBothFrom) {
+            float2* both = reinterpret_cast<float2*>(parts + long_items(p.lists));
+            a.slopes = reinterpret_cast<float*>(both + p.lists.num_sets);
+            a.both = both;
+            hipLaunchKernelGGL(both_kernel, dim3((unsigned)((p.lists.num_sets + kBlock - 1) / kBlock)), dim3(kBlock), 0, stream,
+                               values, ref, p.lists.num_sets, both);
+            if ((e = hipGetLastError()) != hipSuccess) return e;
+        }
     }
     const int64_t want = (p.num_pairs + kBlock - 1) / kBlock;
     const int grid = (int)(want < 1 ? 1 : want > kPairGrid ? kPairGrid : want);
@@ -1393,7 +1440,8 @@ hipError_t launch_preference(const PairLayout& p, PairArgs a, const float* value
 }
 
 int64_t preference_work_bytes(const PairLayout& p) {
-    return 8 * ((int64_t)kPairGrid + long_items(p.lists) + long_items(p.seqs)) + 4 * (p.num_pairs + 2 * p.seqs.num_sets);
+    return 8 * ((int64_t)kPairGrid + long_items(p.lists) + long_items(p.seqs)) + 4 * (p.num_pairs + 2 * p.seqs.num_sets) +
+           (!p.has_seqs && p.lists.num_sets >= kBothFrom ? 8 * p.lists.num_sets : 0);
 }
 
 }  // namespace pb

@@ -498,6 +498,11 @@ hipError_t launch_predict_bins(const uint8_t* bins, int64_t N, int64_t ld, int32
 constexpr int kSetTileRows = 512;
 constexpr int kSetTileSets = 128;
 constexpr int kSetShort = kSetTileRows - 8;
+// Where at least kSetMany sets have more than kSetLean rows, those up to kSetShort go to a wave each as well:
+// it spends about 300 vector instructions on one, a tile about 700 on 512 rows. Fewer are not worth the
+// launch (100k sets of up to 40k rows: 43 + 60 us so, 55 + 51 in tiles; a launch takes 4 to 6 us).
+constexpr int kSetLean = 256;
+constexpr int kSetMany = 4096;
 constexpr int kSetMidRows = 2048;
 constexpr int kSetWideRows = 8192;
 struct SetItem {
@@ -577,6 +582,7 @@ struct PairArgs {
     int64_t num_pairs;
     const float* values;
     const float* ref;
+    const float2* both;  // values and references side by side, or NULL
     const float* weights;
     float beta, smoothing, scale;
     float* margins;
