@@ -26,7 +26,6 @@ constexpr float kLowest = -3.402823466e38f;
 constexpr int kRun = 8;                                     // consecutive rows of a lane
 constexpr int kWideRuns = kSetWideRows / (kRun * kBlock);   // runs of a thread of a longer set
 constexpr int kTileRounds = kSetTileSets / kWave;           // sets of a tile per lane
-constexpr int kTileAhead = 2;                               // and of those, asked for with the rows
 // Values from which on they are laid beside their references first: two arrays of them pass a quarter of an
 // XCD's 4 MB L2, and every pair's four reads miss it more and more.
 constexpr int64_t kBothFrom = 1 << 17;
@@ -40,6 +39,9 @@ static_assert(kSetTileRows == kRun * kWave, "a lane holds one run of a tile");
 // and log2(e)'s own move the result by at most |x| 2^-23 of itself, as a unit in the last place of x does.
 // Results below 2^-126 are 0; e^-inf is 0 and NaN stays NaN.
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * 1.44269502162933349609375f); }
+
+// log x for x = 0 or above 1/2: 0 gives -inf, NaN stays NaN.
+__device__ __forceinline__ float log_of(float x) { return __builtin_amdgcn_logf(x) * 0.69314718055994530942f; }
 
 // Maxima that pass a NaN over (fmaxf first quiets operands that the compiler cannot see through).
 __device__ __forceinline__ float max2(float a, float b) {
@@ -129,22 +131,6 @@ __device__ __forceinline__ void put_row(float (&x)[kRun], int k, float v) {
     for (int j = 0; j < kRun; ++j) x[j] = j == k ? v : x[j];
 }
 
-template <int TYPE>
-__device__ __forceinline__ void load_scores(const ChoiceArgs& a, const Span& s, int i, float (&x)[kRun]) {
-    if (TYPE == PB_F32) {
-        const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(a.scores) + s.q0 + i);
-        const float4 t = p[0], u = p[1];
-        x[0] = t.x, x[1] = t.y, x[2] = t.z, x[3] = t.w;
-        x[4] = u.x, x[5] = u.y, x[6] = u.z, x[7] = u.w;
-    } else {
-        const uint4 t = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.scores) + s.q0 + i);
-        x[0] = half_value<TYPE>(t.x & 0xffffu), x[1] = half_value<TYPE>(t.x >> 16);
-        x[2] = half_value<TYPE>(t.y & 0xffffu), x[3] = half_value<TYPE>(t.y >> 16);
-        x[4] = half_value<TYPE>(t.z & 0xffffu), x[5] = half_value<TYPE>(t.z >> 16);
-        x[6] = half_value<TYPE>(t.w & 0xffffu), x[7] = half_value<TYPE>(t.w >> 16);
-    }
-}
-
 // A run of the rows' gradients, 0 where `off` has a bit.
 __device__ __forceinline__ void load_floats(const ChoiceArgs& a, const Span& s, int i, const float* p, uint32_t off,
                                             float (&x)[kRun]) {
@@ -211,56 +197,90 @@ struct Buckets {
     __device__ __forceinline__ int at(int k) const { return (int)(w[k >> 2] >> (8 * (k & 3)) & 0xffu); }
 };
 
-// A run's logits: -inf where `off` has a bit, outside [lo, hi) and where masked.
+// A run as it lies in memory, asked for but not waited for; nothing where it goes row by row.
+template <int TYPE, bool MASK, bool BIAS>
+struct RawRun {
+    uint4 score[TYPE == PB_F32 ? 2 : 1];
+    uint2 mask;
+    int4 pos[2];
+
+    __device__ __forceinline__ void load(const ChoiceArgs& a, const Span& s, int i) {
+        if (!whole_run(a, s, i)) return;
+        if (TYPE == PB_F32) {
+            const uint4* p = reinterpret_cast<const uint4*>(static_cast<const float*>(a.scores) + s.q0 + i);
+            score[0] = p[0];
+            score[TYPE == PB_F32 ? 1 : 0] = p[1];
+        } else {
+            score[0] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.scores) + s.q0 + i);
+        }
+        if (MASK) mask = *reinterpret_cast<const uint2*>(a.mask + s.q0 + i);
+        if (BIAS) {
+            const int4* p = reinterpret_cast<const int4*>(a.positions + s.q0 + i);
+            pos[0] = p[0];
+            pos[1] = p[1];
+        }
+    }
+
+    // the logits: -inf where `off` has a bit, outside [lo, hi) and where masked
+    __device__ __forceinline__ void logits(const ChoiceArgs& a, const BiasShared* bias, const Span& s, int i,
+                                           float (&x)[kRun], uint32_t& off, Buckets& buckets) const {
+        off = outside(s, i);
+        buckets.w[0] = buckets.w[1] = 0;
+        if (whole_run(a, s, i)) {
+            const uint32_t w[8] = {score[0].x, score[0].y, score[0].z, score[0].w, score[TYPE == PB_F32 ? 1 : 0].x,
+                                   score[TYPE == PB_F32 ? 1 : 0].y, score[TYPE == PB_F32 ? 1 : 0].z,
+                                   score[TYPE == PB_F32 ? 1 : 0].w};
+#pragma unroll
+            for (int k = 0; k < kRun; ++k)
+                x[k] = TYPE == PB_F32 ? __uint_as_float(w[k]) : half_value<TYPE>(k & 1 ? w[k >> 1] >> 16 : w[k >> 1] & 0xffffu);
+            if (MASK) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    off |= (mask.x >> (8 * k) & 0xffu) == 0 ? 1u << k : 0u;
+                    off |= (mask.y >> (8 * k) & 0xffu) == 0 ? 16u << k : 0u;
+                }
+            }
+            if (BIAS) {
+                const int32_t q[kRun] = {pos[0].x, pos[0].y, pos[0].z, pos[0].w, pos[1].x, pos[1].y, pos[1].z, pos[1].w};
+#pragma unroll
+                for (int k = 0; k < kRun; ++k) {
+                    const uint32_t b = bucket_of(a, *bias, q[k]);
+                    buckets.w[k >> 2] |= b << (8 * (k & 3));
+                    x[k] += bias->table[b];
+                }
+            }
+        } else {
+            const uint32_t out = off;
+#pragma unroll 1
+            for (int k = 0; k < kRun; ++k) {
+                if (out >> k & 1u) continue;
+                const int64_t row = s.q0 + i + k;
+                float v = load_score<TYPE>(a.scores, row * a.stride);
+                if (BIAS) {
+                    const uint32_t b = bucket_of(a, *bias, a.positions[row]);
+                    if (k < 4)
+                        buckets.w[0] |= b << (8 * k);
+                    else
+                        buckets.w[1] |= b << (8 * (k - 4));
+                    v += bias->table[b];
+                }
+                if (MASK && !a.mask[row]) off |= 1u << k;
+                put_row(x, k, v);
+            }
+        }
+        if (off) {
+#pragma unroll
+            for (int k = 0; k < kRun; ++k) x[k] = off >> k & 1u ? -kInf : x[k];
+        }
+    }
+};
+
 template <int TYPE, bool MASK, bool BIAS>
 __device__ __forceinline__ void load_logits(const ChoiceArgs& a, const BiasShared* bias, const Span& s, int i,
                                             float (&x)[kRun], uint32_t& off, Buckets& buckets) {
-    off = outside(s, i);
-    buckets.w[0] = buckets.w[1] = 0;
-    if (whole_run(a, s, i)) {
-        load_scores<TYPE>(a, s, i, x);
-        if (MASK) {
-            const uint2 m = *reinterpret_cast<const uint2*>(a.mask + s.q0 + i);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                off |= (m.x >> (8 * k) & 0xffu) == 0 ? 1u << k : 0u;
-                off |= (m.y >> (8 * k) & 0xffu) == 0 ? 16u << k : 0u;
-            }
-        }
-        if (BIAS) {
-            const int4* p = reinterpret_cast<const int4*>(a.positions + s.q0 + i);
-            const int4 t = p[0], u = p[1];
-            const int32_t pos[kRun] = {t.x, t.y, t.z, t.w, u.x, u.y, u.z, u.w};
-#pragma unroll
-            for (int k = 0; k < kRun; ++k) {
-                const uint32_t b = bucket_of(a, *bias, pos[k]);
-                buckets.w[k >> 2] |= b << (8 * (k & 3));
-                x[k] += bias->table[b];
-            }
-        }
-    } else {
-        const uint32_t out = off;
-#pragma unroll 1
-        for (int k = 0; k < kRun; ++k) {
-            if (out >> k & 1u) continue;
-            const int64_t row = s.q0 + i + k;
-            float v = load_score<TYPE>(a.scores, row * a.stride);
-            if (BIAS) {
-                const uint32_t b = bucket_of(a, *bias, a.positions[row]);
-                if (k < 4)
-                    buckets.w[0] |= b << (8 * k);
-                else
-                    buckets.w[1] |= b << (8 * (k - 4));
-                v += bias->table[b];
-            }
-            if (MASK && !a.mask[row]) off |= 1u << k;
-            put_row(x, k, v);
-        }
-    }
-    if (off) {
-#pragma unroll
-        for (int k = 0; k < kRun; ++k) x[k] = off >> k & 1u ? -kInf : x[k];
-    }
+    RawRun<TYPE, MASK, BIAS> raw;
+    raw.load(a, s, i);
+    raw.logits(a, bias, s, i, x, off, buckets);
 }
 
 // One logit.
@@ -331,8 +351,12 @@ __device__ __forceinline__ Soft wave_soft(Soft l) {
 // A lane's from parts first, first + step, ... of a set.
 __device__ __forceinline__ Soft join_parts(const float2* parts, int n, int first, int step) {
     Soft l{kLowest, 0.0f};
-    for (int j = first; j < n; j += step) l.top = fmaxf(l.top, parts[j].x);
-    for (int j = first; j < n; j += step) l.sum += parts[j].y * exp_of(parts[j].x - l.top);
+    for (int j = first; j < n; j += step) {
+        const float2 p = parts[j];
+        const float top = fmaxf(l.top, p.x);
+        l.sum = l.sum * exp_of(l.top - top) + p.y * exp_of(p.x - top);
+        l.top = top;
+    }
     return l;
 }
 
@@ -414,14 +438,14 @@ __device__ __forceinline__ PolicyIn load_policy(const ChoiceArgs& a, int64_t g) 
 
 __device__ __forceinline__ float policy_step(const ChoiceArgs& a, const PolicyIn& in, float lp, bool tally, double (&sum)[3]) {
     const float w = in.w * a.scale;
-    const float ratio = expf(lp - in.old);
+    const float ratio = exp_of(lp - in.old);
     const float free = ratio * in.adv;
     const float held = fminf(fmaxf(ratio, a.ratio_min), a.ratio_max) * in.adv;
     const bool clipped = free > held;
     float kl = 0.0f, slope = clipped ? 0.0f : -free;
     if (a.ref) {
         const float d = in.ref - lp;
-        const float e = expf(d);
+        const float e = exp_of(d);
         kl = e - d - 1.0f;
         slope += a.kl_weight * (1.0f - e);
     }
@@ -580,68 +604,86 @@ __device__ __forceinline__ void read_run(const float* p, float (&x)[kRun]) {
     x[4] = u.x, x[5] = u.y, x[6] = u.z, x[7] = u.w;
 }
 
+// What a tile reads, all of it asked for before anything is waited for: a lane's run, and the lane's sets.
+template <int MODE, int TYPE, bool MASK, bool BIAS>
+struct TileIn {
+    Span sp;
+    int set0, sets;
+    RawRun<TYPE, MASK, BIAS> raw;
+    int32_t begin[kTileRounds], chosen[kTileRounds];
+    float given[kTileRounds], lse[kTileRounds];
+    PolicyIn pol[kTileRounds];
+
+    __device__ __forceinline__ void load(const ChoiceArgs& a, const SetItem& im, int lane) {
+        sp = span_of(a, im);
+        set0 = im.set0;
+        sets = im.sets;
+        if (kRun * lane < sp.hi) raw.load(a, sp, kRun * lane);
+#pragma unroll
+        for (int r = 0; r < kTileRounds; ++r) {
+            const int s = r * kWave + lane;
+            const int64_t g = (int64_t)set0 + s;
+            chosen[r] = -1;
+            given[r] = lse[r] = 0.0f;
+            if (s < sets) {
+                begin[r] = (int)(a.off[g] - sp.q0);
+                if (MODE != kRows && MODE != kRowsBack) chosen[r] = a.chosen[g];
+                if (MODE == kStepsBack) given[r] = a.grad[g];
+                if (MODE == kStepsBack || MODE == kRowsBack) lse[r] = a.lse[g];
+                if (MODE == kPolicy) pol[r] = load_policy(a, g);
+            }
+        }
+    }
+};
+
 // One tile of short sets by one wave.
 template <int MODE, int TYPE, bool MASK, bool BIAS>
-__device__ __forceinline__ void tile_pass(const ChoiceArgs& a, const SetItem& im, TileShared& sh, const BiasShared* bias,
-                                          TableSum& table, double (&tally)[3]) {
+__device__ __forceinline__ void tile_pass(const ChoiceArgs& a, TileIn<MODE, TYPE, MASK, BIAS>& in, TileShared& sh,
+                                          const BiasShared* bias, TableSum& table, double (&tally)[3]) {
     constexpr bool GRAD = MODE == kRowsBack || MODE == kStepsBack || MODE == kPolicy;
     constexpr bool STEPS = MODE != kRows && MODE != kRowsBack;
     constexpr bool SOFT = MODE == kRows || MODE == kSteps || MODE == kPolicy;
     const int lane = (int)threadIdx.x & (kWave - 1);
-    const Span sp = span_of(a, im);
+    const Span sp = in.sp;
     const int i0 = kRun * lane;
-    // everything the tile reads is asked for before anything is waited for
     float x[kRun], d[kRun];
     uint32_t off = 0xffu;
     Buckets buckets{{0, 0}};
 #pragma unroll
     for (int k = 0; k < kRun; ++k) x[k] = -kInf, d[k] = 0.0f;
     if (i0 < sp.hi) {
-        load_logits<TYPE, MASK, BIAS>(a, bias, sp, i0, x, off, buckets);
+        in.raw.logits(a, bias, sp, i0, x, off, buckets);
         if (MODE == kRowsBack) load_floats(a, sp, i0, a.grad, off, d);
     }
-    int32_t begin[kTileRounds], chosen[kTileRounds];
-    float given[kTileRounds], lse[kTileRounds];
-    PolicyIn pol[kTileAhead];
-#pragma unroll
-    for (int r = 0; r < kTileRounds; ++r) {
-        const int s = r * kWave + lane;
-        const int64_t g = (int64_t)im.set0 + s;
-        chosen[r] = -1;
-        given[r] = lse[r] = 0.0f;
-        if (s < im.sets) {
-            begin[r] = (int)(a.off[g] - sp.q0);
-            if (STEPS) chosen[r] = a.chosen[g];
-            if (MODE == kStepsBack) given[r] = a.grad[g];
-            if (!SOFT) lse[r] = a.lse[g];
-            if (MODE == kPolicy && r < kTileAhead) pol[r < kTileAhead ? r : 0] = load_policy(a, g);
-        }
-    }
+    int32_t (&begin)[kTileRounds] = in.begin;
+    int32_t (&chosen)[kTileRounds] = in.chosen;
     wave_sync();  // the last tile's values have been read
     *reinterpret_cast<uint4*>(&sh.head[i0]) = make_uint4(0, 0, 0, 0);
     if (STEPS) write_run(&sh.x[i0], x);
 #pragma unroll
     for (int r = 0; r < kTileRounds; ++r) {
         const int s = r * kWave + lane;
-        if (s < im.sets) {
+        if (s < in.sets) {
             sh.begin[s] = (uint16_t)begin[r];
-            if (!SOFT) sh.shift[s] = lse[r];
+            if (!SOFT) sh.shift[s] = in.lse[r];
         }
     }
-    if (lane == 0) sh.begin[im.sets] = (uint16_t)sp.hi;
+    if (lane == 0) sh.begin[in.sets] = (uint16_t)sp.hi;
     wave_sync();
-    // which set each row is of, and the chosen rows' logits (a choice outside its set is none)
+    // which set each row is of, and the chosen rows' logits (a choice outside its set or masked is none)
     int end[kTileRounds];
     float picked[kTileRounds];
 #pragma unroll
     for (int r = 0; r < kTileRounds; ++r) {
         const int s = r * kWave + lane;
-        if (s < im.sets) {
+        if (s < in.sets) {
             end[r] = sh.begin[s + 1];
             if (end[r] > begin[r]) sh.head[begin[r]] = (uint16_t)(s + 1);
             if (STEPS) {
                 if (chosen[r] >= end[r] - begin[r]) chosen[r] = -1;
                 picked[r] = chosen[r] >= 0 ? sh.x[begin[r] + chosen[r]] : -kInf;
+                // a masked row's logit is -inf, as one of that score is: the mask says which
+                if (MASK && chosen[r] >= 0 && picked[r] == -kInf && !a.mask[sp.q0 + begin[r] + chosen[r]]) chosen[r] = -1;
             }
         }
     }
@@ -689,27 +731,24 @@ __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, const SetItem& im
         for (int r = 0; r < kTileRounds; ++r) {
             const int s = r * kWave + lane;
             coef[r] = 0.0f;
-            if (s < im.sets) {
-                const int64_t g = (int64_t)im.set0 + s;
+            if (s < in.sets) {
+                const int64_t g = (int64_t)in.set0 + s;
                 const bool empty = end[r] == begin[r];
-                const float top = SOFT ? (empty ? 0.0f : sh.shift[s]) : lse[r];
+                const float top = SOFT ? (empty ? 0.0f : sh.shift[s]) : in.lse[r];
                 const float sum = SOFT && !empty ? sh.factor[s] : 0.0f;
-                const float ls = SOFT ? logf(sum) : 0.0f;
+                const float ls = SOFT ? log_of(sum) : 0.0f;
                 if (MODE == kRows || MODE == kSteps) a.lse_out[g] = top + ls;
                 if (MODE == kRows) {
                     sh.shift[s] = top;
                     sh.factor[s] = ls;
                 }
                 if (STEPS) {
-                    // left out: a choice outside the set or masked, a set without probability. A masked row's
-                    // logit is -inf, as one of that score is: the mask says which.
-                    bool counts = chosen[r] >= 0 && (SOFT ? sum != 0.0f : top != -kInf);
-                    if (MASK && counts && picked[r] == -kInf) counts = a.mask[sp.q0 + begin[r] + chosen[r]] != 0;
+                    // left out: a choice outside the set or masked, a set without probability
+                    const bool counts = chosen[r] >= 0 && (SOFT ? sum != 0.0f : top != -kInf);
                     const float lp = SOFT && counts ? (picked[r] - top) - ls : 0.0f;
                     if (SOFT) a.log_probs[g] = lp;
-                    if (MODE == kStepsBack && counts) coef[r] = given[r];
-                    if (MODE == kPolicy && counts) 
-                        coef[r] = policy_step(a, r < kTileAhead ? pol[r < kTileAhead ? r : 0] : load_policy(a, g), lp, true, tally);
+                    if (MODE == kStepsBack && counts) coef[r] = in.given[r];
+                    if (MODE == kPolicy && counts) coef[r] = policy_step(a, in.pol[r], lp, true, tally);
                     if (GRAD) sh.factor[s] = counts ? (SOFT ? -coef[r] * __builtin_amdgcn_rcpf(sum) : -coef[r]) : 0.0f;
                     if (!counts) chosen[r] = -1;
                 }
@@ -723,7 +762,7 @@ __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, const SetItem& im
         wave_sync();
 #pragma unroll
         for (int r = 0; r < kTileRounds; ++r)
-            if (r * kWave + lane < im.sets && chosen[r] >= 0) sh.x[begin[r] + chosen[r]] = coef[r];
+            if (r * kWave + lane < in.sets && chosen[r] >= 0) sh.x[begin[r] + chosen[r]] = coef[r];
     }
     wave_sync();
     if (MODE == kRows) {
@@ -773,20 +812,14 @@ __device__ __forceinline__ void wide_pass(const ChoiceArgs& a, const SetItem& im
     const Span sp = span_of(a, im);
     const int64_t g = im.set0;
     const bool first = im.part == 0 && tid == 0;
-    float v[kWideRuns][kRun], d[kWideRuns][kRun];
-    uint32_t off[kWideRuns];
-    Buckets buckets[kWideRuns];
+    // the parts' sums first, then the rows: the ones are joined while the others are on their way
+    Soft joined{kLowest, 0.0f};
+    if (SOFT && !ALONE && im.parts > 1) joined = join_parts(a.parts + (index - im.part), im.parts, tid, THREADS);
+    RawRun<TYPE, MASK, BIAS> raw[kWideRuns];
 #pragma unroll
     for (int j = 0; j < kWideRuns; ++j) {
         const int i = kRun * (j * THREADS + tid);
-        off[j] = 0xffu;
-        buckets[j].w[0] = buckets[j].w[1] = 0;
-#pragma unroll
-        for (int k = 0; k < kRun; ++k) v[j][k] = -kInf, d[j][k] = 0.0f;
-        if (kRun * (j * THREADS + wave0) < sp.hi && i < sp.hi) {
-            load_logits<TYPE, MASK, BIAS>(a, bias, sp, i, v[j], off[j], buckets[j]);
-            if (MODE == kRowsBack) load_floats(a, sp, i, a.grad, off[j], d[j]);
-        }
+        if (kRun * (j * THREADS + wave0) < sp.hi && i < sp.hi) raw[j].load(a, sp, i);
     }
     // what the set has beside its rows, asked for with them
     const float lse = SOFT ? 0.0f : a.lse[g];
@@ -801,13 +834,28 @@ __device__ __forceinline__ void wide_pass(const ChoiceArgs& a, const SetItem& im
         if (MASK) counts = a.mask[r0 + c] != 0;
         if (SOFT) xc = one_logit<TYPE, BIAS>(a, bias, r0 + c);
     }
-    const int live = sp.hi <= kRun * wave0 ? 0 : (sp.hi - kRun * wave0 + kRun * THREADS - 1) / (kRun * THREADS);  // the wave's runs
     Soft t{0.0f, 0.0f};
+    if (SOFT && !ALONE && im.parts > 1) t = block_soft(wave_soft(joined), shs);
+    float v[kWideRuns][kRun], d[kWideRuns][kRun];
+    uint32_t off[kWideRuns];
+    Buckets buckets[kWideRuns];
+#pragma unroll
+    for (int j = 0; j < kWideRuns; ++j) {
+        const int i = kRun * (j * THREADS + tid);
+        off[j] = 0xffu;
+        buckets[j].w[0] = buckets[j].w[1] = 0;
+#pragma unroll
+        for (int k = 0; k < kRun; ++k) v[j][k] = -kInf, d[j][k] = 0.0f;
+        if (kRun * (j * THREADS + wave0) < sp.hi && i < sp.hi) {
+            raw[j].logits(a, bias, sp, i, v[j], off[j], buckets[j]);
+            if (MODE == kRowsBack) load_floats(a, sp, i, a.grad, off[j], d[j]);
+        }
+    }
+    const int live = sp.hi <= kRun * wave0 ? 0 : (sp.hi - kRun * wave0 + kRun * THREADS - 1) / (kRun * THREADS);  // the wave's runs
     float own = 1.0f;  // what the wave's exponentials are relative to, over the set's maximum
     if (SOFT) {
         Soft w;
         if (!ALONE && im.parts > 1) {
-            t = block_soft(wave_soft(join_parts(a.parts + (index - im.part), im.parts, tid, THREADS)), shs);
             w.top = t.top;
         } else {
             w.top = kLowest;
@@ -836,7 +884,7 @@ __device__ __forceinline__ void wide_pass(const ChoiceArgs& a, const SetItem& im
             if (GRAD && !ALONE) own = exp_of(w.top - t.top);
         }
     }
-    const float ls = SOFT ? logf(t.sum) : 0.0f;
+    const float ls = SOFT ? log_of(t.sum) : 0.0f;
     if ((MODE == kRows || MODE == kSteps) && first) a.lse_out[g] = t.top + ls;
     if (MODE == kRows) {
 #pragma unroll
@@ -928,7 +976,7 @@ __global__ __launch_bounds__(kBlock) void split_steps_kernel(ChoiceArgs a, const
     const Soft t = wave_soft(join_parts(a.parts + firsts[k], im.parts, lane, kWave));
     bool counts = c >= 0 && c < size && t.sum != 0.0f;
     if (MASK && counts) counts = a.mask[r0 + c] != 0;
-    const float ls = logf(t.sum);
+    const float ls = log_of(t.sum);
     if (lane == 0) {
         a.lse_out[g] = t.top + ls;
         a.log_probs[g] = counts ? (one_logit<TYPE, BIAS>(a, &bias, r0 + c) - t.top) - ls : 0.0f;
@@ -940,20 +988,26 @@ __global__ __launch_bounds__(kBlock) void split_steps_kernel(ChoiceArgs a, const
 template <int MODE, bool TABLE>
 __device__ __forceinline__ void leave_sums(const ChoiceArgs& a, int block, double (&tally)[3], TableSum& table,
                                            unsigned long long (*bins)[kBins], const int* bad, double* shd) {
-    const int tid = (int)threadIdx.x, wave = tid / kWave, lane = tid & (kWave - 1);
+    const int tid = (int)threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid & (kWave - 1);
     const int head = MODE == kPolicy ? 3 : 0;
     const int cols = head + (TABLE ? a.num_buckets : 0);
     double* mine = a.sums + (int64_t)block * cols;
     if (MODE == kPolicy) {
 #pragma unroll
-        for (int j = 0; j < 3; ++j) {
-            const double t = block_sum(tally[j], shd);
-            if (tid == 0) {
-                if (a.blocks == 1)
-                    a.stats[j] = (float)t;
-                else
-                    mine[j] = t;
-            }
+        for (int m = kWave / 2; m >= 1; m >>= 1)
+#pragma unroll
+            for (int j = 0; j < 3; ++j) tally[j] += __shfl_xor(tally[j], m);
+        if (lane == 0)
+#pragma unroll
+            for (int j = 0; j < 3; ++j) shd[wave * 3 + j] = tally[j];
+        __syncthreads();
+        if (tid < 3) {
+            double t = shd[tid];
+            for (int w = 1; w < kWaves; ++w) t += shd[w * 3 + tid];
+            if (a.blocks == 1)
+                a.stats[tid] = (float)t;
+            else
+                mine[tid] = t;
         }
     }
     if (TABLE) {
@@ -984,30 +1038,37 @@ __device__ __forceinline__ void leave_sums(const ChoiceArgs& a, int block, doubl
 template <int MODE, bool BIAS>
 constexpr bool kTable = BIAS && (MODE == kRowsBack || MODE == kStepsBack || MODE == kPolicy);
 
-// Waves per SIMD that a kernel's registers leave room for: as many as go without spilling.
-template <int MODE, bool BIAS>
-constexpr int kTileWaves = MODE == kPolicy ? 4 : 5;
-
 // The tiles, one a wave at a time.
 template <int MODE, int TYPE, bool MASK, bool BIAS>
-__global__ __launch_bounds__(kBlock, (kTileWaves<MODE, BIAS>)) void tile_kernel(ChoiceArgs a) {
+__global__ __launch_bounds__(kBlock, 4) void tile_kernel(ChoiceArgs a) {
     constexpr bool TABLE = kTable<MODE, BIAS>;
     __shared__ TileShared tiles[kWaves];
     __shared__ BiasShared bias;
     __shared__ unsigned long long bins[TABLE ? kWaves : 1][kBins];
     __shared__ int bad[kMaxBuckets];
-    __shared__ double shd[kWaves];
-    const int tid = (int)threadIdx.x, wave = tid / kWave;
+    __shared__ double shd[kWaves * 3];
+    const int tid = (int)threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     TableSum table;
     if (TABLE) {
         for (int b = tid; b < kMaxBuckets; b += kBlock) bad[b] = 0;
         table.start(a, bins[wave], bad);
     }
-    if (BIAS) stage_bias(a, bias);
     double tally[3] = {0.0, 0.0, 0.0};
-    for (int it = __builtin_amdgcn_readfirstlane((int)blockIdx.x * kWaves + wave); it < a.num_tiles;
-         it += (int)gridDim.x * kWaves)
-        tile_pass<MODE, TYPE, MASK, BIAS>(a, a.tiles[it], tiles[wave], &bias, table, tally);
+    const int lane = tid & (kWave - 1), step = (int)gridDim.x * kWaves;
+    int it = __builtin_amdgcn_readfirstlane((int)blockIdx.x * kWaves + wave);
+    SetItem next = a.tiles[min(it, a.num_tiles - 1)];
+    TileIn<MODE, TYPE, MASK, BIAS> in;
+    // The first tile is asked for before the bias is staged (a wave beyond the tiles asks for the last one
+    // and leaves it), which with the table's gradient costs more registers than it gains.
+    if (!TABLE) in.load(a, next, lane);
+    if (BIAS) stage_bias(a, bias);
+    while (it < a.num_tiles) {
+        if (TABLE) in.load(a, next, lane);
+        next = a.tiles[min(it + step, a.num_tiles - 1)];
+        tile_pass<MODE, TYPE, MASK, BIAS>(a, in, tiles[wave], &bias, table, tally);
+        it += step;
+        if (!TABLE && it < a.num_tiles) in.load(a, next, lane);
+    }
     leave_sums<MODE, TABLE>(a, (int)blockIdx.x, tally, table, bins, bad, shd);
 }
 
@@ -1021,8 +1082,8 @@ __global__ __launch_bounds__(kBlock) void wide_kernel(ChoiceArgs a, int mid_bloc
     __shared__ int bad[kMaxBuckets];
     __shared__ Soft shs[kWaves];
     __shared__ float shf[kWaves];
-    __shared__ double shd[kWaves];
-    const int tid = (int)threadIdx.x, wave = tid / kWave;
+    __shared__ double shd[kWaves * 3];
+    const int tid = (int)threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     TableSum table;
     if (TABLE) {
         for (int b = tid; b < kMaxBuckets; b += kBlock) bad[b] = 0;
@@ -1031,8 +1092,14 @@ __global__ __launch_bounds__(kBlock) void wide_kernel(ChoiceArgs a, int mid_bloc
     if (BIAS) stage_bias(a, bias);
     double tally[3] = {0.0, 0.0, 0.0};
     if ((int)blockIdx.x < mid_blocks) {
-        for (int it = __builtin_amdgcn_readfirstlane((int)blockIdx.x * kWaves + wave); it < a.num_mid; it += mid_blocks * kWaves)
-            wide_pass<MODE, TYPE, MASK, BIAS, kWave>(a, a.wide[it], it, shs, shf, &bias, table, tally);
+        const int step = mid_blocks * kWaves;
+        int it = __builtin_amdgcn_readfirstlane((int)blockIdx.x * kWaves + wave);
+        SetItem next = a.wide[min(it, a.num_mid - 1)];
+        for (; it < a.num_mid; it += step) {
+            const SetItem im = next;
+            next = a.wide[min(it + step, a.num_mid - 1)];
+            wide_pass<MODE, TYPE, MASK, BIAS, kWave>(a, im, it, shs, shf, &bias, table, tally);
+        }
     } else {
         const int n = a.num_mid + (MODE == kSteps ? a.num_whole : a.num_wide);
         for (int it = a.num_mid + (int)blockIdx.x - mid_blocks; it < n; it += (int)gridDim.x - mid_blocks)
@@ -1224,7 +1291,17 @@ __global__ __launch_bounds__(kBlock) void both_kernel(const float* __restrict__ 
 __device__ __forceinline__ float list_slope(const SumArgs& a, const int64_t* list_off, int64_t g, int sub, int L) {
     double t = 0.0;
     const int64_t e = list_off[g + 1];
-    for (int64_t i = list_off[g] + sub; i < e; i += L) t += sum_term<true>(a, i);
+    for (int64_t i0 = list_off[g] + sub; i0 < e; i0 += 4 * L) {  // four in flight; past the end none
+        double v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int64_t i = i0 + (int64_t)k * L;
+            v[k] = sum_term<true>(a, min(i, e - 1));
+            if (i >= e) v[k] = 0.0;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) t += v[k];
+    }
     for (int m = 1; m < L; m <<= 1) t += __shfl_xor(t, m);
     return (float)t;
 }
