@@ -564,8 +564,8 @@ int pb_sets_destroy(pb_sets* sets);
 #define PB_F16 2
 
 /* Scores of the rows of a pb_sets. num_buckets 0: no position bias. Else table_dev float32
- * [num_buckets] (at most 256), positions_dev int32 [rows] and buckets_dev uint8 [2 (reach + 1)], every
- * entry below num_buckets: a row at position q takes bucket buckets_dev[min(|q|, reach)] for q <= 0 and
+ * [num_buckets] (at most 256), positions_dev int32 [rows] and buckets_dev uint8 [2 (reach + 1)] (an
+ * entry of num_buckets or more counts as the last bucket): a row at position q takes bucket buckets_dev[min(|q|, reach)] for q <= 0 and
  * buckets_dev[reach + 1 + min(q, reach)] for q > 0. */
 typedef struct {
     const void* scores_dev;       /* score_type [rows], element i at i * score_stride */

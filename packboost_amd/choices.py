@@ -72,9 +72,10 @@ class _Handle:
     _destroy = ""
 
     def close(self) -> None:
-        """Frees the device memory; no call that uses it may still be running."""
+        """Frees the device memory, once the calls that use it have ended."""
         h, self._handle = getattr(self, "_handle", None), None
         if h is not None and h.value:
+            torch.cuda.synchronize(self.device)
             getattr(_hip.load(), self._destroy)(h)
 
     def __del__(self) -> None:  # pragma: no cover - best effort
@@ -203,14 +204,16 @@ class PreferencePairs(_Handle):
         self.device = _home(device, winners, losers, offsets)
         self.num_pairs = int(w.size)
         self.num_values = int(num_values) if off is None else int(off.size - 1)
-        if self.num_values < 0 or (w.size and (min(w.min(), l.min()) < 0 or max(w.max(), l.max()) >= self.num_values)):
-            raise ValueError(f"pairs must name values in [0, {self.num_values})")
+        if self.num_values < 0:
+            raise ValueError(f"num_values must not be negative, got {self.num_values}")
         self.num_steps = self.num_values if off is None else int(off[-1])
         h = ctypes.c_void_p()
         with torch.cuda.device(self.device):
-            _hip.check(_hip.load().pb_pairs_create(
-                w.ctypes.data, l.ctypes.data, self.num_pairs, self.num_values,
-                None if off is None else off.ctypes.data, ctypes.byref(h)), "pb_pairs_create")
+            rc = _hip.load().pb_pairs_create(w.ctypes.data, l.ctypes.data, self.num_pairs, self.num_values,
+                                             None if off is None else off.ctypes.data, ctypes.byref(h))
+            if rc == _hip.PB_ERR_RANGE:
+                raise ValueError(f"pairs must name values in [0, {self.num_values})")
+            _hip.check(rc, "pb_pairs_create")
         self._handle = h
         self._work_bytes = int(_hip.load().pb_preference_work_bytes(h))
 

@@ -2,7 +2,7 @@
 // the device), argument checks, workspaces.
 #include <algorithm>
 #include <memory>
-#include <new>
+#include <exception>
 #include <string>
 #include <vector>
 
@@ -116,7 +116,8 @@ int sets_create(const int64_t* off, int64_t num_sets, pb_sets** out) {
     if (off[0] != 0) return pb::api_fail(PB_ERR_INVALID, "pb_sets_create: offsets must start at 0");
     for (int64_t g = 0; g < num_sets; ++g)
         if (off[g + 1] < off[g]) return pb::api_fail(PB_ERR_INVALID, "pb_sets_create: offsets must not decrease");
-    if (off[num_sets] > ((int64_t)1 << 40)) return pb::api_fail(PB_ERR_UNSUPPORTED, "pb_sets_create: more than 2^40 rows");
+    if (off[num_sets] > ((int64_t)1 << 37))  // what the sums of the bias table's gradient hold
+        return pb::api_fail(PB_ERR_UNSUPPORTED, "pb_sets_create: more than 2^37 rows");
     Layout lay;
     lay_out(off, num_sets, lay);
     const size_t tiles = lay.tiles.size(), mid = lay.mid.size(), whole = lay.whole.size();
@@ -262,7 +263,7 @@ int pb_sets_create(const int64_t* offsets_host, int64_t num_sets, pb_sets** out)
     if (!offsets_host) return pb::api_fail(PB_ERR_INVALID, "pb_sets_create: null offsets");
     try {
         return sets_create(offsets_host, num_sets, out);
-    } catch (const std::bad_alloc&) {
+    } catch (const std::exception&) {
         return pb::api_fail(PB_ERR_NOMEM, "pb_sets_create: out of host memory");
     }
 }
@@ -348,7 +349,7 @@ int pb_pairs_create(const int64_t* winners_host, const int64_t* losers_host, int
         return pb::api_fail(PB_ERR_INVALID, "pb_pairs_create: bad shape or null pairs");
     try {
         return pairs_create(winners_host, losers_host, num_pairs, num_values, seq_offsets_host, out);
-    } catch (const std::bad_alloc&) {
+    } catch (const std::exception&) {
         return pb::api_fail(PB_ERR_NOMEM, "pb_pairs_create: out of host memory");
     }
 }

@@ -181,13 +181,13 @@ struct BiasShared {
 __device__ __forceinline__ uint32_t bucket_of(const ChoiceArgs& a, const BiasShared& b, int32_t q) {
     const uint32_t d = q < 0 ? 0u - (uint32_t)q : (uint32_t)q;
     const uint32_t i = min(d, (uint32_t)a.reach) + (q > 0 ? (uint32_t)a.reach + 1u : 0u);
-    return a.reach < kLookup / 2 ? b.lookup[i] : a.buckets[i];
+    return a.reach < kLookup / 2 ? b.lookup[i] : min((uint32_t)a.buckets[i], (uint32_t)a.num_buckets - 1u);
 }
 
 __device__ __forceinline__ void stage_bias(const ChoiceArgs& a, BiasShared& b) {
     for (int i = (int)threadIdx.x; i < a.num_buckets; i += kBlock) b.table[i] = a.table[i];
     if (a.reach < kLookup / 2)
-        for (int i = (int)threadIdx.x; i < 2 * (a.reach + 1); i += kBlock) b.lookup[i] = a.buckets[i];
+        for (int i = (int)threadIdx.x; i < 2 * (a.reach + 1); i += kBlock) b.lookup[i] = (uint8_t)min((int)a.buckets[i], a.num_buckets - 1);
     __syncthreads();
 }
 
