@@ -1,9 +1,12 @@
 // C-ABI host layer of the choice and preference operators: their layouts (built on the host, kept on
 // the device), argument checks, workspaces.
 #include <algorithm>
+#include <atomic>
 #include <memory>
 #include <exception>
 #include <string>
+#include <system_error>
+#include <thread>
 #include <vector>
 
 #include "pb_internal.h"
@@ -157,35 +160,70 @@ int sets_create(const int64_t* off, int64_t num_sets, pb_sets** out) {
     return PB_OK;
 }
 
+constexpr int64_t kManyPairs = 1 << 17;  // from which on several threads lay pairs out
+
+// f(0) .. f(threads - 1), a thread each; those that cannot be started run here.
+template <class F>
+void in_threads(int threads, const F& f) {
+    std::vector<std::thread> running;
+    running.reserve((size_t)threads);
+    for (int t = 1; t < threads; ++t) {
+        try {
+            running.emplace_back(f, t);
+        } catch (const std::system_error&) {
+            f(t);
+        }
+    }
+    f(0);
+    for (std::thread& r : running) r.join();
+}
+
 int pairs_create(const int64_t* winners, const int64_t* losers, int64_t num_pairs, int64_t num_values,
                  const int64_t* seq_off, pb_pairs** out) {
     if (num_values >= INT32_MAX || num_pairs >= ((int64_t)1 << 30))
         return pb::api_fail(PB_ERR_UNSUPPORTED, "pb_pairs_create: at most 2^30 pairs and 2^31 - 2 values");
+    // [winners | losers | entries], the entries of a value in the order of its pairs: a counting sort, each
+    // thread over all pairs for the values of its range (their counters and lists are its alone)
     std::vector<int64_t> off((size_t)num_values + 1, 0);
-    for (int64_t p = 0; p < num_pairs; ++p) {
-        if (winners[p] < 0 || winners[p] >= num_values || losers[p] < 0 || losers[p] >= num_values)
-            return pb::api_fail(PB_ERR_RANGE, "pb_pairs_create: a pair names a value out of range");
-        ++off[(size_t)winners[p] + 1];
-        ++off[(size_t)losers[p] + 1];
-    }
+    const size_t words = (size_t)num_pairs * 4;
+    const std::unique_ptr<int32_t[]> host(new int32_t[words]);  // first touched by the threads
+    int32_t* entries = host.get() + 2 * num_pairs;
+    const int threads = num_pairs < kManyPairs ? 1 : (int)std::min(8u, std::max(1u, std::thread::hardware_concurrency()));
+    std::atomic<bool> in_range{true};
+    in_threads(threads, [&](int t) {
+        const int64_t p0 = num_pairs * t / threads, p1 = num_pairs * (t + 1) / threads;
+        for (int64_t p = p0; p < p1; ++p) {
+            const int64_t w = winners[p], l = losers[p];
+            if (w < 0 || w >= num_values || l < 0 || l >= num_values) {
+                in_range = false;
+                return;
+            }
+            host[(size_t)p] = (int32_t)w;
+            host[(size_t)(num_pairs + p)] = (int32_t)l;
+        }
+    });
+    if (!in_range) return pb::api_fail(PB_ERR_RANGE, "pb_pairs_create: a pair names a value out of range");
+    const int32_t *w32 = host.get(), *l32 = w32 + num_pairs;
+    const auto each_of = [&](int t, const auto& f) {  // f(value, pair, side) of the thread's values, in pair order
+        const int32_t v0 = (int32_t)(num_values * t / threads), v1 = (int32_t)(num_values * (t + 1) / threads);
+        for (int64_t p = 0; p < num_pairs; ++p) {
+            if (w32[p] >= v0 && w32[p] < v1) f(w32[p], (int32_t)p, 0);
+            if (l32[p] >= v0 && l32[p] < v1) f(l32[p], (int32_t)p, 1);
+        }
+    };
+    in_threads(threads, [&](int t) { each_of(t, [&](int32_t v, int32_t, int) { ++off[(size_t)v + 1]; }); });
     for (int64_t v = 0; v < num_values; ++v) off[(size_t)v + 1] += off[(size_t)v];
-    // [winners | losers | entries], the entries of a value in the order of its pairs
-    std::vector<int32_t> host((size_t)num_pairs * 4);
     std::vector<int64_t> next(off.begin(), off.end() - 1);
-    int32_t* entries = host.data() + 2 * num_pairs;
-    for (int64_t p = 0; p < num_pairs; ++p) {
-        host[(size_t)p] = (int32_t)winners[p];
-        host[(size_t)(num_pairs + p)] = (int32_t)losers[p];
-        entries[next[(size_t)winners[p]]++] = (int32_t)(p * 2);
-        entries[next[(size_t)losers[p]]++] = (int32_t)(p * 2 + 1);
-    }
+    in_threads(threads, [&](int t) {
+        each_of(t, [&](int32_t v, int32_t p, int side) { entries[next[(size_t)v]++] = p * 2 + side; });
+    });
     std::unique_ptr<pb_pairs, void (*)(pb_pairs*)> h(new pb_pairs(), free_pairs);
     int rc = sets_create(off.data(), num_values, &h->lists);
     if (rc == PB_OK && seq_off) rc = sets_create(seq_off, num_values, &h->seqs);
     if (rc == PB_OK) {
         hipError_t e = hipGetDevice(&h->device);
-        if (e == hipSuccess) e = hipMalloc(&h->arena, std::max<size_t>(256, host.size() * 4));
-        if (e == hipSuccess && !host.empty()) e = hipMemcpy(h->arena, host.data(), host.size() * 4, hipMemcpyHostToDevice);
+        if (e == hipSuccess) e = hipMalloc(&h->arena, std::max<size_t>(256, words * 4));
+        if (e == hipSuccess && words > 0) e = hipMemcpy(h->arena, host.get(), words * 4, hipMemcpyHostToDevice);
         if (e != hipSuccess) rc = pb::api_hip_fail(e, "pb_pairs_create");
     }
     if (rc != PB_OK) return rc;
