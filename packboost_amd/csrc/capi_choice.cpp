@@ -53,40 +53,90 @@ int32_t team_of(int64_t rows, int64_t sets, int64_t largest) {
 
 struct Layout {
     std::vector<SetItem> tiles, mid, whole, parts;
+    std::vector<pb::TileSegment> segments;
     std::vector<int32_t> split;  // the first part of each split set, within `parts`
 };
 
-void lay_out(const int64_t* off, int64_t num_sets, Layout& out) {
-    SetItem tile{};
-    int64_t largest = 0;
-    auto flush = [&] {
-        if (tile.sets == 0) return;
-        tile.team = team_of(tile.rows, tile.sets, largest);
-        out.tiles.push_back(tile);
-        tile = SetItem{};
-        largest = 0;
-    };
+// The tile that is being filled.
+class TileFill {
+  public:
+    TileFill(Layout& out, bool segments) : out_(out), most_segments_(segments ? pb::kTileSegments : 1) {}
+
+    // a longer set lies between the sets before and those after
+    void interrupt() { broken_ = tile_.sets > 0; }
+
+    void add(int64_t row0, int64_t size, int64_t set) {
+        if (tile_.sets > 0 && !fits(row0, size)) flush();
+        if (tile_.sets == 0) {
+            tile_.row0 = row0;
+            tile_.set0 = (int32_t)set;
+            row0_ = row0;
+            rows_ = lane0_ = 0;
+        } else if (broken_) {
+            if (tile_.parts == 0) tile_.part = (int32_t)out_.segments.size();
+            lane0_ = lanes();
+            row0_ = row0;
+            rows_ = 0;
+            out_.segments.push_back({row0, 0, (int32_t)set, (int32_t)lane0_, tile_.sets});
+            ++tile_.parts;
+        }
+        broken_ = false;
+        rows_ += size;
+        (tile_.parts == 0 ? tile_.rows : out_.segments.back().rows) = (int32_t)rows_;
+        total_ += size;
+        ++tile_.sets;
+        largest_ = std::max(largest_, size);
+    }
+
+    void flush() {
+        broken_ = false;
+        if (tile_.sets == 0) return;
+        tile_.team = team_of(total_, tile_.sets, largest_);
+        out_.tiles.push_back(tile_);
+        tile_ = SetItem{};
+        total_ = largest_ = 0;
+    }
+
+  private:
+    static int64_t lanes_of(int64_t row0, int64_t rows) { return rows == 0 ? 0 : ((row0 & 7) + rows + 7) / 8; }
+    int64_t lanes() const { return lane0_ + lanes_of(row0_, rows_); }
+    bool fits(int64_t row0, int64_t size) const {
+        if (tile_.sets == pb::kSetTileSets) return false;
+        if (!broken_) return lane0_ + lanes_of(row0_, rows_ + size) <= pb::kWave;
+        return tile_.parts + 1 < most_segments_ && lanes() + lanes_of(row0, size) <= pb::kWave;
+    }
+
+    Layout& out_;
+    const int most_segments_;
+    SetItem tile_{};
+    bool broken_ = false;
+    int64_t row0_ = 0, rows_ = 0, lane0_ = 0;  // of the last segment
+    int64_t total_ = 0, largest_ = 0;
+};
+
+void lay_out(const int64_t* off, int64_t num_sets, bool segments, Layout& out) {
+    TileFill tiles(out, segments);
     int64_t many = 0;
     for (int64_t g = 0; g < num_sets; ++g) many += off[g + 1] - off[g] > pb::kSetLean;
     const int64_t most_short = many >= pb::kSetMany ? pb::kSetLean : pb::kSetShort;
     for (int64_t g = 0; g < num_sets; ++g) {
         const int64_t size = off[g + 1] - off[g];
-        if (size > most_short) {
-            flush();
-            SetItem im{};
-            im.row0 = off[g];
-            im.rows = (int32_t)std::min<int64_t>(size, pb::kSetWideRows);
-            im.set0 = (int32_t)g;
-            im.sets = 1;
-            im.parts = 1;
-            if ((off[g] & 7) + size <= pb::kSetMidRows) {
-                out.mid.push_back(im);
-                continue;
-            }
-            if ((off[g] & 7) + size <= pb::kSetWideRows) {
-                out.whole.push_back(im);
-                continue;
-            }
+        if (size <= most_short) {
+            tiles.add(off[g], size, g);
+            continue;
+        }
+        tiles.interrupt();
+        SetItem im{};
+        im.row0 = off[g];
+        im.rows = (int32_t)std::min<int64_t>(size, pb::kSetWideRows);
+        im.set0 = (int32_t)g;
+        im.sets = 1;
+        im.parts = 1;
+        if ((off[g] & 7) + size <= pb::kSetMidRows) {
+            out.mid.push_back(im);
+        } else if ((off[g] & 7) + size <= pb::kSetWideRows) {
+            out.whole.push_back(im);
+        } else {
             const int64_t most = pb::kSetWideRows - 8;
             const int64_t want = (size + most - 1) / most;
             const int64_t each = ((size + want - 1) / want + 7) / 8 * 8;  // at most `most`, itself a multiple of 8
@@ -97,24 +147,15 @@ void lay_out(const int64_t* off, int64_t num_sets, Layout& out) {
                 im.rows = (int32_t)std::min(each, off[g + 1] - im.row0);
                 out.parts.push_back(im);
             }
-            continue;
         }
-        if (tile.sets > 0 && ((tile.row0 & 7) + tile.rows + size > pb::kSetTileRows || tile.sets == pb::kSetTileSets))
-            flush();
-        if (tile.sets == 0) {
-            tile.row0 = off[g];
-            tile.set0 = (int32_t)g;
-        }
-        tile.rows += (int32_t)size;
-        ++tile.sets;
-        largest = std::max(largest, size);
     }
-    flush();
+    tiles.flush();
 }
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
-int sets_create(const int64_t* off, int64_t num_sets, pb_sets** out) {
+// segments: tiles may hold sets from either side of longer ones (not where sums are laid out).
+int sets_create(const int64_t* off, int64_t num_sets, bool segments, pb_sets** out) {
     if (num_sets < 0 || num_sets >= INT32_MAX) return pb::api_fail(PB_ERR_UNSUPPORTED, "pb_sets_create: num_sets must lie in [0, 2^31 - 1)");
     if (off[0] != 0) return pb::api_fail(PB_ERR_INVALID, "pb_sets_create: offsets must start at 0");
     for (int64_t g = 0; g < num_sets; ++g)
@@ -122,7 +163,7 @@ int sets_create(const int64_t* off, int64_t num_sets, pb_sets** out) {
     if (off[num_sets] > ((int64_t)1 << 37))  // what the sums of the bias table's gradient hold
         return pb::api_fail(PB_ERR_UNSUPPORTED, "pb_sets_create: more than 2^37 rows");
     Layout lay;
-    lay_out(off, num_sets, lay);
+    lay_out(off, num_sets, segments, lay);
     const size_t tiles = lay.tiles.size(), mid = lay.mid.size(), whole = lay.whole.size();
     std::vector<SetItem>& items = lay.tiles;  // the tiles, the wide items
     items.insert(items.end(), lay.mid.begin(), lay.mid.end());
@@ -133,10 +174,13 @@ int sets_create(const int64_t* off, int64_t num_sets, pb_sets** out) {
     const size_t b_off = round256(sizeof(int64_t) * (size_t)(num_sets + 1));
     const size_t b_items = round256(sizeof(SetItem) * items.size());
     const size_t b_split = round256(sizeof(int32_t) * split.size());
-    std::vector<char> host(b_off + b_items + b_split);
+    const size_t b_segments = round256(sizeof(pb::TileSegment) * lay.segments.size());
+    std::vector<char> host(b_off + b_items + b_split + b_segments);
     std::copy_n(off, num_sets + 1, reinterpret_cast<int64_t*>(host.data()));
     std::copy(items.begin(), items.end(), reinterpret_cast<SetItem*>(host.data() + b_off));
     std::copy(split.begin(), split.end(), reinterpret_cast<int32_t*>(host.data() + b_off + b_items));
+    std::copy(lay.segments.begin(), lay.segments.end(),
+              reinterpret_cast<pb::TileSegment*>(host.data() + b_off + b_items + b_split));
     pb_sets* h = new pb_sets();
     hipError_t e = hipGetDevice(&h->device);
     if (e == hipSuccess) e = hipMalloc(&h->arena, host.size());
@@ -149,6 +193,7 @@ int sets_create(const int64_t* off, int64_t num_sets, pb_sets** out) {
     h->s.tiles = reinterpret_cast<SetItem*>(h->arena + b_off);
     h->s.wide = h->s.tiles + tiles;
     h->s.split = reinterpret_cast<int32_t*>(h->arena + b_off + b_items);
+    h->s.segments = reinterpret_cast<pb::TileSegment*>(h->arena + b_off + b_items + b_split);
     h->s.num_tiles = (int32_t)tiles;
     h->s.num_mid = (int32_t)mid;
     h->s.num_wide = (int32_t)(items.size() - tiles - mid);
@@ -218,8 +263,8 @@ int pairs_create(const int64_t* winners, const int64_t* losers, int64_t num_pair
         each_of(t, [&](int32_t v, int32_t p, int side) { entries[next[(size_t)v]++] = p * 2 + side; });
     });
     std::unique_ptr<pb_pairs, void (*)(pb_pairs*)> h(new pb_pairs(), free_pairs);
-    int rc = sets_create(off.data(), num_values, &h->lists);
-    if (rc == PB_OK && seq_off) rc = sets_create(seq_off, num_values, &h->seqs);
+    int rc = sets_create(off.data(), num_values, false, &h->lists);
+    if (rc == PB_OK && seq_off) rc = sets_create(seq_off, num_values, false, &h->seqs);
     if (rc == PB_OK) {
         hipError_t e = hipGetDevice(&h->device);
         if (e == hipSuccess) e = hipMalloc(&h->arena, std::max<size_t>(256, words * 4));
@@ -300,7 +345,7 @@ int pb_sets_create(const int64_t* offsets_host, int64_t num_sets, pb_sets** out)
     *out = nullptr;
     if (!offsets_host) return pb::api_fail(PB_ERR_INVALID, "pb_sets_create: null offsets");
     try {
-        return sets_create(offsets_host, num_sets, out);
+        return sets_create(offsets_host, num_sets, true, out);
     } catch (const std::exception&) {
         return pb::api_fail(PB_ERR_NOMEM, "pb_sets_create: out of host memory");
     }

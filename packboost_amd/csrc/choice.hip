@@ -367,18 +367,15 @@ struct Segments {
     uint32_t heads, tails;
     uint32_t steps;  // a bit for each step of the scan that stays within the lane's set
 
-    // raw: the sets that start at the lane's rows, 0 for none; rows first .. last - 1 of the lane count
-    __device__ __forceinline__ void start(const int (&raw)[kRun], int lane, int first, int last) {
+    // raw: the sets that start at the lane's rows, 0 for none. A set ends where the next one starts: rows
+    // between them that are of no set hold what changes neither a maximum nor a sum.
+    __device__ __forceinline__ void start(const int (&raw)[kRun], int lane) {
         heads = 0;
 #pragma unroll
         for (int k = 0; k < kRun; ++k) heads |= raw[k] ? 1u << k : 0u;
         const unsigned long long m = __ballot(heads != 0);
-        const unsigned long long next = __ballot((heads & 1u) != 0) >> 1;
+        const unsigned long long next = __ballot((heads & 1u) != 0) >> 1 | 1ull << (kWave - 1);
         tails = heads >> 1 | (uint32_t)(next >> lane & 1ull) << (kRun - 1);
-        if (last >= 1 && last <= kRun) tails |= 1u << (last - 1);
-        const uint32_t from = first <= 0 ? 0xffu : first >= kRun ? 0u : 0xffu << first;
-        const uint32_t upto = last <= 0 ? 0u : last >= kRun ? 0xffu : (1u << last) - 1u;
-        tails &= from & upto;
         const unsigned long long below = m & (~0ull >> (kWave - 1 - lane));
         const int at = below ? kWave - 1 - __clzll((long long)below) : 0;  // the last lane up to this one with a head
         const int room = min(lane - at, lane & 15);  // lanes down to it, in the row of 16
@@ -585,12 +582,11 @@ __global__ __launch_bounds__(kBlock) void part_kernel(ChoiceArgs a, int first) {
 // What a wave keeps of its tile in LDS.
 struct TileShared {
     float x[kSetTileRows];          // logits, then what the chosen rows' gradients are more than the others'
-    float shift[kSetTileSets];      // per set: maximum, or lse
+    float shift[kSetTileSets + 4];  // per set: maximum, or lse
     union {
         uint16_t head[kSetTileRows];  // the set that starts at a row, from 1; 0: none
-        float factor[kSetTileSets];   // later: sum of exponentials, then what the rows' are multiplied by
+        float factor[kSetTileSets + 4];  // later: sum of exponentials, then what the rows' are multiplied by
     };
-    uint16_t begin[kSetTileSets + 4];
 };
 
 __device__ __forceinline__ void write_run(float* p, const float (&x)[kRun]) {
@@ -607,26 +603,50 @@ __device__ __forceinline__ void read_run(const float* p, float (&x)[kRun]) {
 // What a tile reads, all of it asked for before anything is waited for: a lane's run, and the lane's sets.
 template <int MODE, int TYPE, bool MASK, bool BIAS>
 struct TileIn {
-    Span sp;
-    int set0, sets;
+    Span sp;   // of the lane's run alone
+    int sets;
     RawRun<TYPE, MASK, BIAS> raw;
-    int32_t begin[kTileRounds], chosen[kTileRounds];
+    int32_t set[kTileRounds], begin[kTileRounds], end[kTileRounds], chosen[kTileRounds];  // begin, end: rows of the tile
     float given[kTileRounds], lse[kTileRounds];
     PolicyIn pol[kTileRounds];
 
     __device__ __forceinline__ void load(const ChoiceArgs& a, const SetItem& im, int lane) {
-        sp = span_of(a, im);
-        set0 = im.set0;
+        int64_t row0 = im.row0, rows = im.rows;
+        int lane0 = 0;
+        int64_t base[kTileRounds];
         sets = im.sets;
-        if (kRun * lane < sp.hi) raw.load(a, sp, kRun * lane);
 #pragma unroll
         for (int r = 0; r < kTileRounds; ++r) {
-            const int s = r * kWave + lane;
-            const int64_t g = (int64_t)set0 + s;
+            set[r] = im.set0 + r * kWave + lane;
+            base[r] = row0 & ~(int64_t)(kRun - 1);
+        }
+        for (int e = 0; e < im.parts; ++e) {  // the tile's further segments
+            const TileSegment seg = a.segments[im.part + e];
+            if (lane >= seg.lane0) {
+                row0 = seg.row0;
+                rows = seg.rows;
+                lane0 = seg.lane0;
+            }
+#pragma unroll
+            for (int r = 0; r < kTileRounds; ++r)
+                if (r * kWave + lane >= seg.first) {
+                    set[r] = seg.set0 + r * kWave + lane - seg.first;
+                    base[r] = (seg.row0 & ~(int64_t)(kRun - 1)) - kRun * seg.lane0;
+                }
+        }
+        sp.q0 = (row0 & ~(int64_t)(kRun - 1)) + kRun * (lane - lane0);
+        sp.lo = (int)max(row0 - sp.q0, (int64_t)0);  // below kRun
+        sp.hi = (int)min(row0 + rows - sp.q0, (int64_t)kRun);
+        sp.end = (int)min(a.rows - sp.q0, (int64_t)kRun);
+        if (sp.hi > 0) raw.load(a, sp, 0);
+#pragma unroll
+        for (int r = 0; r < kTileRounds; ++r) {
+            const int64_t g = set[r];
             chosen[r] = -1;
             given[r] = lse[r] = 0.0f;
-            if (s < sets) {
-                begin[r] = (int)(a.off[g] - sp.q0);
+            if (r * kWave + lane < sets) {
+                begin[r] = (int)(a.off[g] - base[r]);
+                end[r] = (int)(a.off[g + 1] - base[r]);
                 if (MODE != kRows && MODE != kRowsBack) chosen[r] = a.chosen[g];
                 if (MODE == kStepsBack) given[r] = a.grad[g];
                 if (MODE == kStepsBack || MODE == kRowsBack) lse[r] = a.lse[g];
@@ -651,39 +671,34 @@ __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, TileIn<MODE, TYPE
     Buckets buckets{{0, 0}};
 #pragma unroll
     for (int k = 0; k < kRun; ++k) x[k] = -kInf, d[k] = 0.0f;
-    if (i0 < sp.hi) {
-        in.raw.logits(a, bias, sp, i0, x, off, buckets);
-        if (MODE == kRowsBack) load_floats(a, sp, i0, a.grad, off, d);
+    if (sp.hi > 0) {
+        in.raw.logits(a, bias, sp, 0, x, off, buckets);
+        if (MODE == kRowsBack) load_floats(a, sp, 0, a.grad, off, d);
     }
-    int32_t (&begin)[kTileRounds] = in.begin;
+    const int32_t (&begin)[kTileRounds] = in.begin;
+    const int32_t (&end)[kTileRounds] = in.end;
     int32_t (&chosen)[kTileRounds] = in.chosen;
     wave_sync();  // the last tile's values have been read
     *reinterpret_cast<uint4*>(&sh.head[i0]) = make_uint4(0, 0, 0, 0);
     if (STEPS) write_run(&sh.x[i0], x);
+    if (!SOFT) {
 #pragma unroll
-    for (int r = 0; r < kTileRounds; ++r) {
-        const int s = r * kWave + lane;
-        if (s < in.sets) {
-            sh.begin[s] = (uint16_t)begin[r];
-            if (!SOFT) sh.shift[s] = in.lse[r];
-        }
+        for (int r = 0; r < kTileRounds; ++r)
+            if (r * kWave + lane < in.sets) sh.shift[r * kWave + lane] = in.lse[r];
     }
-    if (lane == 0) sh.begin[in.sets] = (uint16_t)sp.hi;
     wave_sync();
     // which set each row is of, and the chosen rows' logits (a choice outside its set or masked is none)
-    int end[kTileRounds];
     float picked[kTileRounds];
 #pragma unroll
     for (int r = 0; r < kTileRounds; ++r) {
         const int s = r * kWave + lane;
         if (s < in.sets) {
-            end[r] = sh.begin[s + 1];
             if (end[r] > begin[r]) sh.head[begin[r]] = (uint16_t)(s + 1);
             if (STEPS) {
                 if (chosen[r] >= end[r] - begin[r]) chosen[r] = -1;
                 picked[r] = chosen[r] >= 0 ? sh.x[begin[r] + chosen[r]] : -kInf;
                 // a masked row's logit is -inf, as one of that score is: the mask says which
-                if (MASK && chosen[r] >= 0 && picked[r] == -kInf && !a.mask[sp.q0 + begin[r] + chosen[r]]) chosen[r] = -1;
+                if (MASK && chosen[r] >= 0 && picked[r] == -kInf && !a.mask[a.off[in.set[r]] + chosen[r]]) chosen[r] = -1;
             }
         }
     }
@@ -701,13 +716,13 @@ __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, TileIn<MODE, TYPE
         const unsigned long long below = __ballot(last != 0) & ((1ull << lane) - 1ull);
         const int from = below ? kWave - 1 - __clzll((long long)below) : lane;
         const int carried = __shfl(last, from);
-        int now = below ? carried : 1;
+        int now = below ? carried : kSetTileSets + 1;  // before the first set: a slot of none
 #pragma unroll
         for (int k = 0; k < kRun; ++k) {
             now = raw[k] ? raw[k] : now;
             id[k] = now;
         }
-        if (SOFT || MODE == kRowsBack) seg.start(raw, lane, sp.lo - i0, sp.hi - i0);
+        if (SOFT || MODE == kRowsBack) seg.start(raw, lane);
     }
     float v[kRun];
     if (SOFT) {
@@ -732,7 +747,7 @@ __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, TileIn<MODE, TYPE
             const int s = r * kWave + lane;
             coef[r] = 0.0f;
             if (s < in.sets) {
-                const int64_t g = (int64_t)in.set0 + s;
+                const int64_t g = in.set[r];
                 const bool empty = end[r] == begin[r];
                 const float top = SOFT ? (empty ? 0.0f : sh.shift[s]) : in.lse[r];
                 const float sum = SOFT && !empty ? sh.factor[s] : 0.0f;
@@ -789,11 +804,11 @@ __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, TileIn<MODE, TYPE
 #pragma unroll
         for (int k = 0; k < kRun; ++k) v[k] = off >> k & 1u ? 0.0f : v[k];
     }
-    if (i0 < sp.hi) {
+    if (sp.hi > 0) {
         if (MODE == kRows)
-            store_run<PB_F32>(a, sp, i0, a.log_probs, v);
+            store_run<PB_F32>(a, sp, 0, a.log_probs, v);
         else
-            store_run<TYPE>(a, sp, i0, a.grad_scores, v);
+            store_run<TYPE>(a, sp, 0, a.grad_scores, v);
     }
     if (BIAS && GRAD) table.add(v, buckets);
 }
@@ -1427,6 +1442,7 @@ hipError_t launch_choice(int mode, const SetLayout& s, ChoiceArgs a, int32_t typ
     a.off = s.off;
     a.tiles = s.tiles;
     a.wide = s.wide;
+    a.segments = s.segments;
     a.num_tiles = s.num_tiles;
     a.num_wide = s.num_wide;
     a.num_mid = s.num_mid;

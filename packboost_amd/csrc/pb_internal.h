@@ -489,12 +489,14 @@ hipError_t launch_predict_bins(const uint8_t* bins, int64_t N, int64_t ld, int32
                                hipStream_t s);
 
 // ---- choices and preferences (choice.hip) ----
-// A table of ragged sets laid out for wavefronts and workgroups. Tiles, for a wave each, in row order: runs
-// of consecutive sets of at most kSetShort rows, at most kSetTileSets of them; their rows, counted from the
-// multiple of 8 at or before the first, are at most kSetTileRows; `team`: lanes of 1 << team to a set, where
-// a wave's lanes are shared out by sets. Wide items: first longer sets of at most kSetMidRows rows counted
-// the same way, for a wave each; then, for a workgroup each, sets of at most kSetWideRows rows and the parts
-// (part `part` of `parts`) of those that are longer, a set's consecutive; `split` names the first of each.
+// A table of ragged sets laid out for wavefronts and workgroups. Tiles, for a wave each: sets of at most
+// kSetShort rows, at most kSetTileSets of them, in segments of consecutive ones. A segment starts at a
+// lane, its rows counted from the multiple of 8 at or before the first, 8 to a lane; between segments lie
+// longer sets. `rows`, `set0` are the first segment's, `sets` the tile's, `parts` further segments are at
+// `part` of the list. Layouts for sums have one segment to a tile, and `team`: lanes of 1 << team to a set.
+// Wide items: first longer sets of at most kSetMidRows rows counted the same way, for a wave each; then, for
+// a workgroup each, sets of at most kSetWideRows rows and the parts (part `part` of `parts`) of those that
+// are longer, a set's consecutive; `split` names the first of each.
 constexpr int kSetTileRows = 512;
 constexpr int kSetTileSets = 128;
 constexpr int kSetShort = kSetTileRows - 8;
@@ -515,9 +517,18 @@ struct SetItem {
     int32_t parts;
 };
 static_assert(sizeof(SetItem) == 32, "an item is 32 bytes");
+struct TileSegment {
+    int64_t row0;
+    int32_t rows;
+    int32_t set0;
+    int32_t lane0;  // its first lane
+    int32_t first;  // its first set among the tile's
+};
+constexpr int kTileSegments = 8;
 struct SetLayout {
     const int64_t* off;    // [num_sets + 1]
     const SetItem* tiles;  // [num_tiles]
+    const TileSegment* segments;
     const SetItem* wide;   // [num_mid + num_wide], of the last num_wide the first num_whole whole sets
     const int32_t* split;  // [num_split], indices of wide items
     int32_t num_tiles;
@@ -545,6 +556,7 @@ struct ChoiceArgs {
     const int64_t* off;
     const SetItem* tiles;
     const SetItem* wide;
+    const TileSegment* segments;
     int32_t num_tiles;
     int32_t num_mid;
     int32_t num_wide;
