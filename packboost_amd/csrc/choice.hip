@@ -298,16 +298,45 @@ __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_wave_barrier();
 }
 
-template <class F>
-__device__ __forceinline__ F wave_sum(F v) {
-#pragma unroll
-    for (int m = kWave / 2; m >= 1; m >>= 1) v += __shfl_xor(v, m);
-    return v;
+template <int CTRL>
+__device__ __forceinline__ float lane_move(float v) {  // lanes without a source keep their own
+    const int i = __float_as_int(v);
+    return __int_as_float(__builtin_amdgcn_update_dpp(i, i, CTRL, 0xf, 0xf, false));
 }
 
-__device__ __forceinline__ float wave_max(float v) {
+struct TakeMax {
+    static constexpr float kNone = kLowest;
+    static __device__ __forceinline__ float of(float a, float b) { return max2(a, b); }
+};
+struct TakeSum {
+    static constexpr float kNone = 0.0f;
+    static __device__ __forceinline__ float of(float a, float b) { return a + b; }
+};
+
+// One step of a reduction by moves between lanes (CTRL of the rows in ROWS; the others take nothing).
+template <class OP, int CTRL, int ROWS>
+__device__ __forceinline__ float reduce_step(float v) {
+    return OP::of(__int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(OP::kNone), __float_as_int(v), CTRL, ROWS, 0xf, false)), v);
+}
+
+// A wave's lanes, the result in all of them: within rows of 16 lanes, then between rows.
+template <class OP>
+__device__ __forceinline__ float wave_reduce(float v) {
+    v = reduce_step<OP, 0x111, 0xf>(v);  // row_shr:1
+    v = reduce_step<OP, 0x112, 0xf>(v);  // row_shr:2
+    v = reduce_step<OP, 0x114, 0xf>(v);  // row_shr:4
+    v = reduce_step<OP, 0x118, 0xf>(v);  // row_shr:8
+    v = reduce_step<OP, 0x142, 0xa>(v);  // row_bcast:15
+    v = reduce_step<OP, 0x143, 0xc>(v);  // row_bcast:31
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), kWave - 1));
+}
+
+__device__ __forceinline__ float wave_max(float v) { return wave_reduce<TakeMax>(v); }
+__device__ __forceinline__ float wave_sum(float v) { return wave_reduce<TakeSum>(v); }
+
+__device__ __forceinline__ double wave_sum(double v) {
 #pragma unroll
-    for (int m = kWave / 2; m >= 1; m >>= 1) v = max2(v, __shfl_xor(v, m));
+    for (int m = kWave / 2; m >= 1; m >>= 1) v += __shfl_xor(v, m);
     return v;
 }
 
@@ -382,21 +411,6 @@ struct Segments {
         steps = (room >= 1 ? 1u : 0u) | (room >= 2 ? 2u : 0u) | (room >= 4 ? 4u : 0u) | (room >= 8 ? 8u : 0u) |
                 ((lane & 16) != 0 && (lane & ~15) - 1 >= at ? 16u : 0u) | (lane >= 32 && 31 >= at ? 32u : 0u);
     }
-};
-
-template <int CTRL>
-__device__ __forceinline__ float lane_move(float v) {  // lanes without a source keep their own
-    const int i = __float_as_int(v);
-    return __int_as_float(__builtin_amdgcn_update_dpp(i, i, CTRL, 0xf, 0xf, false));
-}
-
-struct TakeMax {
-    static constexpr float kNone = kLowest;
-    static __device__ __forceinline__ float of(float a, float b) { return max2(a, b); }
-};
-struct TakeSum {
-    static constexpr float kNone = 0.0f;
-    static __device__ __forceinline__ float of(float a, float b) { return a + b; }
 };
 
 // out[id[k] - 1] = the reduction of x over the set that row k ends; `before`: the lane's rows up to its
