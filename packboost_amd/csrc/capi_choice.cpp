@@ -116,12 +116,9 @@ class TileFill {
 
 void lay_out(const int64_t* off, int64_t num_sets, bool segments, Layout& out) {
     TileFill tiles(out, segments);
-    int64_t many = 0;
-    for (int64_t g = 0; g < num_sets; ++g) many += off[g + 1] - off[g] > pb::kSetLean;
-    const int64_t most_short = many >= pb::kSetMany ? pb::kSetLean : pb::kSetShort;
     for (int64_t g = 0; g < num_sets; ++g) {
         const int64_t size = off[g + 1] - off[g];
-        if (size <= most_short) {
+        if (size <= pb::kSetShort) {
             tiles.add(off[g], size, g);
             continue;
         }

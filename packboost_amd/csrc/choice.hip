@@ -6,10 +6,13 @@
 // lse = m + log s and log p_i = (x_i - m) - log s; a set without probability (empty, all masked) has
 // s = 0 and lse = -inf. The gradient of a step's log p_c is [i = c] - p_i, of all rows' d_i - p_i sum d.
 //
-// Work is laid out once per table of sets. A wavefront takes a tile of consecutive short sets, 8 rows a
-// lane, and reduces them by a segmented scan over the lanes, whose cost does not depend on how the rows
-// fall into sets; a workgroup takes one longer set, or a part of it, in registers. Parts of a set are
-// reduced by a pass before (part_kernel). Every sum has a fixed order (lanes, waves, workgroups), so
+// Work is laid out once per table of sets. A wavefront takes a tile of short sets, 8 rows a lane, and
+// reduces them by a segmented scan over the lanes, whose cost does not depend on how the rows fall into
+// sets; a wave or a workgroup takes one longer set, or a part of it, in registers. Parts of a set are
+// reduced by a pass before (part_kernel). All of it is bound by memory at best: a row has 8 to 20 bytes and
+// some 20 operations, so every row is read once, in 16-byte accesses, and what is read is asked for before
+// anything is waited for (teams of lanes that walked each set's rows in LDS took 15 us for tiles that take
+// 5 to 7 us so). Every sum has a fixed order (lanes, waves, workgroups), so
 // results do not change from run to run. Maxima, sums of exponentials and log-probabilities are float32;
 // losses and the table's gradient are joined in double, each rounded once when it is written.
 #include <algorithm>
@@ -26,9 +29,10 @@ constexpr float kLowest = -3.402823466e38f;
 constexpr int kRun = 8;                                     // consecutive rows of a lane
 constexpr int kWideRuns = kSetWideRows / (kRun * kBlock);   // runs of a thread of a longer set
 constexpr int kTileRounds = kSetTileSets / kWave;           // sets of a tile per lane
-// Values from which on they are laid beside their references first: two arrays of them pass a quarter of an
-// XCD's 4 MB L2, and every pair's four reads miss it more and more.
-constexpr int64_t kBothFrom = 1 << 17;
+// Values are laid beside their references first where both are many: the two arrays pass an XCD's 4 MB of
+// L2, and a pair's four reads become two (us a call, so / without: 1M values, 4M pairs 207 / 259; 512k, 512k
+// 39 / 42; 128k, 512k 35 / 37; with fewer pairs the launch costs more: 256k, 256k 25 / 22; 128k, 128k 21 / 18).
+constexpr int64_t kBothValues = 1 << 17, kBothPairs = 1 << 19;
 constexpr int kJoin = 8;
 constexpr int kPairs = 4;                                   // pairs a thread has in flight
 constexpr int kBins = 256;     // LDS words of the table's gradient per wave: buckets x copies
@@ -413,8 +417,8 @@ struct Segments {
     }
 };
 
-// out[id[k] - 1] = the reduction of x over the set that row k ends; `before`: the lane's rows up to its
-// first head belong to a set that began in a lane below.
+// out[id[k] - 1] = the reduction of x over the set that row k ends. The lane's rows before its first head
+// are of a set that began in a lane below. 24 vector instructions for the scan, 6 a row.
 template <class OP>
 __device__ __forceinline__ void segment_reduce(const Segments& seg, const float (&x)[kRun], const int (&id)[kRun],
                                                int lane, float* out) {
@@ -538,7 +542,8 @@ struct TableSum {
 };
 
 // The maximum and the sum of exponentials of a part of a set, or (listwise backward) the sum of its
-// rows' gradients.
+// rows' gradients. 11 vector instructions a row and one barrier: bound by reading the rows (4096 sets of
+// 32000 bfloat16 scores, 262 MB: 60 us, 4.4 TB/s).
 template <int MODE, int TYPE, bool MASK, bool BIAS>
 __global__ __launch_bounds__(kBlock) void part_kernel(ChoiceArgs a, int first) {
     __shared__ Soft sh[kWaves];
@@ -670,7 +675,12 @@ struct TileIn {
     }
 };
 
-// One tile of short sets by one wave.
+// One tile of short sets by one wave: the maximum and the sum of exponentials by two segmented scans, which
+// leave them in LDS by set; a lane to a set then forms log-probabilities, losses and slopes, 64 sets at a
+// time; the rows take their set's factor from LDS. About 700 vector instructions for 512 rows, 1200 with
+// mask, bias and the policy's steps: past the first few thousand tiles their issue bounds it, before that
+// the chain from the loads to the stores. 2.4M rows of 100k sets with mask and bias: log-probabilities of
+// the steps 9.5 us, their backward with the table's gradient 13.4 us; the policy loss of 480k sets 22.6 us.
 template <int MODE, int TYPE, bool MASK, bool BIAS>
 __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, TileIn<MODE, TYPE, MASK, BIAS>& in, TileShared& sh,
                                           const BiasShared* bias, TableSum& table, double (&tally)[3]) {
@@ -828,7 +838,11 @@ __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, TileIn<MODE, TYPE
 }
 
 // One set of more than kSetShort rows by a wave (THREADS 64), or a longer one or a part of it by a
-// workgroup. A wave passes over runs beyond its rows.
+// workgroup. A wave passes over runs beyond its rows. The rows stay in registers from the load to the
+// store, one exponential each, so that a set of up to kSetWideRows rows is read once; a longer one's parts are
+// read a second time. Bound by memory for sets of thousands of rows (backward of 4096 sets of 32000
+// bfloat16 scores, 524 MB: 86 us, 6.1 TB/s), by the instructions a set takes beside its rows (about 250)
+// for hundreds (100k policy steps, 34M of their 40M rows here: 47 us, 2.9 TB/s).
 template <int MODE, int TYPE, bool MASK, bool BIAS, int THREADS>
 __device__ __forceinline__ void wide_pass(const ChoiceArgs& a, const SetItem& im, int32_t index, Soft* shs, float* shf,
                                           const BiasShared* bias, TableSum& table, double (&tally)[3]) {
@@ -992,7 +1006,7 @@ __device__ __forceinline__ void wide_pass(const ChoiceArgs& a, const SetItem& im
     }
 }
 
-// The steps of the sets in parts, from the parts' maxima and sums: a wave to a set.
+// The steps of the sets in parts, from the parts' maxima and sums: a wave to a set (4096 sets: 5 us).
 template <int TYPE, bool MASK, bool BIAS>
 __global__ __launch_bounds__(kBlock) void split_steps_kernel(ChoiceArgs a, const int32_t* __restrict__ firsts, int n) {
     __shared__ BiasShared bias;
@@ -1138,7 +1152,8 @@ __global__ __launch_bounds__(kBlock) void wide_kernel(ChoiceArgs a, int mid_bloc
 }
 
 // out[j] = sum over the workgroups' sums [n][cols] of column j, in a fixed order; the first `head`
-// columns go to stats, the others to the table's gradient.
+// columns go to stats, the others to the table's gradient. A launch of its own (3 to 5 us, most of it
+// latency): joining in the last workgroup to finish would have every workgroup write back its L2 first.
 __global__ __launch_bounds__(kBlock) void join_kernel(const double* __restrict__ sums, int32_t n, int32_t cols,
                                                       int32_t head, float* __restrict__ stats,
                                                       float* __restrict__ table) {
@@ -1161,7 +1176,10 @@ __global__ __launch_bounds__(kBlock) void join_kernel(const double* __restrict__
 
 // ------------------------------------------------------------------------------ preferences
 // Sums over sets in double: of (value - ref) over a sequence's steps, or of the signed slopes of the
-// pairs that a value is in (list entry: pair * 2 + (1 where it is the loser)).
+// pairs that a value is in (list entry: pair * 2 + (1 where it is the loser)). A pair's slope is computed once
+// and gathered twice, in the lists' order: no atomics, so hubs (values in thousands of pairs) cost
+// what their entries cost and sums keep their order. Bound by the gathers, which find little of 20 MB of
+// slopes in an XCD's 4 MB of L2: 10M entries of 1M lists 148 us, 3.6 TB/s of 64-byte lines.
 struct SumArgs {
     const int64_t* off;
     const SetItem* tiles;
@@ -1256,7 +1274,9 @@ __global__ __launch_bounds__(kBlock) void set_join_kernel(SumArgs a, const int32
 
 // z = beta (a_w - a_l); the loss w [(1 - e) softplus(-z) + e softplus(z)] and its slope
 // beta w (sigmoid(z) - (1 - e)). Sequences' values come from their sums, others' as value - ref, the
-// differences taken in double: both can be large where z is small.
+// differences taken in double: both can be large where z is small. Bound by the gathers of the values: 5M
+// pairs of 1M values, values and references side by side, 94 us (160 us in arrays of their own). Four
+// pairs are in flight a thread.
 __global__ __launch_bounds__(kBlock) void pair_kernel(PairArgs a) {
     __shared__ double sh[kWaves];
     double sum = 0.0;
@@ -1309,7 +1329,7 @@ __global__ __launch_bounds__(kBlock) void pair_kernel(PairArgs a) {
     }
 }
 
-// Values beside their references, so that a pair finds both in one access.
+// Values beside their references, so that a pair finds both in one access (1M: 5 us).
 __global__ __launch_bounds__(kBlock) void both_kernel(const float* __restrict__ values, const float* __restrict__ ref,
                                                       int64_t n, float2* __restrict__ both) {
     const int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x;
@@ -1336,7 +1356,8 @@ __device__ __forceinline__ float list_slope(const SumArgs& a, const int64_t* lis
 }
 
 // out[i] = the slope of step i's sequence: per_set[sequence], or (per_set NULL) the sum over the sequence's
-// list of pairs, where no list is long.
+// list of pairs, where no list is long (300k steps of 4001 sequences in 6000 pairs: 9 us, against 8 + 4 in
+// two launches and what they cost the host).
 __global__ __launch_bounds__(kBlock) void spread_kernel(SumArgs a, const float* __restrict__ per_set,
                                                         const int64_t* __restrict__ list_off) {
     __shared__ double sh[kWaves];
@@ -1426,6 +1447,10 @@ SumArgs sum_args(const SetLayout& s) {
     return a;
 }
 
+bool side_by_side(const PairLayout& p) {
+    return !p.has_seqs && p.lists.num_sets >= kBothValues && p.num_pairs >= kBothPairs;
+}
+
 template <bool PAIRS>
 hipError_t launch_set_sum(const SetLayout& s, const SumArgs& a, hipStream_t stream) {
     const int grid = long_items(s) + tile_groups(s) + (PAIRS && a.num_sums > 0 ? 1 : 0);
@@ -1504,7 +1529,7 @@ hipError_t launch_preference(const PairLayout& p, PairArgs a, const float* value
     } else {
         a.values = values;
         a.ref = ref;
-        if (ref && p.lists.num_sets >= kBothFrom) {
+        if (ref && side_by_side(p)) {
             float2* both = reinterpret_cast<float2*>(parts + long_items(p.lists));
             a.slopes = reinterpret_cast<float*>(both + p.lists.num_sets);
             a.both = both;
@@ -1548,7 +1573,7 @@ hipError_t launch_preference(const PairLayout& p, PairArgs a, const float* value
 
 int64_t preference_work_bytes(const PairLayout& p) {
     return 8 * ((int64_t)kPairGrid + long_items(p.lists) + long_items(p.seqs)) + 4 * (p.num_pairs + 2 * p.seqs.num_sets) +
-           (!p.has_seqs && p.lists.num_sets >= kBothFrom ? 8 * p.lists.num_sets : 0);
+           (side_by_side(p) ? 8 * p.lists.num_sets : 0);
 }
 
 }  // namespace pb

@@ -497,14 +497,14 @@ hipError_t launch_predict_bins(const uint8_t* bins, int64_t N, int64_t ld, int32
 // Wide items: first longer sets of at most kSetMidRows rows counted the same way, for a wave each; then, for
 // a workgroup each, sets of at most kSetWideRows rows and the parts (part `part` of `parts`) of those that
 // are longer, a set's consecutive; `split` names the first of each.
+// A wave waits for no other wave, so it takes what its registers hold (the policy loss of 40000 sets of 600
+// rows in bfloat16: 41 us, by workgroups 108; of 20000 of 2000 rows 35 and 62; steps in float32 with their
+// backward 150 and 330, 202 and 236). Segments save the lanes that a tile ended by a longer set would leave
+// empty (100k sets of 1 to 100k rows, most of them short: 84 us, 88 without; neither way where few are
+// short).
 constexpr int kSetTileRows = 512;
 constexpr int kSetTileSets = 128;
 constexpr int kSetShort = kSetTileRows - 8;
-// Where at least kSetMany sets have more than kSetLean rows, those up to kSetShort go to a wave each as well:
-// it spends about 300 vector instructions on one, a tile about 700 on 512 rows. Fewer are not worth the
-// launch (100k sets of up to 40k rows: 43 + 60 us so, 55 + 51 in tiles; a launch takes 4 to 6 us).
-constexpr int kSetLean = 256;
-constexpr int kSetMany = 4096;
 constexpr int kSetMidRows = 2048;
 constexpr int kSetWideRows = 8192;
 struct SetItem {
