@@ -677,7 +677,8 @@ struct TileIn {
 
 // One tile of short sets by one wave: the maximum and the sum of exponentials by two segmented scans, which
 // leave them in LDS by set; a lane to a set then forms log-probabilities, losses and slopes, 64 sets at a
-// time; the rows take their set's factor from LDS. About 700 vector instructions for 512 rows, 1200 with
+// time; the rows take their set's factor from LDS. A tile of one set has no need of the scans (policy steps
+// of 30000 sets of 300 rows: 32 us, 40 with them; 66 and 73 for steps in float32 with their backward). About 700 vector instructions for 512 rows, 1200 with
 // mask, bias and the policy's steps: past the first few thousand tiles their issue bounds it, before that
 // the chain from the loads to the stores. 2.4M rows of 100k sets with mask and bias: log-probabilities of
 // the steps 9.5 us, their backward with the table's gradient 13.4 us; the policy loss of 480k sets 22.6 us.
@@ -690,6 +691,7 @@ __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, TileIn<MODE, TYPE
     const int lane = (int)threadIdx.x & (kWave - 1);
     const Span sp = in.sp;
     const int i0 = kRun * lane;
+    const bool alone = in.sets == 1;
     float x[kRun], d[kRun];
     uint32_t off = 0xffu;
     Buckets buckets{{0, 0}};
@@ -703,7 +705,7 @@ __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, TileIn<MODE, TYPE
     const int32_t (&end)[kTileRounds] = in.end;
     int32_t (&chosen)[kTileRounds] = in.chosen;
     wave_sync();  // the last tile's values have been read
-    *reinterpret_cast<uint4*>(&sh.head[i0]) = make_uint4(0, 0, 0, 0);
+    if (!alone) *reinterpret_cast<uint4*>(&sh.head[i0]) = make_uint4(0, 0, 0, 0);
     if (STEPS) write_run(&sh.x[i0], x);
     if (!SOFT) {
 #pragma unroll
@@ -717,7 +719,7 @@ __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, TileIn<MODE, TYPE
     for (int r = 0; r < kTileRounds; ++r) {
         const int s = r * kWave + lane;
         if (s < in.sets) {
-            if (end[r] > begin[r]) sh.head[begin[r]] = (uint16_t)(s + 1);
+            if (!alone && end[r] > begin[r]) sh.head[begin[r]] = (uint16_t)(s + 1);
             if (STEPS) {
                 if (chosen[r] >= end[r] - begin[r]) chosen[r] = -1;
                 picked[r] = chosen[r] >= 0 ? sh.x[begin[r] + chosen[r]] : -kInf;
@@ -728,8 +730,32 @@ __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, TileIn<MODE, TYPE
     }
     wave_sync();
     int id[kRun];
-    Segments seg;
-    {
+    float v[kRun];
+    if (alone) {
+#pragma unroll
+        for (int k = 0; k < kRun; ++k) id[k] = 1;
+        if (SOFT) {
+            float top = TakeMax::kNone, sum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kRun; k += 2) top = max3(top, x[k], x[k + 1]);
+            top = wave_max(top);
+#pragma unroll
+            for (int k = 0; k < kRun; ++k) sum += v[k] = exp_of(x[k] - top);
+            sum = wave_sum(sum);
+            if (lane == 0) {
+                sh.shift[0] = top;
+                sh.factor[0] = sum;
+            }
+        }
+        if (MODE == kRowsBack) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kRun; ++k) sum += d[k];
+            sum = wave_sum(sum);
+            if (lane == 0) sh.factor[0] = sum;
+        }
+        wave_sync();
+    } else {
         const uint4 w = *reinterpret_cast<const uint4*>(&sh.head[i0]);
         const int raw[kRun] = {(int)(w.x & 0xffffu), (int)(w.x >> 16), (int)(w.y & 0xffffu), (int)(w.y >> 16),
                                (int)(w.z & 0xffffu), (int)(w.z >> 16), (int)(w.w & 0xffffu), (int)(w.w >> 16)};
@@ -746,22 +772,20 @@ __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, TileIn<MODE, TYPE
             now = raw[k] ? raw[k] : now;
             id[k] = now;
         }
+        Segments seg;
         if (SOFT || MODE == kRowsBack) seg.start(raw, lane);
-    }
-    float v[kRun];
-    if (SOFT) {
-        segment_reduce<TakeMax>(seg, x, id, lane, sh.shift);
-        wave_sync();
+        if (SOFT) {
+            segment_reduce<TakeMax>(seg, x, id, lane, sh.shift);
+            wave_sync();
 #pragma unroll
-        for (int k = 0; k < kRun; ++k) {
-            v[k] = exp_of(x[k] - sh.shift[id[k] - 1]);
+            for (int k = 0; k < kRun; ++k) v[k] = exp_of(x[k] - sh.shift[id[k] - 1]);
+            segment_reduce<TakeSum>(seg, v, id, lane, sh.factor);
+            wave_sync();
         }
-        segment_reduce<TakeSum>(seg, v, id, lane, sh.factor);
-        wave_sync();
-    }
-    if (MODE == kRowsBack) {
-        segment_reduce<TakeSum>(seg, d, id, lane, sh.factor);
-        wave_sync();
+        if (MODE == kRowsBack) {
+            segment_reduce<TakeSum>(seg, d, id, lane, sh.factor);
+            wave_sync();
+        }
     }
     // a lane to a set: log-probabilities, losses, slopes
     float coef[kTileRounds];
@@ -842,7 +866,7 @@ __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, TileIn<MODE, TYPE
 // store, one exponential each, so that a set of up to kSetWideRows rows is read once; a longer one's parts are
 // read a second time. Bound by memory for sets of thousands of rows (backward of 4096 sets of 32000
 // bfloat16 scores, 524 MB: 86 us, 6.1 TB/s), by the instructions a set takes beside its rows (about 250)
-// for hundreds (100k policy steps, 34M of their 40M rows here: 47 us, 2.9 TB/s).
+// for hundreds (100k policy steps, 29M of their 40M rows here: 38 us, 3.1 TB/s).
 template <int MODE, int TYPE, bool MASK, bool BIAS, int THREADS>
 __device__ __forceinline__ void wide_pass(const ChoiceArgs& a, const SetItem& im, int32_t index, Soft* shs, float* shf,
                                           const BiasShared* bias, TableSum& table, double (&tally)[3]) {
