@@ -564,9 +564,9 @@ int pb_sets_destroy(pb_sets* sets);
 #define PB_F16 2
 
 /* Scores of the rows of a pb_sets. num_buckets 0: no position bias. Else table_dev float32
- * [num_buckets] (at most 256), positions_dev int32 [rows] and buckets_dev uint8 [2 (reach + 1)] (an
- * entry of num_buckets or more counts as the last bucket): a row at position q takes bucket buckets_dev[min(|q|, reach)] for q <= 0 and
- * buckets_dev[reach + 1 + min(q, reach)] for q > 0. */
+ * [num_buckets] (at most 256), positions_dev int32 [rows] and buckets_dev uint8 [2 (reach + 1)]: a row
+ * at position q takes bucket buckets_dev[min(|q|, reach)] for q <= 0 and buckets_dev[reach + 1 + min(q, reach)]
+ * for q > 0 (an entry of num_buckets or more counts as the last bucket). */
 typedef struct {
     const void* scores_dev;       /* score_type [rows], element i at i * score_stride */
     const uint8_t* mask_dev;      /* NULL, or [rows]: 0 leaves a row out */
@@ -614,7 +614,7 @@ typedef struct {
  * stats_dev float32 [3]: the loss, scale * sum of w * kl, scale * sum of w over steps whose bound holds
  * (r A above the clipped product). log_probs_dev: the steps', as pb_choice_log_probs gives them. The
  * gradients are the loss's, laid out as in pb_choice_log_probs_backward. One pass over the scores
- * (sets of more than 2048 rows are read twice). */
+ * (sets of more than about 8190 rows are read twice). */
 int pb_policy_loss(const pb_sets* sets, const pb_choice_scores* scores, const pb_policy_terms* terms,
                    const int32_t* chosen_dev, float* stats_dev, float* log_probs_dev, void* grad_scores_dev,
                    float* grad_table_dev, void* work_dev, int64_t work_bytes, void* stream);
@@ -625,6 +625,9 @@ int pb_policy_loss(const pb_sets* sets, const pb_choice_scores* scores, const pb
 typedef struct pb_pairs pb_pairs;
 int pb_pairs_create(const int64_t* winners_host, const int64_t* losers_host, int64_t num_pairs, int64_t num_values,
                     const int64_t* seq_offsets_host, pb_pairs** out);
+/* The same from pairs on the device, written by work on `stream`; waits for it. */
+int pb_pairs_create_from_device(const int64_t* winners_dev, const int64_t* losers_dev, int64_t num_pairs,
+                                int64_t num_values, const int64_t* seq_offsets_host, void* stream, pb_pairs** out);
 int pb_pairs_destroy(pb_pairs* pairs);
 int64_t pb_preference_work_bytes(const pb_pairs* pairs);
 

@@ -41,7 +41,8 @@ EXPORTED_SYMBOLS = (
     "pb_era_corr_work_elems", "pb_era_corr_rows", "pb_fold_tree",
     "pb_rowlist_facts_get", "pb_set_gradients",
     "pb_sets_create", "pb_sets_destroy", "pb_choice_work_bytes", "pb_choice_log_probs",
-    "pb_choice_log_probs_backward", "pb_policy_loss", "pb_pairs_create", "pb_pairs_destroy",
+    "pb_choice_log_probs_backward", "pb_policy_loss", "pb_pairs_create", "pb_pairs_create_from_device",
+    "pb_pairs_destroy",
     "pb_preference_work_bytes", "pb_preference_loss",
 )
 
@@ -190,6 +191,7 @@ _SIGNATURES = {
     "pb_policy_loss": (ctypes.c_int, [_VP, ctypes.POINTER(PbChoiceScores), ctypes.POINTER(PbPolicyTerms)] + [_VP] * 6 +
                        [_I64, _VP]),
     "pb_pairs_create": (ctypes.c_int, [_VP, _VP, _I64, _I64, _VP, ctypes.POINTER(_VP)]),
+    "pb_pairs_create_from_device": (ctypes.c_int, [_VP, _VP, _I64, _I64, _VP, _VP, ctypes.POINTER(_VP)]),
     "pb_pairs_destroy": (ctypes.c_int, [_VP]),
     "pb_preference_work_bytes": (_I64, [_VP]),
     "pb_preference_loss": (ctypes.c_int, [_VP] * 4 + [_F32] * 3 + [_VP] * 4 + [_I64, _VP]),

@@ -1,12 +1,9 @@
 // C-ABI host layer of the choice and preference operators: their layouts (built on the host, kept on
 // the device), argument checks, workspaces.
 #include <algorithm>
-#include <atomic>
 #include <memory>
 #include <exception>
 #include <string>
-#include <system_error>
-#include <thread>
 #include <vector>
 
 #include "pb_internal.h"
@@ -202,72 +199,59 @@ int sets_create(const int64_t* off, int64_t num_sets, bool segments, pb_sets** o
     return PB_OK;
 }
 
-constexpr int64_t kManyPairs = 1 << 17;  // from which on several threads lay pairs out
+// Device memory for the time of a call.
+struct DeviceScratch {
+    void* at = nullptr;
+    ~DeviceScratch() {
+        if (at) (void)hipFree(at);
+    }
+};
 
-// f(0) .. f(threads - 1), a thread each; those that cannot be started run here.
-template <class F>
-void in_threads(int threads, const F& f) {
-    std::vector<std::thread> running;
-    running.reserve((size_t)threads);
-    for (int t = 1; t < threads; ++t) {
-        try {
-            running.emplace_back(f, t);
-        } catch (const std::system_error&) {
-            f(t);
+// The pairs by index: on the host, or (from_device) on the device, where `stream` has written them.
+int pairs_create(const char* who, const int64_t* winners, const int64_t* losers, int64_t num_pairs, int64_t num_values,
+                 const int64_t* seq_off, bool from_device, hipStream_t stream, pb_pairs** out) {
+    const auto bad = [&](int code, const char* what) {
+        return pb::api_fail(code, (std::string(who) + ": " + what).c_str());
+    };
+    if (num_values >= INT32_MAX || num_pairs >= ((int64_t)1 << 30))
+        return bad(PB_ERR_UNSUPPORTED, "at most 2^30 pairs and 2^31 - 2 values");
+    const char* range = "a pair names a value out of range";
+    std::vector<int32_t> host;  // winners, losers
+    if (!from_device && num_pairs > 0) {
+        host.resize((size_t)num_pairs * 2);
+        for (int64_t i = 0; i < 2 * num_pairs; ++i) {
+            const int64_t v = i < num_pairs ? winners[i] : losers[i - num_pairs];
+            if (v < 0 || v >= num_values) return bad(PB_ERR_RANGE, range);
+            host[(size_t)i] = (int32_t)v;
         }
     }
-    f(0);
-    for (std::thread& r : running) r.join();
-}
-
-int pairs_create(const int64_t* winners, const int64_t* losers, int64_t num_pairs, int64_t num_values,
-                 const int64_t* seq_off, pb_pairs** out) {
-    if (num_values >= INT32_MAX || num_pairs >= ((int64_t)1 << 30))
-        return pb::api_fail(PB_ERR_UNSUPPORTED, "pb_pairs_create: at most 2^30 pairs and 2^31 - 2 values");
-    // [winners | losers | entries], the entries of a value in the order of its pairs: a counting sort, each
-    // thread over all pairs for the values of its range (their counters and lists are its alone)
-    std::vector<int64_t> off((size_t)num_values + 1, 0);
-    const size_t words = (size_t)num_pairs * 4;
-    const std::unique_ptr<int32_t[]> host(new int32_t[words]);  // first touched by the threads
-    int32_t* entries = host.get() + 2 * num_pairs;
-    const int threads = num_pairs < kManyPairs ? 1 : (int)std::min(8u, std::max(1u, std::thread::hardware_concurrency()));
-    std::atomic<bool> in_range{true};
-    in_threads(threads, [&](int t) {
-        const int64_t p0 = num_pairs * t / threads, p1 = num_pairs * (t + 1) / threads;
-        for (int64_t p = p0; p < p1; ++p) {
-            const int64_t w = winners[p], l = losers[p];
-            if (w < 0 || w >= num_values || l < 0 || l >= num_values) {
-                in_range = false;
-                return;
-            }
-            host[(size_t)p] = (int32_t)w;
-            host[(size_t)(num_pairs + p)] = (int32_t)l;
-        }
-    });
-    if (!in_range) return pb::api_fail(PB_ERR_RANGE, "pb_pairs_create: a pair names a value out of range");
-    const int32_t *w32 = host.get(), *l32 = w32 + num_pairs;
-    const auto each_of = [&](int t, const auto& f) {  // f(value, pair, side) of the thread's values, in pair order
-        const int32_t v0 = (int32_t)(num_values * t / threads), v1 = (int32_t)(num_values * (t + 1) / threads);
-        for (int64_t p = 0; p < num_pairs; ++p) {
-            if (w32[p] >= v0 && w32[p] < v1) f(w32[p], (int32_t)p, 0);
-            if (l32[p] >= v0 && l32[p] < v1) f(l32[p], (int32_t)p, 1);
-        }
-    };
-    in_threads(threads, [&](int t) { each_of(t, [&](int32_t v, int32_t, int) { ++off[(size_t)v + 1]; }); });
-    for (int64_t v = 0; v < num_values; ++v) off[(size_t)v + 1] += off[(size_t)v];
-    std::vector<int64_t> next(off.begin(), off.end() - 1);
-    in_threads(threads, [&](int t) {
-        each_of(t, [&](int32_t v, int32_t p, int side) { entries[next[(size_t)v]++] = p * 2 + side; });
-    });
     std::unique_ptr<pb_pairs, void (*)(pb_pairs*)> h(new pb_pairs(), free_pairs);
+    std::vector<int64_t> off((size_t)num_values + 1, 0);
+    hipError_t e = hipGetDevice(&h->device);
+    if (e == hipSuccess) e = hipMalloc(&h->arena, std::max<size_t>(256, (size_t)num_pairs * 16));
+    if (e == hipSuccess && num_pairs > 0) {
+        DeviceScratch work;
+        int32_t wrong = 0;
+        e = hipMalloc(&work.at, pb::pair_layout_bytes(num_pairs, num_values));
+        int32_t* flag = static_cast<int32_t*>(work.at);
+        if (e == hipSuccess && from_device) {
+            if ((e = hipMemcpyAsync(flag, &wrong, sizeof(wrong), hipMemcpyHostToDevice, stream)) == hipSuccess &&
+                (e = pb::launch_narrow_pairs(winners, losers, num_pairs, num_values, h->arena, flag, stream)) == hipSuccess &&
+                (e = hipMemcpyAsync(&wrong, flag, sizeof(wrong), hipMemcpyDeviceToHost, stream)) == hipSuccess)
+                e = hipStreamSynchronize(stream);
+            if (e == hipSuccess && wrong) return bad(PB_ERR_RANGE, range);
+        } else if (e == hipSuccess) {
+            e = hipMemcpy(h->arena, host.data(), host.size() * sizeof(int32_t), hipMemcpyHostToDevice);
+        }
+        if (e == hipSuccess) e = pb::launch_pair_layout(h->arena, num_pairs, num_values, work.at, stream);
+        if (e == hipSuccess)
+            e = hipMemcpyAsync(off.data(), work.at, off.size() * sizeof(int64_t), hipMemcpyDeviceToHost, stream);
+        const hipError_t waited = hipStreamSynchronize(stream);  // whatever was enqueued uses `work` and `off`
+        if (e == hipSuccess) e = waited;
+    }
+    if (e != hipSuccess) return pb::api_hip_fail(e, who);
     int rc = sets_create(off.data(), num_values, false, &h->lists);
     if (rc == PB_OK && seq_off) rc = sets_create(seq_off, num_values, false, &h->seqs);
-    if (rc == PB_OK) {
-        hipError_t e = hipGetDevice(&h->device);
-        if (e == hipSuccess) e = hipMalloc(&h->arena, std::max<size_t>(256, words * 4));
-        if (e == hipSuccess && words > 0) e = hipMemcpy(h->arena, host.get(), words * 4, hipMemcpyHostToDevice);
-        if (e != hipSuccess) rc = pb::api_hip_fail(e, "pb_pairs_create");
-    }
     if (rc != PB_OK) return rc;
     h->p.winners = h->arena;
     h->p.losers = h->arena + num_pairs;
@@ -278,6 +262,22 @@ int pairs_create(const int64_t* winners, const int64_t* losers, int64_t num_pair
     if (h->seqs) h->p.seqs = h->seqs->s;
     *out = h.release();
     return PB_OK;
+}
+
+int pairs_entry(const char* who, const int64_t* winners, const int64_t* losers, int64_t num_pairs, int64_t num_values,
+                const int64_t* seq_off, bool from_device, hipStream_t stream, pb_pairs** out) {
+    const auto bad = [&](int code, const char* what) {
+        return pb::api_fail(code, (std::string(who) + ": " + what).c_str());
+    };
+    try {
+        if (!out) return bad(PB_ERR_INVALID, "null output");
+        *out = nullptr;
+        if (num_pairs < 0 || num_values < 0 || (num_pairs > 0 && (!winners || !losers)))
+            return bad(PB_ERR_INVALID, "bad shape or null pairs");
+        return pairs_create(who, winners, losers, num_pairs, num_values, seq_off, from_device, stream, out);
+    } catch (const std::exception&) {
+        return pb::api_fail(PB_ERR_NOMEM, "pairs: out of host memory");
+    }
 }
 
 // Sums that a workgroup leaves (none where there is one workgroup, which writes the results itself).
@@ -423,15 +423,14 @@ int pb_policy_loss(const pb_sets* s, const pb_choice_scores* in, const pb_policy
 
 int pb_pairs_create(const int64_t* winners_host, const int64_t* losers_host, int64_t num_pairs, int64_t num_values,
                     const int64_t* seq_offsets_host, pb_pairs** out) {
-    if (!out) return pb::api_fail(PB_ERR_INVALID, "pb_pairs_create: null output");
-    *out = nullptr;
-    if (num_pairs < 0 || num_values < 0 || (num_pairs > 0 && (!winners_host || !losers_host)))
-        return pb::api_fail(PB_ERR_INVALID, "pb_pairs_create: bad shape or null pairs");
-    try {
-        return pairs_create(winners_host, losers_host, num_pairs, num_values, seq_offsets_host, out);
-    } catch (const std::exception&) {
-        return pb::api_fail(PB_ERR_NOMEM, "pb_pairs_create: out of host memory");
-    }
+    return pairs_entry("pb_pairs_create", winners_host, losers_host, num_pairs, num_values, seq_offsets_host, false,
+                       nullptr, out);
+}
+
+int pb_pairs_create_from_device(const int64_t* winners_dev, const int64_t* losers_dev, int64_t num_pairs,
+                                int64_t num_values, const int64_t* seq_offsets_host, void* stream, pb_pairs** out) {
+    return pairs_entry("pb_pairs_create_from_device", winners_dev, losers_dev, num_pairs, num_values, seq_offsets_host,
+                       true, (hipStream_t)stream, out);
 }
 
 int pb_pairs_destroy(pb_pairs* pairs) {

@@ -609,6 +609,15 @@ hipError_t launch_preference(const PairLayout& p, PairArgs a, const float* value
                              char* work, hipStream_t stream);
 int64_t preference_work_bytes(const PairLayout& p);
 
+// ---- layout of pairs (pairs.hip) ----
+// pairs: int32 [winners | losers | entries]; fills the entries, and int64 [num_values + 1] list starts at
+// the head of `work` (pair_layout_bytes). num_pairs and num_values are at least 1, the pairs in range.
+size_t pair_layout_bytes(int64_t num_pairs, int64_t num_values);
+hipError_t launch_pair_layout(int32_t* pairs, int64_t num_pairs, int64_t num_values, void* work, hipStream_t stream);
+// int64 pairs as int32 [winners | losers]; *bad becomes 1 if one is out of range (taken as 0).
+hipError_t launch_narrow_pairs(const int64_t* winners, const int64_t* losers, int64_t num_pairs, int64_t num_values,
+                               int32_t* out, int32_t* bad, hipStream_t stream);
+
 // Sets the calling thread's error message (pb_last_error) and returns the code (capi.cpp).
 int api_fail(int code, const char* msg);
 int api_hip_fail(hipError_t e, const char* where);
