@@ -47,6 +47,53 @@ __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f
 // log x for x = 0 or above 1/2: 0 gives -inf, NaN stays NaN.
 __device__ __forceinline__ float log_of(float x) { return __builtin_amdgcn_logf(x) * 0.69314718055994530942f; }
 
+// What a step of a policy has once is taken to below float32's rounding: its loss terms cancel (advantages of
+// both signs, e^d - d - 1 of a small d), and its ratio is held against bounds. All in double it took half as
+// long again (policy loss of 480k sets 32 us, 24 so, 22.7 in float32 alone).
+//
+// log x within 2^-30 for finite x above 1/2 (else as log_of): x = 2^k m, m in [2/3, 4/3), and
+// log m = 2 (f + f^3 / 3 + ... + f^11 / 11), f = (m - 1) / (m + 1) with the quotient's remainder, |f| <= 1/5.
+__device__ __forceinline__ double fine_log(float x) {
+    if (!(x > 0.5f && x < kInf)) return (double)log_of(x);
+    const float half = __builtin_amdgcn_frexp_mantf(x);  // [1/2, 1)
+    const bool low = half < 0.666666687f;
+    const float m = low ? 2.0f * half : half;
+    const int k = __builtin_amdgcn_frexp_expf(x) - (low ? 1 : 0);
+    const float n = m - 1.0f, s = m + 1.0f, rest = m - (s - 1.0f);  // n, s + rest exact
+    const float inv = __builtin_amdgcn_rcpf(s), f = n * inv, q = f * f;
+    float p = 1.0f / 11;
+    p = __builtin_fmaf(p, q, 1.0f / 9);
+    p = __builtin_fmaf(p, q, 1.0f / 7);
+    p = __builtin_fmaf(p, q, 1.0f / 5);
+    p = __builtin_fmaf(p, q, 1.0f / 3);
+    const float small = __builtin_fmaf(p * q, f, (__builtin_fmaf(-f, s, n) - f * rest) * inv);
+    return __builtin_fma((double)k, 0.69314718055994531, 2.0 * ((double)f + (double)small));
+}
+
+// e^x and what it is more than the first terms of its series, e^x - 1 and e^x - 1 - x, a unit or so in the last
+// place of each: x = k log 2 + r, |r| <= log(2) / 2, and seven terms of r's series. Without the series for |x|
+// of 87 and more, infinities and NaN.
+struct FineExp {
+    float all, less_one, less_line;
+    __device__ __forceinline__ explicit FineExp(double x) {
+        const float hi = (float)x, lo = (float)(x - (double)hi);
+        const float k = __builtin_rintf(hi * 1.44269504f);
+        float r = __builtin_fmaf(k, -0.693145751953125f, hi);
+        r = __builtin_fmaf(k, -1.42860682e-6f, r) + lo;
+        float p = 1.0f / 5040;
+        p = __builtin_fmaf(p, r, 1.0f / 720);
+        p = __builtin_fmaf(p, r, 1.0f / 120);
+        p = __builtin_fmaf(p, r, 1.0f / 24);
+        p = __builtin_fmaf(p, r, 1.0f / 6);
+        p = __builtin_fmaf(p, r, 0.5f);
+        p *= r * r;
+        const bool near = __builtin_fabsf(hi) < 87.0f;
+        all = near ? __builtin_amdgcn_ldexpf(1.0f + (r + p), (int)k) : exp_of(hi);
+        less_one = k == 0.0f ? r + p : all - 1.0f;
+        less_line = k == 0.0f ? p : (all - 1.0f) - hi;
+    }
+};
+
 // Maxima that pass a NaN over (fmaxf first quiets operands that the compiler cannot see through).
 __device__ __forceinline__ float max2(float a, float b) {
     float r;
@@ -451,18 +498,18 @@ __device__ __forceinline__ PolicyIn load_policy(const ChoiceArgs& a, int64_t g) 
     return PolicyIn{a.advantages[g], a.old[g], a.ref ? a.ref[g] : 0.0f, a.weights ? a.weights[g] : 1.0f};
 }
 
-__device__ __forceinline__ float policy_step(const ChoiceArgs& a, const PolicyIn& in, float lp, bool tally, double (&sum)[3]) {
+// A step's gradient with respect to its log-probability lp, and its part of the sums.
+__device__ __forceinline__ float policy_step(const ChoiceArgs& a, const PolicyIn& in, double lp, bool tally, double (&sum)[3]) {
     const float w = in.w * a.scale;
-    const float ratio = exp_of(lp - in.old);
+    const float ratio = FineExp(lp - (double)in.old).all;
     const float free = ratio * in.adv;
     const float held = fminf(fmaxf(ratio, a.ratio_min), a.ratio_max) * in.adv;
     const bool clipped = free > held;
     float kl = 0.0f, slope = clipped ? 0.0f : -free;
     if (a.ref) {
-        const float d = in.ref - lp;
-        const float e = exp_of(d);
-        kl = e - d - 1.0f;
-        slope += a.kl_weight * (1.0f - e);
+        const FineExp e((double)in.ref - lp);
+        kl = e.less_line;
+        slope -= a.kl_weight * e.less_one;
     }
     if (tally) {
         sum[0] += (double)(w * (a.kl_weight * kl - (clipped ? held : free)));
@@ -681,7 +728,7 @@ struct TileIn {
 // of 30000 sets of 300 rows: 32 us, 40 with them; 66 and 73 for steps in float32 with their backward). About 700 vector instructions for 512 rows, 1200 with
 // mask, bias and the policy's steps: past the first few thousand tiles their issue bounds it, before that
 // the chain from the loads to the stores. 2.4M rows of 100k sets with mask and bias: log-probabilities of
-// the steps 9.5 us, their backward with the table's gradient 13.4 us; the policy loss of 480k sets 22.6 us.
+// the steps 9.2 us, their backward with the table's gradient 12.9 us; the policy loss of 480k sets 24.0 us.
 template <int MODE, int TYPE, bool MASK, bool BIAS>
 __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, TileIn<MODE, TYPE, MASK, BIAS>& in, TileShared& sh,
                                           const BiasShared* bias, TableSum& table, double (&tally)[3]) {
@@ -808,10 +855,14 @@ __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, TileIn<MODE, TYPE
                 if (STEPS) {
                     // left out: a choice outside the set or masked, a set without probability
                     const bool counts = chosen[r] >= 0 && (SOFT ? sum != 0.0f : top != -kInf);
-                    const float lp = SOFT && counts ? (picked[r] - top) - ls : 0.0f;
-                    if (SOFT) a.log_probs[g] = lp;
+                    float lp = SOFT && counts ? (picked[r] - top) - ls : 0.0f;
                     if (MODE == kStepsBack && counts) coef[r] = in.given[r];
-                    if (MODE == kPolicy && counts) coef[r] = policy_step(a, in.pol[r], lp, true, tally);
+                    if (MODE == kPolicy && counts) {
+                        const double fine = ((double)picked[r] - (double)top) - fine_log(sum);
+                        lp = (float)fine;
+                        coef[r] = policy_step(a, in.pol[r], fine, true, tally);
+                    }
+                    if (SOFT) a.log_probs[g] = lp;
                     if (GRAD) sh.factor[s] = counts ? (SOFT ? -coef[r] * __builtin_amdgcn_rcpf(sum) : -coef[r]) : 0.0f;
                     if (!counts) chosen[r] = -1;
                 }
@@ -866,7 +917,7 @@ __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, TileIn<MODE, TYPE
 // store, one exponential each, so that a set of up to kSetWideRows rows is read once; a longer one's parts are
 // read a second time. Bound by memory for sets of thousands of rows (backward of 4096 sets of 32000
 // bfloat16 scores, 524 MB: 86 us, 6.1 TB/s), by the instructions a set takes beside its rows (about 250)
-// for hundreds (100k policy steps, 29M of their 40M rows here: 38 us, 3.1 TB/s).
+// for hundreds (100k policy steps, 29M of their 40M rows here: 41 us, 2.8 TB/s).
 template <int MODE, int TYPE, bool MASK, bool BIAS, int THREADS>
 __device__ __forceinline__ void wide_pass(const ChoiceArgs& a, const SetItem& im, int32_t index, Soft* shs, float* shf,
                                           const BiasShared* bias, TableSum& table, double (&tally)[3]) {
@@ -983,12 +1034,13 @@ __device__ __forceinline__ void wide_pass(const ChoiceArgs& a, const SetItem& im
     float extra = 0.0f;
     if (STEPS) {
         counts = counts && (SOFT ? t.sum != 0.0f : lse != -kInf);
-        const float lp = SOFT && counts ? (xc - t.top) - ls : 0.0f;
+        const double fine = MODE == kPolicy && counts ? ((double)xc - (double)t.top) - fine_log(t.sum) : 0.0;
+        const float lp = MODE == kPolicy ? (float)fine : SOFT && counts ? (xc - t.top) - ls : 0.0f;
         if (SOFT && first) a.log_probs[g] = lp;
         if (GRAD) {
             float coef = 0.0f;
             if (MODE == kStepsBack && counts) coef = given;
-            if (MODE == kPolicy && counts) coef = policy_step(a, pol, lp, first, tally);
+            if (MODE == kPolicy && counts) coef = policy_step(a, pol, fine, first, tally);
             const float f = counts ? (SOFT ? -coef * __builtin_amdgcn_rcpf(t.sum) : -coef) : 0.0f;
             const float fw = f * own;
             const int64_t row = r0 + c - sp.q0;
