@@ -725,7 +725,7 @@ struct TileIn {
 // One tile of short sets by one wave: the maximum and the sum of exponentials by two segmented scans, which
 // leave them in LDS by set; a lane to a set then forms log-probabilities, losses and slopes, 64 sets at a
 // time; the rows take their set's factor from LDS. A tile of one set has no need of the scans (policy steps
-// of 30000 sets of 300 rows: 32 us, 40 with them; 66 and 73 for steps in float32 with their backward). About 700 vector instructions for 512 rows, 1200 with
+// of 30000 sets of 300 rows: 37 us, 44 with them; 68 and 76 for steps in float32 with their backward). About 700 vector instructions for 512 rows, 1200 with
 // mask, bias and the policy's steps: past the first few thousand tiles their issue bounds it, before that
 // the chain from the loads to the stores. 2.4M rows of 100k sets with mask and bias: log-probabilities of
 // the steps 9.2 us, their backward with the table's gradient 12.9 us; the policy loss of 480k sets 24.0 us.

@@ -498,10 +498,10 @@ hipError_t launch_predict_bins(const uint8_t* bins, int64_t N, int64_t ld, int32
 // a workgroup each, sets of at most kSetWideRows rows and the parts (part `part` of `parts`) of those that
 // are longer, a set's consecutive; `split` names the first of each.
 // A wave waits for no other wave, so it takes what its registers hold (the policy loss of 40000 sets of 600
-// rows in bfloat16: 41 us, by workgroups 108; of 20000 of 2000 rows 35 and 62; steps in float32 with their
-// backward 150 and 330, 202 and 236). Segments save the lanes that a tile ended by a longer set would leave
-// empty (100k sets of 1 to 100k rows, most of them short: 84 us, 88 without; neither way where few are
-// short).
+// rows in bfloat16: 46 us, by workgroups 125; of 20000 of 2000 rows 38 and 70; steps in float32 with their
+// backward 145 and 326, 203 and 235; 28 to 30 us either way for a few hundred sets). Segments save the lanes
+// that a tile ended by a longer set would leave empty (100k sets of 1 to 100k rows, most of them short: 91 us,
+// 95 without; steps in float32 287 and 290; 1 us either way for a few thousand sets).
 constexpr int kSetTileRows = 512;
 constexpr int kSetTileSets = 128;
 constexpr int kSetShort = kSetTileRows - 8;

@@ -22,7 +22,7 @@ def draw(values, pairs, hubs, seed):
 # around the entries of a wave and a workgroup, and around the digits that a value has
 @pytest.mark.parametrize("values,pairs", [(1, 1), (1, 5000), (2, 31), (3, 32), (255, 33), (256, 511), (257, 512),
                                           (300, 513), (7, 2047), (65_535, 2048), (65_536, 2049), (65_537, 20_000),
-                                          (100_003, 300_001), ((1 << 24) + 3, 4097)])
+                                          (100_003, 300_001), (70_001, 530_003), ((1 << 24) + 3, 4097)])
 @pytest.mark.parametrize("hubs", [False, True])
 def test_gradients(hip, values, pairs, hubs):
     """The slopes of a value's pairs, summed in double: each is below 1 and off by at most 40 U (margins of up to
