@@ -612,7 +612,8 @@ typedef struct {
 /* With r = exp(log p - old), A the advantage and d = ref - log p, summed over the steps:
  *   loss = scale * w * (kl_weight * kl - min(r A, clip(r, ratio_min, ratio_max) A)), kl = e^d - d - 1.
  * stats_dev float32 [3]: the loss, scale * sum of w * kl, scale * sum of w over steps whose bound holds
- * (r A above the clipped product). log_probs_dev: the steps', as pb_choice_log_probs gives them. The
+ * (r A above the clipped product). Steps of weight 0, a KL term of weight 0 and a ratio of advantage 0 count
+ * for nothing, also where they overflow. log_probs_dev: the steps', as pb_choice_log_probs gives them. The
  * gradients are the loss's, laid out as in pb_choice_log_probs_backward. One pass over the scores
  * (sets of more than about 8190 rows are read twice). */
 int pb_policy_loss(const pb_sets* sets, const pb_choice_scores* scores, const pb_policy_terms* terms,

@@ -354,7 +354,8 @@ def policy_loss(scores: torch.Tensor, sets: ChoiceSets, chosen: torch.Tensor, ad
 
     over the steps (sets) that are not left out (see choice_log_probs). advantages, old_log_probs,
     ref_log_probs and weights (w, default 1) are float32 per set; without ref_log_probs there is no KL
-    term. scale is the caller's mean: 1 / the number of steps, or 1 for the sum that a boosting round
+    term. What has weight, kl_weight or advantage 0 counts for nothing, also where it overflows (`kl` tells the
+    KL term whatever its weight). scale is the caller's mean: 1 / the number of steps, or 1 for the sum that a boosting round
     takes."""
     c, keep = _scores(scores, sets, mask, bias)
     dev, g = sets.device, sets.num_sets

@@ -498,21 +498,26 @@ __device__ __forceinline__ PolicyIn load_policy(const ChoiceArgs& a, int64_t g) 
     return PolicyIn{a.advantages[g], a.old[g], a.ref ? a.ref[g] : 0.0f, a.weights ? a.weights[g] : 1.0f};
 }
 
-// A step's gradient with respect to its log-probability lp, and its part of the sums.
+// A step's gradient with respect to its log-probability lp, and its part of the sums. Ratio and KL term may
+// overflow: where their weight, kl_weight or advantage is 0 they count for nothing all the same.
 __device__ __forceinline__ float policy_step(const ChoiceArgs& a, const PolicyIn& in, double lp, bool tally, double (&sum)[3]) {
     const float w = in.w * a.scale;
+    if (w == 0.0f) return 0.0f;
     const float ratio = FineExp(lp - (double)in.old).all;
-    const float free = ratio * in.adv;
+    const float free = in.adv == 0.0f && ratio == kInf ? 0.0f : ratio * in.adv;
     const float held = fminf(fmaxf(ratio, a.ratio_min), a.ratio_max) * in.adv;
     const bool clipped = free > held;
-    float kl = 0.0f, slope = clipped ? 0.0f : -free;
+    float kl = 0.0f, term = 0.0f, slope = clipped ? 0.0f : -free;
     if (a.ref) {
         const FineExp e((double)in.ref - lp);
         kl = e.less_line;
-        slope -= a.kl_weight * e.less_one;
+        if (a.kl_weight != 0.0f) {
+            term = a.kl_weight * kl;
+            slope -= a.kl_weight * e.less_one;
+        }
     }
     if (tally) {
-        sum[0] += (double)(w * (a.kl_weight * kl - (clipped ? held : free)));
+        sum[0] += (double)(w * (term - (clipped ? held : free)));
         sum[1] += (double)(w * kl);
         sum[2] += clipped ? (double)w : 0.0;
     }
