@@ -635,7 +635,8 @@ int64_t pb_preference_work_bytes(const pb_pairs* pairs);
 /* Paired log ratios: z = beta (a_winner - a_loser), a = values - ref (ref_dev NULL: 0), summed over each
  * run's steps where the pairs have runs; loss_dev[0] = scale * sum of w (-(1 - e) log s(z) - e log s(-z))
  * with s the sigmoid, e label_smoothing and w weights_dev [num_pairs] (NULL: 1). grad_dev: the loss's
- * gradient, one entry per value (per step); margins_dev [num_pairs]: z. All float32. */
+ * gradient, one entry per value (per step); margins_dev [num_pairs]: z. All float32. A pair of weight 0 and a
+ * side of the loss whose factor (1 - e or e) is 0 count for nothing, also where z is infinite. */
 int pb_preference_loss(const pb_pairs* pairs, const float* values_dev, const float* ref_dev, const float* weights_dev,
                        float beta, float label_smoothing, float scale, float* loss_dev, float* grad_dev,
                        float* margins_dev, void* work_dev, int64_t work_bytes, void* stream);

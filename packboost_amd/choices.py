@@ -393,7 +393,8 @@ def preference_loss(values: torch.Tensor, pairs: PreferencePairs, *, ref_values:
 
     values and ref_values are float32 per value (per step), weights (w, default 1) per pair. Values are
     scores of rows (a reward model) or log-probabilities of steps (choice_log_probs with `chosen`, whose
-    backward takes the gradient on); the ref_values those of a reference model."""
+    backward takes the gradient on); the ref_values those of a reference model. A pair of weight 0 and a
+    side of the loss whose factor is 0 count for nothing, also where the margin is infinite."""
     if not isinstance(pairs, PreferencePairs):
         raise ValueError("pairs must be PreferencePairs")
     dev, n = pairs.device, pairs.num_steps

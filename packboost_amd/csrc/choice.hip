@@ -1393,12 +1393,14 @@ __global__ __launch_bounds__(kBlock) void pair_kernel(PairArgs a) {
             const float z = (float)((double)a.beta * d[k]);
             const float ws = weight[k] * a.scale;
             const float t = expf(-fabsf(z)), soft = log1pf(t);
-            const float e = a.smoothing;
+            const float e = a.smoothing, h = 1.0f - e;
             const float up = z > 0.0f ? 1.0f / (1.0f + t) : t / (1.0f + t);    // sigmoid(z)
             const float down = z > 0.0f ? t / (1.0f + t) : 1.0f / (1.0f + t);  // sigmoid(-z)
             __builtin_nontemporal_store(z, a.margins + p);
-            a.slopes[p] = a.beta * ws * (e * up - (1.0f - e) * down);
-            sum += (double)(ws * ((1.0f - e) * (soft + fmaxf(-z, 0.0f)) + e * (soft + fmaxf(z, 0.0f))));
+            a.slopes[p] = ws == 0.0f ? 0.0f : a.beta * ws * (e * up - h * down);
+            // a term of factor 0 counts for nothing, whatever its margin
+            const float lost = (h == 0.0f ? 0.0f : h * (soft + fmaxf(-z, 0.0f))) + (e == 0.0f ? 0.0f : e * (soft + fmaxf(z, 0.0f)));
+            if (ws != 0.0f) sum += (double)(ws * lost);
         }
     }
     sum = block_sum(sum, sh);

@@ -89,3 +89,45 @@ def test_steps_without_advantage(hip):
     r = policy_case(s, SIZES, chosen, np.zeros(len(SIZES)), lp - 100.0)
     assert float(r.loss) == 0.0 and float(r.clipped) == 0.0
     assert torch.equal(r.grad_scores, torch.zeros_like(r.grad_scores))
+
+
+@pytest.mark.parametrize("ref", [False, True])
+def test_preference_terms_of_no_weight(hip, ref):
+    """Margins that are infinite on the side of a factor of 0, and pairs of weight 0, count for nothing."""
+    from packboost_amd import PreferencePairs, preference_loss
+
+    inf, nan = math.inf, math.nan
+    v = torch.tensor([0.5, 0.25, -inf, 1.0, nan], device=DEV)
+    kw = dict(ref_values=torch.zeros(5, device=DEV)) if ref else {}
+    alone = preference_loss(v[:2].contiguous(), PreferencePairs([0], [1], num_values=2), beta=1.0)
+    # the loser cannot be had at all: the loss's limit is 0, and so is the slope's
+    r = preference_loss(v, PreferencePairs([0, 3], [1, 2], num_values=5), beta=1.0, **kw)
+    assert float(r.loss) == float(alone.loss) and float(r.margins[1]) == inf
+    assert r.grad.tolist() == alone.grad.tolist() + [0.0, 0.0, 0.0]
+    # the same with labels the other way round
+    one = preference_loss(v[:2].contiguous(), PreferencePairs([0], [1], num_values=2), beta=1.0, label_smoothing=1.0)
+    r = preference_loss(v, PreferencePairs([0, 2], [1, 3], num_values=5), beta=1.0, label_smoothing=1.0, **kw)
+    assert float(r.loss) == float(one.loss) and r.grad.tolist() == one.grad.tolist() + [0.0, 0.0, 0.0]
+    # weight 0: margins of -inf, inf and NaN
+    w = torch.tensor([1.0, 0.0, 0.0, 0.0], device=DEV)
+    for e in (0.0, 0.25, 1.0):
+        want = preference_loss(v[:2].contiguous(), PreferencePairs([0], [1], num_values=2), beta=1.0, label_smoothing=e)
+        r = preference_loss(v, PreferencePairs([0, 2, 3, 4], [1, 3, 2, 0], num_values=5), beta=1.0, label_smoothing=e,
+                            weights=w, **kw)
+        assert float(r.loss) == float(want.loss) and r.grad.tolist() == want.grad.tolist() + [0.0, 0.0, 0.0]
+    # what does count stays visible
+    assert float(preference_loss(v, PreferencePairs([2], [3], num_values=5), beta=1.0, **kw).loss) == inf
+    assert math.isnan(float(preference_loss(v, PreferencePairs([4], [3], num_values=5), beta=1.0, **kw).loss))
+
+
+def test_preference_of_steps_that_cannot_be(hip):
+    """A choice whose score is -inf has log-probability -inf; the sequence that holds it loses for nothing."""
+    from packboost_amd import ChoiceSets, PreferencePairs, choice_log_probs, preference_loss
+
+    s = torch.tensor([0.0, 1.0, -math.inf, 0.5, 0.0, 0.0], device=DEV)
+    lp, _ = choice_log_probs(s, ChoiceSets([0, 2, 4, 6]), chosen=torch.zeros(3, dtype=torch.int32, device=DEV))
+    assert float(lp[1]) == -math.inf
+    r = preference_loss(lp, PreferencePairs([0, 0], [1, 2], offsets=[0, 1, 2, 3]), beta=0.5)
+    z = 0.5 * (float(lp[0]) - float(lp[2]))
+    assert float(r.loss) == pytest.approx(math.log1p(math.exp(-z)), rel=8 * U)
+    assert torch.isfinite(r.grad).all() and float(r.grad[1]) == 0.0
