@@ -594,7 +594,9 @@ int pb_choice_log_probs(const pb_sets* sets, const pb_choice_scores* scores, con
 
 /* Gradients of the scores (score_type [rows], stride 1, 0 where masked) and of the bias table (float32
  * [num_buckets]) from grad_dev, that of the rows' (chosen_dev NULL) or the steps' log-probabilities;
- * masked rows' entries are not used. lse_dev: pb_choice_log_probs' for the same scores. */
+ * masked rows' entries are not used. lse_dev: pb_choice_log_probs' for the same scores. A bucket's rows are
+ * summed in whole numbers of 2^-34 or less of its largest gradient (a wave's at a time, in a fixed
+ * order), then in double, and rounded once. */
 int pb_choice_log_probs_backward(const pb_sets* sets, const pb_choice_scores* scores, const int32_t* chosen_dev,
                                  const float* grad_dev, const float* lse_dev, void* grad_scores_dev,
                                  float* grad_table_dev, void* work_dev, int64_t work_bytes, void* stream);

@@ -391,6 +391,15 @@ __device__ __forceinline__ double wave_sum(double v) {
     return v;
 }
 
+// v of another lane; CTRL as in lane_move
+template <int CTRL>
+__device__ __forceinline__ double lane_move(double v) {
+    const long long b = __double_as_longlong(v);
+    const int lo = __builtin_amdgcn_update_dpp((int)b, (int)b, CTRL, 0xf, 0xf, false);
+    const int hi = __builtin_amdgcn_update_dpp((int)(b >> 32), (int)(b >> 32), CTRL, 0xf, 0xf, false);
+    return __longlong_as_double((long long)hi << 32 | (uint32_t)lo);
+}
+
 template <class F>
 __device__ F block_sum(F v, F* sh) {
     v = wave_sum(v);
@@ -524,72 +533,124 @@ __device__ __forceinline__ float policy_step(const ChoiceArgs& a, const PolicyIn
     return w * slope;
 }
 
-// The table's gradient as a wave gathers it: bins of whole numbers in units of 2^(e - 38), 2^e above
-// every gradient so far, so that their sums do not depend on the order of the atomics. A gradient is
-// rounded to 2^(e - 30) (what that takes is below 2^-31 * 2^e a row); a larger one raises e and halves what
-// the bins hold so often, to the nearest. Copies of the bins keep lanes that meet in a bucket apart. 2^25
-// rows of a wave fit.
+// The table's gradient as a wave gathers it: bins of whole numbers, bin i's in units of 2^-shift[i], so that
+// their sums do not depend on the order of the atomics. A bucket has copies of its bin, which keep lanes that
+// meet in it apart. Each bin's own gradients set its unit, so that what other buckets hold takes no bits from
+// it: a first one, and each one of 2^38 units or more, makes room for 16 times itself, and the bin is brought to
+// the larger unit, to the nearest. A gradient is so rounded to 2^-34 or less of the largest in its bin (one unit
+// for the whole wave lost a bucket's sum where another held gradients of 2^31 times its own; it took 27.2 us a call
+// where this takes 28.2, for the policy loss of 480k sets). A wave's rows, at most about 2^24, stay below 2^62 units.
 struct TableSum {
-    unsigned long long* bins;  // [kBins] of this wave
+    static constexpr int kUnset = 300;             // above every unit's exponent: any gradient but 0 is too large
+    static constexpr float kMost = 274877906944.0f;  // 2^38
+    unsigned long long* bins;  // [kBins] of this wave: bucket b's from b << copy_bits on
+    int* shift;                // [kBins]
     int* bad;                  // [num_buckets]: a gradient that is not finite
-    int copies, e;
-    float limit;               // 2^e, 0 before the first gradient
+    int copy_bits;
+    bool fresh;  // no gradient yet
 
-    __device__ void start(const ChoiceArgs& a, unsigned long long* b, int* flags) {
+    __device__ __forceinline__ void start(const ChoiceArgs& a, unsigned long long* b, int* shifts, int* flags) {
         bins = b;
+        shift = shifts;
         bad = flags;
-        copies = 1;
-        while (copies * 2 * a.num_buckets <= kBins && copies < 32) copies *= 2;
-        e = 0;
-        limit = 0.0f;
-        for (int i = (int)threadIdx.x & (kWave - 1); i < kBins; i += kWave) bins[i] = 0;
+        fresh = true;
+        copy_bits = 0;
+        while ((a.num_buckets << (copy_bits + 1)) <= kBins && copy_bits < 5) ++copy_bits;
+        for (int i = (int)threadIdx.x & (kWave - 1); i < kBins; i += kWave) {
+            bins[i] = 0;
+            shift[i] = kUnset;
+        }
         wave_sync();
     }
 
-    // raises e above every lane's `big`, finite; the whole wave
-    __device__ __forceinline__ void make_room(float big) {
-        if (__any(big >= limit && big > 0.0f)) {
-            int now;
-            (void)frexpf(wave_max(big), &now);
-            const int by = limit > 0.0f ? min(now - e, 62) : 62;
+    __device__ __forceinline__ int bin_of(int b) const {
+        return (b << copy_bits) + ((int)threadIdx.x & ((1 << copy_bits) - 1));
+    }
+
+    // larger units for the bins of the rows in `over`; the whole wave. Which rows these are was decided with the
+    // units before, so that the new ones are the same in any order.
+    __device__ __forceinline__ void make_room(const float (&g)[kRun], const Buckets& buckets, uint32_t over) {
+        const int lane = (int)threadIdx.x & (kWave - 1);
+        int was[kBins / kWave];
+        if (!fresh) {
+#pragma unroll
+            for (int j = 0; j < kBins / kWave; ++j) was[j] = shift[j * kWave + lane];
             wave_sync();
-#pragma unroll 1
-            for (int i = (int)threadIdx.x & (kWave - 1); i < kBins; i += kWave) {
-                const long long t = (long long)bins[i];
-                bins[i] = (unsigned long long)((t + (1ll << (by - 1))) >> by);
+        }
+        bool finite = true;
+#pragma unroll
+        for (int k = 0; k < kRun; ++k) {
+            const bool in = fabsf(g[k]) < kInf;
+            finite = finite && in;
+            atomicMin(&shift[bin_of(buckets.at(k))], in && (over >> k & 1u) ? 34 - __builtin_amdgcn_frexp_expf(g[k]) : kUnset);
+        }
+        if (!finite) {
+#pragma unroll
+            for (int k = 0; k < kRun; ++k)
+                if (!(fabsf(g[k]) < kInf)) bad[buckets.at(k)] = 1;
+        }
+        wave_sync();
+        if (!fresh) {
+#pragma unroll
+            for (int j = 0; j < kBins / kWave; ++j) {
+                const int i = j * kWave + lane, by = was[j] == kUnset ? 0 : was[j] - shift[i];
+                if (by > 0) {
+                    const long long t = (long long)bins[i];
+                    bins[i] = by > 62 ? 0ull : (unsigned long long)((t + (1ll << (by - 1))) >> by);
+                }
             }
             wave_sync();
-            e = now;
-            limit = ldexpf(1.0f, now);
         }
+        fresh = false;
     }
 
     __device__ __forceinline__ void add(const float (&g)[kRun], const Buckets& buckets) {
-        float big = 0.0f;
+        float t[kRun];
+        uint32_t over = 0;
 #pragma unroll
         for (int k = 0; k < kRun; ++k) {
-            const float m = fabsf(g[k]);
-            big = m < kInf ? fmaxf(big, m) : big;
+            t[k] = __builtin_amdgcn_ldexpf(g[k], fresh ? kUnset : shift[bin_of(buckets.at(k))]);
+            over |= fabsf(t[k]) < kMost ? 0u : 1u << k;
         }
-        make_room(big);
-        const int mine = (int)threadIdx.x & (copies - 1);
+        if (__any(over != 0)) {
+            make_room(g, buckets, over);
+#pragma unroll
+            for (int k = 0; k < kRun; ++k)
+                t[k] = fabsf(g[k]) < kInf ? __builtin_amdgcn_ldexpf(g[k], shift[bin_of(buckets.at(k))]) : 0.0f;
+        }
 #pragma unroll
         for (int k = 0; k < kRun; ++k) {
-            if (g[k] == 0.0f) continue;
-            const int b = buckets.at(k);
-            if (fabsf(g[k]) < kInf) {
-                const long long t = (long long)__float2int_rn(ldexpf(g[k], 30 - e)) << 8;
-                atomicAdd(&bins[b * copies + mine], (unsigned long long)t);
-            } else {
-                bad[b] = 1;
-            }
+            // the nearest whole number: the low bits of t + 1.5 2^52
+            const long long n = __double_as_longlong((double)t[k] + 6755399441055744.0) - 0x4338000000000000ll;
+            atomicAdd(&bins[bin_of(buckets.at(k))], (unsigned long long)n);
         }
     }
 
-    __device__ __forceinline__ double value(int b) const {  // of bucket b
-        long long t = 0;
-        for (int c = 0; c < copies; ++c) t += (long long)bins[b * copies + c];
-        return ldexp((double)t, e - 38);
+    // The buckets' sums in the place of the bins, a double each; the whole wave. A bucket's slot lies at or before
+    // its bins, all of which have been read.
+    __device__ __forceinline__ void finish() {
+        const int lane = (int)threadIdx.x & (kWave - 1);
+        double v[kBins / kWave];
+        wave_sync();
+#pragma unroll
+        for (int j = 0; j < kBins / kWave; ++j) {
+            const int i = j * kWave + lane;
+            v[j] = ldexp((double)(long long)bins[i], -shift[i]);
+        }
+        wave_sync();
+#pragma unroll
+        for (int j = 0; j < kBins / kWave; ++j) {  // lanes of one bucket, which hold the same after each step
+            if (copy_bits > 0) v[j] += lane_move<0xb1>(v[j]);   // quad_perm:[1,0,3,2]
+            if (copy_bits > 1) v[j] += lane_move<0x4e>(v[j]);   // quad_perm:[2,3,0,1]
+            if (copy_bits > 2) v[j] += lane_move<0x141>(v[j]);  // row_half_mirror
+            if (copy_bits > 3) v[j] += lane_move<0x140>(v[j]);  // row_mirror
+            if (copy_bits > 4) v[j] += __shfl_xor(v[j], 16);
+        }
+        if ((lane & ((1 << copy_bits) - 1)) == 0)
+#pragma unroll
+            for (int j = 0; j < kBins / kWave; ++j)
+                reinterpret_cast<double*>(bins)[(j * kWave + lane) >> copy_bits] = v[j];
+        wave_sync();
     }
 };
 
@@ -1135,17 +1196,7 @@ __device__ __forceinline__ void leave_sums(const ChoiceArgs& a, int block, doubl
         }
     }
     if (TABLE) {
-        // each wave's values in the place of its bins: bucket b's are all read before slot b is written,
-        // since a lane's bucket lies at or after the lane's slot and the wave takes 64 at a time
-        double* own = reinterpret_cast<double*>(bins[wave]);
-        wave_sync();
-#pragma unroll 1
-        for (int b0 = 0; b0 < a.num_buckets; b0 += kWave) {
-            const double t = b0 + lane < a.num_buckets ? table.value(b0 + lane) : 0.0;
-            wave_sync();
-            if (b0 + lane < a.num_buckets) own[b0 + lane] = t;
-            wave_sync();
-        }
+        table.finish();
         __syncthreads();
         for (int b = tid; b < a.num_buckets; b += kBlock) {
             double t = 0.0;
@@ -1169,13 +1220,14 @@ __global__ __launch_bounds__(kBlock, 4) void tile_kernel(ChoiceArgs a) {
     __shared__ TileShared tiles[kWaves];
     __shared__ BiasShared bias;
     __shared__ unsigned long long bins[TABLE ? kWaves : 1][kBins];
+    __shared__ int shifts[TABLE ? kWaves : 1][kBins];
     __shared__ int bad[kMaxBuckets];
     __shared__ double shd[kWaves * 3];
     const int tid = (int)threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     TableSum table;
     if (TABLE) {
         for (int b = tid; b < kMaxBuckets; b += kBlock) bad[b] = 0;
-        table.start(a, bins[wave], bad);
+        table.start(a, bins[wave], shifts[wave], bad);
     }
     double tally[3] = {0.0, 0.0, 0.0};
     const int lane = tid & (kWave - 1), step = (int)gridDim.x * kWaves;
@@ -1203,6 +1255,7 @@ __global__ __launch_bounds__(kBlock) void wide_kernel(ChoiceArgs a, int mid_bloc
     constexpr bool TABLE = kTable<MODE, BIAS>;
     __shared__ BiasShared bias;
     __shared__ unsigned long long bins[TABLE ? kWaves : 1][kBins];
+    __shared__ int shifts[TABLE ? kWaves : 1][kBins];
     __shared__ int bad[kMaxBuckets];
     __shared__ Soft shs[kWaves];
     __shared__ float shf[kWaves];
@@ -1211,7 +1264,7 @@ __global__ __launch_bounds__(kBlock) void wide_kernel(ChoiceArgs a, int mid_bloc
     TableSum table;
     if (TABLE) {
         for (int b = tid; b < kMaxBuckets; b += kBlock) bad[b] = 0;
-        table.start(a, bins[wave], bad);
+        table.start(a, bins[wave], shifts[wave], bad);
     }
     if (BIAS) stage_bias(a, bias);
     double tally[3] = {0.0, 0.0, 0.0};

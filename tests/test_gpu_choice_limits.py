@@ -131,3 +131,104 @@ def test_preference_of_steps_that_cannot_be(hip):
     z = 0.5 * (float(lp[0]) - float(lp[2]))
     assert float(r.loss) == pytest.approx(math.log1p(math.exp(-z)), rel=8 * U)
     assert torch.isfinite(r.grad).all() and float(r.grad[1]) == 0.0
+
+
+def bucket_case(sizes, far_sets, seed=0, num=16, reach=32):
+    """Sets whose positions name buckets up to the reference, but for those of `far_sets`, which name the ones
+    after it."""
+    from packboost_amd import ChoiceSets, PositionBias, PositionBuckets
+
+    r = np.random.default_rng(seed)
+    off = offsets_of(sizes)
+    n = int(off[-1])
+    pos = -(np.arange(n) % 23).astype(np.int32)
+    far = np.repeat(np.isin(np.arange(len(sizes)), list(far_sets)), sizes)
+    pos[far] = 1 - pos[far]
+    pb = PositionBuckets(num, reach)
+    table = (0.3 * r.standard_normal(num)).astype(np.float32)
+    s = r.standard_normal(n).astype(np.float32)
+    d = {"off": off, "size": np.diff(off), "keep": np.ones(n, bool), "ids": pb(pos).astype(np.int64), "r": r,
+         "c": np.floor(r.random(len(sizes)) * np.diff(off)).astype(np.int64), "sets": ChoiceSets(off), "scores": torch.from_numpy(s).to(DEV),
+         "bias": PositionBias(torch.from_numpy(table).to(DEV), torch.from_numpy(pos).to(DEV), pb)}
+    d["x"] = s.astype(np.float64) + table.astype(np.float64)[d["ids"]]
+    d["chosen"] = torch.from_numpy(d["c"].astype(np.int32)).to(DEV)
+    return d
+
+
+def check_buckets(d, got, g, size, room=0.0):
+    """A bucket's sum is off by what its own rows' gradients are off by (`size`, the sum of a row's absolute terms,
+    and `room`), by 2^-30 of its own largest one a row, and by its rounding. No other bucket's size comes in."""
+    nb = d["bias"].buckets.num_buckets
+    tol = U * (4 * np.abs(d["x"]).max() + 100)
+    want = np.bincount(d["ids"], g, minlength=nb)
+    big = np.zeros(nb)
+    np.maximum.at(big, d["ids"], np.abs(g))
+    lim = np.bincount(d["ids"], size * (tol + 4 * U) + room, minlength=nb) + np.bincount(d["ids"], minlength=nb) * big * 2.0 ** -30
+    assert np.all(np.abs(got.double().cpu().numpy() - want) <= lim + 2 * U * np.abs(want))
+    near = np.unique(d["ids"][d["ids"] < nb // 2])
+    assert np.all(lim[near] < 1e-3 * np.bincount(d["ids"], np.abs(g), minlength=nb)[near])  # the bound says something
+
+
+OUTLIERS = {
+    "tile": ([3] * 300, [0]),
+    "tile_last": ([5] * 400, [399]),
+    "tiles": ([4] * 1_200_000, [0, 40_000, 1_199_999]),  # more than one to a wave
+    "wave": ([600, 900, 600, 700], [0]),
+    "group": ([3000, 5000, 2500], [1]),
+    "parts": ([30_000, 20_000], [0]),
+    "mixture": ([3, 700, 3, 4000, 2, 20_000, 3] * 3, [0, 3]),
+}
+
+
+@pytest.mark.parametrize("case", list(OUTLIERS))
+@pytest.mark.parametrize("size", [1e8, 1e30])
+def test_a_buckets_gradient_is_its_own(hip, case, size):
+    """A few steps' gradients 1e8 (1e30) times the others', whose rows lie in buckets of their own: the other
+    buckets' gradients keep their bits."""
+    from packboost_amd import choice_log_probs, choice_log_probs_backward
+
+    sizes, far = OUTLIERS[case]
+    d = bucket_case(sizes, far, seed=len(sizes))
+    p, _, _, ok, _, at = reference(d)
+    _, lse = choice_log_probs(d["scores"], d["sets"], chosen=d["chosen"], bias=d["bias"])
+    up = d["r"].uniform(0.5, 1.0, len(sizes)).astype(np.float32)
+    up[far] *= size
+    _, gt = choice_log_probs_backward(torch.from_numpy(up).to(DEV), d["scores"], lse, d["sets"], chosen=d["chosen"], bias=d["bias"])
+    check_buckets(d, gt, *back(d, p, ok, at, up.astype(np.float64)))
+    rows = d["r"].standard_normal(len(d["x"])).astype(np.float32)
+    rows[np.repeat(np.isin(np.arange(len(sizes)), far), sizes)] *= size
+    _, gt = choice_log_probs_backward(torch.from_numpy(rows).to(DEV), d["scores"], lse, d["sets"], bias=d["bias"])
+    u = rows.astype(np.float64)
+    total, absolute = (np.repeat(per_set(d, np.add, v, 0.0), d["size"]) for v in (u, np.abs(u)))
+    # the sum of a set's gradients passes at most 100 roundings
+    check_buckets(d, gt, u - p * total, np.abs(u) + p * absolute, 100 * U * p * absolute)
+
+
+def test_policy_with_a_stale_step(hip):
+    """The ratio is not held where the advantage is below 0: a log-probability 20 nats off takes e^20."""
+    from packboost_amd import policy_loss
+
+    d = bucket_case([4] * 2000, [7], seed=3)
+    p, _, _, ok, step, at = reference(d)
+    old = (step - 0.01).astype(np.float32)
+    old[7] -= 20
+    adv = np.where(np.arange(2000) == 7, -1.0, d["r"].uniform(0.5, 1, 2000)).astype(np.float32)
+    r = policy_loss(d["scores"], d["sets"], d["chosen"], torch.from_numpy(adv).to(DEV), torch.from_numpy(old).to(DEV), bias=d["bias"])
+    _, _, _, slope, w = policy_reference({"advantages": adv, "old_log_probs": old}, ok, step, 0.2, 0.2, 0.0, 1.0)
+    tol = U * (4 * np.abs(d["x"]).max() + 100)
+    g, size = back(d, p, ok, at, slope)
+    check_buckets(d, r.grad_table, g, size, size * (tol + 16 * U))
+
+
+def test_bucket_gradients_that_grow(hip):
+    """A bucket's gradients rise by many powers of two along the rows, each bucket's in its own way."""
+    from packboost_amd import choice_log_probs, choice_log_probs_backward
+
+    sets = 700_000  # more than a tile a wave
+    d = bucket_case([8] * sets, range(1, sets, 2), seed=5)
+    p, _, _, ok, _, at = reference(d)
+    i = np.arange(sets)
+    up = np.where(i % 2, 2.0 ** (i // 2 % 120 - 60), 2.0 ** (40 - i // 2 % 90)).astype(np.float32) * d["r"].uniform(0.5, 1, sets).astype(np.float32)
+    _, lse = choice_log_probs(d["scores"], d["sets"], chosen=d["chosen"], bias=d["bias"])
+    _, gt = choice_log_probs_backward(torch.from_numpy(up).to(DEV), d["scores"], lse, d["sets"], chosen=d["chosen"], bias=d["bias"])
+    check_buckets(d, gt, *back(d, p, ok, at, up.astype(np.float64)))
