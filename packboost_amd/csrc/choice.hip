@@ -511,7 +511,6 @@ __device__ __forceinline__ PolicyIn load_policy(const ChoiceArgs& a, int64_t g) 
 // overflow: where their weight, kl_weight or advantage is 0 they count for nothing all the same.
 __device__ __forceinline__ float policy_step(const ChoiceArgs& a, const PolicyIn& in, double lp, bool tally, double (&sum)[3]) {
     const float w = in.w * a.scale;
-    if (w == 0.0f) return 0.0f;
     const float ratio = FineExp(lp - (double)in.old).all;
     const float free = in.adv == 0.0f && ratio == kInf ? 0.0f : ratio * in.adv;
     const float held = fminf(fmaxf(ratio, a.ratio_min), a.ratio_max) * in.adv;
@@ -526,11 +525,11 @@ __device__ __forceinline__ float policy_step(const ChoiceArgs& a, const PolicyIn
         }
     }
     if (tally) {
-        sum[0] += (double)(w * (term - (clipped ? held : free)));
-        sum[1] += (double)(w * kl);
+        sum[0] += w == 0.0f ? 0.0 : (double)(w * (term - (clipped ? held : free)));
+        sum[1] += w == 0.0f ? 0.0 : (double)(w * kl);
         sum[2] += clipped ? (double)w : 0.0;
     }
-    return w * slope;
+    return w == 0.0f ? 0.0f : w * slope;
 }
 
 // The table's gradient as a wave gathers it: bins of whole numbers, bin i's in units of 2^-shift[i], so that
