@@ -594,7 +594,8 @@ int pb_choice_log_probs(const pb_sets* sets, const pb_choice_scores* scores, con
 
 /* Gradients of the scores (score_type [rows], stride 1, 0 where masked) and of the bias table (float32
  * [num_buckets]) from grad_dev, that of the rows' (chosen_dev NULL) or the steps' log-probabilities;
- * masked rows' entries are not used. lse_dev: pb_choice_log_probs' for the same scores. A bucket's rows are
+ * masked rows' entries are not used. lse_dev: pb_choice_log_probs' for the same scores; where it is 16 or
+ * more in size its rounding is made up for, by another sum over the set. A bucket's rows are
  * summed in whole numbers of 2^-34 or less of its largest gradient (a wave's at a time, in a fixed
  * order), then in double, and rounded once. */
 int pb_choice_log_probs_backward(const pb_sets* sets, const pb_choice_scores* scores, const int32_t* chosen_dev,

@@ -316,9 +316,10 @@ def choice_log_probs_backward(grad: torch.Tensor, scores: torch.Tensor, lse: tor
                               bias: PositionBias | None = None) -> tuple[torch.Tensor, torch.Tensor | None]:
     """(gradient of the scores, gradient of the bias table or None) from `grad`, that of the
     log-probabilities `choice_log_probs` gave for the same arguments (per row, or per step with
-    `chosen`). lse is that call's. Masked rows and steps left out take and give no gradient. A bucket's
-    gradient is its rows' sum, each rounded to 2^-34 or less of the bucket's largest, in an order that is
-    always the same."""
+    `chosen`). lse is that call's; where it is 16 or more in size, its rounding, which an offset of the
+    scores brings, is made up for by another sum over the set. Masked rows and steps left out take and give
+    no gradient. A bucket's gradient is its rows' sum, each rounded to 2^-34 or less of the bucket's largest,
+    in an order that is always the same."""
     c, keep = _scores(scores, sets, mask, bias)
     dev = sets.device
     grad = _column("grad", grad, sets.num_rows if chosen is None else sets.num_sets, dev, torch.float32)

@@ -400,6 +400,13 @@ __device__ __forceinline__ double lane_move(double v) {
     return __longlong_as_double((long long)hi << 32 | (uint32_t)lo);
 }
 
+// Backward passes take a set's probabilities as exp(x - lse), from an lse that is rounded: all of them are off
+// by up to |lse| 2^-24 of themselves, 2^-20 at kFarLse (where a set of ordinary scores stays below). A common
+// offset of the scores, which a softmax does not see, must not grow that. So beyond kFarLse the exponentials of
+// the set are summed anew and divided by their sum, which costs sets in parts another reading of them.
+constexpr float kFarLse = 16.0f;
+__device__ __forceinline__ bool far_lse(float lse) { return __builtin_fabsf(lse) >= kFarLse && __builtin_fabsf(lse) < kInf; }
+
 template <class F>
 __device__ F block_sum(F v, F* sh) {
     v = wave_sum(v);
@@ -653,50 +660,28 @@ struct TableSum {
     }
 };
 
-// The maximum and the sum of exponentials of a part of a set, or (listwise backward) the sum of its
-// rows' gradients. 11 vector instructions a row and one barrier: bound by reading the rows (4096 sets of
-// 32000 bfloat16 scores, 262 MB: 60 us, 4.4 TB/s).
+// The maximum and the sum of exponentials of a part of a set. 11 vector instructions a row and one barrier: bound
+// by reading the rows (4096 sets of 32000 bfloat16 scores, 262 MB: 60 us, 4.4 TB/s).
 template <int MODE, int TYPE, bool MASK, bool BIAS>
 __global__ __launch_bounds__(kBlock) void part_kernel(ChoiceArgs a, int first) {
     __shared__ Soft sh[kWaves];
-    __shared__ float shf[kWaves];
     __shared__ BiasShared bias;
     const int it = first + (int)blockIdx.x;
     const Span s = span_of(a, a.wide[it]);
-    if (BIAS && MODE != kRowsBack) stage_bias(a, bias);
+    if (BIAS) stage_bias(a, bias);
     float v[kWideRuns][kRun];
-    float sum = 0.0f;
 #pragma unroll
     for (int j = 0; j < kWideRuns; ++j) {
         const int i = kRun * (j * kBlock + (int)threadIdx.x);
 #pragma unroll
-        for (int k = 0; k < kRun; ++k) v[j][k] = MODE == kRowsBack ? 0.0f : -kInf;
+        for (int k = 0; k < kRun; ++k) v[j][k] = -kInf;
         if (i < s.hi) {
-            if (MODE == kRowsBack) {
-                uint32_t off = outside(s, i);
-                if (MASK) {
-                    const uint32_t out = off;
-                    for (int k = 0; k < kRun; ++k)
-                        if (!(out >> k & 1u) && !a.mask[s.q0 + i + k]) off |= 1u << k;
-                }
-                load_floats(a, s, i, a.grad, off, v[j]);
-            } else {
-                uint32_t off;
-                Buckets buckets;
-                load_logits<TYPE, MASK, BIAS>(a, &bias, s, i, v[j], off, buckets);
-            }
+            uint32_t off;
+            Buckets buckets;
+            load_logits<TYPE, MASK, BIAS>(a, &bias, s, i, v[j], off, buckets);
         }
     }
-    if (MODE == kRowsBack) {
-#pragma unroll
-        for (int j = 0; j < kWideRuns; ++j)
-#pragma unroll
-            for (int k = 0; k < kRun; ++k) sum += v[j][k];
-        sum = block_sum(sum, shf);
-        if (threadIdx.x == 0) a.parts[it] = make_float2(0.0f, sum);
-        return;
-    }
-    float top = kLowest;
+    float top = kLowest, sum = 0.0f;
 #pragma unroll
     for (int j = 0; j < kWideRuns; ++j)
 #pragma unroll
@@ -708,6 +693,70 @@ __global__ __launch_bounds__(kBlock) void part_kernel(ChoiceArgs a, int first) {
         for (int k = 0; k < kRun; ++k) sum += exp_of(v[j][k] - top);
     const Soft t = block_soft(Soft{top, wave_sum(sum)}, sh);
     if (threadIdx.x == 0) a.parts[it] = make_float2(t.top, t.sum);
+}
+
+// The sum of a part's rows' gradients.
+template <bool MASK>
+__global__ __launch_bounds__(kBlock) void part_grads_kernel(ChoiceArgs a, int first) {
+    __shared__ float shf[kWaves];
+    const int it = first + (int)blockIdx.x;
+    const Span s = span_of(a, a.wide[it]);
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kWideRuns; ++j) {
+        const int i = kRun * (j * kBlock + (int)threadIdx.x);
+        float v[kRun] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+        if (i < s.hi) {
+            uint32_t off = outside(s, i);
+            if (MASK) {
+                const uint32_t out = off;
+                for (int k = 0; k < kRun; ++k)
+                    if (!(out >> k & 1u) && !a.mask[s.q0 + i + k]) off |= 1u << k;
+            }
+            load_floats(a, s, i, a.grad, off, v);
+        }
+#pragma unroll
+        for (int k = 0; k < kRun; ++k) sum += v[k];
+    }
+    sum = block_sum(sum, shf);
+    if (threadIdx.x == 0) a.parts[it].y = sum;
+}
+
+// The sum of exp(x - lse) of the parts [first, first + n) whose set's lse is far (far_lse). A workgroup looks at
+// 64 of its parts at a time, a lane each, so that a table without such sets costs a launch (16384 parts: 3 us).
+template <int TYPE, bool MASK, bool BIAS>
+__global__ __launch_bounds__(kBlock) void part_far_kernel(ChoiceArgs a, int first, int n) {
+    __shared__ float shf[kWaves];
+    __shared__ BiasShared bias;
+    const int lane = (int)threadIdx.x & (kWave - 1), step = (int)gridDim.x;
+    bool staged = false;
+    for (int64_t i0 = blockIdx.x; i0 < n; i0 += (int64_t)step * kWave) {
+        const int64_t mine = i0 + (int64_t)step * lane;
+        unsigned long long far = __ballot(mine < n && far_lse(a.lse[a.wide[first + (mine < n ? mine : 0)].set0]));
+        for (; far; far &= far - 1) {  // the same in all waves
+            const int it = first + (int)(i0 + (int64_t)step * (__ffsll((long long)far) - 1));
+            const SetItem im = a.wide[it];
+            const Span s = span_of(a, im);
+            const float lse = a.lse[im.set0];
+            if (BIAS && !staged) stage_bias(a, bias);
+            staged = true;
+            float sum = 0.0f;
+#pragma unroll 1
+            for (int j = 0; j < kWideRuns; ++j) {
+                const int i = kRun * (j * kBlock + (int)threadIdx.x);
+                if (i < s.hi) {
+                    float v[kRun];
+                    uint32_t off;
+                    Buckets buckets;
+                    load_logits<TYPE, MASK, BIAS>(a, &bias, s, i, v, off, buckets);
+#pragma unroll
+                    for (int k = 0; k < kRun; ++k) sum += exp_of(v[k] - lse);
+                }
+            }
+            sum = block_sum(sum, shf);
+            if (threadIdx.x == 0) a.parts[it].x = sum;
+        }
+    }
 }
 
 // What a wave keeps of its tile in LDS.
@@ -899,6 +948,30 @@ __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, TileIn<MODE, TYPE
             wave_sync();
         }
     }
+    float anew[kTileRounds];  // what a set's exponentials over a far lse sum to
+#pragma unroll
+    for (int r = 0; r < kTileRounds; ++r) anew[r] = 1.0f;
+    if (!SOFT) {
+        bool far = false;
+#pragma unroll
+        for (int r = 0; r < kTileRounds; ++r) far = far || (r * kWave + lane < in.sets && far_lse(in.lse[r]));
+        if (__any(far)) {  // a lane walks a set: a scan here would take registers from tables without such sets
+            float e[kRun];
+#pragma unroll
+            for (int k = 0; k < kRun; ++k) e[k] = exp_of(x[k] - sh.shift[id[k] - 1]);
+            write_run(&sh.x[i0], e);  // the logits there have been read
+            wave_sync();
+#pragma unroll
+            for (int r = 0; r < kTileRounds; ++r)
+                if (r * kWave + lane < in.sets && far_lse(in.lse[r])) {
+                    double t = 0.0;
+                    for (int i = begin[r]; i < end[r]; ++i) t += (double)sh.x[i];
+                    anew[r] = (float)t;
+                    if (MODE == kRowsBack) sh.factor[r * kWave + lane] /= (float)t;
+                }
+            wave_sync();
+        }
+    }
     // a lane to a set: log-probabilities, losses, slopes
     float coef[kTileRounds];
     if (SOFT || STEPS) {
@@ -928,7 +1001,7 @@ __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, TileIn<MODE, TYPE
                         coef[r] = policy_step(a, in.pol[r], fine, true, tally);
                     }
                     if (SOFT) a.log_probs[g] = lp;
-                    if (GRAD) sh.factor[s] = counts ? (SOFT ? -coef[r] * __builtin_amdgcn_rcpf(sum) : -coef[r]) : 0.0f;
+                    if (GRAD) sh.factor[s] = counts ? (SOFT ? -coef[r] * __builtin_amdgcn_rcpf(sum) : -coef[r] / anew[r]) : 0.0f;
                     if (!counts) chosen[r] = -1;
                 }
             }
@@ -1076,6 +1149,21 @@ __device__ __forceinline__ void wide_pass(const ChoiceArgs& a, const SetItem& im
 #pragma unroll
                 for (int k = 0; k < kRun; ++k) v[j][k] = v[j][k] == -kInf ? -kInf : (v[j][k] - t.top) - ls;
     }
+    float anew = 1.0f;  // what the exponentials over a far lse sum to
+    if (!SOFT && far_lse(lse)) {
+        anew = 0.0f;
+        if (!ALONE && im.parts > 1) {
+            const float2* parts = a.parts + (index - im.part);
+            for (int j = tid; j < im.parts; j += THREADS) anew += parts[j].x;
+        } else {
+#pragma unroll
+            for (int j = 0; j < kWideRuns; ++j)
+                if (j < live)
+#pragma unroll
+                    for (int k = 0; k < kRun; ++k) anew += exp_of(v[j][k] - lse);
+        }
+        anew = ALONE ? wave_sum(anew) : block_sum(anew, shf);
+    }
     if (MODE == kRowsBack) {
         float total = 0.0f;
         if (!ALONE && im.parts > 1) {
@@ -1087,7 +1175,7 @@ __device__ __forceinline__ void wide_pass(const ChoiceArgs& a, const SetItem& im
 #pragma unroll
                 for (int k = 0; k < kRun; ++k) total += d[j][k];
         }
-        total = ALONE ? wave_sum(total) : block_sum(total, shf);
+        total = (ALONE ? wave_sum(total) : block_sum(total, shf)) / anew;
 #pragma unroll
         for (int j = 0; j < kWideRuns; ++j)
             if (j < live)
@@ -1106,7 +1194,7 @@ __device__ __forceinline__ void wide_pass(const ChoiceArgs& a, const SetItem& im
             float coef = 0.0f;
             if (MODE == kStepsBack && counts) coef = given;
             if (MODE == kPolicy && counts) coef = policy_step(a, pol, fine, first, tally);
-            const float f = counts ? (SOFT ? -coef * __builtin_amdgcn_rcpf(t.sum) : -coef) : 0.0f;
+            const float f = counts ? (SOFT ? -coef * __builtin_amdgcn_rcpf(t.sum) : -coef / anew) : 0.0f;
             const float fw = f * own;
             const int64_t row = r0 + c - sp.q0;
             if (counts && row >= sp.lo && row < sp.hi) {
@@ -1531,9 +1619,18 @@ template <int MODE, int TYPE, bool MASK, bool BIAS>
 hipError_t launch_choice_as(const SetLayout& s, const ChoiceArgs& a, hipStream_t stream) {
     hipError_t e = hipSuccess;
     const int parts = s.num_wide - s.num_whole;
-    if (MODE != kStepsBack && parts > 0) {
-        hipLaunchKernelGGL((part_kernel<MODE, TYPE, MASK, BIAS>), dim3(parts), dim3(kBlock), 0, stream, a,
-                           s.num_mid + s.num_whole);
+    if (parts > 0) {
+        const int first = s.num_mid + s.num_whole;
+        if constexpr (MODE == kRowsBack || MODE == kStepsBack) {
+            if (MODE == kRowsBack) {
+                hipLaunchKernelGGL(part_grads_kernel<MASK>, dim3(parts), dim3(kBlock), 0, stream, a, first);
+                if ((e = hipGetLastError()) != hipSuccess) return e;
+            }
+            hipLaunchKernelGGL((part_far_kernel<TYPE, MASK, BIAS>), dim3(std::min(parts, kChoiceGrid)), dim3(kBlock), 0, stream,
+                               a, first, parts);
+        } else {
+            hipLaunchKernelGGL((part_kernel<MODE, TYPE, MASK, BIAS>), dim3(parts), dim3(kBlock), 0, stream, a, first);
+        }
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
     if (s.num_tiles > 0) {

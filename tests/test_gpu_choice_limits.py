@@ -232,3 +232,70 @@ def test_bucket_gradients_that_grow(hip):
     _, lse = choice_log_probs(d["scores"], d["sets"], chosen=d["chosen"], bias=d["bias"])
     _, gt = choice_log_probs_backward(torch.from_numpy(up).to(DEV), d["scores"], lse, d["sets"], chosen=d["chosen"], bias=d["bias"])
     check_buckets(d, gt, *back(d, p, ok, at, up.astype(np.float64)))
+
+
+@pytest.mark.parametrize("offset", [16.0, -100.0, 8192.0, -8192.0])
+@pytest.mark.parametrize("sizes", [[2] * 300, [60, 1, 0, 200, 30], [700, 3000, 5], [9000, 2], [30_000, 9000, 700, 3, 17_000]])
+def test_an_offset_of_the_scores_changes_nothing(hip, sizes, offset):
+    """Scores in units of 2^-10 below 8 and an offset below 2^13 add without rounding: the gradients are the
+    softmax's of the scores alone, in a bound without the offset."""
+    from packboost_amd import ChoiceSets, choice_log_probs, choice_log_probs_backward
+
+    r = np.random.default_rng(len(sizes))
+    off = offsets_of(sizes)
+    n, g = int(off[-1]), len(sizes)
+    x = r.integers(-8 << 10, 8 << 10, n) / 1024.0
+    d = {"off": off, "size": np.diff(off), "x": x, "keep": np.ones(n, bool),
+         "c": np.floor(r.random(g) * np.diff(off)).astype(np.int64)}
+    p, _, _, ok, _, at = reference(d)
+    sets, tol = ChoiceSets(off), U * (4 * 8 + 100)
+    chosen = torch.from_numpy(d["c"].astype(np.int32)).to(DEV)
+    scores = torch.from_numpy((x + offset).astype(np.float32)).to(DEV)
+    assert np.array_equal(scores.double().cpu().numpy(), x + offset)
+    up = r.standard_normal(g).astype(np.float32)
+    _, lse = choice_log_probs(scores, sets, chosen=chosen)
+    gs, _ = choice_log_probs_backward(torch.from_numpy(up).to(DEV), scores, lse, sets, chosen=chosen)
+    want, size = back(d, p, ok, at, up.astype(np.float64))
+    assert np.all(np.abs(gs.double().cpu().numpy() - want) <= size * (tol + 4 * U) + U * np.abs(want))
+    rows = r.standard_normal(n).astype(np.float32)
+    _, lse = choice_log_probs(scores, sets)
+    gs, _ = choice_log_probs_backward(torch.from_numpy(rows).to(DEV), scores, lse, sets)
+    u = rows.astype(np.float64)
+    total, absolute = (np.repeat(per_set(d, np.add, v, 0.0), sizes) for v in (u, np.abs(u)))
+    want = u - p * total
+    room = np.abs(u) * 4 * U + p * absolute * (tol + 104 * U) + U * np.abs(want)
+    assert np.all(np.abs(gs.double().cpu().numpy() - want) <= room)
+
+
+@pytest.mark.parametrize("score", [3.0e9, -3.0e9, 1e30])
+@pytest.mark.parametrize("size", [3, 700, 2500, 20_000])
+def test_equal_scores_of_any_size(hip, size, score):
+    """A uniform choice, whose lse has no room for the log of the number of rows."""
+    from packboost_amd import ChoiceSets, choice_log_probs, choice_log_probs_backward
+
+    sets = ChoiceSets([0, size])
+    s = torch.full((size,), score, device=DEV)
+    chosen = torch.zeros(1, dtype=torch.int32, device=DEV)
+    _, lse = choice_log_probs(s, sets, chosen=chosen)
+    gs, _ = choice_log_probs_backward(torch.ones(1, device=DEV), s, lse, sets, chosen=chosen)
+    want = np.full(size, -1.0 / size)
+    want[0] += 1.0
+    assert np.all(np.abs(gs.double().cpu().numpy() - want) <= 8 * U / size + U * np.abs(want))
+
+
+def test_a_neighbour_far_off_changes_nothing(hip):
+    """Sets of one tile, one of them offset: the others' gradients are to the bit what they are without it."""
+    from packboost_amd import ChoiceSets, choice_log_probs, choice_log_probs_backward
+
+    s = torch.randn(90, device=DEV)
+    moved = s.clone()
+    moved[30:60] += 4096.0
+    sets, chosen = ChoiceSets([0, 30, 60, 90]), torch.zeros(3, dtype=torch.int32, device=DEV)
+    out = []
+    for t in (s, moved):
+        lp, lse = choice_log_probs(t, sets, chosen=chosen)
+        rows, _ = choice_log_probs_backward(t.abs() * 1e-3, t, lse, sets)
+        out.append((lp, lse, choice_log_probs_backward(torch.ones(3, device=DEV), t, lse, sets, chosen=chosen)[0], rows))
+    for a, b in zip(*out):
+        k = len(a) // 3
+        assert torch.equal(a[:k], b[:k]) and torch.equal(a[2 * k:], b[2 * k:])
