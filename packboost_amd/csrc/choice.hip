@@ -1412,6 +1412,7 @@ struct SumArgs {
     const int32_t* entries;
     const float* slopes;
     float* out;
+    double* totals;      // in the place of `out`, for sequences: their sums nearly cancel in pairs
     double* parts;
     const double* sums;  // the pairs' workgroups' losses [num_sums], joined by a workgroup more
     int32_t num_sums;
@@ -1437,6 +1438,14 @@ __device__ __forceinline__ double sum_term(const SumArgs& a, int64_t i) {
 }
 
 template <bool PAIRS>
+__device__ __forceinline__ void put_sum(const SumArgs& a, int64_t g, double t) {
+    if (PAIRS)
+        a.out[g] = (float)t;
+    else
+        a.totals[g] = t;
+}
+
+template <bool PAIRS>
 __global__ __launch_bounds__(kBlock) void set_sum_kernel(SumArgs a) {
     constexpr int kPer = kSetTileRows / kWave;
     __shared__ double xs[kWaves][kSetTileRows];
@@ -1449,7 +1458,7 @@ __global__ __launch_bounds__(kBlock) void set_sum_kernel(SumArgs a) {
         t = block_sum(t, sh);
         if (tid == 0) {
             if (im.parts == 1)
-                a.out[im.set0] = (float)t;
+                put_sum<PAIRS>(a, im.set0, t);
             else
                 a.parts[blockIdx.x] = t;
         }
@@ -1478,11 +1487,12 @@ __global__ __launch_bounds__(kBlock) void set_sum_kernel(SumArgs a) {
         double t = 0.0;
         for (int i = b + sub; i < e; i += L) t += xs[wave][i];
         for (int m = 1; m < L; m <<= 1) t += __shfl_xor(t, m);
-        if (sub == 0) a.out[g] = (float)t;
+        if (sub == 0) put_sum<PAIRS>(a, g, t);
     }
 }
 
 // The sets that were summed in parts.
+template <bool PAIRS>
 __global__ __launch_bounds__(kBlock) void set_join_kernel(SumArgs a, const int32_t* __restrict__ list) {
     __shared__ double sh[kWaves];
     const int32_t it = list[blockIdx.x];
@@ -1490,12 +1500,12 @@ __global__ __launch_bounds__(kBlock) void set_join_kernel(SumArgs a, const int32
     double t = 0.0;
     for (int j = (int)threadIdx.x; j < im.parts; j += kBlock) t += a.parts[it + j];
     t = block_sum(t, sh);
-    if (threadIdx.x == 0) a.out[im.set0] = (float)t;
+    if (threadIdx.x == 0) put_sum<PAIRS>(a, im.set0, t);
 }
 
 // z = beta (a_w - a_l); the loss w [(1 - e) softplus(-z) + e softplus(z)] and its slope
-// beta w (sigmoid(z) - (1 - e)). Sequences' values come from their sums, others' as value - ref, the
-// differences taken in double: both can be large where z is small. Bound by the gathers of the values: 5M
+// beta w (sigmoid(z) - (1 - e)). Sequences' values come from their sums in double, others' as value
+// - ref, the differences taken in double: both can be large where z is small. Bound by the gathers of the values: 5M
 // pairs of 1M values, values and references side by side, 94 us (160 us in arrays of their own). Four
 // pairs are in flight a thread.
 __global__ __launch_bounds__(kBlock) void pair_kernel(PairArgs a) {
@@ -1513,7 +1523,10 @@ __global__ __launch_bounds__(kBlock) void pair_kernel(PairArgs a) {
             l[k] = __builtin_nontemporal_load(a.losers + p);
             weight[k] = a.weights ? __builtin_nontemporal_load(a.weights + p) : 1.0f;
         }
-        if (a.both) {
+        if (a.totals) {
+#pragma unroll
+            for (int k = 0; k < kPairs; ++k) d[k] = a.totals[w[k]] - a.totals[l[k]];
+        } else if (a.both) {
 #pragma unroll
             for (int k = 0; k < kPairs; ++k) {
                 const float2 t = a.both[w[k]], u = a.both[l[k]];
@@ -1690,7 +1703,7 @@ hipError_t launch_set_sum(const SetLayout& s, const SumArgs& a, hipStream_t stre
     hipLaunchKernelGGL(set_sum_kernel<PAIRS>, dim3(grid), dim3(kBlock), 0, stream, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || s.num_split == 0) return e;
-    hipLaunchKernelGGL(set_join_kernel, dim3(s.num_split), dim3(kBlock), 0, stream, a, s.split);
+    hipLaunchKernelGGL(set_join_kernel<PAIRS>, dim3(s.num_split), dim3(kBlock), 0, stream, a, s.split);
     return hipGetLastError();
 }
 
@@ -1744,9 +1757,9 @@ hipError_t launch_preference(const PairLayout& p, PairArgs a, const float* value
     a.num_pairs = p.num_pairs;
     a.sums = reinterpret_cast<double*>(work);
     double* parts = a.sums + kPairGrid;
-    a.slopes = reinterpret_cast<float*>(parts + long_items(p.lists) + long_items(p.seqs));
-    float* seq_sum = a.slopes + p.num_pairs;
-    float* seq_grad = seq_sum + p.seqs.num_sets;
+    double* totals = parts + long_items(p.lists) + long_items(p.seqs);
+    a.slopes = reinterpret_cast<float*>(totals + p.seqs.num_sets);
+    float* seq_grad = a.slopes + p.num_pairs;
     const bool seqs = p.has_seqs;
     hipError_t e = hipSuccess;
     if (seqs) {
@@ -1754,10 +1767,9 @@ hipError_t launch_preference(const PairLayout& p, PairArgs a, const float* value
         sa.parts = parts;
         sa.values = values;
         sa.ref = ref;
-        sa.out = seq_sum;
+        sa.totals = totals;
         if ((e = launch_set_sum<false>(p.seqs, sa, stream)) != hipSuccess) return e;
-        a.values = seq_sum;
-        a.ref = nullptr;
+        a.totals = totals;
     } else {
         a.values = values;
         a.ref = ref;
@@ -1804,7 +1816,7 @@ hipError_t launch_preference(const PairLayout& p, PairArgs a, const float* value
 }
 
 int64_t preference_work_bytes(const PairLayout& p) {
-    return 8 * ((int64_t)kPairGrid + long_items(p.lists) + long_items(p.seqs)) + 4 * (p.num_pairs + 2 * p.seqs.num_sets) +
+    return 8 * ((int64_t)kPairGrid + long_items(p.lists) + long_items(p.seqs) + p.seqs.num_sets) + 4 * (p.num_pairs + p.seqs.num_sets) +
            (side_by_side(p) ? 8 * p.lists.num_sets : 0);
 }
 

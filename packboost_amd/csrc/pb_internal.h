@@ -595,6 +595,7 @@ struct PairArgs {
     const float* values;
     const float* ref;
     const float2* both;  // values and references side by side, or NULL
+    const double* totals;  // sequences' sums, or NULL
     const float* weights;
     float beta, smoothing, scale;
     float* margins;

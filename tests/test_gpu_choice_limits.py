@@ -299,3 +299,24 @@ def test_a_neighbour_far_off_changes_nothing(hip):
     for a, b in zip(*out):
         k = len(a) // 3
         assert torch.equal(a[:k], b[:k]) and torch.equal(a[2 * k:], b[2 * k:])
+
+
+@pytest.mark.parametrize("length", [400, 1900, 7000, 10_000, 30_000])
+def test_long_sequences_that_nearly_cancel(hip, length):
+    """Sequences' sums are large and their differences small: a margin is the difference of two sums in double,
+    rounded once (and beta's own rounding)."""
+    from packboost_amd import PreferencePairs, preference_loss
+
+    r = np.random.default_rng(length)
+    seqs = 8
+    off = offsets_of([length] * seqs)
+    v = (-4 * r.random(length * seqs)).astype(np.float32)
+    a = np.array([v[b:e].astype(np.float64).sum() for b, e in zip(off[:-1], off[1:])])
+    for k in range(1, seqs):  # a last step that brings the sum next to the first sequence's
+        v[off[k + 1] - 1] += np.float32(a[0] - a[k] + r.uniform(-1, 1))
+    a = np.array([v[b:e].astype(np.float64).sum() for b, e in zip(off[:-1], off[1:])])
+    w, l = np.repeat(np.arange(seqs), seqs), np.tile(np.arange(seqs), seqs)
+    out = preference_loss(torch.from_numpy(v).to(DEV), PreferencePairs(w, l, offsets=off), beta=0.5)
+    z = 0.5 * (a[w] - a[l])
+    # a term (2 on average) passes at most 2^8 additions in double, here and there
+    assert np.all(np.abs(out.margins.double().cpu().numpy() - z) <= 2.1 * U * np.abs(z) + 2.0 ** -44 * length)
