@@ -70,27 +70,29 @@ __device__ __forceinline__ double fine_log(float x) {
     return __builtin_fma((double)k, 0.69314718055994531, 2.0 * ((double)f + (double)small));
 }
 
-// e^x and what it is more than the first terms of its series, e^x - 1 and e^x - 1 - x, a unit or so in the last
-// place of each: x = k log 2 + r, |r| <= log(2) / 2, and seven terms of r's series. Without the series for |x|
-// of 87 and more, infinities and NaN.
+// e^x, e^x - 1 and e^x - 1 - x, within 1, 1 and 4 units in the last place: x = k log 2 + r, |r| <= log(2) / 2, and
+// eight terms of r's series (r^2 / 2 + ... + r^8 / 40320 in float32, what is joined with 1, 2^k and x in double).
+// From |x| of 200 on, infinities and NaN as of e^x.
 struct FineExp {
     float all, less_one, less_line;
     __device__ __forceinline__ explicit FineExp(double x) {
-        const float hi = (float)x, lo = (float)(x - (double)hi);
-        const float k = __builtin_rintf(hi * 1.44269504f);
-        float r = __builtin_fmaf(k, -0.693145751953125f, hi);
-        r = __builtin_fmaf(k, -1.42860682e-6f, r) + lo;
-        float p = 1.0f / 5040;
+        const float hi = (float)x, k = __builtin_rintf(hi * 1.44269504f);
+        const double rest = __builtin_fma((double)k, -0.69314718055994531, x);
+        const float r = (float)rest;
+        float p = 1.0f / 40320;
+        p = __builtin_fmaf(p, r, 1.0f / 5040);
         p = __builtin_fmaf(p, r, 1.0f / 720);
         p = __builtin_fmaf(p, r, 1.0f / 120);
         p = __builtin_fmaf(p, r, 1.0f / 24);
         p = __builtin_fmaf(p, r, 1.0f / 6);
         p = __builtin_fmaf(p, r, 0.5f);
         p *= r * r;
-        const bool near = __builtin_fabsf(hi) < 87.0f;
-        all = near ? __builtin_amdgcn_ldexpf(1.0f + (r + p), (int)k) : exp_of(hi);
-        less_one = k == 0.0f ? r + p : all - 1.0f;
-        less_line = k == 0.0f ? p : (all - 1.0f) - hi;
+        const bool near = __builtin_fabsf(hi) < 200.0f;
+        const int n = near ? (int)k : 0;
+        const double unit = ldexp(1.0, n), one = n == 0 ? rest + (double)p : __builtin_fma(unit, rest + (double)p, unit - 1.0);
+        all = near ? __builtin_amdgcn_ldexpf(1.0f + (r + p), n) : exp_of(hi);
+        less_one = near ? (float)one : all - 1.0f;
+        less_line = !near ? (hi > 0.0f ? all : (all - 1.0f) - hi) : n == 0 ? p : (float)(one - x);
     }
 };
 

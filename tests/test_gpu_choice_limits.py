@@ -320,3 +320,32 @@ def test_long_sequences_that_nearly_cancel(hip, length):
     z = 0.5 * (a[w] - a[l])
     # a term (2 on average) passes at most 2^8 additions in double, here and there
     assert np.all(np.abs(out.margins.double().cpu().numpy() - z) <= 2.1 * U * np.abs(z) + 2.0 ** -44 * length)
+
+
+def test_kl_term_near_its_zero(hip):
+    """A set of one row has log p = 0, so ref_log_probs is d itself: e^d - d - 1, and its slope e^d - 1 on one
+    of two equal rows. Both are formed without cancellation that the formula does not have: within 5 units in
+    the last place (a unit is at most 2^-23 of the value)."""
+    from packboost_amd import ChoiceSets, policy_loss
+
+    d = np.concatenate([np.linspace(-2.2, 2.2, 2001), [1e-4, -1e-4, 0.3465, 0.3467, -0.3465, -0.3467, 0.351, 1e-15, 0.0, 80.0, -80.0]])
+    d = d.astype(np.float32)
+    one = torch.ones(1, device=DEV)
+    zero = torch.zeros(1, dtype=torch.int32, device=DEV)
+    sets, row = ChoiceSets([0, 1]), torch.zeros(1, device=DEV)
+    refs = torch.from_numpy(d).to(DEV)
+    got = torch.stack([policy_loss(row, sets, zero, one, row, ref_log_probs=refs[i: i + 1], kl_weight=1.0).kl for i in range(len(d))])
+    x = d.astype(np.float64)
+    want = np.expm1(x) - x
+    small = np.abs(x) < 0.1  # where that cancels too: the series
+    want[small] = sum(x[small] ** k / math.factorial(k) for k in range(2, 14))
+    assert np.all(np.abs(got.double().cpu().numpy() - want) <= 5 * 2 * U * np.abs(want))
+    # slopes: two equal rows, log p = -log 2 in more bits than float32's
+    n = len(d)
+    ref = (d - math.log(2)).astype(np.float32)
+    r = policy_loss(torch.zeros(2 * n, device=DEV), ChoiceSets(np.arange(n + 1) * 2), torch.zeros(n, dtype=torch.int32, device=DEV),
+                    torch.zeros(n, device=DEV), torch.zeros(n, device=DEV), ref_log_probs=torch.from_numpy(ref).to(DEV), kl_weight=1.0)
+    gap = ref.astype(np.float64) + math.log(2)
+    want = -0.5 * np.expm1(gap)
+    # log 2 itself is known to 2^-30
+    assert np.all(np.abs(r.grad_scores[::2].double().cpu().numpy() - want) <= 5 * 2 * U * np.abs(want) + 2.0 ** -30 * np.exp(gap))
