@@ -40,9 +40,26 @@ constexpr int kLookup = 2048;  // bytes of the position lookup kept in LDS
 static_assert(kSetTileRows == kRun * kWave, "a lane holds one run of a tile");
 
 // e^x of a difference to a set's maximum or lse: 2^(x log2(e)) in two instructions. The product's rounding
-// and log2(e)'s own move the result by at most |x| 2^-23 of itself, as a unit in the last place of x does.
-// Results below 2^-126 are 0; e^-inf is 0 and NaN stays NaN.
+// and log2(e)'s own move the result by at most |x| 2^-24 of itself and a unit, 64 2^-24 at x = -87. Sums of
+// exponentials take it, in which a term of size e^x weighs so much; gradients rounded to 16 bits, too. Results
+// below 2^-126 are 0; e^-inf is 0 and NaN stays NaN.
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * 1.44269502162933349609375f); }
+
+// The same within 2 2^-24 beside the instruction's own error, for gradients in float32: e = 2^t, t the rounded
+// product, and e (x - t log 2) for what the rounding took (four instructions a row: for bfloat16 scores 3 us of the
+// 103 of the policy loss of 40M rows).
+__device__ __forceinline__ float close_exp(float x) {
+    const float d = __builtin_elementwise_maximum(x, -200.0f);  // a NaN is the larger one
+    const float t = d * 1.44269502162933349609375f, e = __builtin_amdgcn_exp2f(t);
+    const float rest = __builtin_fmaf(t, 1.904654299957e-9f, __builtin_fmaf(t, -0.693147182464599609375f, d));
+    return __builtin_fmaf(e, rest, e);
+}
+
+template <int MODE, int TYPE, bool BIAS>
+__device__ __forceinline__ float row_exp(float x) {
+    constexpr bool GRAD = MODE == kRowsBack || MODE == kStepsBack || MODE == kPolicy;
+    return GRAD && (TYPE == PB_F32 || BIAS) ? close_exp(x) : exp_of(x);
+}
 
 // log x for x = 0 or above 1/2: 0 gives -inf, NaN stays NaN.
 __device__ __forceinline__ float log_of(float x) { return __builtin_amdgcn_logf(x) * 0.69314718055994530942f; }
@@ -903,7 +920,7 @@ __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, TileIn<MODE, TYPE
             for (int k = 0; k < kRun; k += 2) top = max3(top, x[k], x[k + 1]);
             top = wave_max(top);
 #pragma unroll
-            for (int k = 0; k < kRun; ++k) sum += v[k] = exp_of(x[k] - top);
+            for (int k = 0; k < kRun; ++k) sum += v[k] = row_exp<MODE, TYPE, BIAS>(x[k] - top);
             sum = wave_sum(sum);
             if (lane == 0) {
                 sh.shift[0] = top;
@@ -941,7 +958,7 @@ __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, TileIn<MODE, TYPE
             segment_reduce<TakeMax>(seg, x, id, lane, sh.shift);
             wave_sync();
 #pragma unroll
-            for (int k = 0; k < kRun; ++k) v[k] = exp_of(x[k] - sh.shift[id[k] - 1]);
+            for (int k = 0; k < kRun; ++k) v[k] = row_exp<MODE, TYPE, BIAS>(x[k] - sh.shift[id[k] - 1]);
             segment_reduce<TakeSum>(seg, v, id, lane, sh.factor);
             wave_sync();
         }
@@ -960,7 +977,7 @@ __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, TileIn<MODE, TYPE
         if (__any(far)) {  // a lane walks a set: a scan here would take registers from tables without such sets
             float e[kRun];
 #pragma unroll
-            for (int k = 0; k < kRun; ++k) e[k] = exp_of(x[k] - sh.shift[id[k] - 1]);
+            for (int k = 0; k < kRun; ++k) e[k] = row_exp<MODE, TYPE, BIAS>(x[k] - sh.shift[id[k] - 1]);
             write_run(&sh.x[i0], e);  // the logits there have been read
             wave_sync();
 #pragma unroll
@@ -1027,7 +1044,7 @@ __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, TileIn<MODE, TYPE
     if (MODE == kRowsBack) {
 #pragma unroll
         for (int k = 0; k < kRun; ++k)
-            v[k] = d[k] - (x[k] == -kInf ? 0.0f : exp_of(x[k] - sh.shift[id[k] - 1]) * sh.factor[id[k] - 1]);
+            v[k] = d[k] - (x[k] == -kInf ? 0.0f : row_exp<MODE, TYPE, BIAS>(x[k] - sh.shift[id[k] - 1]) * sh.factor[id[k] - 1]);
     }
     if (STEPS) {
         float own[kRun];
@@ -1035,7 +1052,7 @@ __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, TileIn<MODE, TYPE
 #pragma unroll
         for (int k = 0; k < kRun; ++k) {
             const float f = sh.factor[id[k] - 1];
-            const float e = SOFT ? v[k] : exp_of(x[k] - sh.shift[id[k] - 1]);
+            const float e = SOFT ? v[k] : row_exp<MODE, TYPE, BIAS>(x[k] - sh.shift[id[k] - 1]);
             v[k] = (f == 0.0f ? 0.0f : f * e) + own[k];
         }
     }
@@ -1131,7 +1148,7 @@ __device__ __forceinline__ void wide_pass(const ChoiceArgs& a, const SetItem& im
                 if (j < live)
 #pragma unroll
                     for (int k = 0; k < kRun; ++k) {
-                        const float e = exp_of(v[j][k] - w.top);
+                        const float e = row_exp<MODE, TYPE, BIAS>(v[j][k] - w.top);
                         w.sum += e;
                         if (GRAD) v[j][k] = e;
                     }
@@ -1139,7 +1156,7 @@ __device__ __forceinline__ void wide_pass(const ChoiceArgs& a, const SetItem& im
         if (ALONE || im.parts == 1) {
             w.sum = wave_sum(w.sum);
             t = ALONE ? w : block_soft(w, shs);
-            if (GRAD && !ALONE) own = exp_of(w.top - t.top);
+            if (GRAD && !ALONE) own = row_exp<MODE, TYPE, BIAS>(w.top - t.top);
         }
     }
     const float ls = SOFT ? log_of(t.sum) : 0.0f;
@@ -1162,7 +1179,7 @@ __device__ __forceinline__ void wide_pass(const ChoiceArgs& a, const SetItem& im
             for (int j = 0; j < kWideRuns; ++j)
                 if (j < live)
 #pragma unroll
-                    for (int k = 0; k < kRun; ++k) anew += exp_of(v[j][k] - lse);
+                    for (int k = 0; k < kRun; ++k) anew += row_exp<MODE, TYPE, BIAS>(v[j][k] - lse);
         }
         anew = ALONE ? wave_sum(anew) : block_sum(anew, shf);
     }
@@ -1183,7 +1200,7 @@ __device__ __forceinline__ void wide_pass(const ChoiceArgs& a, const SetItem& im
             if (j < live)
 #pragma unroll
                 for (int k = 0; k < kRun; ++k)
-                    v[j][k] = d[j][k] - (v[j][k] == -kInf ? 0.0f : exp_of(v[j][k] - lse) * total);
+                    v[j][k] = d[j][k] - (v[j][k] == -kInf ? 0.0f : row_exp<MODE, TYPE, BIAS>(v[j][k] - lse) * total);
     }
     int at = -kRun;  // the chosen row, as the span counts
     float extra = 0.0f;
@@ -1208,7 +1225,7 @@ __device__ __forceinline__ void wide_pass(const ChoiceArgs& a, const SetItem& im
                 if (j < live)
 #pragma unroll
                     for (int k = 0; k < kRun; ++k) {
-                        const float e = SOFT ? v[j][k] : exp_of(v[j][k] - lse);
+                        const float e = SOFT ? v[j][k] : row_exp<MODE, TYPE, BIAS>(v[j][k] - lse);
                         v[j][k] = f == 0.0f ? 0.0f : fw * e;
                     }
         }

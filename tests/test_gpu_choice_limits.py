@@ -349,3 +349,48 @@ def test_kl_term_near_its_zero(hip):
     want = -0.5 * np.expm1(gap)
     # log 2 itself is known to 2^-30
     assert np.all(np.abs(r.grad_scores[::2].double().cpu().numpy() - want) <= 5 * 2 * U * np.abs(want) + 2.0 ** -30 * np.exp(gap))
+
+
+def test_small_probabilities_keep_their_bits(hip):
+    """Two rows, {0, -t}: the second's probability, down to e^-87, is good to 10 units of itself (the exponential
+    2, sum and quotient 2 each, products) and what the difference to a rounded lse takes."""
+    from packboost_amd import ChoiceSets, choice_log_probs, choice_log_probs_backward, policy_loss
+
+    t = np.arange(1, 2000) * 0.0434
+    t = np.round(t * 65536) / 65536  # differences without rounding
+    g = len(t)
+    x = np.stack([np.zeros(g), -t], 1).reshape(-1)
+    s = torch.from_numpy(x.astype(np.float32)).to(DEV)
+    assert np.array_equal(s.double().cpu().numpy(), x)
+    sets, c, one = ChoiceSets(np.arange(g + 1) * 2), torch.zeros(g, dtype=torch.int32, device=DEV), torch.ones(g, device=DEV)
+    p = np.exp(-t) / (1 + np.exp(-t))
+    lp, lse = choice_log_probs(s, sets, chosen=c)
+    shift = lse.double().cpu().numpy()
+    room = (10 * U + np.where(shift != 0, U * (np.abs(t + shift) + np.abs(shift)), 0.0)) * p
+    gs, _ = choice_log_probs_backward(one, s, lse, sets, chosen=c)
+    assert np.all(np.abs(gs.double().cpu().numpy()[1::2] + p) <= room)
+    rows = torch.tensor([1.0, 0.0], device=DEV).repeat(g)
+    gs, _ = choice_log_probs_backward(rows, s, lse, sets)
+    assert np.all(np.abs(gs.double().cpu().numpy()[1::2] + p) <= room)
+    gs = policy_loss(s, sets, c, one, lp).grad_scores.double().cpu().numpy()[1::2]
+    ratio = np.exp(-np.log1p(np.exp(-t)) - lp.double().cpu().numpy())  # a rounding of lp away from 1
+    assert np.all(np.abs(gs - ratio * p) <= 12 * U * p)
+
+
+@pytest.mark.parametrize("size", [700, 2500, 9000])
+def test_small_probabilities_of_longer_sets(hip, size):
+    """The same by a wave, a workgroup and in parts, whose sums of positive terms pass at most 43 roundings more."""
+    from packboost_amd import ChoiceSets, policy_loss
+
+    r = np.random.default_rng(size)
+    x = -np.round(r.uniform(0, 86.9, size) * 1024) / 1024
+    x[0], x[-1] = 0.0, -86.5
+    d = {"off": offsets_of([size]), "size": np.array([size]), "x": x, "keep": np.ones(size, bool), "c": np.array([0])}
+    p, lp, *_ = reference(d)
+    s = torch.from_numpy(x.astype(np.float32)).to(DEV)
+    one, old = torch.ones(1, device=DEV), torch.from_numpy(lp[:1].astype(np.float32)).to(DEV)
+    gs = policy_loss(s, ChoiceSets([0, size]), torch.zeros(1, dtype=torch.int32, device=DEV), one, old).grad_scores
+    want = math.exp(lp[0] - float(old[0])) * p
+    other = np.arange(size) != 0
+    # what lies below 2^-126 may be 0
+    assert np.all(np.abs(gs.double().cpu().numpy() - want)[other] <= 55 * U * want[other] + 2.0 ** -126)
