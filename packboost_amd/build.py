@@ -52,10 +52,15 @@ def compile_flags() -> list[str]:
 # selection. One build of the single-feature histogram tile that spilled returned wrong plane
 # counts for a code generation it took only with the spills, so a spill here fails the build.
 NO_SCRATCH = re.compile(r"hist_era_kernel|seg_score_kernel|des_score|kcuts_kernel")
+# Kernels that must not spill vector registers: the choice operators'. (The policy's wide_kernel with a bias has
+# 36 bytes of scratch reserved, for kernel arguments that end in lanes of a vector register; nothing in it is
+# read or written.)
+NO_SPILLS = re.compile(r"tile_kernel|wide_kernel|part_kernel|part_grads_kernel|part_far_kernel|split_steps_kernel")
 
 
 def spilling_kernels(remarks: str) -> list[str]:
-    """Names of NO_SCRATCH kernels whose kernel-resource-usage remarks report ScratchSize > 0."""
+    """Names of NO_SCRATCH kernels whose kernel-resource-usage remarks report ScratchSize > 0, and of NO_SPILLS
+    kernels for which they report spilled VGPRs or more scratch than those 36 bytes."""
     out, name = [], None
     for line in remarks.splitlines():
         m = re.search(r"Function Name: (\S+)", line)
@@ -63,7 +68,11 @@ def spilling_kernels(remarks: str) -> list[str]:
             name = m.group(1)
             continue
         m = re.search(r"ScratchSize \[bytes/lane\]: (\d+)", line)
-        if m and name and int(m.group(1)) > 0 and NO_SCRATCH.search(name):
+        if m and name and (int(m.group(1)) > 0 and NO_SCRATCH.search(name)
+                           or int(m.group(1)) > 36 and NO_SPILLS.search(name)):
+            out.append(name)
+        m = re.search(r"VGPRs Spill: (\d+)", line)
+        if m and name and int(m.group(1)) > 0 and NO_SPILLS.search(name) and name not in out:
             out.append(name)
     return out
 
@@ -83,8 +92,8 @@ def build(verbose: bool = False) -> Path:
             raise RuntimeError(f"hipcc failed for {src}:\n{res.stdout}\n{res.stderr}")
         spilled = spilling_kernels(res.stderr)
         if spilled:
-            raise RuntimeError(f"{src}: register spills (scratch) in {', '.join(spilled)}; the histogram "
-                               "and scorer kernels must fit their registers")
+            raise RuntimeError(f"{src}: register spills (scratch) in {', '.join(spilled)}; the histogram, "
+                               "scorer and choice kernels must fit their registers")
         if verbose:
             warn = "\n".join(l for l in res.stderr.splitlines() if "remark:" not in l)
             if warn.strip():

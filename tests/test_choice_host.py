@@ -99,3 +99,18 @@ def test_choice_struct_layouts_match_header():
         subprocess.run([cc, "-std=c11", "-I", str(ROOT / "include"), str(src), "-o", str(exe)], check=True)
         got = dict(line.split() for line in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.splitlines())
     assert {k: int(v) for k, v in got.items()} == want
+
+
+def test_build_refuses_spills_of_the_choice_kernels():
+    """What the compiler reports of a kernel that spills, and of one that only has a frame reserved."""
+    from packboost_amd.build import spilling_kernels
+
+    def remarks(name, scratch, vgprs):
+        return "\n".join(f"choice.hip:1:0: remark:     {v} [-Rpass-analysis=kernel-resource-usage]" for v in (
+            f"Function Name: {name}", "VGPRs: 96", f"ScratchSize [bytes/lane]: {scratch}", "SGPRs Spill: 40",
+            f"VGPRs Spill: {vgprs}", "LDS Size [bytes/block]: 0"))
+
+    wide, tile, other = "_ZN2pb11wide_kernelILi4E", "_ZN2pb11tile_kernelILi3E", "_ZN2pb11join_kernelE"
+    assert spilling_kernels("\n".join((remarks(wide, 36, 0), remarks(tile, 0, 0), remarks(other, 64, 3)))) == []
+    assert spilling_kernels("\n".join((remarks(tile, 20, 4), remarks(wide, 80, 0)))) == [tile, wide]
+    assert spilling_kernels(remarks("_ZN2pb15hist_era_kernelE", 4, 0)) == ["_ZN2pb15hist_era_kernelE"]
