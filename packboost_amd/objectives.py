@@ -34,6 +34,16 @@ def _array(name: str, v, n: int, dtype) -> np.ndarray:
     return np.ascontiguousarray(a, dtype=dtype)
 
 
+def _indices(name: str, v, n: int) -> np.ndarray:
+    """int32 [n] of whole numbers that it holds."""
+    a = np.asarray(v.detach().cpu().numpy() if isinstance(v, torch.Tensor) else v)
+    if a.size and not np.issubdtype(a.dtype, np.integer):
+        raise ValueError(f"{name} must be integers, got {a.dtype}")
+    if a.size and (a.min() < -2 ** 31 or a.max() > 2 ** 31 - 1):
+        raise ValueError(f"{name} must lie in int32's range")
+    return _array(name, a, n, np.int32)
+
+
 def _to(device: torch.device, a: np.ndarray | None) -> torch.Tensor | None:
     return None if a is None else torch.from_numpy(a).to(device)
 
@@ -102,9 +112,9 @@ class _Choices(Objective):
         if self._off.size == 0 or self._off[0] != 0 or np.any(self._off[1:] < self._off[:-1]):
             raise ValueError("offsets must start at 0 and not decrease")
         self._g, self._n = self._off.size - 1, int(self._off[-1])
-        self._chosen = _array("chosen", chosen, self._g, np.int32)
+        self._chosen = _indices("chosen", chosen, self._g)
         self._mask = None if mask is None else _array("mask", mask, self._n, bool)
-        self._positions = None if positions is None else _array("positions", positions, self._n, np.int32)
+        self._positions = None if positions is None else _indices("positions", positions, self._n)
         if buckets is not None and positions is None:
             raise ValueError("buckets need positions")
         self._buckets = buckets if buckets is not None or positions is None else PositionBuckets()

@@ -114,3 +114,25 @@ def test_build_refuses_spills_of_the_choice_kernels():
     assert spilling_kernels("\n".join((remarks(wide, 36, 0), remarks(tile, 0, 0), remarks(other, 64, 3)))) == []
     assert spilling_kernels("\n".join((remarks(tile, 20, 4), remarks(wide, 80, 0)))) == [tile, wide]
     assert spilling_kernels(remarks("_ZN2pb15hist_era_kernelE", 4, 0)) == ["_ZN2pb15hist_era_kernelE"]
+
+
+def test_objectives_refuse_indices_that_a_cast_would_change():
+    """Choices and positions are int32: what int32 does not hold, or what is no whole number, is not cut to fit."""
+    from packboost_amd import ChoicePreferenceObjective, PolicyObjective
+
+    off, one = [0, 2, 5], np.ones(2)
+    policy = lambda chosen=(0, 1), positions=None: PolicyObjective(off, chosen, one, one, positions=positions)
+    sequences = lambda chosen=(0, 1), positions=None: ChoicePreferenceObjective(off, chosen, [0, 1, 2], [0], [1], positions=positions)
+    place = np.arange(5)
+    for build in (policy, sequences):
+        for bad in ([0, 2 ** 32 + 1], [0, -2 ** 31 - 1], [0.0, 1.7], np.array([0.0, 1.0]), np.array([False, True]),
+                    np.array([0, 2 ** 64 - 1], dtype=np.uint64)):
+            with pytest.raises(ValueError, match="chosen"):
+                build(chosen=bad)
+        for bad in (place + 2 ** 32, place + 0.5, place.astype(np.float32)):
+            with pytest.raises(ValueError, match="positions"):
+                build(positions=bad)
+        for good in ([-1, 2 ** 31 - 1], np.array([0, 1], dtype=np.uint8), np.array([0, 7], dtype=np.int64)):
+            kept = build(chosen=good, positions=place.astype(np.int64))
+            assert kept._chosen.dtype == np.int32 and kept._chosen.tolist() == np.asarray(good).tolist()
+            assert kept._positions.dtype == np.int32 and kept._positions.tolist() == place.tolist()
