@@ -121,6 +121,7 @@ class _Choices(Objective):
         self._bias_rate = float(bias_rate)
         self.table: np.ndarray | None = None
         self._sets: ChoiceSets | None = None
+        self._bias: PositionBias | None = None
 
     def _bind_sets(self, perm, num_rows, device) -> np.ndarray | None:
         """Lays out the sets over the fit's rows; returns the order of the sets there (None: the caller's)."""

@@ -136,3 +136,38 @@ def test_objectives_refuse_indices_that_a_cast_would_change():
             kept = build(chosen=good, positions=place.astype(np.int64))
             assert kept._chosen.dtype == np.int32 and kept._chosen.tolist() == np.asarray(good).tolist()
             assert kept._positions.dtype == np.int32 and kept._positions.tolist() == place.tolist()
+
+
+@pytest.mark.parametrize("kind", ["policy", "sequences"])
+def test_a_bind_that_fails_is_released(monkeypatch, kind):
+    """Whatever fails after the sets are laid out (here: memory for the mask) is what the caller hears of, and
+    the sets are closed."""
+    import torch
+
+    from packboost_amd import ChoicePreferenceObjective, PolicyObjective, objectives
+
+    closed = []
+
+    class Sets:
+        def __init__(self, offsets, *, device=None):
+            pass
+
+        def close(self):
+            closed.append(self)
+
+    def no_memory(device, a):
+        raise MemoryError("out of device memory")
+
+    monkeypatch.setattr(objectives, "ChoiceSets", Sets)
+    monkeypatch.setattr(objectives, "_to", no_memory)
+    one, mask = np.ones(2), np.ones(5, bool)
+    obj = (PolicyObjective([0, 2, 5], [0, 1], one, one, mask=mask) if kind == "policy" else
+           ChoicePreferenceObjective([0, 2, 5], [0, 1], [0, 1, 2], [0], [1], mask=mask))
+    with pytest.raises(MemoryError):
+        try:  # as a fit does
+            obj.bind(None, 5, torch.device("cpu"))
+        finally:
+            obj.release()
+    assert len(closed) == 1
+    obj.release()
+    assert len(closed) == 1 and obj.table is None
