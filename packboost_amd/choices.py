@@ -12,9 +12,12 @@ clipped policy loss with a KL term, its value and gradients in one pass; `prefer
 paired log ratios on values or on sequences of steps.
 
 All of them run on the device as HIP kernels on torch's current stream, allocate their outputs from
-torch's allocator and wait for nothing, so a caller may capture them in a graph. Row and step
+torch's allocator and wait for nothing, so a caller may capture them in a graph. The sets, pairs, buckets
+and tensors of a captured call have to outlive the graph; sets and pairs are laid out before the capture,
+and PositionBuckets that the device has not seen are sent there before it by `on`. Row and step
 quantities are 1-D device tensors; scores are float32, bfloat16 or float16 (their gradient has the same
-type), everything else is float32.
+type), everything else is float32. The gradients are returned, not recorded: tensors that require
+gradients are read like any others, and nothing here is part of autograd's graph.
 """
 
 from __future__ import annotations
@@ -72,17 +75,34 @@ def _column(name: str, t, n: int, device: torch.device, *dtypes: torch.dtype) ->
     return t if t.stride(0) == 1 or n <= 1 else t.contiguous()
 
 
+_dropped: list = []  # (destroy, handle, device): closed, not freed yet
+
+
+def _free_dropped() -> None:
+    """Frees the layouts that were closed. A capture allows neither the wait nor the free: they stay until the
+    next layout is made or closed outside of one."""
+    while _dropped and not torch.cuda.is_current_stream_capturing():
+        destroy, h, device = _dropped.pop()
+        torch.cuda.synchronize(device)
+        getattr(_hip.load(), destroy)(h)
+
+
 class _Handle:
     """A layout the library keeps on the device."""
 
     _destroy = ""
 
+    def _before(self) -> None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"{type(self).__name__} cannot be laid out while a graph is captured")
+        _free_dropped()
+
     def close(self) -> None:
-        """Frees the device memory, once the calls that use it have ended."""
+        """Frees the device memory, once the calls that use it have ended (and a capture, if one is going on)."""
         h, self._handle = getattr(self, "_handle", None), None
         if h is not None and h.value:
-            torch.cuda.synchronize(self.device)
-            getattr(_hip.load(), self._destroy)(h)
+            _dropped.append((self._destroy, h, self.device))
+            _free_dropped()
 
     def __del__(self) -> None:  # pragma: no cover - best effort
         try:
@@ -111,6 +131,7 @@ class ChoiceSets(_Handle):
         if off.size == 0 or off[0] != 0 or np.any(off[1:] < off[:-1]):
             raise ValueError("offsets must start at 0 and not decrease")
         self.device = _home(device, offsets)
+        self._before()
         self.num_sets, self.num_rows = int(off.size - 1), int(off[-1])
         h = ctypes.c_void_p()
         with torch.cuda.device(self.device):
@@ -169,9 +190,12 @@ class PositionBuckets:
         return self.lookup[np.minimum(np.abs(q), self.reach) + (q > 0) * (self.reach + 1)]
 
     def on(self, device: torch.device) -> torch.Tensor:
+        """The lookup on a device, sent there at the first call."""
         t = self._on.get(device)
         if t is None:
-            t = self._on[device] = torch.from_numpy(self.lookup).to(device)
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"PositionBuckets have not been on {device} yet: call on(device) before the capture")
+            t = self._on[_device(device)] = torch.from_numpy(self.lookup).to(device)
         return t
 
 
@@ -199,6 +223,7 @@ class PreferencePairs(_Handle):
     def __init__(self, winners, losers, *, num_values: int | None = None, offsets=None, device=None) -> None:
         self._handle = None
         self.device = _home(device, winners, losers, offsets)
+        self._before()
         here = all(isinstance(t, torch.Tensor) and t.device == self.device for t in (winners, losers))
         table = _device_int64 if here else _host_int64
         w, l = table("winners", winners), table("losers", losers)

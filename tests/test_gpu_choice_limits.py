@@ -394,3 +394,37 @@ def test_small_probabilities_of_longer_sets(hip, size):
     other = np.arange(size) != 0
     # what lies below 2^-126 may be 0
     assert np.all(np.abs(gs.double().cpu().numpy() - want)[other] <= 55 * U * want[other] + 2.0 ** -126)
+
+
+def test_layouts_and_buckets_around_a_capture(hip):
+    """A layout that goes while a graph is captured leaves the capture whole and is freed after it; what needs the
+    host is refused inside one, by name."""
+    from packboost_amd import ChoiceSets, PositionBias, PositionBuckets, PreferencePairs, choice_log_probs, choices
+
+    s = torch.randn(5, device=DEV)
+    pos = torch.arange(5, dtype=torch.int32, device=DEV)
+    bias = PositionBias(torch.randn(8, device=DEV), pos, PositionBuckets(8, 16))
+    fresh = PositionBias(bias.table, pos, PositionBuckets(8, 16))
+    bias.buckets.on(s.device)
+    sets, other, pairs = ChoiceSets([0, 2, 5]), ChoiceSets([0, 5]), PreferencePairs([0], [1], num_values=2)
+    want = choice_log_probs(s, sets, bias=bias)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for build in (lambda: ChoiceSets([0, 2]), lambda: PreferencePairs([0], [1], num_values=2),
+                      lambda: choice_log_probs(s, sets, bias=fresh)):
+            with pytest.raises(RuntimeError, match="captur"):
+                build()
+        other.close()
+        del pairs
+        assert len(choices._dropped) == 2
+        got = choice_log_probs(s, sets, bias=bias)
+    with pytest.raises(ValueError, match="closed"):
+        choice_log_probs(s, other)
+    for k in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        ChoiceSets([0, 2]).close()
+        assert not choices._dropped
+    assert torch.equal(choice_log_probs(s, sets, bias=fresh)[0], want[0])
