@@ -291,7 +291,7 @@ class PackBoost:
         if objective is not None and not isinstance(objective, Objective):
             raise TypeError("objective must be a packboost_amd Objective")
         if y is None and objective is not None:
-            y = np.zeros(int(X.shape[0]), dtype=np.float32)
+            y = np.zeros(len(X), dtype=np.float32)
         y_np = np.asarray(y.detach().cpu().numpy() if isinstance(y, torch.Tensor) else y,
                           dtype=np.float32)
         if y_np.ndim != 1:

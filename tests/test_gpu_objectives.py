@@ -287,3 +287,13 @@ def test_refusals(hip):
     with pytest.raises(ValueError):
         fit(PreferenceObjective([0], [1], label_smoothing=2.0))
     fit(PolicyObjective(off, chosen, one, one))  # and the model still fits
+
+
+def test_rows_as_a_list(hip):
+    """Without targets, features in any form that a fit takes with them."""
+    from packboost_amd import PackBoost, PreferenceObjective
+
+    X = np.random.default_rng(2).standard_normal((200, 4)).astype(np.float32)
+    obj = lambda: PreferenceObjective(np.arange(100), np.arange(100, 200))
+    a, b = (PackBoost(config()).fit(t, None, None, num_rounds=2, objective=obj()) for t in (X, X.tolist()))
+    same_trees(a, b)
