@@ -967,7 +967,9 @@ __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, TileIn<MODE, TYPE
             wave_sync();
         }
     }
-    float anew[kTileRounds];  // what a set's exponentials over a far lse sum to
+    // What a set's exponentials over a far lse sum to, 1 where that is not asked for: every step divides by it. (With
+    // the division under a branch on whether the tile has such a set, the compiler dropped the other branch's sign.)
+    float anew[kTileRounds];
 #pragma unroll
     for (int r = 0; r < kTileRounds; ++r) anew[r] = 1.0f;
     if (!SOFT) {

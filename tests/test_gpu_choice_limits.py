@@ -10,7 +10,8 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_choices import DEV, U, back, offsets_of, per_set, policy_reference, reference
+from test_gpu_choices import (DEV, LAYOUTS, U, back, bound_lp, check_grads, make, offsets_of, per_set, policy_reference,
+                              reference, same_or_close)
 
 pytestmark = pytest.mark.gpu
 
@@ -428,3 +429,34 @@ def test_layouts_and_buckets_around_a_capture(hip):
         ChoiceSets([0, 2]).close()
         assert not choices._dropped
     assert torch.equal(choice_log_probs(s, sets, bias=fresh)[0], want[0])
+
+
+@pytest.mark.parametrize("dtype,masked,biased", [("f32", False, False), ("f32", True, True), ("f32", False, True),
+                                                 ("bf16", True, False), ("bf16", True, True), ("f16", False, True),
+                                                 ("f16", True, False), ("f32", True, False)])
+@pytest.mark.parametrize("layout", ["small", "empties", "wave", "tile_edges", "mixed", "long_pair"])
+def test_offset_scores_of_every_kind(hip, layout, dtype, masked, biased):
+    """Scores near 64, whose sets are summed anew in the backward passes: masks, biases, 16-bit scores and every
+    kind of set, in the bounds of test_gpu_choices."""
+    from packboost_amd import choice_log_probs, choice_log_probs_backward
+
+    d = make(LAYOUTS[layout], dtype, masked, biased, seed=33)
+    kw = dict(mask=d["mask"], bias=d["bias"])
+    moved = (d["scores"].float() + 64).to(d["scores"].dtype)
+    by = (moved.double() - d["scores"].double()).cpu().numpy()
+    d["x"] = np.where(d["keep"], d["x"] + np.where(d["keep"], by, 0.0), -np.inf)
+    p, _, lse, ok, step, at = reference(d)
+    tol = bound_lp(d)
+    got, got_lse = choice_log_probs(moved, d["sets"], chosen=d["chosen"], **kw)
+    same_or_close(got, step, tol)
+    same_or_close(got_lse, lse, tol)
+    up = d["r"].standard_normal(len(step)).astype(np.float32)
+    gs, gt = choice_log_probs_backward(torch.from_numpy(up).to(DEV), moved, got_lse, d["sets"], chosen=d["chosen"], **kw)
+    g, size = back(d, p, ok, at, up.astype(np.float64))
+    check_grads(d, gs, gt, g, size, tol)
+    rows = d["r"].standard_normal(len(d["x"])).astype(np.float32)
+    gs, gt = choice_log_probs_backward(torch.from_numpy(rows).to(DEV), moved, got_lse, d["sets"], **kw)
+    u = np.where(d["keep"], rows.astype(np.float64), 0.0)
+    total, absolute = (np.repeat(per_set(d, np.add, v, 0.0), d["size"]) for v in (u, np.abs(u)))
+    check_grads(d, gs, gt, np.where(d["keep"], u - p * total, 0.0),
+                np.abs(u) + p * absolute * (1 + 100 * U / (tol + 4 * U)), tol)
