@@ -55,7 +55,7 @@ NO_SCRATCH = re.compile(r"hist_era_kernel|seg_score_kernel|des_score|kcuts_kerne
 # Kernels that must not spill vector registers: the choice operators'. (The policy's wide_kernel with a bias has
 # 36 bytes of scratch reserved, for kernel arguments that end in lanes of a vector register; nothing in it is
 # read or written.)
-NO_SPILLS = re.compile(r"tile_kernel|wide_kernel|part_kernel|part_grads_kernel|part_far_kernel|split_steps_kernel")
+NO_SPILLS = re.compile(r"\d(?:tile|wide|part|part_grads|part_far|split_steps)_kernel")
 
 
 def spilling_kernels(remarks: str) -> list[str]:
