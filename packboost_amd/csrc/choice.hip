@@ -629,6 +629,10 @@ struct TableSum {
         fresh = false;
     }
 
+    // ALL: zeros are added, too, without a branch a row. The policy's tiles take that (28.5 us a call for 480k sets, 28.7
+    // else); the backward passes' keep the registers of five waves a SIMD without it (steps of 100k sets 48.2 us from
+    // call to result, 50.8 else).
+    template <bool ALL>
     __device__ __forceinline__ void add(const float (&g)[kRun], const Buckets& buckets) {
         float t[kRun];
         uint32_t over = 0;
@@ -645,6 +649,7 @@ struct TableSum {
         }
 #pragma unroll
         for (int k = 0; k < kRun; ++k) {
+            if (!ALL && t[k] == 0.0f) continue;
             // the nearest whole number: the low bits of t + 1.5 2^52
             const long long n = __double_as_longlong((double)t[k] + 6755399441055744.0) - 0x4338000000000000ll;
             atomicAdd(&bins[bin_of(buckets.at(k))], (unsigned long long)n);
@@ -909,6 +914,31 @@ __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, TileIn<MODE, TYPE
         }
     }
     wave_sync();
+    // What a set's exponentials over a far lse sum to, 1 where that is not asked for: every gradient is divided by it.
+    // (With the division under a branch on whether the tile has such a set, the compiler dropped the other
+    // branch's sign.) A lane walks its set's logits: scans would take registers from tables without such sets.
+    float anew[kTileRounds];
+#pragma unroll
+    for (int r = 0; r < kTileRounds; ++r) anew[r] = 1.0f;
+    if (!SOFT) {
+        bool far = false;
+#pragma unroll
+        for (int r = 0; r < kTileRounds; ++r) far = far || (r * kWave + lane < in.sets && far_lse(in.lse[r]));
+        if (__any(far)) {
+            if (!STEPS) {
+                write_run(&sh.x[i0], x);
+                wave_sync();
+            }
+#pragma unroll
+            for (int r = 0; r < kTileRounds; ++r)
+                if (r * kWave + lane < in.sets && far_lse(in.lse[r])) {
+                    double t = 0.0;
+                    for (int i = begin[r]; i < end[r]; ++i) t += (double)exp_of(sh.x[i] - in.lse[r]);
+                    anew[r] = (float)t;
+                }
+            wave_sync();
+        }
+    }
     int id[kRun];
     float v[kRun];
     if (alone) {
@@ -967,32 +997,6 @@ __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, TileIn<MODE, TYPE
             wave_sync();
         }
     }
-    // What a set's exponentials over a far lse sum to, 1 where that is not asked for: every step divides by it. (With
-    // the division under a branch on whether the tile has such a set, the compiler dropped the other branch's sign.)
-    float anew[kTileRounds];
-#pragma unroll
-    for (int r = 0; r < kTileRounds; ++r) anew[r] = 1.0f;
-    if (!SOFT) {
-        bool far = false;
-#pragma unroll
-        for (int r = 0; r < kTileRounds; ++r) far = far || (r * kWave + lane < in.sets && far_lse(in.lse[r]));
-        if (__any(far)) {  // a lane walks a set: a scan here would take registers from tables without such sets
-            float e[kRun];
-#pragma unroll
-            for (int k = 0; k < kRun; ++k) e[k] = row_exp<MODE, TYPE, BIAS>(x[k] - sh.shift[id[k] - 1]);
-            write_run(&sh.x[i0], e);  // the logits there have been read
-            wave_sync();
-#pragma unroll
-            for (int r = 0; r < kTileRounds; ++r)
-                if (r * kWave + lane < in.sets && far_lse(in.lse[r])) {
-                    double t = 0.0;
-                    for (int i = begin[r]; i < end[r]; ++i) t += (double)sh.x[i];
-                    anew[r] = (float)t;
-                    if (MODE == kRowsBack) sh.factor[r * kWave + lane] /= (float)t;
-                }
-            wave_sync();
-        }
-    }
     // a lane to a set: log-probabilities, losses, slopes
     float coef[kTileRounds];
     if (SOFT || STEPS) {
@@ -1029,6 +1033,11 @@ __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, TileIn<MODE, TYPE
         }
     }
     if (MODE == kSteps) return;
+    if (MODE == kRowsBack) {
+#pragma unroll
+        for (int r = 0; r < kTileRounds; ++r)
+            if (r * kWave + lane < in.sets && end[r] > begin[r]) sh.factor[r * kWave + lane] /= anew[r];
+    }
     if (STEPS) {  // the chosen rows' own part
         const float none[kRun] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
         write_run(&sh.x[i0], none);
@@ -1068,7 +1077,7 @@ __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, TileIn<MODE, TYPE
         else
             store_run<TYPE>(a, sp, 0, a.grad_scores, v);
     }
-    if (BIAS && GRAD) table.add(v, buckets);
+    if (BIAS && GRAD) table.add<MODE == kPolicy>(v, buckets);
 }
 
 // One set of more than kSetShort rows by a wave (THREADS 64), or a longer one or a part of it by a
@@ -1250,7 +1259,7 @@ __device__ __forceinline__ void wide_pass(const ChoiceArgs& a, const SetItem& im
                         if (at - i == k) v[j][k] += extra;
                 }
                 if (i < sp.hi) store_run<TYPE>(a, sp, i, a.grad_scores, v[j]);
-                if (BIAS) table.add(v[j], buckets[j]);
+                if (BIAS) table.add<MODE == kPolicy>(v[j], buckets[j]);
             }
         }
     }
