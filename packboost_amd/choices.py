@@ -16,7 +16,9 @@ torch's allocator and wait for nothing, so a caller may capture them in a graph.
 and tensors of a captured call have to outlive the graph; sets and pairs are laid out before the capture,
 and PositionBuckets that the device has not seen are sent there before it by `on`. Row and step
 quantities are 1-D device tensors; scores are float32, bfloat16 or float16 (their gradient has the same
-type), everything else is float32. The gradients are returned, not recorded: tensors that require
+type), everything else is float32. Tables whose rows start off a 16-byte boundary and scores with a stride
+are read row by row, which takes 1.3 to 5 times as long (see whole_run in csrc/choice.hip); columns with a
+stride other than the scores are copied. The gradients are returned, not recorded: tensors that require
 gradients are read like any others, and nothing here is part of autograd's graph.
 """
 

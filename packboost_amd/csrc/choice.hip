@@ -10,11 +10,11 @@
 // reduces them by a segmented scan over the lanes, whose cost does not depend on how the rows fall into
 // sets; a wave or a workgroup takes one longer set, or a part of it, in registers. Parts of a set are
 // reduced by a pass before (part_kernel). All of it is bound by memory at best: a row has 8 to 20 bytes and
-// some 20 operations, so every row is read once, in 16-byte accesses, and what is read is asked for before
-// anything is waited for (teams of lanes that walked each set's rows in LDS took 15 us for tiles that take
-// 5 to 7 us so). Every sum has a fixed order (lanes, waves, workgroups), so
+// some 20 operations, so every row is read once, in 16-byte accesses, and scores, masks, positions and what
+// the sets have are asked for before anything is waited for (teams of lanes that walked each set's rows in
+// LDS took 15 us for tiles that take 5 to 7 us so). Every sum has a fixed order (lanes, waves, workgroups), so
 // results do not change from run to run. Maxima, sums of exponentials and log-probabilities are float32;
-// losses and the table's gradient are joined in double, each rounded once when it is written.
+// losses, the table's gradient and sequences' sums are joined in double, each rounded once when it is written.
 #include <algorithm>
 
 #include "pb_internal.h"
@@ -66,7 +66,8 @@ __device__ __forceinline__ float log_of(float x) { return __builtin_amdgcn_logf(
 
 // What a step of a policy has once is taken to below float32's rounding: its loss terms cancel (advantages of
 // both signs, e^d - d - 1 of a small d), and its ratio is held against bounds. All in double it took half as
-// long again (policy loss of 480k sets 32 us, 24 so, 22.7 in float32 alone).
+// long again (tiles of 480k sets, before the table's bins had units of their own: 32 us, 24 so, 22.7 in float32
+// alone).
 //
 // log x within 2^-30 for finite x above 1/2 (else as log_of): x = 2^k m, m in [2/3, 4/3), and
 // log m = 2 (f + f^3 / 3 + ... + f^11 / 11), f = (m - 1) / (m + 1) with the quotient's remainder, |f| <= 1/5.
@@ -193,7 +194,9 @@ __device__ __forceinline__ uint32_t outside(const Span& s, int i) {
 }
 
 // Whether a run goes in accesses of 16 bytes: the addresses are aligned (a.vec) and all its rows lie in the
-// table. Else it goes row by row, in a rolled loop, within [lo, hi).
+// table. Else it goes row by row, in a rolled loop, within [lo, hi). That is what a table whose rows start off a
+// 16-byte boundary, or whose scores have a stride, costs the whole call (us, aligned / one row off / stride 2: steps of
+// 100k sets 28 / 44 / 52; policy of 480k sets 28 / 38 / 40; 4096 sets of 32000 bfloat16 scores 154 / 509 / 707).
 __device__ __forceinline__ bool whole_run(const ChoiceArgs& a, const Span& s, int i) { return a.vec && i + kRun <= s.end; }
 
 __device__ __forceinline__ void put_row(float (&x)[kRun], int k, float v) {
@@ -747,7 +750,8 @@ __global__ __launch_bounds__(kBlock) void part_grads_kernel(ChoiceArgs a, int fi
 }
 
 // The sum of exp(x - lse) of the parts [first, first + n) whose set's lse is far (far_lse). A workgroup looks at
-// 64 of its parts at a time, a lane each, so that a table without such sets costs a launch (16384 parts: 3 us).
+// 64 of its parts at a time, a lane each, so that a table without such sets costs a launch (16384 parts: 4.7 us, and
+// 43 more where all are: 4096 sets of 32000 in bfloat16).
 template <int TYPE, bool MASK, bool BIAS>
 __global__ __launch_bounds__(kBlock) void part_far_kernel(ChoiceArgs a, int first, int n) {
     __shared__ float shf[kWaves];
@@ -804,7 +808,8 @@ __device__ __forceinline__ void read_run(const float* p, float (&x)[kRun]) {
     x[4] = u.x, x[5] = u.y, x[6] = u.z, x[7] = u.w;
 }
 
-// What a tile reads, all of it asked for before anything is waited for: a lane's run, and the lane's sets.
+// What a tile reads, asked for before anything is waited for: a lane's run, and the lane's sets. (The rows' given
+// gradients, of the rows' backward, are asked for when the logits have come.)
 template <int MODE, int TYPE, bool MASK, bool BIAS>
 struct TileIn {
     Span sp;   // of the lane's run alone
@@ -863,10 +868,13 @@ struct TileIn {
 // One tile of short sets by one wave: the maximum and the sum of exponentials by two segmented scans, which
 // leave them in LDS by set; a lane to a set then forms log-probabilities, losses and slopes, 64 sets at a
 // time; the rows take their set's factor from LDS. A tile of one set has no need of the scans (policy steps
-// of 30000 sets of 300 rows: 37 us, 44 with them; 68 and 76 for steps in float32 with their backward). About 700 vector instructions for 512 rows, 1200 with
-// mask, bias and the policy's steps: past the first few thousand tiles their issue bounds it, before that
-// the chain from the loads to the stores. 2.4M rows of 100k sets with mask and bias: log-probabilities of
-// the steps 9.2 us, their backward with the table's gradient 12.9 us; the policy loss of 480k sets 24.0 us.
+// of 30000 sets of 300 rows: 37 us, 44 with them; 68 and 76 for steps in float32 with their backward). With mask and
+// bias a tile of 512 rows takes 504 vector instructions for the steps, 814 for their backward and 1465 for the
+// policy; a SIMD issues in 45 to 47 % of the time, and waves wait for half of theirs. So what bounds a few
+// thousand tiles is the chain from the loads to the stores, of one tile a wave, and how many waves are resident:
+// four a SIMD in the policy's, whose last workgroups run a second round. 2.4M rows of 100k sets: steps 9.1 us, their
+// backward with the table's gradient 14.0 us; the policy loss of 480k sets 25.4 us. Tens of thousands of tiles
+// issue in 69 % (40M rows in bfloat16: 43.5 us).
 template <int MODE, int TYPE, bool MASK, bool BIAS>
 __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, TileIn<MODE, TYPE, MASK, BIAS>& in, TileShared& sh,
                                           const BiasShared* bias, TableSum& table, double (&tally)[3]) {
@@ -1084,8 +1092,8 @@ __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, TileIn<MODE, TYPE
 // workgroup. A wave passes over runs beyond its rows. The rows stay in registers from the load to the
 // store, one exponential each, so that a set of up to kSetWideRows rows is read once; a longer one's parts are
 // read a second time. Bound by memory for sets of thousands of rows (backward of 4096 sets of 32000
-// bfloat16 scores, 524 MB: 86 us, 6.1 TB/s), by the instructions a set takes beside its rows (about 250)
-// for hundreds (100k policy steps, 29M of their 40M rows here: 41 us, 2.8 TB/s).
+// bfloat16 scores, 524 MB: 87.5 us, 6.0 TB/s), by the instructions a set takes beside its rows (about 250)
+// for hundreds (100k policy steps, 29M of their 40M rows here: 42.4 us, 2.7 TB/s).
 template <int MODE, int TYPE, bool MASK, bool BIAS, int THREADS>
 __device__ __forceinline__ void wide_pass(const ChoiceArgs& a, const SetItem& im, int32_t index, Soft* shs, float* shf,
                                           const BiasShared* bias, TableSum& table, double (&tally)[3]) {
@@ -1430,7 +1438,8 @@ __global__ __launch_bounds__(kBlock) void join_kernel(const double* __restrict__
 // pairs that a value is in (list entry: pair * 2 + (1 where it is the loser)). A pair's slope is computed once
 // and gathered twice, in the lists' order: no atomics, so hubs (values in thousands of pairs) cost
 // what their entries cost and sums keep their order. Bound by the gathers, which find little of 20 MB of
-// slopes in an XCD's 4 MB of L2: 10M entries of 1M lists 148 us, 3.6 TB/s of 64-byte lines.
+// slopes in an XCD's 4 MB of L2: 10M entries of 1M lists 149 to 152 us, 3.6 TB/s of 64-byte lines. They
+// are taken in the caller's order of the pairs; an order in which neighbouring entries share lines is not tried.
 struct SumArgs {
     const int64_t* off;
     const SetItem* tiles;
@@ -1536,7 +1545,7 @@ __global__ __launch_bounds__(kBlock) void set_join_kernel(SumArgs a, const int32
 // z = beta (a_w - a_l); the loss w [(1 - e) softplus(-z) + e softplus(z)] and its slope
 // beta w (sigmoid(z) - (1 - e)). Sequences' values come from their sums in double, others' as value
 // - ref, the differences taken in double: both can be large where z is small. Bound by the gathers of the values: 5M
-// pairs of 1M values, values and references side by side, 94 us (160 us in arrays of their own). Four
+// pairs of 1M values, values and references side by side, 93 us (160 us in arrays of their own). Four
 // pairs are in flight a thread.
 __global__ __launch_bounds__(kBlock) void pair_kernel(PairArgs a) {
     __shared__ double sh[kWaves];

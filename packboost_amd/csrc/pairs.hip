@@ -5,7 +5,7 @@
 // lanes below that hold its digit, so equal digits keep their order and the layout has one result only.
 //
 // A pass reads an entry twice and writes it once (4 + 8 + 8 bytes) at places that are scattered over 256
-// runs, and is bound by those writes: for 10M entries of 1M values 16 to 27 us to count and 87 to 211 us to
+// runs, and is bound by those writes: for 10M entries of 1M values 16 to 27 us to count and 87 to 226 us to
 // write, three passes of them, 0.65 ms in all. What a caller waits for is the device memory taken for the
 // call and the list starts that go to the host, whose lists' work is laid out there (4.4 ms).
 #include "pb_internal.h"

@@ -585,7 +585,7 @@ struct ChoiceArgs {
     void* grad_scores;
     float* grad_table;
     float* stats;   // policy: loss, kl, clipped weight
-    float2* parts;  // [num_mid + num_wide] maximum and sum of the parts of split sets
+    float2* parts;  // [num_mid + num_wide] of the parts of split sets: maximum and sum; backward: sum over a far lse, sum of gradients
     double* sums;   // [choice_grid][3 (policy) + num_buckets (gradient)]
 };
 struct PairArgs {

@@ -12,7 +12,8 @@ shrink with the table.
 The two objectives on choices can learn a position bias beside the trees: a bucket of positions is
 fitted like a leaf, table -= bias_rate * (sum of its rows' gradients) / (number of its rows), each
 round, and taken into account in the scores' gradients; the model's own predictions are free of it.
-`table` holds it after the fit.
+`table` holds it after the fit; a saved model holds the trees alone, so who serves with the bias keeps
+`table` beside it.
 
 Rows are the fit's, in the order they are passed in; a set's rows must be of one era (the fit sorts rows
 by era, which keeps them together).
