@@ -751,7 +751,7 @@ __global__ __launch_bounds__(kBlock) void part_grads_kernel(ChoiceArgs a, int fi
 
 // The sum of exp(x - lse) of the parts [first, first + n) whose set's lse is far (far_lse). A workgroup looks at
 // 64 of its parts at a time, a lane each, so that a table without such sets costs a launch (16384 parts: 4.7 us, and
-// 43 more where all are: 4096 sets of 32000 in bfloat16).
+// 42 more where all are: 4096 sets of 32000 in bfloat16).
 template <int TYPE, bool MASK, bool BIAS>
 __global__ __launch_bounds__(kBlock) void part_far_kernel(ChoiceArgs a, int first, int n) {
     __shared__ float shf[kWaves];
@@ -924,7 +924,7 @@ __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, TileIn<MODE, TYPE
     wave_sync();
     // What a set's exponentials over a far lse sum to, 1 where that is not asked for: every gradient is divided by it.
     // (With the division under a branch on whether the tile has such a set, the compiler dropped the other
-    // branch's sign.) A lane walks its set's logits: scans would take registers from tables without such sets.
+    // branch's sign.) Lanes walk the sets' logits: scans would take registers from tables without such sets.
     float anew[kTileRounds];
 #pragma unroll
     for (int r = 0; r < kTileRounds; ++r) anew[r] = 1.0f;
@@ -937,13 +937,26 @@ __device__ __forceinline__ void tile_pass(const ChoiceArgs& a, TileIn<MODE, TYPE
                 write_run(&sh.x[i0], x);
                 wave_sync();
             }
+            // as many lanes to a set as there are (8M rows in sets of 30 to 400: 21 to 23 us, 18 to 19 without far sets; by
+            // a lane to a set 26 to 133)
+            if (in.sets <= kWave / 2) {
+                const int bits = in.sets > 1 ? __clz(in.sets - 1) - 26 : 6, team = lane >> bits, from = min(team, in.sets - 1);
+                const int e = __shfl(end[0], from);
+                const float lse = __shfl(in.lse[0], from);
+                double t = 0.0;
+                for (int i = __shfl(begin[0], from) + (lane & ((1 << bits) - 1)); i < e; i += 1 << bits) t += (double)exp_of(sh.x[i] - lse);
+                for (int m = 1; m < 1 << bits; m *= 2) t += __shfl_xor(t, m);
+                t = __shfl(t, (lane << bits) & (kWave - 1));
+                if (lane < in.sets && far_lse(in.lse[0])) anew[0] = (float)t;
+            } else {
 #pragma unroll
-            for (int r = 0; r < kTileRounds; ++r)
-                if (r * kWave + lane < in.sets && far_lse(in.lse[r])) {
-                    double t = 0.0;
-                    for (int i = begin[r]; i < end[r]; ++i) t += (double)exp_of(sh.x[i] - in.lse[r]);
-                    anew[r] = (float)t;
-                }
+                for (int r = 0; r < kTileRounds; ++r)
+                    if (r * kWave + lane < in.sets && far_lse(in.lse[r])) {
+                        double t = 0.0;
+                        for (int i = begin[r]; i < end[r]; ++i) t += (double)exp_of(sh.x[i] - in.lse[r]);
+                        anew[r] = (float)t;
+                    }
+            }
             wave_sync();
         }
     }
