@@ -460,3 +460,17 @@ def test_offset_scores_of_every_kind(hip, layout, dtype, masked, biased):
     total, absolute = (np.repeat(per_set(d, np.add, v, 0.0), d["size"]) for v in (u, np.abs(u)))
     check_grads(d, gs, gt, np.where(d["keep"], u - p * total, 0.0),
                 np.abs(u) + p * absolute * (1 + 100 * U / (tol + 4 * U)), tol)
+
+
+@pytest.mark.parametrize("size", [3, 700, 3000, 9000])
+def test_a_choice_that_cannot_be(hip, size):
+    """A chosen row whose score is -inf: its log-probability is -inf, its ratio 0 and its KL term inf, which without
+    weight changes nothing."""
+    from packboost_amd import ChoiceSets, policy_loss
+
+    s = torch.zeros(size, device=DEV)
+    s[1] = -math.inf
+    one = torch.ones(1, device=DEV)
+    r = policy_loss(s, ChoiceSets([0, size]), torch.ones(1, dtype=torch.int32, device=DEV), one, -one, ref_log_probs=-one)
+    assert float(r.log_probs[0]) == -math.inf and float(r.kl) == math.inf
+    assert float(r.loss) == 0.0 and torch.equal(r.grad_scores, torch.zeros_like(s))
