@@ -581,10 +581,13 @@ typedef struct {
 } pb_choice_scores;
 
 /* Bytes of the workspace (16-byte aligned; none where this is 0) of a call on these sets: op PB_LOG_PROBS
- * (pb_choice_log_probs), PB_BACKWARD or PB_POLICY; -1: bad argument. */
+ * (pb_choice_log_probs), PB_BACKWARD, PB_POLICY, PB_REPORT_BACKWARD (pb_choice_report_backward) or PB_DISTILL
+ * (pb_distillation_loss); -1: bad argument. */
 #define PB_LOG_PROBS 0
 #define PB_BACKWARD 1
 #define PB_POLICY 2
+#define PB_REPORT_BACKWARD 3
+#define PB_DISTILL 4
 int64_t pb_choice_work_bytes(const pb_sets* sets, int32_t op, int32_t num_buckets);
 
 /* chosen_dev NULL: log_probs_dev float32 [rows], every row's (-inf where masked). Else (int32
@@ -622,6 +625,52 @@ typedef struct {
 int pb_policy_loss(const pb_sets* sets, const pb_choice_scores* scores, const pb_policy_terms* terms,
                    const int32_t* chosen_dev, float* stats_dev, float* log_probs_dev, void* grad_scores_dev,
                    float* grad_table_dev, void* work_dev, int64_t work_bytes, void* stream);
+
+/* What a model says of each set, at a temperature T in [2^-20, 2^20]: p is the softmax of the logits over T.
+ * log_probs_dev (float32 [num_sets], with chosen_dev): the chosen rows' log p, 0 for a step left out. entropy_dev
+ * float32 [num_sets]: -sum of p log p, 0 for a set without probability; lse_dev as pb_choice_log_probs gives it, of the
+ * logits over T. top_index_dev int32 and top_log_probs_dev float32 [num_sets][top], top in [0, 64]: the rows of
+ * largest logit by their index within the set, and their log p; equal logits (as float32, the bias added) by index, NaN above
+ * all. Rows left out and rows of logit -inf are not listed; behind the last row stand -1 and -inf. Sets of more than
+ * 2^31 - 1 rows have no lists (PB_ERR_UNSUPPORTED). The workspace has pb_choice_report_work_bytes (-1: bad argument). */
+int64_t pb_choice_report_work_bytes(const pb_sets* sets, int32_t top);
+int pb_choice_report(const pb_sets* sets, const pb_choice_scores* scores, const int32_t* chosen_dev, float temperature,
+                     int32_t top, float* log_probs_dev, float* entropy_dev, float* lse_dev, int32_t* top_index_dev,
+                     float* top_log_probs_dev, void* work_dev, int64_t work_bytes, void* stream);
+
+/* Gradients of the scores and the bias table (laid out as in pb_choice_log_probs_backward) from those of the
+ * chosen rows' log-probabilities (with chosen_dev, or NULL) and of the entropies (or NULL), float32 [num_sets]
+ * each, as pb_choice_report gave them for the same arguments. The sets' sums are formed anew. */
+int pb_choice_report_backward(const pb_sets* sets, const pb_choice_scores* scores, const int32_t* chosen_dev,
+                              float temperature, const float* grad_log_probs_dev, const float* grad_entropy_dev,
+                              void* grad_scores_dev, float* grad_table_dev, void* work_dev, int64_t work_bytes,
+                              void* stream);
+
+/* A teacher of which each set's best rows are known: [num_sets][entries], entries in [1, 64]. */
+typedef struct {
+    const int32_t* index_dev;  /* rows by their index within the set; outside of it: none */
+    const void* logits_dev;    /* logit_type */
+    const float* weights_dev;  /* float32 [num_sets], or NULL: 1 */
+    int32_t entries;
+    int32_t logit_type;        /* PB_F32, PB_BF16, PB_F16 */
+    int32_t tail;              /* 0: logits; else log-probabilities at the temperature, what they leave counts */
+    float temperature, scale;
+    int32_t reserved;
+} pb_teacher;
+
+/* The divergence of the student (the scores' softmax p at the temperature T) from the teacher. The entries count that
+ * name a row that is not masked, the first of those that name one row. q is the softmax of the teacher's logits over T
+ * within the entries that count; or (tail) q = exp of the log-probabilities, and rho = 1 - sum of q stands against
+ * the student's probability pi of the rows not listed. Where no such row has probability, or the q sum to 1 or more, they
+ * are divided by their sum and rho is 0.
+ *   kl_dev float32 [num_sets] = sum of q (log q - log p) + rho (log rho - log pi),
+ *   loss_dev[0] = scale T^2 * sum of w kl.
+ * Sets in which the teacher's entries or the student have no probability are left out (kl 0, no gradient); sets of weight
+ * 0 count for nothing, also where their divergence is infinite. The gradients are the loss's, laid out as in
+ * pb_choice_log_probs_backward. */
+int pb_distillation_loss(const pb_sets* sets, const pb_choice_scores* scores, const pb_teacher* teacher, float* loss_dev,
+                         float* kl_dev, void* grad_scores_dev, float* grad_table_dev, void* work_dev, int64_t work_bytes,
+                         void* stream);
 
 /* Pairs of values (winner, loser), by index in [0, num_values). seq_offsets_host (int64 [num_values + 1],
  * or NULL): the values are sums over runs of consecutive steps, run k [seq_offsets[k], seq_offsets[k + 1]).

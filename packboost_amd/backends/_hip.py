@@ -44,6 +44,7 @@ EXPORTED_SYMBOLS = (
     "pb_choice_log_probs_backward", "pb_policy_loss", "pb_pairs_create", "pb_pairs_create_from_device",
     "pb_pairs_destroy",
     "pb_preference_work_bytes", "pb_preference_loss",
+    "pb_choice_report_work_bytes", "pb_choice_report", "pb_choice_report_backward", "pb_distillation_loss",
 )
 
 
@@ -80,7 +81,7 @@ class PbFitBuffers(ctypes.Structure):
 
 
 PB_F32, PB_BF16, PB_F16 = 0, 1, 2
-PB_LOG_PROBS, PB_BACKWARD, PB_POLICY = 0, 1, 2
+PB_LOG_PROBS, PB_BACKWARD, PB_POLICY, PB_REPORT_BACKWARD, PB_DISTILL = 0, 1, 2, 3, 4
 
 
 class PbChoiceScores(ctypes.Structure):
@@ -97,6 +98,14 @@ class PbPolicyTerms(ctypes.Structure):
         ("advantages_dev", ctypes.c_void_p), ("old_log_probs_dev", ctypes.c_void_p),
         ("ref_log_probs_dev", ctypes.c_void_p), ("weights_dev", ctypes.c_void_p), ("ratio_min", ctypes.c_float),
         ("ratio_max", ctypes.c_float), ("kl_weight", ctypes.c_float), ("scale", ctypes.c_float),
+    ]
+
+
+class PbTeacher(ctypes.Structure):
+    _fields_ = [
+        ("index_dev", ctypes.c_void_p), ("logits_dev", ctypes.c_void_p), ("weights_dev", ctypes.c_void_p),
+        ("entries", ctypes.c_int32), ("logit_type", ctypes.c_int32), ("tail", ctypes.c_int32),
+        ("temperature", ctypes.c_float), ("scale", ctypes.c_float), ("reserved", ctypes.c_int32),
     ]
 
 
@@ -190,6 +199,11 @@ _SIGNATURES = {
     "pb_choice_log_probs_backward": (ctypes.c_int, [_VP, ctypes.POINTER(PbChoiceScores)] + [_VP] * 6 + [_I64, _VP]),
     "pb_policy_loss": (ctypes.c_int, [_VP, ctypes.POINTER(PbChoiceScores), ctypes.POINTER(PbPolicyTerms)] + [_VP] * 6 +
                        [_I64, _VP]),
+    "pb_choice_report_work_bytes": (_I64, [_VP, _I32]),
+    "pb_choice_report": (ctypes.c_int, [_VP, ctypes.POINTER(PbChoiceScores), _VP, _F32, _I32] + [_VP] * 6 + [_I64, _VP]),
+    "pb_choice_report_backward": (ctypes.c_int, [_VP, ctypes.POINTER(PbChoiceScores), _VP, _F32] + [_VP] * 5 + [_I64, _VP]),
+    "pb_distillation_loss": (ctypes.c_int, [_VP, ctypes.POINTER(PbChoiceScores), ctypes.POINTER(PbTeacher)] + [_VP] * 5 +
+                             [_I64, _VP]),
     "pb_pairs_create": (ctypes.c_int, [_VP, _VP, _I64, _I64, _VP, ctypes.POINTER(_VP)]),
     "pb_pairs_create_from_device": (ctypes.c_int, [_VP, _VP, _I64, _I64, _VP, _VP, ctypes.POINTER(_VP)]),
     "pb_pairs_destroy": (ctypes.c_int, [_VP]),

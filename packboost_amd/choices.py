@@ -9,7 +9,9 @@ model's scores give each row a probability within its set:
 `choice_log_probs` computes them for every row, or for the row chosen in each set (a step), and
 `choice_log_probs_backward` takes gradients back to the scores and the bias table. `policy_loss` is the
 clipped policy loss with a KL term, its value and gradients in one pass; `preference_loss` is the loss of
-paired log ratios on values or on sequences of steps.
+paired log ratios on values or on sequences of steps. `choice_report` tells how sure a model is of each set, the
+entropy and the rows it finds most probable, at a temperature; `choice_report_backward` trains with that, and
+`distillation_loss` on what such a report of a larger model lists.
 
 All of them run on the device as HIP kernels on torch's current stream, allocate their outputs from
 torch's allocator and wait for nothing, so a caller may capture them in a graph. The sets, pairs, buckets
@@ -34,6 +36,7 @@ import torch
 from .backends import _hip
 
 MAX_BUCKETS = 256
+MAX_TOP = 64
 _SCORE_TYPES = {torch.float32: _hip.PB_F32, torch.bfloat16: _hip.PB_BF16, torch.float16: _hip.PB_F16}
 
 
@@ -145,6 +148,13 @@ class ChoiceSets(_Handle):
         n = self._work.get((op, num_buckets))
         if n is None:
             n = self._work[op, num_buckets] = int(_hip.load().pb_choice_work_bytes(self._open(), op, num_buckets))
+        return (_empty(n, self.device, torch.uint8), n) if n else (None, 0)
+
+
+    def _report_workspace(self, top: int) -> tuple[torch.Tensor | None, int]:
+        n = self._work.get((-1, top))
+        if n is None:
+            n = self._work[-1, top] = int(_hip.load().pb_choice_report_work_bytes(self._open(), top))
         return (_empty(n, self.device, torch.uint8), n) if n else (None, 0)
 
 
@@ -272,6 +282,21 @@ class PreferenceLoss(NamedTuple):
     loss: torch.Tensor     # float32 scalar
     grad: torch.Tensor     # float32 per value, or per step of the sequences
     margins: torch.Tensor  # float32 per pair: beta * (log ratio of the winner - the loser's)
+
+
+class ChoiceReport(NamedTuple):
+    log_probs: torch.Tensor | None      # float32 per set: the chosen row's, 0 where left out; None without `chosen`
+    entropy: torch.Tensor               # float32 per set, 0 for a set without probability
+    lse: torch.Tensor                   # float32 per set, -inf for a set without probability
+    top_index: torch.Tensor | None      # int32 [sets, top] within the set, -1 behind the last; None where top is 0
+    top_log_probs: torch.Tensor | None  # float32 [sets, top], -inf behind the last
+
+
+class DistillationLoss(NamedTuple):
+    loss: torch.Tensor               # float32 scalar
+    grad_scores: torch.Tensor        # the scores' type, per row
+    grad_table: torch.Tensor | None  # float32 per bucket
+    kl: torch.Tensor                 # float32 per set: the divergence, 0 where left out
 
 
 def _scores(scores, sets: ChoiceSets, mask, bias) -> tuple[_hip.PbChoiceScores, list]:
@@ -409,6 +434,124 @@ def policy_loss(scores: torch.Tensor, sets: ChoiceSets, chosen: torch.Tensor, ad
             sets._open(), c, t, chosen.data_ptr(), stats.data_ptr(), lp.data_ptr(), gs.data_ptr(), _hip.ptr(gt),
             _hip.ptr(work), size, _hip.stream_ptr()), "pb_policy_loss")
     return PolicyLoss(stats[0], gs, gt, lp, stats[1], stats[2])
+
+
+def _temperature(v: float) -> float:
+    v = float(v)
+    if not 2.0 ** -20 <= v <= 2.0 ** 20:
+        raise ValueError(f"temperature must lie in [2^-20, 2^20], got {v}")
+    return v
+
+
+def choice_report(scores: torch.Tensor, sets: ChoiceSets, *, chosen: torch.Tensor | None = None, top: int = 0,
+                  mask: torch.Tensor | None = None, bias: PositionBias | None = None,
+                  temperature: float = 1.0) -> ChoiceReport:
+    """What a model says of each set, with p the softmax of its logits over the temperature: the chosen rows'
+    log-probabilities (see choice_log_probs), the entropy -sum p log p, the log of the sum of exponentials, and the
+    `top` (at most 64) rows of largest logit with their log-probabilities, best first.
+
+    Logits are compared as float32, the bias added; equal ones are listed by index, NaN above all. Masked rows and
+    rows of logit -inf are not listed. Sets of more than 2^31 - 1 rows have no lists."""
+    c, keep = _scores(scores, sets, mask, bias)
+    dev, g, top = sets.device, sets.num_sets, int(top)
+    if not 0 <= top <= MAX_TOP:
+        raise ValueError(f"top must lie in [0, {MAX_TOP}], got {top}")
+    temperature = _temperature(temperature)
+    if chosen is not None:
+        chosen = _column("chosen", chosen, g, dev, torch.int32)
+    with _on(dev):
+        lp = None if chosen is None else _empty(g, dev)
+        entropy, lse = _empty(g, dev), _empty(g, dev)
+        index = torch.empty((g, top), dtype=torch.int32, device=dev) if top else None
+        best = torch.empty((g, top), dtype=torch.float32, device=dev) if top else None
+        work, size = sets._report_workspace(top)
+        _hip.check(_hip.load().pb_choice_report(
+            sets._open(), c, _hip.ptr(chosen), temperature, top, _hip.ptr(lp), entropy.data_ptr(), lse.data_ptr(),
+            _hip.ptr(index), _hip.ptr(best), _hip.ptr(work), size, _hip.stream_ptr()), "pb_choice_report")
+    return ChoiceReport(lp, entropy, lse, index, best)
+
+
+def choice_report_backward(grad_log_probs: torch.Tensor | None, grad_entropy: torch.Tensor | None,
+                           scores: torch.Tensor, sets: ChoiceSets, *, chosen: torch.Tensor | None = None,
+                           mask: torch.Tensor | None = None, bias: PositionBias | None = None,
+                           temperature: float = 1.0) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """(gradient of the scores, gradient of the bias table or None) from those of the chosen rows'
+    log-probabilities and of the entropies (float32 per set, or None: 0) that `choice_report` gave for the same
+    arguments. Masked rows take and give no gradient; steps left out give none through their log-probability. The
+    sets' sums are formed anew, so a common offset of the scores does not matter."""
+    c, keep = _scores(scores, sets, mask, bias)
+    dev, g = sets.device, sets.num_sets
+    if grad_log_probs is not None and chosen is None:
+        raise ValueError("grad_log_probs need chosen")
+    if chosen is not None:
+        chosen = _column("chosen", chosen, g, dev, torch.int32)
+    if grad_log_probs is not None:
+        grad_log_probs = _column("grad_log_probs", grad_log_probs, g, dev, torch.float32)
+    if grad_entropy is not None:
+        grad_entropy = _column("grad_entropy", grad_entropy, g, dev, torch.float32)
+    temperature = _temperature(temperature)
+    with _on(dev):
+        gs = _empty(sets.num_rows, dev, scores.dtype)
+        gt = _empty(c.num_buckets, dev) if bias is not None else None
+        work, size = sets._workspace(_hip.PB_REPORT_BACKWARD, c.num_buckets)
+        _hip.check(_hip.load().pb_choice_report_backward(
+            sets._open(), c, _hip.ptr(chosen), temperature, _hip.ptr(grad_log_probs), _hip.ptr(grad_entropy),
+            gs.data_ptr(), _hip.ptr(gt), _hip.ptr(work), size, _hip.stream_ptr()), "pb_choice_report_backward")
+    return gs, gt
+
+
+def _list_of(name: str, t, sets: ChoiceSets, *dtypes: torch.dtype) -> torch.Tensor:
+    """t as the kernels read it: a list per set, one after the other."""
+    if not isinstance(t, torch.Tensor) or t.device != sets.device:
+        raise ValueError(f"{name} must be a tensor on {sets.device}")
+    if t.dim() != 2 or t.shape[0] != sets.num_sets or not 1 <= t.shape[1] <= MAX_TOP:
+        raise ValueError(f"{name} must have shape [{sets.num_sets}, 1 to {MAX_TOP}], got {tuple(t.shape)}")
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name} must be {' or '.join(str(d)[6:] for d in dtypes)}, got {str(t.dtype)[6:]}")
+    return t.contiguous()
+
+
+def distillation_loss(scores: torch.Tensor, sets: ChoiceSets, teacher_index: torch.Tensor, teacher_logits: torch.Tensor, *,
+                      tail: bool = False, weights: torch.Tensor | None = None, mask: torch.Tensor | None = None,
+                      bias: PositionBias | None = None, temperature: float = 1.0,
+                      scale: float = 1.0) -> DistillationLoss:
+    """The divergence of the scores' softmax from a teacher of which each set's best rows are known, and its gradients.
+
+    teacher_index: int32 [sets, k], k at most 64, rows by their index within the set (outside of it: none);
+    teacher_logits [sets, k]: float32, bfloat16 or float16. An entry counts whose row is not masked, of entries
+    that name one row the first. With p the student's softmax at the temperature T,
+
+        tail=False   teacher_logits are logits, q their softmax at T within the set's entries that count, rho = 0
+        tail=True    teacher_logits are log-probabilities at T (top_log_probs of a choice_report at T), q their
+                     exponentials, and rho = 1 - sum q stands against pi, the sum of p over the rows not listed
+                     (q / sum q and rho = 0 where there is no such row or the q sum to 1 or more)
+
+        kl = sum q (log q - log p) + rho (log rho - log pi);  loss = scale * T^2 * sum of w * kl
+
+    over the sets. weights (w, default 1) are float32 per set; a set of weight 0 counts for nothing, also where its
+    divergence is infinite. A set in which the teacher's entries or the student have no probability is left out."""
+    c, keep = _scores(scores, sets, mask, bias)
+    dev, g = sets.device, sets.num_sets
+    index = _list_of("teacher_index", teacher_index, sets, torch.int32)
+    logits = _list_of("teacher_logits", teacher_logits, sets, *_SCORE_TYPES)
+    if index.shape != logits.shape:
+        raise ValueError(f"teacher_index and teacher_logits differ in shape ({tuple(index.shape)} and {tuple(logits.shape)})")
+    t = _hip.PbTeacher()
+    t.index_dev, t.logits_dev = index.data_ptr(), logits.data_ptr()
+    t.entries, t.logit_type, t.tail = index.shape[1], _SCORE_TYPES[logits.dtype], bool(tail)
+    if weights is not None:
+        weights = _column("weights", weights, g, dev, torch.float32)
+        t.weights_dev = weights.data_ptr()
+    t.temperature, t.scale = _temperature(temperature), _finite("scale", scale)
+    with _on(dev):
+        loss, kl = _empty(1, dev), _empty(g, dev)
+        gs = _empty(sets.num_rows, dev, scores.dtype)
+        gt = _empty(c.num_buckets, dev) if bias is not None else None
+        work, size = sets._workspace(_hip.PB_DISTILL, c.num_buckets)
+        _hip.check(_hip.load().pb_distillation_loss(
+            sets._open(), c, t, loss.data_ptr(), kl.data_ptr(), gs.data_ptr(), _hip.ptr(gt), _hip.ptr(work), size,
+            _hip.stream_ptr()), "pb_distillation_loss")
+    return DistillationLoss(loss[0], gs, gt, kl)
 
 
 def preference_loss(values: torch.Tensor, pairs: PreferencePairs, *, ref_values: torch.Tensor | None = None,

@@ -12,6 +12,7 @@ struct pb_sets {
     pb::SetLayout s;
     int32_t device;
     char* arena;  // offsets, items and split list
+    int64_t largest;
 };
 
 struct pb_pairs {
@@ -195,6 +196,7 @@ int sets_create(const int64_t* off, int64_t num_sets, bool segments, pb_sets** o
     h->s.num_split = (int32_t)split.size();
     h->s.num_sets = num_sets;
     h->s.rows = off[num_sets];
+    for (int64_t g = 0; g < num_sets; ++g) h->largest = std::max(h->largest, off[g + 1] - off[g]);
     *out = h;
     return PB_OK;
 }
@@ -291,22 +293,18 @@ int64_t work_need(const pb_sets* s, int32_t op, int32_t num_buckets) {
     return 8 * (sum_cols(s, op, num_buckets) * pb::choice_grid(s->s) + parts);
 }
 
-// Checks what every choice call takes and fills the arguments it shares.
-int choice_args(const char* who, int32_t op, const pb_sets* s, const pb_choice_scores* in, void* work,
-                int64_t work_bytes, pb::ChoiceArgs& a) {
+// Checks what every choice call takes (its workspace of `need` bytes among it) and fills the arguments it shares.
+int scores_args(const char* who, const pb_sets* s, const pb_choice_scores* in, const void* work, int64_t work_bytes,
+                int64_t need, pb::ChoiceArgs& a) {
     const auto bad = [&](int code, const char* what) {
         return pb::api_fail(code, (std::string(who) + ": " + what).c_str());
     };
-    if (!s || !in) return bad(PB_ERR_INVALID, "null argument");
     if (s->s.rows > 0 && !in->scores_dev) return bad(PB_ERR_INVALID, "null scores");
     if (in->score_type != PB_F32 && in->score_type != PB_BF16 && in->score_type != PB_F16)
         return bad(PB_ERR_UNSUPPORTED, "scores must be float32, bfloat16 or float16");
-    if (in->num_buckets < 0 || in->num_buckets > pb::kMaxBuckets)
-        return bad(PB_ERR_UNSUPPORTED, "at most 256 position buckets");
     if (in->num_buckets > 0 && (!in->table_dev || !in->buckets_dev || (s->s.rows > 0 && !in->positions_dev)))
         return bad(PB_ERR_INVALID, "a position bias needs its table, buckets and positions");
     if (in->num_buckets > 0 && in->reach < 0) return bad(PB_ERR_INVALID, "reach must not be negative");
-    const int64_t sums = sum_cols(s, op, in->num_buckets) * pb::choice_grid(s->s), need = work_need(s, op, in->num_buckets);
     if (need > 0 && (!work || work_bytes < need)) return bad(PB_ERR_INVALID, "workspace too small");
     if (reinterpret_cast<uintptr_t>(work) & 15) return bad(PB_ERR_INVALID, "workspace must be 16-byte aligned");
     a.num_buckets = in->num_buckets;
@@ -317,8 +315,41 @@ int choice_args(const char* who, int32_t op, const pb_sets* s, const pb_choice_s
     a.table = in->num_buckets > 0 ? in->table_dev : nullptr;
     a.buckets = in->buckets_dev;
     a.reach = in->reach;
+    return PB_OK;
+}
+
+// What comes before anything that reads the handle or asks for a number of buckets.
+int check_scores(const char* who, const pb_sets* s, const pb_choice_scores* in) {
+    if (!s || !in) return pb::api_fail(PB_ERR_INVALID, (std::string(who) + ": null argument").c_str());
+    if (in->num_buckets < 0 || in->num_buckets > pb::kMaxBuckets)
+        return pb::api_fail(PB_ERR_UNSUPPORTED, (std::string(who) + ": at most 256 position buckets").c_str());
+    return PB_OK;
+}
+
+int choice_args(const char* who, int32_t op, const pb_sets* s, const pb_choice_scores* in, void* work,
+                int64_t work_bytes, pb::ChoiceArgs& a) {
+    int rc = check_scores(who, s, in);
+    if (rc == PB_OK) rc = scores_args(who, s, in, work, work_bytes, work_need(s, op, in->num_buckets), a);
+    if (rc != PB_OK) return rc;
     a.sums = static_cast<double*>(work);
-    a.parts = reinterpret_cast<float2*>(a.sums + sums);
+    a.parts = reinterpret_cast<float2*>(a.sums + sum_cols(s, op, in->num_buckets) * pb::choice_grid(s->s));
+    return PB_OK;
+}
+
+// The temperature's part of a report's arguments, and the length of the lists.
+int report_args(const char* who, float temperature, int32_t top, pb::ReportArgs& a) {
+    const auto bad = [&](int code, const char* what) {
+        return pb::api_fail(code, (std::string(who) + ": " + what).c_str());
+    };
+    if (!(temperature >= 0x1p-20f && temperature <= 0x1p20f)) return bad(PB_ERR_INVALID, "the temperature must lie in [2^-20, 2^20]");
+    if (top > pb::kMaxTop) return bad(PB_ERR_UNSUPPORTED, "at most 64 entries to a list");
+    a.temp = temperature;
+    a.inv_temp = 1.0 / (double)temperature;
+    const double heat = 1.4426950408889634 * a.inv_temp;
+    a.heat_hi = (float)heat;
+    a.heat_lo = (float)(heat - (double)a.heat_hi);
+    a.heat_low = (float)(-200.0 / heat);  // 2^-200 is 0
+    a.top = top;
     return PB_OK;
 }
 
@@ -354,8 +385,13 @@ int pb_sets_destroy(pb_sets* sets) {
 }
 
 int64_t pb_choice_work_bytes(const pb_sets* s, int32_t op, int32_t num_buckets) {
-    if (!s || op < PB_LOG_PROBS || op > PB_POLICY || num_buckets < 0 || num_buckets > pb::kMaxBuckets) return -1;
+    if (!s || op < PB_LOG_PROBS || op > PB_DISTILL || num_buckets < 0 || num_buckets > pb::kMaxBuckets) return -1;
+    if (op >= PB_REPORT_BACKWARD) return pb::soft_grads_work_bytes(s->s, op == PB_DISTILL, num_buckets);
     return work_need(s, op, num_buckets);
+}
+
+int64_t pb_choice_report_work_bytes(const pb_sets* s, int32_t top) {
+    return !s || top < 0 || top > pb::kMaxTop ? -1 : pb::report_work_bytes(s->s, top);
 }
 
 int pb_choice_log_probs(const pb_sets* s, const pb_choice_scores* in, const int32_t* chosen_dev, float* log_probs_dev,
@@ -419,6 +455,88 @@ int pb_policy_loss(const pb_sets* s, const pb_choice_scores* in, const pb_policy
     a.grad_scores = grad_scores_dev;
     a.grad_table = grad_table_dev;
     return launch("pb_policy_loss", pb::kPolicy, s, a, in->score_type, stream);
+}
+
+int pb_choice_report(const pb_sets* s, const pb_choice_scores* in, const int32_t* chosen_dev, float temperature, int32_t top,
+                     float* log_probs_dev, float* entropy_dev, float* lse_dev, int32_t* top_index_dev,
+                     float* top_log_probs_dev, void* work_dev, int64_t work_bytes, void* stream) {
+    const char* who = "pb_choice_report";
+    pb::ReportArgs a{};
+    int rc = check_scores(who, s, in);
+    if (rc == PB_OK && top < 0) rc = pb::api_fail(PB_ERR_INVALID, "pb_choice_report: a list has at least 0 entries");
+    if (rc == PB_OK) rc = report_args(who, temperature, top, a);
+    if (rc == PB_OK && top > 0 && s->largest > INT32_MAX)
+        rc = pb::api_fail(PB_ERR_UNSUPPORTED, "pb_choice_report: lists name rows of sets of at most 2^31 - 1 rows");
+    if (rc == PB_OK) rc = scores_args(who, s, in, work_dev, work_bytes, pb::report_work_bytes(s->s, top), a);
+    if (rc != PB_OK || s->s.num_sets == 0) return rc;
+    if (!entropy_dev || !lse_dev || (chosen_dev && !log_probs_dev) || (top > 0 && (!top_index_dev || !top_log_probs_dev)))
+        return pb::api_fail(PB_ERR_INVALID, "pb_choice_report: null output");
+    a.chosen = chosen_dev;
+    a.log_probs = log_probs_dev;
+    a.entropy = entropy_dev;
+    a.lse_out = lse_dev;
+    a.top_index = top_index_dev;
+    a.top_log_probs = top_log_probs_dev;
+    const hipError_t e = pb::launch_report(s->s, a, in->score_type, static_cast<char*>(work_dev), (hipStream_t)stream);
+    return e == hipSuccess ? PB_OK : pb::api_hip_fail(e, who);
+}
+
+int pb_choice_report_backward(const pb_sets* s, const pb_choice_scores* in, const int32_t* chosen_dev, float temperature,
+                              const float* grad_log_probs_dev, const float* grad_entropy_dev, void* grad_scores_dev,
+                              float* grad_table_dev, void* work_dev, int64_t work_bytes, void* stream) {
+    const char* who = "pb_choice_report_backward";
+    pb::ReportArgs a{};
+    int rc = check_scores(who, s, in);
+    if (rc == PB_OK) rc = report_args(who, temperature, 0, a);
+    if (rc == PB_OK)
+        rc = scores_args(who, s, in, work_dev, work_bytes, pb::soft_grads_work_bytes(s->s, false, in->num_buckets), a);
+    if (rc != PB_OK) return rc;
+    if (in->num_buckets > 0 && !grad_table_dev) return pb::api_fail(PB_ERR_INVALID, "pb_choice_report_backward: null table gradient");
+    if (s->s.num_sets == 0) return clear(who, grad_table_dev, in->num_buckets, stream);
+    if ((grad_log_probs_dev && !chosen_dev) || (s->s.rows > 0 && !grad_scores_dev))
+        return pb::api_fail(PB_ERR_INVALID, "pb_choice_report_backward: null argument");
+    a.chosen = chosen_dev;
+    a.grad = grad_log_probs_dev;
+    a.grad_entropy = grad_entropy_dev;
+    a.grad_scores = grad_scores_dev;
+    a.grad_table = grad_table_dev;
+    const hipError_t e = pb::launch_soft_grads(false, s->s, a, in->score_type, static_cast<char*>(work_dev), (hipStream_t)stream);
+    return e == hipSuccess ? PB_OK : pb::api_hip_fail(e, who);
+}
+
+int pb_distillation_loss(const pb_sets* s, const pb_choice_scores* in, const pb_teacher* t, float* loss_dev, float* kl_dev,
+                         void* grad_scores_dev, float* grad_table_dev, void* work_dev, int64_t work_bytes, void* stream) {
+    const char* who = "pb_distillation_loss";
+    pb::ReportArgs a{};
+    int rc = check_scores(who, s, in);
+    if (rc == PB_OK && !t) rc = pb::api_fail(PB_ERR_INVALID, "pb_distillation_loss: null argument");
+    if (rc == PB_OK && t->entries < 1) rc = pb::api_fail(PB_ERR_INVALID, "pb_distillation_loss: a list has at least 1 entry");
+    if (rc == PB_OK) rc = report_args(who, t->temperature, t->entries, a);
+    if (rc == PB_OK && t->logit_type != PB_F32 && t->logit_type != PB_BF16 && t->logit_type != PB_F16)
+        rc = pb::api_fail(PB_ERR_UNSUPPORTED, "pb_distillation_loss: the teacher's logits must be float32, bfloat16 or float16");
+    if (rc == PB_OK)
+        rc = scores_args(who, s, in, work_dev, work_bytes, pb::soft_grads_work_bytes(s->s, true, in->num_buckets), a);
+    if (rc != PB_OK) return rc;
+    if (!loss_dev || (in->num_buckets > 0 && !grad_table_dev))
+        return pb::api_fail(PB_ERR_INVALID, "pb_distillation_loss: null argument");
+    if (s->s.num_sets == 0) {
+        rc = clear(who, loss_dev, 1, stream);
+        return rc != PB_OK ? rc : clear(who, grad_table_dev, in->num_buckets, stream);
+    }
+    if (!t->index_dev || !t->logits_dev || !kl_dev || (s->s.rows > 0 && !grad_scores_dev))
+        return pb::api_fail(PB_ERR_INVALID, "pb_distillation_loss: null argument");
+    a.entry_index = t->index_dev;
+    a.entry_logits = t->logits_dev;
+    a.entry_type = t->logit_type;
+    a.tail = t->tail != 0;
+    a.weights = t->weights_dev;
+    a.scale = t->scale;
+    a.stats = loss_dev;
+    a.kl = kl_dev;
+    a.grad_scores = grad_scores_dev;
+    a.grad_table = grad_table_dev;
+    const hipError_t e = pb::launch_soft_grads(true, s->s, a, in->score_type, static_cast<char*>(work_dev), (hipStream_t)stream);
+    return e == hipSuccess ? PB_OK : pb::api_hip_fail(e, who);
 }
 
 int pb_pairs_create(const int64_t* winners_host, const int64_t* losers_host, int64_t num_pairs, int64_t num_values,

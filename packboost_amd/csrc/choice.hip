@@ -1135,7 +1135,12 @@ hipError_t launch_choice(int mode, const SetLayout& s, ChoiceArgs a, int32_t typ
     const int32_t head = mode == kPolicy ? 3 : 0;
     const int32_t cols = head + (a.table && mode != kRows && mode != kSteps ? a.num_buckets : 0);
     if (e != hipSuccess || cols == 0 || a.blocks == 1) return e;
-    hipLaunchKernelGGL(join_kernel, dim3(cols), dim3(kBlock), 0, stream, a.sums, a.blocks, cols, head, a.stats, a.grad_table);
+    return launch_join_sums(a.sums, a.blocks, cols, head, a.stats, a.grad_table, stream);
+}
+
+hipError_t launch_join_sums(const double* sums, int32_t n, int32_t cols, int32_t head, float* stats, float* table,
+                            hipStream_t stream) {
+    hipLaunchKernelGGL(join_kernel, dim3(cols), dim3(kBlock), 0, stream, sums, n, cols, head, stats, table);
     return hipGetLastError();
 }
 

@@ -672,5 +672,33 @@ __device__ __forceinline__ void leave_sums(const ChoiceArgs& a, int block, doubl
     }
 }
 
+// ---- probabilities at a temperature T: p_i = exp((z_i - m) / T) / s
+// log2(e) / T as the sum of two floats, and the distance to the maximum from which on exponentials are 0.
+struct Heat {
+    float hi, lo, low;
+};
+
+// exp(d / T) of d = z - m. EXACT: within 2 units; else the exponent is rounded once, which moves the result by at
+// most |d / T| 2^-24 of itself, in either direction. -inf gives 0, NaN stays NaN.
+template <bool EXACT>
+__device__ __forceinline__ float heat_exp(float distance, const Heat& h) {
+    const float d = __builtin_elementwise_maximum(distance, h.low);  // a NaN is the larger one
+    const float t = d * h.hi;
+    if (!EXACT) return __builtin_amdgcn_exp2f(__builtin_fmaf(d, h.lo, t));
+    const float e = __builtin_amdgcn_exp2f(t), rest = __builtin_fmaf(d, h.lo, __builtin_fmaf(d, h.hi, -t));
+    return __builtin_fmaf(e * 0.693147182464599609375f, rest, e);
+}
+
+// Reductions over teams of 1 << bits neighbouring lanes of a wave, the result in all of them.
+__device__ __forceinline__ double team_sum(double v, int bits) {
+    for (int m = 1; m < 1 << bits; m <<= 1) v += __shfl_xor(v, m);
+    return v;
+}
+
+__device__ __forceinline__ double team_max(double v, int bits) {
+    for (int m = 1; m < 1 << bits; m <<= 1) v = fmax(v, __shfl_xor(v, m));
+    return v;
+}
+
 }  // namespace
 }  // namespace pb

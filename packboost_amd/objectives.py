@@ -8,8 +8,9 @@ shrink with the table.
     PreferenceObjective          rows compared in pairs (a reward model, a ranker)
     ChoicePreferenceObjective    sequences of choices compared in pairs, against a reference model
     PolicyObjective              choices with advantages: the clipped policy loss with a KL term
+    DistillationObjective        sets of which a teacher's best rows are known: the divergence from the teacher
 
-The two objectives on choices can learn a position bias beside the trees: a bucket of positions is
+The objectives on choices can learn a position bias beside the trees: a bucket of positions is
 fitted like a leaf, table -= bias_rate * (sum of its rows' gradients) / (number of its rows), each
 round, and taken into account in the scores' gradients; the model's own predictions are free of it.
 `table` holds it after the fit; a saved model holds the trees alone, so who serves with the bias keeps
@@ -24,8 +25,8 @@ from __future__ import annotations
 import numpy as np
 import torch
 
-from .choices import (ChoiceSets, PositionBias, PositionBuckets, PreferencePairs, _host_int64, choice_log_probs,
-                      choice_log_probs_backward, policy_loss, preference_loss)
+from .choices import (MAX_TOP, ChoiceSets, PositionBias, PositionBuckets, PreferencePairs, _host_int64, _temperature,
+                      choice_log_probs, choice_log_probs_backward, distillation_loss, policy_loss, preference_loss)
 
 
 def _array(name: str, v, n: int, dtype) -> np.ndarray:
@@ -105,15 +106,15 @@ class PreferenceObjective(Objective):
 
 
 class _Choices(Objective):
-    """Sets of rows with one choice each, a mask and a learned position bias."""
+    """Sets of rows, with one choice each where `chosen` is given, a mask and a learned position bias."""
 
-    def __init__(self, offsets, chosen, *, mask=None, positions=None, buckets: PositionBuckets | None = None,
+    def __init__(self, offsets, chosen=None, *, mask=None, positions=None, buckets: PositionBuckets | None = None,
                  bias_rate: float = 0.1) -> None:
         self._off = _host_int64("offsets", offsets)
         if self._off.size == 0 or self._off[0] != 0 or np.any(self._off[1:] < self._off[:-1]):
             raise ValueError("offsets must start at 0 and not decrease")
         self._g, self._n = self._off.size - 1, int(self._off[-1])
-        self._chosen = _indices("chosen", chosen, self._g)
+        self._chosen = None if chosen is None else _indices("chosen", chosen, self._g)
         self._mask = None if mask is None else _array("mask", mask, self._n, bool)
         self._positions = None if positions is None else _indices("positions", positions, self._n)
         if buckets is not None and positions is None:
@@ -204,6 +205,44 @@ class PolicyObjective(_Choices):
     def release(self):
         super().release()
         self._dev = None
+
+
+class DistillationObjective(_Choices):
+    """Sets of which a teacher's best rows are known: distillation_loss on the softmax of the predictions.
+
+    offsets, mask, positions: as ChoiceSets and choice_log_probs take them; teacher_index, teacher_logits [sets, k]
+    (top_index and top_log_probs of a choice_report of the teacher's scores at this temperature, with tail=True, or logits);
+    weights: per set."""
+
+    def __init__(self, offsets, teacher_index, teacher_logits, *, tail: bool = False, weights=None, mask=None,
+                 positions=None, buckets=None, bias_rate: float = 0.1, temperature: float = 1.0) -> None:
+        super().__init__(offsets, mask=mask, positions=positions, buckets=buckets, bias_rate=bias_rate)
+        index, logits = (np.asarray(v.detach().float().cpu().numpy() if isinstance(v, torch.Tensor) and v.is_floating_point()
+                                    else v.detach().cpu().numpy() if isinstance(v, torch.Tensor) else v)
+                         for v in (teacher_index, teacher_logits))
+        if index.ndim != 2 or index.shape[0] != self._g or not 1 <= index.shape[1] <= MAX_TOP:
+            raise ValueError(f"teacher_index must have shape [{self._g}, 1 to {MAX_TOP}], got {index.shape}")
+        if logits.shape != index.shape:
+            raise ValueError(f"teacher_index and teacher_logits differ in shape ({index.shape} and {logits.shape})")
+        self._index = _indices("teacher_index", index.reshape(-1), index.size).reshape(index.shape)
+        self._logits = np.ascontiguousarray(logits, dtype=np.float32)
+        self._weights = None if weights is None else _array("weights", weights, self._g, np.float32)
+        self._args = dict(tail=bool(tail), temperature=_temperature(temperature))
+
+    def bind(self, perm, num_rows, device):
+        order = self._bind_sets(perm, num_rows, device)
+        self._teacher = [self._steps(v, order, device) for v in (self._index, self._logits)]
+        self._wt = self._steps(self._weights, order, device)
+
+    def gradient(self, preds):
+        r = distillation_loss(preds, self._sets, *self._teacher, weights=self._wt, mask=self._mask_dev, bias=self._bias,
+                              **self._args)
+        self._learn(r.grad_table)
+        return r.loss, r.grad_scores
+
+    def release(self):
+        super().release()
+        self._teacher = self._wt = None
 
 
 class ChoicePreferenceObjective(_Choices):
