@@ -21,7 +21,7 @@ CSRC = PKG_DIR / "csrc"
 LIB_NAME = "libpackboost_hip.so"
 LIB_PATH = PKG_DIR / LIB_NAME
 SOURCES = ["hist.hip", "score.hip", "partition.hip", "predict.hip", "metrics.hip", "binning.hip", "rowlist.hip", "segment.hip",
-           "quantile.hip", "choice.hip", "pairs.hip", "report.hip", "distill.hip",
+           "quantile.hip", "choice.hip", "pairs.hip", "report.hip", "report_grads.hip", "distill.hip",
            "capi.cpp", "capi_choice.cpp"]
 ARCH = "gfx950"
 

@@ -7,6 +7,7 @@
 #include <vector>
 
 #include "pb_internal.h"
+#include "report.h"
 
 struct pb_sets {
     pb::SetLayout s;

@@ -689,16 +689,142 @@ __device__ __forceinline__ float heat_exp(float distance, const Heat& h) {
     return __builtin_fmaf(e * 0.693147182464599609375f, rest, e);
 }
 
-// Reductions over teams of 1 << bits neighbouring lanes of a wave, the result in all of them.
-__device__ __forceinline__ double team_sum(double v, int bits) {
-    for (int m = 1; m < 1 << bits; m <<= 1) v += __shfl_xor(v, m);
+// e^x in double within 2^-46 of itself: x = k log 2 + r, |r| <= log(2) / 2, and eleven terms of r's series. -inf gives 0,
+// NaN and infinity give NaN.
+__device__ __forceinline__ double exp_near(double x) {
+    x = x < -800.0 ? -800.0 : x;
+    const double k = __builtin_rint(x * 1.4426950408889634);
+    const double r = __builtin_fma(k, -2.3190468138462996e-17, __builtin_fma(k, -0.69314718055994529, x));
+    double p = 1.0 / 39916800;
+    p = __builtin_fma(p, r, 1.0 / 3628800);
+    p = __builtin_fma(p, r, 1.0 / 362880);
+    p = __builtin_fma(p, r, 1.0 / 40320);
+    p = __builtin_fma(p, r, 1.0 / 5040);
+    p = __builtin_fma(p, r, 1.0 / 720);
+    p = __builtin_fma(p, r, 1.0 / 120);
+    p = __builtin_fma(p, r, 1.0 / 24);
+    p = __builtin_fma(p, r, 1.0 / 6);
+    p = __builtin_fma(p, r, 0.5);
+    p = __builtin_fma(p, r, 1.0);
+    p = __builtin_fma(p, r, 1.0);
+    return ldexp(p, (int)k);
+}
+
+// log x in double within 2^-31 beside its rounding, and as close relative to itself near 1: x = 2^k m, m in [2/3, 4/3),
+// log m = 2 (f + f^3 / 3 + ... + f^13 / 13), f = (m - 1) / (m + 1), the terms after the first in float. 0 gives -inf.
+__device__ __forceinline__ double log_near(double x) {
+    if (!(x > 0.0 && x < (double)kInf)) return (double)log_of((float)x);
+    const double half = __builtin_amdgcn_frexp_mant(x);  // [1/2, 1)
+    const bool low = half < 0.66666666666666663;
+    const double m = low ? 2.0 * half : half;
+    const int k = __builtin_amdgcn_frexp_exp(x) - (low ? 1 : 0);
+    const double n = m - 1.0, s = m + 1.0, inv = (double)__builtin_amdgcn_rcpf((float)s);
+    const double f0 = n * inv, f = __builtin_fma(__builtin_fma(-f0, s, n), inv, f0);
+    const float g = (float)f, q = g * g;
+    float p = 1.0f / 13;
+    p = __builtin_fmaf(p, q, 1.0f / 11);
+    p = __builtin_fmaf(p, q, 1.0f / 9);
+    p = __builtin_fmaf(p, q, 1.0f / 7);
+    p = __builtin_fmaf(p, q, 1.0f / 5);
+    p = __builtin_fmaf(p, q, 1.0f / 3);
+    return __builtin_fma((double)k, 0.69314718055994531, 2.0 * (f + (double)(p * q * g)));
+}
+
+// Reductions over teams of 1 << bits neighbouring lanes of a wave, the result in all of them. Lanes that mirror each
+// other hold the same after the steps before.
+template <class F>
+__device__ __forceinline__ double team_reduce(double v, int bits, F f) {
+    if (bits > 0) v = f(v, lane_move<0xb1>(v));   // quad_perm:[1,0,3,2]
+    if (bits > 1) v = f(v, lane_move<0x4e>(v));   // quad_perm:[2,3,0,1]
+    if (bits > 2) v = f(v, lane_move<0x141>(v));  // row_half_mirror
+    if (bits > 3) v = f(v, lane_move<0x140>(v));  // row_mirror
+    if (bits > 4) v = f(v, __shfl_xor(v, 16));
+    if (bits > 5) v = f(v, __shfl_xor(v, 32));
     return v;
 }
 
-__device__ __forceinline__ double team_max(double v, int bits) {
-    for (int m = 1; m < 1 << bits; m <<= 1) v = fmax(v, __shfl_xor(v, m));
-    return v;
+__device__ __forceinline__ double team_sum(double v, int bits) {
+    return team_reduce(v, bits, [](double a, double b) { return a + b; });
 }
+
+__device__ __forceinline__ double team_max(double v, int bits) {
+    return team_reduce(v, bits, [](double a, double b) { return fmax(a, b); });
+}
+
+// What a wave reads of a tile of short sets, asked for before anything is waited for: a lane's run, and where the lane's
+// sets lie.
+template <int TYPE, bool MASK, bool BIAS>
+struct TileRows {
+    Span sp;  // of the lane's run alone
+    int sets;
+    RawRun<TYPE, MASK, BIAS> raw;
+    int32_t set[kTileRounds], begin[kTileRounds], end[kTileRounds];  // begin, end: rows of the tile
+
+    __device__ __forceinline__ void load(const ChoiceArgs& a, const SetItem& im, int lane) {
+        int64_t row0 = im.row0, rows = im.rows;
+        int lane0 = 0;
+        int64_t base[kTileRounds];
+        sets = im.sets;
+#pragma unroll
+        for (int r = 0; r < kTileRounds; ++r) {
+            set[r] = im.set0 + r * kWave + lane;
+            base[r] = row0 & ~(int64_t)(kRun - 1);
+        }
+        for (int e = 0; e < im.parts; ++e) {  // the tile's further segments
+            const TileSegment seg = a.segments[im.part + e];
+            if (lane >= seg.lane0) {
+                row0 = seg.row0;
+                rows = seg.rows;
+                lane0 = seg.lane0;
+            }
+#pragma unroll
+            for (int r = 0; r < kTileRounds; ++r)
+                if (r * kWave + lane >= seg.first) {
+                    set[r] = seg.set0 + r * kWave + lane - seg.first;
+                    base[r] = (seg.row0 & ~(int64_t)(kRun - 1)) - kRun * seg.lane0;
+                }
+        }
+        sp.q0 = (row0 & ~(int64_t)(kRun - 1)) + kRun * (lane - lane0);
+        sp.lo = (int)max(row0 - sp.q0, (int64_t)0);  // below kRun
+        sp.hi = (int)min(row0 + rows - sp.q0, (int64_t)kRun);
+        sp.end = (int)min(a.rows - sp.q0, (int64_t)kRun);
+        if (sp.hi > 0) raw.load(a, sp, 0);
+#pragma unroll
+        for (int r = 0; r < kTileRounds; ++r) {
+            begin[r] = end[r] = 0;
+            if (r * kWave + lane < sets) {
+                begin[r] = (int)(a.off[set[r]] - base[r]);
+                end[r] = (int)(a.off[set[r] + 1] - base[r]);
+            }
+        }
+    }
+};
+
+// The sets of a tile's rows, and how they are reduced. `head` has the set that starts at a row, from 1, 0 for none.
+struct TileSets {
+    int id[kRun];  // the row's set, from 1; a slot of none before the first
+    Segments seg;
+
+    __device__ __forceinline__ void find(const uint16_t* head, int lane) {
+        const uint4 w = *reinterpret_cast<const uint4*>(&head[kRun * lane]);
+        const int raw[kRun] = {(int)(w.x & 0xffffu), (int)(w.x >> 16), (int)(w.y & 0xffffu), (int)(w.y >> 16),
+                               (int)(w.z & 0xffffu), (int)(w.z >> 16), (int)(w.w & 0xffffu), (int)(w.w >> 16)};
+        int last = 0;
+#pragma unroll
+        for (int k = 0; k < kRun; ++k) last = raw[k] ? raw[k] : last;
+        // the set that the rows before the lane's first head are of: the last head's below
+        const unsigned long long below = __ballot(last != 0) & ((1ull << lane) - 1ull);
+        const int from = below ? kWave - 1 - __clzll((long long)below) : lane;
+        const int carried = __shfl(last, from);
+        int now = below ? carried : kSetTileSets + 1;
+#pragma unroll
+        for (int k = 0; k < kRun; ++k) {
+            now = raw[k] ? raw[k] : now;
+            id[k] = now;
+        }
+        seg.start(raw, lane);
+    }
+};
 
 }  // namespace
 }  // namespace pb

@@ -588,24 +588,6 @@ struct ChoiceArgs {
     float2* parts;  // [num_mid + num_wide] of the parts of split sets: maximum and sum; backward: sum over a far lse, sum of gradients
     double* sums;   // [choice_grid][3 (policy) + num_buckets (gradient)]
 };
-// Reports on choices and distillation (report.hip, distill.hip).
-constexpr int kMaxTop = 64;  // entries of a set's list, a lane each
-struct ReportArgs : ChoiceArgs {
-    double inv_temp;
-    float temp;
-    float heat_hi, heat_lo, heat_low;  // log2(e) / T in two parts; see Heat
-    int32_t top;                       // entries of each set's list
-    float* entropy;
-    int32_t* top_index;
-    float* top_log_probs;
-    const float* grad_entropy;
-    // the teacher's
-    const int32_t* entry_index;
-    const void* entry_logits;
-    int32_t entry_type;
-    bool tail;
-    float* kl;
-};
 struct PairArgs {
     const int32_t* winners;
     const int32_t* losers;
@@ -627,11 +609,6 @@ hipError_t launch_choice(int mode, const SetLayout& s, ChoiceArgs a, int32_t typ
 // The workgroups' sums [n][cols], joined in a fixed order: the first `head` columns to stats, the others to table.
 hipError_t launch_join_sums(const double* sums, int32_t n, int32_t cols, int32_t head, float* stats, float* table,
                             hipStream_t stream);
-int64_t report_work_bytes(const SetLayout& s, int32_t top);
-hipError_t launch_report(const SetLayout& s, ReportArgs a, int32_t type, char* work, hipStream_t stream);
-// distill: the loss's gradient, else that of the log-probabilities and entropies; `sums` are in the workspace
-int64_t soft_grads_work_bytes(const SetLayout& s, bool distill, int32_t num_buckets);
-hipError_t launch_soft_grads(bool distill, const SetLayout& s, ReportArgs a, int32_t type, char* work, hipStream_t stream);
 hipError_t launch_preference(const PairLayout& p, PairArgs a, const float* values, const float* ref, float* grad,
                              char* work, hipStream_t stream);
 int64_t preference_work_bytes(const PairLayout& p);

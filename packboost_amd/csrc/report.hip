@@ -10,6 +10,7 @@
 #include <algorithm>
 
 #include "choice_rows.h"
+#include "report.h"
 
 namespace pb {
 namespace {
