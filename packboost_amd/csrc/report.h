@@ -19,6 +19,7 @@ struct ReportArgs : ChoiceArgs {
     int32_t top;                       // entries of each set's list
     int32_t team_bits;                 // 1 << team_bits lanes take it
     SoftSums* part_sums;               // of the parts of split sets, by wide item
+    unsigned long long* part_keys;     // [top] of each, best first
     float* entropy;
     int32_t* top_index;
     float* top_log_probs;

@@ -6,7 +6,10 @@
 // probability has s = 0, lse -inf and entropy 0. Rows are ranked by z, equal ones by index, NaN above all; rows of z = -inf
 // are not ranked.
 //
-// A workgroup to a set: its rows are read once for the maximum, once for the sums, and once for each entry of its list.
+// Rows are laid out and read as choice.hip has them, each once: tiles of short sets by a wave, longer sets by a wave or a
+// workgroup that holds them in registers, what is longer still in parts that a second kernel joins. In a tile, a row of
+// a short set counts the rows that rank above it. Of longer sets a bound is found first that at least as many rows reach as
+// are listed, from the maxima of the lanes; the few rows that reach it are gathered and ranked by counting.
 #include <algorithm>
 
 #include "choice_rows.h"
@@ -15,139 +18,731 @@
 namespace pb {
 namespace {
 
-constexpr int kReportGrid = 4096;
+constexpr int kCountRows = 64;    // rows of a tile's set whose rows count what ranks above them
+constexpr int kWaveList = 256;    // rows that reach the bound: room for a wave's
+constexpr int kGroupList = 512;   // and a workgroup's
+constexpr int kJoinList = kMaxTop * kMaxTop;
 
-// What orders the rows of a set: larger logits first (-0 as 0, NaN above all), then smaller indices; 0 for none.
-__device__ __forceinline__ unsigned long long rank_key(float z, uint32_t index) {
+// Orders logits as whole numbers: larger first, -0 as 0, NaN above all; 0 for what is not ranked.
+__device__ __forceinline__ uint32_t rank_of(float z) {
+    if (z == -kInf) return 0;
     const uint32_t b = z != z ? 0x7fc00000u : __float_as_uint(z + 0.0f);
-    return (unsigned long long)(b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u)) << 32 | (uint32_t)~index;
+    return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
 
-__device__ __forceinline__ unsigned long long block_max(unsigned long long v, unsigned long long* sh) {
+__device__ __forceinline__ float rank_value(uint32_t r) { return __uint_as_float(r & 0x80000000u ? r ^ 0x80000000u : ~r); }
+
+// A row of a list: its rank, then smaller indices first. 0 for none.
+__device__ __forceinline__ unsigned long long key_of(float z, uint32_t index) {
+    return (unsigned long long)rank_of(z) << 32 | (uint32_t)~index;
+}
+
+__device__ __forceinline__ float list_log_prob(const ReportArgs& a, float z, float top, double log_sum) {
+    return (float)(((double)z - (double)top) * a.inv_temp - log_sum);
+}
+
+// What a set's sums say, by one lane.
+__device__ __forceinline__ void put_report(const ReportArgs& a, int64_t g, const SoftSums& t, double log_sum, bool counts, float z) {
+    const bool none = t.sum == 0.0;
+    const double m = none ? 0.0 : (double)t.top;
+    a.lse_out[g] = (float)(m * a.inv_temp + log_sum);
+    a.entropy[g] = none ? 0.0f : (float)(log_sum - t.along * a.inv_temp / t.sum);
+    if (a.chosen) a.log_probs[g] = counts && !none ? (float)(((double)z - m) * a.inv_temp - log_sum) : 0.0f;
+}
+
+__device__ __forceinline__ void put_entry(const ReportArgs& a, int64_t at, int32_t index, float log_prob) {
+    a.top_index[at] = index;
+    a.top_log_probs[at] = log_prob;
+}
+
+// ------------------------------------------------------------------------------------ lists of longer sets
+template <int THREADS, int LIST>
+struct RankGroup {
+    static constexpr int kGroupWaves = THREADS / kWave;
+    unsigned long long list[LIST];
+    uint32_t bound[kGroupWaves], count[2][kGroupWaves];
+    uint32_t size;
+};
+
+// The number of a group's lanes' v, the same in every lane; `turn` is 0 and 1 in turn.
+template <int THREADS, int LIST>
+__device__ __forceinline__ uint32_t group_count(uint32_t wave_count, RankGroup<THREADS, LIST>& sh, int& turn) {
+    if (THREADS == kWave) return wave_count;
+    turn ^= 1;
+    if ((threadIdx.x & (kWave - 1)) == 0) sh.count[turn][threadIdx.x / kWave] = wave_count;
+    __syncthreads();
+    uint32_t n = 0;
+    for (int w = 0; w < THREADS / kWave; ++w) n += sh.count[turn][w];
+    return n;
+}
+
+template <int RUNS, class F>
+__device__ __forceinline__ uint32_t wave_count(int live, F f) {
+    uint32_t n = 0;
 #pragma unroll
-    for (int m = kWave / 2; m >= 1; m >>= 1) {
-        const unsigned long long t = __shfl_xor(v, m);
-        v = t > v ? t : v;
-    }
-    __syncthreads();
-    if ((threadIdx.x & (kWave - 1)) == 0) sh[threadIdx.x / kWave] = v;
-    __syncthreads();
-    for (int w = 0; w < kWaves; ++w) v = sh[w] > v ? sh[w] : v;
-    return v;
+    for (int j = 0; j < RUNS; ++j)
+        if (j < live)
+#pragma unroll
+            for (int k = 0; k < kRun; ++k) n += (uint32_t)__popcll(__ballot(f(j, k)));
+    return n;
 }
 
-// f(rows from the set's first, logits) for every run of rows [r0, r1), a thread a run.
-template <int TYPE, bool MASK, bool BIAS, class F>
-__device__ __forceinline__ void each_run(const ReportArgs& a, const BiasShared* bias, int64_t r0, int64_t r1, F f) {
-    constexpr int64_t kPiece = 1 << 20;
-    for (int64_t p0 = r0; p0 < r1; p0 += kPiece) {
-        Span s;
-        s.q0 = p0 & ~(int64_t)(kRun - 1);
-        s.lo = (int)(p0 - s.q0);
-        s.hi = s.lo + (int)min(kPiece, r1 - p0);
-        s.end = (int)min(a.rows - s.q0, (int64_t)1 << 30);
-        for (int i = kRun * (int)threadIdx.x; i < s.hi; i += kRun * kBlock) {
-            float z[kRun];
-            uint32_t off;
-            Buckets buckets;
-            load_logits<TYPE, MASK, BIAS>(a, bias, s, i, z, off, buckets);
-            f(s.q0 + i - r0, z);
+// The largest bound, in steps of 2^16 of the ranks, that at least n of the wave's COUNT x 64 maxima reach; 0 if there are
+// fewer. So many rows reach it at least.
+template <int COUNT>
+__device__ __forceinline__ uint32_t wave_bound(const uint32_t (&most)[COUNT], uint32_t n) {
+    uint32_t t = 0;
+    for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit >>= 1) {
+        uint32_t c = 0;
+#pragma unroll
+        for (int j = 0; j < COUNT; ++j) c += (uint32_t)__popcll(__ballot(most[j] >= (t | bit)));
+        if (c >= n) t |= bit;
+    }
+    return t;
+}
+
+// The rows of a group's logits v (run j, row k: row kRun (j THREADS + tid) + k of the group's, from index0 on within the set)
+// that rank highest, at least a.top of them where there are so many, as keys in sh.list; returns their number.
+template <int THREADS, int LIST, int RUNS>
+__device__ __forceinline__ int gather_best(const ReportArgs& a, const float (&v)[RUNS][kRun], int live, int64_t index0,
+                                           RankGroup<THREADS, LIST>& sh) {
+    const int tid = (int)threadIdx.x & (THREADS - 1), lane = tid & (kWave - 1);
+    const uint32_t n = (uint32_t)a.top;
+    uint32_t most[RUNS], all[1] = {0};
+#pragma unroll
+    for (int j = 0; j < RUNS; ++j) {
+        float m = v[j][0];
+#pragma unroll
+        for (int k = 1; k < kRun; ++k) m = max2(m, v[j][k]);
+        most[j] = j < live ? rank_of(m) : 0;
+        all[0] = max(all[0], most[j]);
+    }
+    uint32_t bound;
+    if (THREADS == kWave) {
+        // where the lanes' largest would let many rows through, the runs' have a say, or each row
+        if (n <= 16) {
+            bound = wave_bound<1>(all, n);
+        } else if (RUNS > 1) {
+            bound = wave_bound<RUNS>(most, n);
+        } else {
+            uint32_t each[kRun];
+#pragma unroll
+            for (int k = 0; k < kRun; ++k) each[k] = rank_of(v[0][k]);
+            bound = wave_bound<kRun>(each, n);
+        }
+    } else {
+        // of each wave's rows a share; a wave that has too few leaves it to the others
+        const uint32_t waves = THREADS / kWave;
+        const uint32_t mine = wave_bound<1>(all, (n + waves - 1) / waves);
+        if (lane == 0) sh.bound[tid / kWave] = mine;
+        if (tid == 0) sh.size = 0;
+        __syncthreads();
+        bound = ~0u;
+        for (uint32_t w = 0; w < waves; ++w) bound = min(bound, sh.bound[w]);
+        if (bound == 0) {
+            const uint32_t whole = wave_bound<RUNS>(most, n);
+            __syncthreads();
+            if (lane == 0) sh.bound[tid / kWave] = whole;
+            __syncthreads();
+            for (uint32_t w = 0; w < waves; ++w) bound = max(bound, sh.bound[w]);
+        }
+    }
+    const auto add = [&](bool in, int j, int k, uint32_t& count) {
+        const unsigned long long m = __ballot(in);
+        if (m == 0) return;
+        uint32_t at = count;
+        if (THREADS == kWave) {
+            count += (uint32_t)__popcll(m);
+        } else {
+            if (lane == 0) at = atomicAdd(&sh.size, (uint32_t)__popcll(m));
+            at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at);
+        }
+        at += (uint32_t)__popcll(m & ((1ull << lane) - 1ull));
+        if (in && at < (uint32_t)LIST) sh.list[at] = key_of(v[j][k], (uint32_t)(index0 + kRun * (j * THREADS + tid) + k));
+    };
+    const float least = bound < 0x00800000u ? kLowest : rank_value(bound);
+    uint32_t count = 0;
+    wave_sync();
+#pragma unroll
+    for (int j = 0; j < RUNS; ++j)
+        if (j < live)
+#pragma unroll
+            for (int k = 0; k < kRun; ++k) add(!(v[j][k] < least), j, k, count);
+    if (THREADS != kWave) {
+        __syncthreads();
+        count = sh.size;
+    }
+    wave_sync();
+    if (count <= (uint32_t)LIST) return (int)count;
+    // Too many rows reach the bound, of one value most often: the least rank that a.top rows reach, and of those that have
+    // it the first.
+    int turn = 0;
+    uint32_t t = 0;
+    for (uint32_t bit = 1u << 31; bit != 0; bit >>= 1)
+        if (group_count(wave_count<RUNS>(live, [&](int j, int k) { return rank_of(v[j][k]) >= (t | bit); }), sh, turn) >= n) t |= bit;
+    const uint32_t above = group_count(wave_count<RUNS>(live, [&](int j, int k) { return rank_of(v[j][k]) > t; }), sh, turn);
+    int last = RUNS * THREADS * kRun - 1;
+    for (int bit = RUNS * THREADS * kRun / 2; bit != 0; bit >>= 1)
+        if (above + group_count(wave_count<RUNS>(live, [&](int j, int k) {
+                                    return rank_of(v[j][k]) == t && kRun * (j * THREADS + tid) + k <= last - bit;
+                                }), sh, turn) >= n)
+            last -= bit;
+    if (THREADS != kWave) {
+        if (tid == 0) sh.size = 0;
+        __syncthreads();
+    }
+    count = 0;
+#pragma unroll
+    for (int j = 0; j < RUNS; ++j)
+        if (j < live)
+#pragma unroll
+            for (int k = 0; k < kRun; ++k) {
+                const uint32_t r = rank_of(v[j][k]);
+                add(r > t || (r == t && t != 0 && kRun * (j * THREADS + tid) + k <= last), j, k, count);
+            }
+    if (THREADS != kWave) {
+        __syncthreads();
+        count = sh.size;
+    }
+    wave_sync();
+    return (int)count;
+}
+
+// f(place, key) of the first a.top of n keys, and of none (key 0) behind the last.
+template <int THREADS, class F>
+__device__ __forceinline__ void rank_list(const ReportArgs& a, const unsigned long long* list, int n, F f) {
+    const int tid = (int)threadIdx.x & (THREADS - 1);
+    for (int c = tid; c < n; c += THREADS) {
+        const unsigned long long key = list[c];
+        int place = 0;
+        for (int i = 0; i < n; ++i) place += list[i] > key ? 1 : 0;
+        if (place < a.top) f(place, key);
+    }
+    for (int c = n + tid; c < a.top; c += THREADS) f(c, 0ull);
+}
+
+// ------------------------------------------------------------------------------------ tiles
+struct ReportTile {
+    union {
+        float x[kSetTileRows];        // logits
+        uint32_t rank[kSetTileRows];  // later: their ranks
+    };
+    float top[kSetTileSets + 4];  // per set: maximum
+    union {
+        uint16_t head[kSetTileRows];  // the set that starts at a row, from 1; 0: none
+        float sum[kSetTileSets + 4];  // later: sum of exponentials, then its logarithm
+    };
+    float along[kSetTileSets + 4];     // sum of exponentials times distances
+    uint32_t range[kSetTileSets + 4];  // first row and, 16 bits up, the row behind the last
+    int32_t set[kSetTileSets + 4];
+    int32_t idle[kSetTileSets + 4];    // rows that are not ranked
+    RankGroup<kWave, kWaveList> group;
+};
+
+// The lists of a tile: ranks of 32 bits in LDS. A row compares itself with those of its set that lie before its lane's run,
+// in the run, and after it; what lies before belongs to the set of the run's first row, what lies after to that of its
+// last. 17 vector instructions for a row of LDS and eight of the lane's.
+template <class ROWS>
+__device__ __forceinline__ void tile_lists(const ReportArgs& a, const ROWS& in, const float (&x)[kRun], const int (&id)[kRun],
+                                           ReportTile& sh) {
+    const int lane = (int)threadIdx.x & (kWave - 1), i0 = kRun * lane;
+    uint32_t own[kRun];
+    int place[kRun];
+#pragma unroll
+    for (int k = 0; k < kRun; ++k) {
+        own[k] = rank_of(x[k]);
+        place[k] = 0;
+    }
+    *reinterpret_cast<uint4*>(&sh.rank[i0]) = make_uint4(own[0], own[1], own[2], own[3]);
+    *reinterpret_cast<uint4*>(&sh.rank[i0 + 4]) = make_uint4(own[4], own[5], own[6], own[7]);
+#pragma unroll
+    for (int r = 0; r < kTileRounds; ++r) {
+        const int s = r * kWave + lane;
+        sh.range[s] = (uint32_t)in.begin[r] | (uint32_t)in.end[r] << 16;
+        sh.set[s] = in.set[r];
+        sh.idle[s] = 0;
+    }
+    if (lane < 4) sh.range[kSetTileSets + lane] = 0;
+    wave_sync();
+    uint32_t range[kRun];
+#pragma unroll
+    for (int k = 0; k < kRun; ++k) {
+        range[k] = sh.range[id[k] - 1];
+        const int i = i0 + k;
+        if (own[k] == 0 && i >= (int)(range[k] & 0xffffu) && i < (int)(range[k] >> 16)) atomicAdd(&sh.idle[id[k] - 1], 1);
+    }
+    const auto short_set = [](uint32_t r) { return (int)(r >> 16) - (int)(r & 0xffffu) <= kCountRows; };
+#pragma unroll
+    for (int k = 0; k < kRun; ++k)
+#pragma unroll
+        for (int l = k + 1; l < kRun; ++l) {
+            const bool same = id[k] == id[l], below = own[l] > own[k];
+            place[k] += same && below ? 1 : 0;
+            place[l] += same && !below ? 1 : 0;
+        }
+    uint32_t some = 0;
+#pragma unroll
+    for (int k = 0; k < kRun; ++k) some |= own[k];
+    // rows [i, e) of LDS, four asked for at a time
+    const auto count_rows = [&](int i, int e, const uint32_t (&than)[kRun]) {
+        for (; i + 3 < e; i += 4) {
+            const uint32_t o[4] = {sh.rank[i], sh.rank[i + 1], sh.rank[i + 2], sh.rank[i + 3]};
+#pragma unroll
+            for (int l = 0; l < 4; ++l)
+#pragma unroll
+                for (int k = 0; k < kRun; ++k) place[k] += o[l] > than[k] ? 1 : 0;
+        }
+        for (; i < e; ++i) {
+            const uint32_t o = sh.rank[i];
+#pragma unroll
+            for (int k = 0; k < kRun; ++k) place[k] += o > than[k] ? 1 : 0;
+        }
+    };
+    if (some && short_set(range[0])) {  // of equal ones the rows before rank above
+        uint32_t than[kRun];
+#pragma unroll
+        for (int k = 0; k < kRun; ++k) than[k] = id[k] == id[0] && own[k] != 0 ? own[k] - 1u : ~0u;
+        count_rows((int)(range[0] & 0xffffu), min(i0, (int)(range[0] >> 16)), than);
+    }
+    if (some && short_set(range[kRun - 1])) {
+        uint32_t than[kRun];
+#pragma unroll
+        for (int k = 0; k < kRun; ++k) than[k] = id[k] == id[kRun - 1] ? own[k] : ~0u;
+        count_rows(i0 + kRun, (int)(range[kRun - 1] >> 16), than);
+    }
+#pragma unroll
+    for (int k = 0; k < kRun; ++k)
+        if (own[k] != 0 && place[k] < a.top && short_set(range[k])) {
+            const int s = id[k] - 1;
+            put_entry(a, (int64_t)sh.set[s] * a.top + place[k], i0 + k - (int)(range[k] & 0xffffu),
+                      list_log_prob(a, rank_value(own[k]), sh.top[s], (double)sh.sum[s]));
+        }
+    // behind the last: lists of short sets with fewer ranked rows than entries
+    bool gaps = false;
+#pragma unroll
+    for (int r = 0; r < kTileRounds; ++r) {
+        const int s = r * kWave + lane, size = in.end[r] - in.begin[r];
+        gaps = gaps || (s < in.sets && size <= kCountRows && size - sh.idle[s] < a.top);
+    }
+    if (__any(gaps)) {
+        const int bits = a.team_bits, entries = in.sets << bits, j = lane & ((1 << bits) - 1);
+        for (int e = lane; e < entries; e += kWave) {
+            const int s = e >> bits;
+            const uint32_t r = sh.range[s];
+            if (j < a.top && short_set(r) && j >= (int)(r >> 16) - (int)(r & 0xffffu) - sh.idle[s])
+                put_entry(a, (int64_t)sh.set[s] * a.top + j, -1, -kInf);
+        }
+    }
+    // longer sets, one after the other
+    for (int r = 0; r < kTileRounds; ++r) {
+        const int size = r ? in.end[1] - in.begin[1] : in.end[0] - in.begin[0];
+        for (unsigned long long m = __ballot(r * kWave + lane < in.sets && size > kCountRows); m; m &= m - 1) {
+            const int s = r * kWave + __ffsll((long long)m) - 1;
+            const uint32_t rg = sh.range[s];
+            const int b = (int)(rg & 0xffffu), e = (int)(rg >> 16);
+            float v[1][kRun];
+#pragma unroll
+            for (int k = 0; k < kRun; ++k) {
+                const uint32_t o = b + i0 + k < e ? sh.rank[b + i0 + k] : 0u;
+                v[0][k] = o ? rank_value(o) : -kInf;
+            }
+            const int n = gather_best(a, v, 1, 0, sh.group);
+            rank_list<kWave>(a, sh.group.list, n, [&](int place, unsigned long long key) {
+                const bool there = key != 0;
+                put_entry(a, (int64_t)sh.set[s] * a.top + place, there ? (int32_t)~(uint32_t)key : -1,
+                          there ? list_log_prob(a, rank_value((uint32_t)(key >> 32)), sh.top[s], (double)sh.sum[s]) : -kInf);
+            });
+            wave_sync();
         }
     }
 }
 
 template <int TYPE, bool MASK, bool BIAS>
-__global__ __launch_bounds__(kBlock) void report_kernel(ReportArgs a, int64_t num_sets) {
-    __shared__ BiasShared bias;
-    __shared__ float shf[kWaves];
-    __shared__ double shd[kWaves];
-    __shared__ unsigned long long shk[kWaves];
-    if (BIAS) stage_bias(a, bias);
+__device__ __forceinline__ void report_tile(const ReportArgs& a, const TileRows<TYPE, MASK, BIAS>& in,
+                                            int32_t (&chosen)[kTileRounds], ReportTile& sh, const BiasShared* bias) {
+    const int lane = (int)threadIdx.x & (kWave - 1), i0 = kRun * lane;
     const Heat heat{a.heat_hi, a.heat_lo, a.heat_low};
-    for (int64_t g = blockIdx.x; g < num_sets; g += gridDim.x) {
-        const int64_t r0 = a.off[g], r1 = a.off[g + 1];
-        float top = kLowest;
-        each_run<TYPE, MASK, BIAS>(a, &bias, r0, r1, [&](int64_t, const float(&z)[kRun]) {
+    const bool alone = in.sets == 1;
+    float x[kRun];
+    uint32_t off;
+    Buckets buckets;
 #pragma unroll
-            for (int k = 0; k < kRun; ++k) top = max2(top, z[k]);
-        });
+    for (int k = 0; k < kRun; ++k) x[k] = -kInf;
+    if (in.sp.hi > 0) in.raw.logits(a, bias, in.sp, 0, x, off, buckets);
+    wave_sync();  // the last tile's values have been read
+    *reinterpret_cast<uint4*>(&sh.head[i0]) = make_uint4(0, 0, 0, 0);
+    write_run(&sh.x[i0], x);
+    wave_sync();
+    float picked[kTileRounds];
+#pragma unroll
+    for (int r = 0; r < kTileRounds; ++r) {
+        const int s = r * kWave + lane;
+        picked[r] = -kInf;
+        if (s < in.sets) {
+            if (in.end[r] > in.begin[r]) sh.head[in.begin[r]] = (uint16_t)(s + 1);
+            if (chosen[r] >= in.end[r] - in.begin[r]) chosen[r] = -1;
+            if (chosen[r] >= 0) picked[r] = sh.x[in.begin[r] + chosen[r]];
+            // a masked row's logit is -inf, as one of that score is: the mask says which
+            if (MASK && chosen[r] >= 0 && picked[r] == -kInf && !a.mask[a.off[in.set[r]] + chosen[r]]) chosen[r] = -1;
+        }
+    }
+    wave_sync();
+    TileSets sets;
+    float v[kRun], w[kRun];
+    if (alone) {
+        float top = kLowest, sum = 0.0f, along = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kRun; ++k) sets.id[k] = 1;
+#pragma unroll
+        for (int k = 0; k < kRun; k += 2) top = max3(top, x[k], x[k + 1]);
         top = wave_max(top);
-        __syncthreads();
-        if ((threadIdx.x & (kWave - 1)) == 0) shf[threadIdx.x / kWave] = top;
-        __syncthreads();
-        for (int w = 0; w < kWaves; ++w) top = max2(top, shf[w]);
-        double sum = 0.0, along = 0.0;
-        each_run<TYPE, MASK, BIAS>(a, &bias, r0, r1, [&](int64_t, const float(&z)[kRun]) {
 #pragma unroll
-            for (int k = 0; k < kRun; ++k) {
-                const float e = heat_exp<true>(z[k] - top, heat);
-                sum += (double)e;
-                along += e == 0.0f ? 0.0 : (double)e * (double)(z[k] - top);
-            }
-        });
-        sum = block_sum(sum, shd);
-        along = block_sum(along, shd);
-        const bool none = sum == 0.0;
-        const double log_sum = log(sum);
-        if (threadIdx.x == 0) {
-            const double m = none ? 0.0 : (double)top;
-            a.lse_out[g] = (float)(m * a.inv_temp + log_sum);
-            a.entropy[g] = none ? 0.0f : (float)(log_sum - along * a.inv_temp / sum);
-            if (a.chosen) {
-                const int32_t c = a.chosen[g];
-                bool counts = c >= 0 && c < r1 - r0 && !none;
-                if (MASK && counts) counts = a.mask[r0 + c] != 0;
-                a.log_probs[g] = counts ? (float)(((double)one_logit<TYPE, BIAS>(a, &bias, r0 + c) - m) * a.inv_temp - log_sum) : 0.0f;
-            }
+        for (int k = 0; k < kRun; ++k) {
+            const float d = __builtin_elementwise_maximum(x[k] - top, heat.low), e = heat_exp<TYPE == PB_F32 || BIAS>(d, heat);
+            sum += e;
+            along += e * d;
         }
-        unsigned long long last = ~0ull;
-        for (int j = 0; j < a.top; ++j) {
-            unsigned long long best = 0;
-            if (last != 0)
-                each_run<TYPE, MASK, BIAS>(a, &bias, r0, r1, [&](int64_t i, const float(&z)[kRun]) {
+        sum = wave_sum(sum);
+        along = wave_sum(along);
+        wave_sync();
+        if (lane == 0) {
+            sh.top[0] = top;
+            sh.sum[0] = sum;
+            sh.along[0] = along;
+        }
+    } else {
+        sets.find(sh.head, lane);
+        wave_sync();  // the heads have been read
+        segment_reduce<TakeMax>(sets.seg, x, sets.id, lane, sh.top);
+        wave_sync();
 #pragma unroll
-                    for (int k = 0; k < kRun; ++k) {
-                        const unsigned long long key = z[k] == -kInf ? 0ull : rank_key(z[k], (uint32_t)(i + k));
-                        best = key < last && key > best ? key : best;
-                    }
-                });
-            last = block_max(best, shk);
-            if (threadIdx.x == 0) {
-                const uint32_t i = ~(uint32_t)last;
-                a.top_index[g * a.top + j] = last ? (int32_t)i : -1;
-                a.top_log_probs[g * a.top + j] =
-                    last ? (float)(((double)one_logit<TYPE, BIAS>(a, &bias, r0 + i) - (double)top) * a.inv_temp - log_sum) : -kInf;
-            }
+        for (int k = 0; k < kRun; ++k) {
+            const float d = __builtin_elementwise_maximum(x[k] - sh.top[sets.id[k] - 1], heat.low);
+            v[k] = heat_exp<TYPE == PB_F32 || BIAS>(d, heat);
+            w[k] = v[k] * d;
         }
+        segment_reduce<TakeSum>(sets.seg, v, sets.id, lane, sh.sum);
+        segment_reduce<TakeSum>(sets.seg, w, sets.id, lane, sh.along);
+    }
+    wave_sync();
+#pragma unroll
+    for (int r = 0; r < kTileRounds; ++r) {
+        const int s = r * kWave + lane;
+        if (s < in.sets) {
+            const bool empty = in.end[r] == in.begin[r];
+            const SoftSums t{empty ? kLowest : sh.top[s], empty ? 0.0 : (double)sh.sum[s], empty ? 0.0 : (double)sh.along[s]};
+            const double log_sum = log_near(t.sum);
+            put_report(a, in.set[r], t, log_sum, chosen[r] >= 0, picked[r]);
+            sh.sum[s] = (float)log_sum;
+        }
+    }
+    if (a.top > 0) {
+        wave_sync();
+        tile_lists(a, in, x, sets.id, sh);
     }
 }
 
-template <int TYPE>
-hipError_t launch_report_typed(const SetLayout& s, const ReportArgs& a, hipStream_t stream) {
-    const dim3 grid((unsigned)std::min<int64_t>(s.num_sets, kReportGrid)), block(kBlock);
-    if (a.mask && a.table)
-        hipLaunchKernelGGL((report_kernel<TYPE, true, true>), grid, block, 0, stream, a, s.num_sets);
-    else if (a.mask)
-        hipLaunchKernelGGL((report_kernel<TYPE, true, false>), grid, block, 0, stream, a, s.num_sets);
-    else if (a.table)
-        hipLaunchKernelGGL((report_kernel<TYPE, false, true>), grid, block, 0, stream, a, s.num_sets);
-    else
-        hipLaunchKernelGGL((report_kernel<TYPE, false, false>), grid, block, 0, stream, a, s.num_sets);
-    return hipGetLastError();
+template <int TYPE, bool MASK, bool BIAS>
+__global__ __launch_bounds__(kBlock, 4) void report_tile_kernel(ReportArgs a) {
+    __shared__ ReportTile tiles[kWaves];
+    __shared__ BiasShared bias;
+    const int tid = (int)threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid & (kWave - 1);
+    if (BIAS) stage_bias(a, bias);
+    const int step = (int)gridDim.x * kWaves;
+    for (int it = __builtin_amdgcn_readfirstlane((int)blockIdx.x * kWaves + wave); it < a.num_tiles; it += step) {
+        TileRows<TYPE, MASK, BIAS> in;
+        in.load(a, a.tiles[it], lane);
+        int32_t chosen[kTileRounds];
+#pragma unroll
+        for (int r = 0; r < kTileRounds; ++r) chosen[r] = a.chosen && r * kWave + lane < in.sets ? a.chosen[in.set[r]] : -1;
+        report_tile<TYPE, MASK, BIAS>(a, in, chosen, tiles[wave], &bias);
+    }
 }
+
+// ------------------------------------------------------------------------------------ longer sets
+template <int THREADS, int LIST>
+struct ReportGroup {
+    RankGroup<THREADS, LIST> rank;
+    float top[THREADS / kWave];
+    double sum[THREADS / kWave], along[THREADS / kWave];
+};
+
+// One set of more than kSetShort rows by a wave (THREADS 64), or a longer one or a part of it by a workgroup, its rows in
+// registers.
+template <int TYPE, bool MASK, bool BIAS, int THREADS, int LIST>
+__device__ __forceinline__ void report_pass(const ReportArgs& a, const SetItem& im, int32_t index, ReportGroup<THREADS, LIST>& sh,
+                                            const BiasShared* bias) {
+    constexpr bool EXACT = TYPE == PB_F32 || BIAS;
+    const int tid = (int)threadIdx.x & (THREADS - 1), lane = tid & (kWave - 1);
+    const int wave0 = __builtin_amdgcn_readfirstlane(tid & ~(kWave - 1));  // the wave's first thread
+    const Heat heat{a.heat_hi, a.heat_lo, a.heat_low};
+    const Span sp = span_of(a, im);
+    const int64_t g = im.set0;
+    RawRun<TYPE, MASK, BIAS> raw[kWideRuns];
+#pragma unroll
+    for (int j = 0; j < kWideRuns; ++j) {
+        const int i = kRun * (j * THREADS + tid);
+        if (kRun * (j * THREADS + wave0) < sp.hi && i < sp.hi) raw[j].load(a, sp, i);
+    }
+    const int64_t r0 = a.off[g], size = a.off[g + 1] - r0;
+    bool counts = false;
+    float z = 0.0f;
+    if (a.chosen && im.parts == 1) {
+        const int32_t c = a.chosen[g];
+        counts = c >= 0 && c < size;
+        if (MASK && counts) counts = a.mask[r0 + c] != 0;
+        if (counts) z = one_logit<TYPE, BIAS>(a, bias, r0 + c);
+    }
+    float v[kWideRuns][kRun];
+#pragma unroll
+    for (int j = 0; j < kWideRuns; ++j) {
+        const int i = kRun * (j * THREADS + tid);
+#pragma unroll
+        for (int k = 0; k < kRun; ++k) v[j][k] = -kInf;
+        if (kRun * (j * THREADS + wave0) < sp.hi && i < sp.hi) {
+            uint32_t off;
+            Buckets buckets;
+            raw[j].logits(a, bias, sp, i, v[j], off, buckets);
+        }
+    }
+    const int live = sp.hi <= kRun * wave0 ? 0 : (sp.hi - kRun * wave0 + kRun * THREADS - 1) / (kRun * THREADS);  // the wave's runs
+    SoftSums t{kLowest, 0.0, 0.0};
+#pragma unroll
+    for (int j = 0; j < kWideRuns; ++j)
+        if (j < live)
+#pragma unroll
+            for (int k = 0; k < kRun; k += 2) t.top = max3(t.top, v[j][k], v[j][k + 1]);
+    t.top = wave_max(t.top);
+    float sum = 0.0f, along = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kWideRuns; ++j)
+        if (j < live)
+#pragma unroll
+            for (int k = 0; k < kRun; ++k) {
+                const float d = __builtin_elementwise_maximum(v[j][k] - t.top, heat.low), e = heat_exp<EXACT>(d, heat);
+                sum += e;
+                along = __builtin_fmaf(e, d, along);
+            }
+    t.sum = team_sum((double)sum, 6);
+    t.along = team_sum((double)along, 6);
+    if (THREADS != kWave) {
+        if (lane == 0) {
+            sh.top[tid / kWave] = t.top;
+            sh.sum[tid / kWave] = t.sum;
+            sh.along[tid / kWave] = t.along;
+        }
+        __syncthreads();
+        t = SoftSums{sh.top[0], 0.0, 0.0};
+        for (int w = 1; w < THREADS / kWave; ++w) t.top = max2(t.top, sh.top[w]);
+        for (int w = 0; w < THREADS / kWave; ++w) {
+            const double gap = (double)sh.top[w] - (double)t.top, f = exp_near(gap * a.inv_temp);
+            t.sum += sh.sum[w] * f;
+            t.along += f == 0.0 ? 0.0 : f * (sh.along[w] + sh.sum[w] * gap);
+        }
+    }
+    const double log_sum = log_near(t.sum);
+    if (tid == 0) {
+        if (im.parts == 1)
+            put_report(a, g, t, log_sum, counts, z);
+        else
+            a.part_sums[index] = t;
+    }
+    if (a.top > 0) {
+        const int n = gather_best(a, v, live, sp.q0 - r0, sh.rank);
+        if (im.parts == 1)
+            rank_list<THREADS>(a, sh.rank.list, n, [&](int place, unsigned long long key) {
+                const bool there = key != 0;
+                put_entry(a, g * a.top + place, there ? (int32_t)~(uint32_t)key : -1,
+                          there ? list_log_prob(a, rank_value((uint32_t)(key >> 32)), t.top, log_sum) : -kInf);
+            });
+        else
+            rank_list<THREADS>(a, sh.rank.list, n,
+                               [&](int place, unsigned long long key) { a.part_keys[(int64_t)index * a.top + place] = key; });
+    }
+    if (THREADS != kWave)
+        __syncthreads();  // the list and the sums have been read
+    else
+        wave_sync();
+}
+
+// Workgroups [0, mid_blocks) take the sets for a wave, the others those for a workgroup and the parts, one at a time.
+template <int TYPE, bool MASK, bool BIAS>
+__global__ __launch_bounds__(kBlock) void report_wide_kernel(ReportArgs a, int mid_blocks) {
+    __shared__ union {
+        ReportGroup<kWave, kWaveList> mid[kWaves];
+        ReportGroup<kBlock, kGroupList> whole;
+    } sh;
+    __shared__ BiasShared bias;
+    if (BIAS) stage_bias(a, bias);
+    if ((int)blockIdx.x < mid_blocks) {
+        const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), step = mid_blocks * kWaves;
+        for (int it = (int)blockIdx.x * kWaves + wave; it < a.num_mid; it += step)
+            report_pass<TYPE, MASK, BIAS, kWave, kWaveList>(a, a.wide[it], it, sh.mid[wave], &bias);
+    } else {
+        const int n = a.num_mid + a.num_wide;
+        for (int it = a.num_mid + (int)blockIdx.x - mid_blocks; it < n; it += (int)gridDim.x - mid_blocks)
+            report_pass<TYPE, MASK, BIAS, kBlock, kGroupList>(a, a.wide[it], it, sh.whole, &bias);
+    }
+}
+
+__device__ __forceinline__ uint32_t block_count(uint32_t v, uint32_t* sh) {
+    for (int m = kWave / 2; m >= 1; m >>= 1) v += __shfl_xor(v, m);
+    __syncthreads();
+    if ((threadIdx.x & (kWave - 1)) == 0) sh[threadIdx.x / kWave] = v;
+    __syncthreads();
+    v = 0;
+    for (int w = 0; w < kWaves; ++w) v += sh[w];
+    return v;
+}
+
+// The sets in parts, a workgroup each: sums and lists from those of the parts. With d = top / parts, rounded up, entry d of
+// a part says that d of its rows rank as high: the bound is the (top / d)-th largest of these, which at most top / d parts
+// reach with all of their entries and the others with fewer than d of them, 64 x 64 at most.
+template <int TYPE, bool MASK, bool BIAS>
+__global__ __launch_bounds__(kBlock) void report_join_kernel(ReportArgs a, const int32_t* __restrict__ firsts) {
+    __shared__ unsigned long long list[kJoinList];
+    __shared__ uint32_t shc[kWaves], size;
+    __shared__ float tops[kWaves];
+    __shared__ double sums[kWaves], alongs[kWaves];
+    __shared__ BiasShared bias;
+    const int tid = (int)threadIdx.x, lane = tid & (kWave - 1);
+    const int32_t first = firsts[blockIdx.x];
+    const SetItem im = a.wide[first];
+    const int64_t g = im.set0, r0 = a.off[g];
+    const int n = im.parts;
+    if (BIAS) stage_bias(a, bias);
+    SoftSums t{kLowest, 0.0, 0.0};
+    for (int j = tid; j < n; j += kBlock) t.top = max2(t.top, a.part_sums[first + j].top);
+    t.top = wave_max(t.top);
+    if (lane == 0) tops[tid / kWave] = t.top;
+    if (tid == 0) size = 0;
+    __syncthreads();
+    for (int w = 0; w < kWaves; ++w) t.top = max2(t.top, tops[w]);
+    for (int j = tid; j < n; j += kBlock) {
+        const SoftSums p = a.part_sums[first + j];
+        const double gap = (double)p.top - (double)t.top, f = exp_near(gap * a.inv_temp);
+        t.sum += p.sum * f;
+        t.along += f == 0.0 ? 0.0 : f * (p.along + p.sum * gap);
+    }
+    t.sum = block_sum(t.sum, sums);
+    t.along = block_sum(t.along, alongs);
+    const double log_sum = log_near(t.sum);
+    if (tid == 0) {
+        bool counts = false;
+        float z = 0.0f;
+        if (a.chosen) {
+            const int32_t c = a.chosen[g];
+            counts = c >= 0 && c < a.off[g + 1] - r0;
+            if (MASK && counts) counts = a.mask[r0 + c] != 0;
+            if (counts) z = one_logit<TYPE, BIAS>(a, &bias, r0 + c);
+        }
+        put_report(a, g, t, log_sum, counts, z);
+    }
+    if (a.top == 0) return;
+    const unsigned long long* keys = a.part_keys + (int64_t)first * a.top;
+    const int64_t entries = (int64_t)n * a.top;
+    unsigned long long bound = 0;
+    if (entries > kBlock) {
+        const int d = (a.top + n - 1) / n;
+        const uint32_t want = (uint32_t)((a.top + d - 1) / d);
+        for (int bit = 63; bit >= 0; --bit) {
+            const unsigned long long trial = bound | 1ull << bit;
+            uint32_t c = 0;
+            for (int j = tid; j < n; j += kBlock) c += keys[(int64_t)j * a.top + d - 1] >= trial ? 1u : 0u;
+            if (block_count(c, shc) >= want) bound = trial;
+        }
+    }
+    for (int64_t e0 = 0; e0 < entries; e0 += kBlock) {
+        const int64_t e = e0 + tid;
+        const unsigned long long key = e < entries ? keys[e] : 0ull;
+        if (key != 0 && key >= bound) {
+            const uint32_t at = atomicAdd(&size, 1u);
+            if (at < (uint32_t)kJoinList) list[at] = key;
+        }
+    }
+    __syncthreads();
+    int c = (int)min(size, (uint32_t)kJoinList);
+    if (c > kGroupList) {  // the a.top-th key itself, then what reaches it
+        unsigned long long least = 0;
+        for (int bit = 63; bit >= 0; --bit) {
+            const unsigned long long trial = least | 1ull << bit;
+            uint32_t m = 0;
+            for (int i = tid; i < c; i += kBlock) m += list[i] >= trial ? 1u : 0u;
+            if (block_count(m, shc) >= (uint32_t)a.top) least = trial;
+        }
+        unsigned long long mine[kJoinList / kBlock];
+#pragma unroll
+        for (int i = 0; i < kJoinList / kBlock; ++i) mine[i] = i * kBlock + tid < c ? list[i * kBlock + tid] : 0ull;
+        __syncthreads();
+        if (tid == 0) size = 0;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kJoinList / kBlock; ++i)
+            if (mine[i] >= least && mine[i] != 0) list[atomicAdd(&size, 1u)] = mine[i];
+        __syncthreads();
+        c = (int)size;
+    }
+    rank_list<kBlock>(a, list, c, [&](int place, unsigned long long key) {
+        const bool there = key != 0;
+        put_entry(a, g * a.top + place, there ? (int32_t)~(uint32_t)key : -1,
+                  there ? list_log_prob(a, rank_value((uint32_t)(key >> 32)), t.top, log_sum) : -kInf);
+    });
+}
+
+int tile_blocks(const SetLayout& s) { return std::min((s.num_tiles + kWaves - 1) / kWaves, kChoiceGrid); }
+
+int mid_blocks(const SetLayout& s) { return std::min((s.num_mid + kWaves - 1) / kWaves, kChoiceGrid); }
+
+template <int TYPE, bool MASK, bool BIAS>
+hipError_t launch_as(const SetLayout& s, const ReportArgs& a, hipStream_t stream) {
+    hipError_t e = hipSuccess;
+    const int wide = mid_blocks(s) + std::min(s.num_wide, kChoiceGrid);
+    if (wide > 0) {
+        hipLaunchKernelGGL((report_wide_kernel<TYPE, MASK, BIAS>), dim3(wide), dim3(kBlock), 0, stream, a, mid_blocks(s));
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
+    if (s.num_tiles > 0) {
+        hipLaunchKernelGGL((report_tile_kernel<TYPE, MASK, BIAS>), dim3(tile_blocks(s)), dim3(kBlock), 0, stream, a);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
+    if (s.num_split > 0) {
+        hipLaunchKernelGGL((report_join_kernel<TYPE, MASK, BIAS>), dim3(s.num_split), dim3(kBlock), 0, stream, a, s.split);
+        e = hipGetLastError();
+    }
+    return e;
+}
+
+template <int TYPE>
+hipError_t launch_typed(const SetLayout& s, const ReportArgs& a, hipStream_t stream) {
+    if (a.mask) return a.table ? launch_as<TYPE, true, true>(s, a, stream) : launch_as<TYPE, true, false>(s, a, stream);
+    return a.table ? launch_as<TYPE, false, true>(s, a, stream) : launch_as<TYPE, false, false>(s, a, stream);
+}
+
+int64_t part_items(const SetLayout& s) { return s.num_wide > s.num_whole ? s.num_mid + s.num_wide : 0; }
 
 }  // namespace
 
-int64_t report_work_bytes(const SetLayout&, int32_t) { return 0; }
+int64_t report_work_bytes(const SetLayout& s, int32_t top) { return part_items(s) * ((int64_t)sizeof(SoftSums) + 8 * top); }
 
-hipError_t launch_report(const SetLayout& s, ReportArgs a, int32_t type, char*, hipStream_t stream) {
+hipError_t launch_report(const SetLayout& s, ReportArgs a, int32_t type, char* work, hipStream_t stream) {
     a.off = s.off;
+    a.tiles = s.tiles;
+    a.wide = s.wide;
+    a.segments = s.segments;
+    a.num_tiles = s.num_tiles;
+    a.num_wide = s.num_wide;
+    a.num_mid = s.num_mid;
+    a.num_whole = s.num_whole;
     a.rows = s.rows;
+    a.part_sums = reinterpret_cast<SoftSums*>(work);
+    a.part_keys = reinterpret_cast<unsigned long long*>(work + sizeof(SoftSums) * part_items(s));
+    a.team_bits = 0;
+    while (1 << a.team_bits < a.top) ++a.team_bits;
     const auto at = [](const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; };
     a.vec = a.stride == 1 && at(a.scores, 16) && at(a.mask, 8) && at(a.positions, 16);
-    if (type == PB_BF16) return launch_report_typed<PB_BF16>(s, a, stream);
-    if (type == PB_F16) return launch_report_typed<PB_F16>(s, a, stream);
-    return launch_report_typed<PB_F32>(s, a, stream);
+    if (type == PB_BF16) return launch_typed<PB_BF16>(s, a, stream);
+    if (type == PB_F16) return launch_typed<PB_F16>(s, a, stream);
+    return launch_typed<PB_F32>(s, a, stream);
 }
 
 }  // namespace pb
