@@ -51,9 +51,10 @@ int32_t team_of(int64_t rows, int64_t sets, int64_t largest) {
 }
 
 struct Layout {
-    std::vector<SetItem> tiles, mid, whole, parts;
+    std::vector<SetItem> tiles, mid, whole, parts, half, big;
     std::vector<pb::TileSegment> segments;
     std::vector<int32_t> split;  // the first part of each split set, within `parts`
+    std::vector<int32_t> giant;  // the parts of sets that are not in `half` or `big`, too
 };
 
 // The tile that is being filled.
@@ -136,9 +137,15 @@ void lay_out(const int64_t* off, int64_t num_sets, bool segments, Layout& out) {
             const int64_t most = pb::kSetWideRows - 8;
             const int64_t want = (size + most - 1) / most;
             const int64_t each = ((size + want - 1) / want + 7) / 8 * 8;  // at most `most`, itself a multiple of 8
+            const int64_t span = (off[g] & 7) + size;
+            if (span <= pb::kSetBig) {
+                im.rows = (int32_t)size;
+                (span <= pb::kSetHalfBig ? out.half : out.big).push_back(im);
+            }
             im.parts = (int32_t)((size + each - 1) / each);
             out.split.push_back((int32_t)out.parts.size());
             for (im.part = 0; im.part < im.parts; ++im.part) {
+                if (span > pb::kSetBig) out.giant.push_back((int32_t)out.parts.size());
                 im.row0 = off[g] + im.part * each;
                 im.rows = (int32_t)std::min(each, off[g + 1] - im.row0);
                 out.parts.push_back(im);
@@ -165,8 +172,14 @@ int sets_create(const int64_t* off, int64_t num_sets, bool segments, pb_sets** o
     items.insert(items.end(), lay.mid.begin(), lay.mid.end());
     items.insert(items.end(), lay.whole.begin(), lay.whole.end());
     items.insert(items.end(), lay.parts.begin(), lay.parts.end());
+    const size_t wide_end = items.size(), half = lay.half.size();
+    items.insert(items.end(), lay.half.begin(), lay.half.end());
+    items.insert(items.end(), lay.big.begin(), lay.big.end());
     for (int32_t& first : lay.split) first += (int32_t)(mid + whole);
-    const std::vector<int32_t>& split = lay.split;
+    for (int32_t& part : lay.giant) part += (int32_t)(mid + whole);
+    std::vector<int32_t>& split = lay.split;  // and `giant` behind it
+    const size_t num_split = split.size();
+    split.insert(split.end(), lay.giant.begin(), lay.giant.end());
     const size_t b_off = round256(sizeof(int64_t) * (size_t)(num_sets + 1));
     const size_t b_items = round256(sizeof(SetItem) * items.size());
     const size_t b_split = round256(sizeof(int32_t) * split.size());
@@ -192,9 +205,14 @@ int sets_create(const int64_t* off, int64_t num_sets, bool segments, pb_sets** o
     h->s.segments = reinterpret_cast<pb::TileSegment*>(h->arena + b_off + b_items + b_split);
     h->s.num_tiles = (int32_t)tiles;
     h->s.num_mid = (int32_t)mid;
-    h->s.num_wide = (int32_t)(items.size() - tiles - mid);
+    h->s.num_wide = (int32_t)(wide_end - tiles - mid);
     h->s.num_whole = (int32_t)whole;
-    h->s.num_split = (int32_t)split.size();
+    h->s.num_split = (int32_t)num_split;
+    h->s.big = h->s.tiles + wide_end;
+    h->s.num_big = (int32_t)(items.size() - wide_end);
+    h->s.num_half = (int32_t)half;
+    h->s.giant = h->s.split + num_split;
+    h->s.num_giant = (int32_t)lay.giant.size();
     h->s.num_sets = num_sets;
     h->s.rows = off[num_sets];
     for (int64_t g = 0; g < num_sets; ++g) h->largest = std::max(h->largest, off[g + 1] - off[g]);

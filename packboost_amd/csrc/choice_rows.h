@@ -689,25 +689,24 @@ __device__ __forceinline__ float heat_exp(float distance, const Heat& h) {
     return __builtin_fmaf(e * 0.693147182464599609375f, rest, e);
 }
 
-// e^x in double within 2^-46 of itself: x = k log 2 + r, |r| <= log(2) / 2, and eleven terms of r's series. -inf gives 0,
-// NaN and infinity give NaN.
+// e^x in double within 2^-34 of itself: x = k log 2 + r, |r| <= log(2) / 2, and ten terms of r's series, those from
+// r^4 / 24 on in float. -inf gives 0, NaN and infinity give NaN.
 __device__ __forceinline__ double exp_near(double x) {
     x = x < -800.0 ? -800.0 : x;
-    const double k = __builtin_rint(x * 1.4426950408889634);
-    const double r = __builtin_fma(k, -2.3190468138462996e-17, __builtin_fma(k, -0.69314718055994529, x));
-    double p = 1.0 / 39916800;
-    p = __builtin_fma(p, r, 1.0 / 3628800);
-    p = __builtin_fma(p, r, 1.0 / 362880);
-    p = __builtin_fma(p, r, 1.0 / 40320);
-    p = __builtin_fma(p, r, 1.0 / 5040);
-    p = __builtin_fma(p, r, 1.0 / 720);
-    p = __builtin_fma(p, r, 1.0 / 120);
-    p = __builtin_fma(p, r, 1.0 / 24);
-    p = __builtin_fma(p, r, 1.0 / 6);
-    p = __builtin_fma(p, r, 0.5);
-    p = __builtin_fma(p, r, 1.0);
-    p = __builtin_fma(p, r, 1.0);
-    return ldexp(p, (int)k);
+    const float k = __builtin_rintf((float)x * 1.44269504f);
+    const double r = __builtin_fma((double)k, -0.69314718055994531, x);
+    const float f = (float)r;
+    float p = 1.0f / 3628800;
+    p = __builtin_fmaf(p, f, 1.0f / 362880);
+    p = __builtin_fmaf(p, f, 1.0f / 40320);
+    p = __builtin_fmaf(p, f, 1.0f / 5040);
+    p = __builtin_fmaf(p, f, 1.0f / 720);
+    p = __builtin_fmaf(p, f, 1.0f / 120);
+    p = __builtin_fmaf(p, f, 1.0f / 24);
+    double d = __builtin_fma((double)p, r, 1.0 / 6);
+    d = __builtin_fma(d, r, 0.5);
+    d = __builtin_fma(d, r, 1.0);
+    return ldexp(__builtin_fma(d, r, 1.0), (int)k);
 }
 
 // log x in double within 2^-31 beside its rounding, and as close relative to itself near 1: x = 2^k m, m in [2/3, 4/3),
@@ -715,7 +714,7 @@ __device__ __forceinline__ double exp_near(double x) {
 __device__ __forceinline__ double log_near(double x) {
     if (!(x > 0.0 && x < (double)kInf)) return (double)log_of((float)x);
     const double half = __builtin_amdgcn_frexp_mant(x);  // [1/2, 1)
-    const bool low = half < 0.66666666666666663;
+    const bool low = (float)half < 0.6666667f;
     const double m = low ? 2.0 * half : half;
     const int k = __builtin_amdgcn_frexp_exp(x) - (low ? 1 : 0);
     const double n = m - 1.0, s = m + 1.0, inv = (double)__builtin_amdgcn_rcpf((float)s);

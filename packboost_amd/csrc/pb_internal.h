@@ -507,6 +507,11 @@ constexpr int kSetTileSets = 128;
 constexpr int kSetShort = kSetTileRows - 8;
 constexpr int kSetMidRows = 2048;
 constexpr int kSetWideRows = 8192;
+// Sets of more than kSetWideRows rows are listed whole, too, for operators that have workgroups of 512 and 1024 lanes
+// hold them in registers: `big`, first those of at most kSetHalfBig rows, then those of at most kSetBig; `giant` names the
+// parts of the others.
+constexpr int kSetHalfBig = 32768;
+constexpr int kSetBig = 65536;
 struct SetItem {
     int64_t row0;
     int32_t rows;
@@ -531,6 +536,11 @@ struct SetLayout {
     const TileSegment* segments;
     const SetItem* wide;   // [num_mid + num_wide], of the last num_wide the first num_whole whole sets
     const int32_t* split;  // [num_split], indices of wide items
+    const SetItem* big;    // [num_big], the first num_half of at most kSetHalfBig rows
+    const int32_t* giant;  // [num_giant], indices of wide items
+    int32_t num_big;
+    int32_t num_half;
+    int32_t num_giant;
     int32_t num_tiles;
     int32_t num_mid;
     int32_t num_wide;

@@ -6,14 +6,14 @@ namespace pb {
 namespace {
 
 int64_t sum_cols(const SetLayout& s, bool distill, int32_t num_buckets) {
-    return soft_blocks(s) <= 1 ? 0 : (distill ? 1 : 0) + num_buckets;
+    return soft_blocks(s, num_buckets > 0) <= 1 ? 0 : (distill ? 1 : 0) + num_buckets;
 }
 
 }  // namespace
 
 int64_t soft_grads_work_bytes(const SetLayout& s, bool distill, int32_t num_buckets) {
-    return 8 * sum_cols(s, distill, num_buckets) * soft_blocks(s) +
-           (num_parts(s) > 0 ? (int64_t)sizeof(SoftSums) * (s.num_mid + s.num_wide) : 0);
+    return 8 * sum_cols(s, distill, num_buckets) * soft_blocks(s, num_buckets > 0) +
+           (num_parts(s, num_buckets > 0) > 0 ? (int64_t)sizeof(SoftSums) * (s.num_mid + s.num_wide) : 0);
 }
 
 hipError_t launch_soft_grads(bool distill, const SetLayout& s, ReportArgs a, int32_t type, char* work, hipStream_t stream) {
@@ -25,7 +25,7 @@ hipError_t launch_soft_grads(bool distill, const SetLayout& s, ReportArgs a, int
     a.num_wide = s.num_wide;
     a.num_mid = s.num_mid;
     a.num_whole = s.num_whole;
-    a.blocks = soft_blocks(s);
+    a.blocks = soft_blocks(s, a.num_buckets > 0);
     a.rows = s.rows;
     a.sums = reinterpret_cast<double*>(work);
     a.part_sums = reinterpret_cast<SoftSums*>(a.sums + sum_cols(s, distill, a.num_buckets) * a.blocks);

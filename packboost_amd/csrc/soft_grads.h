@@ -19,6 +19,7 @@
 #pragma once
 
 #include <algorithm>
+#include <type_traits>
 
 #include "choice_rows.h"
 #include "report.h"
@@ -30,9 +31,13 @@ namespace {
 template <int TYPE, bool BIAS>
 constexpr bool kExact = TYPE == PB_F32 || BIAS;
 
-__device__ __forceinline__ float entry_logit(const ReportArgs& a, int64_t i) {
-    if (a.entry_type == PB_F32) return load_score<PB_F32>(a.entry_logits, i);
-    return a.entry_type == PB_BF16 ? load_score<PB_BF16>(a.entry_logits, i) : load_score<PB_F16>(a.entry_logits, i);
+// A teacher's value as it lies in memory, asked for but not waited for, and what it stands for.
+__device__ __forceinline__ uint32_t entry_bits(const ReportArgs& a, int64_t i) {
+    return a.entry_type == PB_F32 ? static_cast<const uint32_t*>(a.entry_logits)[i] : (uint32_t)static_cast<const uint16_t*>(a.entry_logits)[i];
+}
+
+__device__ __forceinline__ float entry_value(const ReportArgs& a, uint32_t bits) {
+    return a.entry_type == PB_F32 ? __uint_as_float(bits) : a.entry_type == PB_BF16 ? bf16_value(bits) : f16_value(bits);
 }
 
 __device__ __forceinline__ double inverse(double d) {
@@ -41,47 +46,67 @@ __device__ __forceinline__ double inverse(double d) {
     return __builtin_fma(__builtin_fma(-d, r, 1.0), r, r);
 }
 
-// One set's divergence and slopes, a lane of its team to an entry: z the student's logit (-inf where the entry does not
-// count), t the teacher's value, top and sum the rest's maximum and sum of exponentials. In double: a divergence is what
-// large terms leave where student and teacher are close, and rho is a difference.
-struct Divergence {
-    double kl;
-    float own;   // gradient of the lane's listed row
-    float rest;  // what the rest's exponentials are multiplied by
+// What a set's list says without the rows that are not listed: zmax the largest listed logit, E = sum of e = exp((z - zmax) / T),
+// mass = sum of part = exp(t), t the teacher's value (over T and less its largest, without tail), and lost = sum of
+// part (t - (z - zmax) / T). In double: a divergence is what large terms leave where student and teacher are close.
+struct ListSide {
+    float zmax;
+    double e, mass, lost;
 };
 
-__device__ __forceinline__ Divergence diverge(const ReportArgs& a, bool on, float z, float t, float rest_top, double rest_sum,
-                                              float weight, int bits) {
+// An entry's terms; z is -inf and t -inf where it does not count.
+struct ListTerms {
+    double e, part, lost;
+    __device__ __forceinline__ ListTerms(const ReportArgs& a, float z, double t, float zmax) {
+        const double x = ((double)z - (double)zmax) * a.inv_temp;
+        e = exp_near(x);
+        part = exp_near(t);
+        lost = part == 0.0 ? 0.0 : part * (t - x);
+    }
+};
+
+// The teacher's value as the terms take it, `most` the largest of the set's.
+__device__ __forceinline__ double entry_term(const ReportArgs& a, bool on, float t, float most) {
+    return !on ? -(double)kInf : a.tail ? (double)t : ((double)t - (most > -kInf ? (double)most : 0.0)) * a.inv_temp;
+}
+
+// What the rows' terms are multiplied by: a listed row's gradient is student e - teacher part, another's rest times its
+// exponential over the rest's maximum. And the set's divergence, where it is asked for.
+struct ListFactors {
+    float student, teacher, rest;
+    double kl;
+};
+
+// From the list's side and the rest's maximum and sum of exponentials; w is the set's weight times scale.
+template <bool KL>
+__device__ __forceinline__ ListFactors list_factors(const ReportArgs& a, const ListSide& l, float rest_top, double rest_sum, float w) {
     const bool has_rest = rest_sum != 0.0;
-    const double top = fmax(team_max((double)z, bits), has_rest ? (double)rest_top : (double)kLowest);
-    const double x = ((double)z - top) * a.inv_temp, e = exp_near(x);  // 0 where the entry does not count
-    const double rest_x = ((double)rest_top - top) * a.inv_temp, rest_e = has_rest ? exp_near(rest_x) : 0.0;
-    const double total = team_sum(e, bits) + (has_rest ? rest_e * rest_sum : 0.0);
-    double given = on ? (a.tail ? (double)t : (double)t * a.inv_temp) : -(double)kInf;
-    if (!a.tail) {
-        const double most = team_max(given, bits);
-        if (most > -(double)kInf) given -= most;
+    const double gap = has_rest ? ((double)rest_top - (double)l.zmax) * a.inv_temp : -(double)kInf, up = fmax(gap, 0.0);
+    const double less = exp_near(up == 0.0 ? gap : -up);  // of the two sides' exponentials one is 1
+    const double ours = up == 0.0 ? 1.0 : less, theirs = up == 0.0 ? less : 1.0;
+    const double total = l.e * ours + (has_rest ? rest_sum * theirs : 0.0);
+    if (l.mass == 0.0 || total == 0.0) return ListFactors{0.0f, 0.0f, 0.0f, 0.0};
+    const bool open = a.tail && has_rest && l.mass < 1.0;
+    const double wt = (double)w * (double)a.temp, per_total = inverse(total), rho = 1.0 - l.mass;
+    const double per = inverse(open ? rest_sum : l.mass);
+    ListFactors f{(float)(wt * ours * per_total), (float)(open ? wt : wt * per),
+                  has_rest ? (float)(wt * (theirs * per_total - (open ? rho * per : 0.0))) : 0.0f, 0.0};
+    if (w == 0.0f) f.student = f.teacher = f.rest = 0.0f;
+    if (KL) {  // one logarithm after the other: beside each other they take the registers of the rows
+        __builtin_amdgcn_sched_barrier(0);
+        const double log_total = log_near(total) + up;  // over the largest listed logit
+        __builtin_amdgcn_sched_barrier(0);
+        const double log_left = log_near(open ? rho : l.mass);
+        __builtin_amdgcn_sched_barrier(0);
+        f.kl = open ? l.lost + l.mass * log_total + rho * (log_left - (gap + log_near(rest_sum) - log_total))
+                    : l.lost * per - log_left + log_total;
     }
-    const double part = exp_near(given), mass = team_sum(part, bits);
-    const double lost = team_sum(part == 0.0 ? 0.0 : part * (given - x), bits);
-    const bool use = mass != 0.0 && total != 0.0;
-    const bool open = a.tail && has_rest && mass < 1.0;
-    const double rho = open ? 1.0 - mass : 0.0, per_mass = open ? 1.0 : inverse(mass);
-    const double log_total = log_near(total), log_left = log_near(open ? rho : mass);
-    Divergence d;
-    d.kl = lost * per_mass;
-    double away = 0.0;  // rho over the rest's sum
-    if (open) {
-        d.kl += mass * log_total + rho * (log_left - (rest_x + log_near(rest_sum) - log_total));
-        away = rho * inverse(rest_sum);
-    } else {
-        d.kl += log_total - log_left;
-    }
-    if (!use) d.kl = 0.0;
-    const double w = use && weight != 0.0f ? (double)weight * (double)a.temp : 0.0, per_total = inverse(total);
-    d.own = w == 0.0 || !on ? 0.0f : (float)(w * (e * per_total - part * per_mass));
-    d.rest = w == 0.0 || !has_rest ? 0.0f : (float)(w * (rest_e * per_total - away));
-    return d;
+    return f;
+}
+
+// A listed row's gradient. A set that counts for nothing has factors of 0, whatever its terms.
+__device__ __forceinline__ float listed_grad(float student, float teacher, float e, float part) {
+    return teacher == 0.0f ? 0.0f : student * e - teacher * part;
 }
 
 // A row's gradient is its exponential times (first + slope (z - m)), from a set's sums.
@@ -102,59 +127,240 @@ struct SoftTile {
         uint16_t head[kSetTileRows];    // the set that starts at a row, from 1; 0: none
         float first[kSetTileSets + 4];  // later: sum of exponentials, then what they are multiplied by
     };
-    union {
-        uint8_t slot[kSetTileRows];     // distillation: the entry that names a row, from 1; 0: none
-        float slope[kSetTileSets + 4];  // entropies: sum of exponentials times distances, then slopes
-    };
+    float slope[kSetTileSets + 4];  // entropies: sum of exponentials times distances, then slopes
+};
+
+struct ListTile : SoftTile {
+    float part[kSetTileRows];    // of listed rows: the teacher's terms
+    double mass[kSetTileSets];   // with tail: their sums
+    uint8_t slot[kSetTileRows];  // the entry that names a row, from 1; 0: none
+    float other[kSetTileSets + 4];  // slope and other: the list's largest logit and teacher's value, then factors
+};
+
+// How a wave takes the lists of a tile: a team of 1 << bits lanes to a set, as many as there are (64 sets at a time), each lane
+// entry after entry, kGroup at a time. So the exponentials of 20 lists of 8 take one group and a reduction over 2 lanes.
+constexpr int kGroup = 4;
+struct ListWalk {
+    int bits, rounds, groups;  // groups: of a round
+
+    __device__ __forceinline__ ListWalk(const ReportArgs& a, int num_sets) {
+        bits = num_sets > 32 ? 0 : num_sets > 1 ? __clz(num_sets - 1) - 26 : 6;
+        bits = min(bits, a.team_bits);
+        rounds = num_sets > kWave ? 2 : 1;
+        groups = (((a.top + (1 << bits) - 1) >> bits) + kGroup - 1) / kGroup;
+    }
+    // entry u of a lane's group
+    __device__ __forceinline__ int entry(int group, int u, int lane) const {
+        return ((group * kGroup + u) << bits) + (lane & ((1 << bits) - 1));
+    }
+};
+static_assert(kTileRounds == 2, "a lane has two sets of a tile");
+
+// A lane's entries of a group, counted over the rounds.
+struct EntryGroup {
+    int32_t c[kGroup];
+    uint32_t t[kGroup];
+
+    __device__ __forceinline__ void load(const ReportArgs& a, const ListWalk& walk, int num_sets, const int32_t (&set)[kTileRounds],
+                                         int index, int lane) {
+        const bool upper = index >= walk.groups;
+        const int team = lane >> walk.bits, group = upper ? index - walk.groups : index;
+        const int64_t list = (int64_t)__shfl(upper ? set[1] : set[0], team) * a.top;
+        const bool there = index < walk.rounds * walk.groups && (upper ? kWave : 0) + team < num_sets;
+#pragma unroll
+        for (int u = 0; u < kGroup; ++u) {
+            const int j = walk.entry(group, u, lane);
+            c[u] = -1;
+            t[u] = 0;
+            if (there && j < a.top) {
+                c[u] = a.entry_index[list + j];
+                t[u] = entry_bits(a, list + j);
+            }
+        }
+    }
 };
 
 template <bool DISTILL, int TYPE, bool MASK, bool BIAS>
 struct SoftTileIn {
     TileRows<TYPE, MASK, BIAS> rows;
     int32_t chosen[kTileRounds];
-    float coef[kTileRounds], h[kTileRounds];
+    float coef[kTileRounds], h[kTileRounds], weight[kTileRounds];
+    EntryGroup ahead[2];  // the first two groups
 
     __device__ __forceinline__ void load(const ReportArgs& a, const SetItem& im, int lane) {
         rows.load(a, im, lane);
-        if (DISTILL) return;
+        if (DISTILL) {
+            const ListWalk walk(a, rows.sets);
+            ahead[0].load(a, walk, rows.sets, rows.set, 0, lane);
+            ahead[1].load(a, walk, rows.sets, rows.set, 1, lane);
+        }
 #pragma unroll
         for (int r = 0; r < kTileRounds; ++r) {
             chosen[r] = -1;
             coef[r] = h[r] = 0.0f;
+            weight[r] = 1.0f;
             if (r * kWave + lane < rows.sets) {
                 const int64_t g = rows.set[r];
-                if (a.grad) {
+                if (DISTILL && a.weights) weight[r] = a.weights[g];
+                if (!DISTILL && a.grad) {
                     chosen[r] = a.chosen[g];
                     coef[r] = a.grad[g];
                 }
-                if (a.grad_entropy) h[r] = a.grad_entropy[g];
+                if (!DISTILL && a.grad_entropy) h[r] = a.grad_entropy[g];
             }
         }
     }
 };
 
-// The entries of a tile's lists, 64 at a time: which set's a lane has, and where that set lies.
-struct EntryLane {
-    int s, j, begin, size;
-    int64_t g;
-    bool there;
+// Where a round's set of the lane's team lies.
+struct RoundSet {
+    int s, begin, size, g, place;
+    bool first;  // the team's first lane, of a set that is there
 
-    template <class ROWS>
-    __device__ __forceinline__ EntryLane(const ReportArgs& a, const ROWS& in, int it, int lane) {
-        const int bits = a.team_bits, first = it << (6 - bits), r = first / kWave;
-        s = first + (lane >> bits);
-        j = lane & ((1 << bits) - 1);
-        const int from = s & (kWave - 1);
-        begin = __shfl(r ? in.begin[1] : in.begin[0], from);
-        size = __shfl(r ? in.end[1] : in.end[0], from) - begin;
-        g = __shfl(r ? in.set[1] : in.set[0], from);
-        there = s < in.sets && j < a.top;
+    template <class IN>
+    __device__ __forceinline__ RoundSet(const ListWalk& walk, const IN& in, int round, int lane) {
+        const int team = lane >> walk.bits;
+        s = round * kWave + team;
+        begin = __shfl(round ? in.begin[1] : in.begin[0], team);
+        size = __shfl(round ? in.end[1] : in.end[0], team) - begin;
+        g = __shfl(round ? in.set[1] : in.set[0], team);
+        place = lane & ((1 << walk.bits) - 1);
+        first = place == 0 && s < in.sets;
     }
 };
-static_assert(kTileRounds == 2, "a lane has two sets of a tile");
+
+// Marks the rows that a tile's lists name, and leaves each list's largest logit and teacher's value. With tail also the
+// teacher's terms, in double: 1 less their sum may be small. (All terms here or all in weigh_listed, where the rows'
+// exponentials lie in registers, would take one wave a SIMD.)
+template <bool MASK, class IN>
+__device__ __forceinline__ void mark_listed(const ReportArgs& a, const ListWalk& walk, IN& all, ListTile& sh, int lane) {
+    const auto& in = all.rows;
+#pragma unroll 1
+    for (int round = 0; round < walk.rounds; ++round) {
+        const RoundSet r(walk, in, round, lane);
+        float zmax = kLowest, tmax = -kInf;
+        double mass = 0.0;
+#pragma unroll 1
+        for (int group = 0; group < walk.groups; ++group) {
+            const int index = round * walk.groups + group;
+            EntryGroup e = index & 1 ? all.ahead[1] : all.ahead[0];
+            if (index > 1) e.load(a, walk, in.sets, in.set, index, lane);
+            bool on[kGroup];
+            float z[kGroup];
+#pragma unroll
+            for (int u = 0; u < kGroup; ++u) {
+                on[u] = e.c[u] >= 0 && e.c[u] < r.size;
+                const int row = on[u] ? r.begin + e.c[u] : 0;
+                z[u] = sh.x[row];
+                on[u] = on[u] && sh.slot[row] == 0;  // of entries that name one row the first counts
+            }
+            if (MASK) {
+#pragma unroll
+                for (int u = 0; u < kGroup; ++u)
+                    if (on[u] && z[u] == -kInf) on[u] = a.mask[a.off[r.g] + e.c[u]] != 0;
+            }
+#pragma unroll
+            for (int u = 0; u < kGroup; ++u)
+                if (on[u]) sh.slot[r.begin + e.c[u]] = (uint8_t)(walk.entry(group, u, lane) + 1);
+            wave_sync();
+            bool lost = false;
+#pragma unroll
+            for (int u = 0; u < kGroup; ++u) lost = lost || (on[u] && sh.slot[r.begin + e.c[u]] != walk.entry(group, u, lane) + 1);
+            if (__any(lost)) {  // entries of this group name one row: one after the other
+#pragma unroll
+                for (int u = 0; u < kGroup; ++u)
+                    if (on[u]) sh.slot[r.begin + e.c[u]] = 0;
+                wave_sync();
+#pragma unroll
+                for (int u = 0; u < kGroup; ++u) {
+                    if (on[u]) on[u] = sh.slot[r.begin + e.c[u]] == 0;
+                    const int named = on[u] ? e.c[u] : -1;
+                    for (int d = 1; d < 1 << walk.bits; ++d) {
+                        const int before = __shfl(named, lane >= d ? lane - d : lane);
+                        if (d <= r.place && before == named) on[u] = false;
+                    }
+                    if (on[u]) sh.slot[r.begin + e.c[u]] = (uint8_t)(walk.entry(group, u, lane) + 1);
+                    wave_sync();
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kGroup; ++u) {
+                zmax = on[u] ? fmaxf(zmax, z[u]) : zmax;
+                tmax = on[u] ? fmaxf(tmax, entry_value(a, e.t[u])) : tmax;
+            }
+            if (a.tail) {
+#pragma unroll
+                for (int u = 0; u < kGroup; ++u) {
+                    const double part = on[u] ? exp_near((double)entry_value(a, e.t[u])) : 0.0;
+                    mass += part;
+                    if (on[u]) sh.part[r.begin + e.c[u]] = (float)part;
+                }
+            }
+        }
+        zmax = (float)team_max((double)zmax, walk.bits);
+        tmax = (float)team_max((double)tmax, walk.bits);
+        if (a.tail) mass = team_sum(mass, walk.bits);
+        if (r.first) {
+            sh.slope[r.s] = zmax;
+            sh.other[r.s] = tmax;
+            sh.mass[r.s] = mass;
+        }
+    }
+}
+
+// The terms of the listed rows, and the sets' factors and divergences.
+template <class IN>
+__device__ __forceinline__ void weigh_listed(const ReportArgs& a, const ListWalk& walk, IN& all, ListTile& sh, int lane,
+                                             double (&tally)[3]) {
+    const auto& in = all.rows;
+    const Heat heat{a.heat_hi, a.heat_lo, a.heat_low};
+#pragma unroll 1
+    for (int round = 0; round < walk.rounds; ++round) {
+        const RoundSet r(walk, in, round, lane);
+        const float w = __shfl(round ? all.weight[1] : all.weight[0], lane >> walk.bits) * a.scale, tmax = sh.other[r.s];
+        const float most = tmax > -kInf ? tmax : 0.0f;
+        ListSide l{sh.slope[r.s], 0.0, 0.0, 0.0};
+#pragma unroll 1
+        for (int group = 0; group < walk.groups; ++group) {
+            const int index = round * walk.groups + group;
+            EntryGroup e = index & 1 ? all.ahead[1] : all.ahead[0];
+            if (index > 1) e.load(a, walk, in.sets, in.set, index, lane);
+#pragma unroll
+            for (int u = 0; u < kGroup; ++u) {
+                bool on = e.c[u] >= 0 && e.c[u] < r.size;
+                const int row = on ? r.begin + e.c[u] : 0;
+                on = on && sh.slot[row] == walk.entry(group, u, lane) + 1;
+                const float z = on ? sh.x[row] : -kInf, t = on ? entry_value(a, e.t[u]) : -kInf;
+                const float student = heat_exp<true>(z - l.zmax, heat);
+                const float part = !a.tail ? heat_exp<true>(t - most, heat) : on ? sh.part[row] : 0.0f;
+                if (on) {
+                    sh.x[row] = student;
+                    sh.part[row] = part;
+                }
+                const double x = ((double)z - (double)l.zmax) * a.inv_temp, given = a.tail ? (double)t : ((double)t - (double)most) * a.inv_temp;
+                l.e += (double)student;
+                l.mass += (double)part;
+                l.lost += part == 0.0f ? 0.0 : (double)part * (given - x);
+            }
+        }
+        l.e = team_sum(l.e, walk.bits);
+        l.mass = a.tail ? sh.mass[min(r.s, kSetTileSets - 1)] : team_sum(l.mass, walk.bits);
+        l.lost = team_sum(l.lost, walk.bits);
+        const ListFactors f = list_factors<true>(a, l, r.size > 0 ? sh.top[r.s] : kLowest, r.size > 0 ? (double)sh.first[r.s] : 0.0, w);
+        wave_sync();
+        if (r.first) {
+            sh.first[r.s] = f.rest;
+            sh.slope[r.s] = f.student;
+            sh.other[r.s] = f.teacher;
+            a.kl[r.g] = (float)f.kl;
+            if (w != 0.0f) tally[0] += (double)w * (double)a.temp * (double)a.temp * f.kl;
+        }
+    }
+}
 
 template <bool DISTILL, int TYPE, bool MASK, bool BIAS>
-__device__ __forceinline__ void soft_tile(const ReportArgs& a, SoftTileIn<DISTILL, TYPE, MASK, BIAS>& all, SoftTile& sh,
+__device__ __forceinline__ void soft_tile(const ReportArgs& a, SoftTileIn<DISTILL, TYPE, MASK, BIAS>& all,
+                                          std::conditional_t<DISTILL, ListTile, SoftTile>& sh,
                                           const BiasShared* bias, TableSum& table, double (&tally)[3]) {
     const TileRows<TYPE, MASK, BIAS>& in = all.rows;
     const int lane = (int)threadIdx.x & (kWave - 1), i0 = kRun * lane;
@@ -169,7 +375,7 @@ __device__ __forceinline__ void soft_tile(const ReportArgs& a, SoftTileIn<DISTIL
     if (sp.hi > 0) in.raw.logits(a, bias, sp, 0, x, off, buckets);
     wave_sync();  // the last tile's values have been read
     *reinterpret_cast<uint4*>(&sh.head[i0]) = make_uint4(0, 0, 0, 0);
-    if (DISTILL) *reinterpret_cast<uint2*>(&sh.slot[i0]) = make_uint2(0, 0);
+    if constexpr (DISTILL) *reinterpret_cast<uint2*>(&sh.slot[i0]) = make_uint2(0, 0);
     write_run(&sh.x[i0], x);
     wave_sync();
 #pragma unroll
@@ -186,29 +392,11 @@ __device__ __forceinline__ void soft_tile(const ReportArgs& a, SoftTileIn<DISTIL
             }
         }
     }
-    const int rounds = DISTILL ? ((in.sets << a.team_bits) + kWave - 1) / kWave : 0;
-    if (DISTILL) {
-        for (int it = 0; it < rounds; ++it) {
-            const EntryLane l(a, in, it, lane);
-            const int32_t c = l.there ? a.entry_index[l.g * a.top + l.j] : -1;
-            bool on = c >= 0 && c < l.size;
-            if (MASK && on && sh.x[l.begin + c] == -kInf) on = a.mask[a.off[l.g] + c] != 0;
-            if (on) sh.slot[l.begin + c] = (uint8_t)(l.j + 1);
-            wave_sync();
-            if (__any(on && sh.slot[l.begin + c] != l.j + 1)) {  // rows named twice: the first entry counts
-                const int named = on ? c : -1;
-                for (int d = 1; d < 1 << a.team_bits; ++d) {
-                    const int before = __shfl(named, lane >= d ? lane - d : lane);
-                    if (d <= l.j && before == named) on = false;
-                }
-                wave_sync();
-                if (on) sh.slot[l.begin + c] = (uint8_t)(l.j + 1);
-            }
-        }
-    }
+    const ListWalk walk(a, DISTILL ? in.sets : 1);
+    if constexpr (DISTILL) mark_listed<MASK>(a, walk, all, sh, lane);
     wave_sync();
     uint2 slots = make_uint2(0, 0);
-    if (DISTILL) {
+    if constexpr (DISTILL) {
         slots = *reinterpret_cast<const uint2*>(&sh.slot[i0]);
         if (slots.x | slots.y) {
 #pragma unroll
@@ -260,30 +448,21 @@ __device__ __forceinline__ void soft_tile(const ReportArgs& a, SoftTileIn<DISTIL
         }
         wave_sync();
     }
-    if (DISTILL) {
-        for (int it = 0; it < rounds; ++it) {
-            const EntryLane l(a, in, it, lane);
-            const int32_t c = l.there ? a.entry_index[l.g * a.top + l.j] : -1;
-            const bool on = c >= 0 && c < l.size && sh.slot[l.begin + c] == l.j + 1;
-            const float t = on ? entry_logit(a, l.g * a.top + l.j) : 0.0f;
-            const float w = l.there ? (a.weights ? a.weights[l.g] : 1.0f) * a.scale : 0.0f;
-            const Divergence r = diverge(a, on, on ? sh.x[l.begin + c] : -kInf, t, sh.top[l.s], l.size > 0 ? (double)sh.first[l.s] : 0.0,
-                                         w, a.team_bits);
-            wave_sync();
-            if (on) sh.x[l.begin + c] = r.own;
-            if (l.there && l.j == 0) {
-                sh.first[l.s] = r.rest;
-                a.kl[l.g] = (float)r.kl;
-                if (w != 0.0f) tally[0] += (double)w * (double)a.temp * (double)a.temp * r.kl;
-            }
-        }
+    if constexpr (DISTILL) {
+        weigh_listed(a, walk, all, sh, lane, tally);
         wave_sync();
-        float own[kRun];
-        read_run(&sh.x[i0], own);
+        float e[kRun], part[kRun];
+        const bool any = (slots.x | slots.y) != 0;
+        if (any) {
+            read_run(&sh.x[i0], e);
+            read_run(&sh.part[i0], part);
+        }
 #pragma unroll
         for (int k = 0; k < kRun; ++k) {
-            const float f = sh.first[sets.id[k] - 1];
-            v[k] = ((k < 4 ? slots.x : slots.y) >> (8 * (k & 3)) & 0xffu) ? own[k] : f == 0.0f ? 0.0f : f * v[k];
+            const int s = sets.id[k] - 1;
+            const float f = sh.first[s];
+            v[k] = f == 0.0f ? 0.0f : f * v[k];
+            if (any && ((k < 4 ? slots.x : slots.y) >> (8 * (k & 3)) & 0xffu)) v[k] = listed_grad(sh.slope[s], sh.other[s], e[k], part[k]);
         }
     } else {
         Slopes f[kTileRounds];
@@ -325,7 +504,7 @@ __device__ __forceinline__ void soft_tile(const ReportArgs& a, SoftTileIn<DISTIL
 
 template <bool DISTILL, int TYPE, bool MASK, bool BIAS>
 __global__ __launch_bounds__(kBlock, DISTILL ? 3 : 4) void soft_tile_kernel(ReportArgs a) {
-    __shared__ SoftTile tiles[kWaves];
+    __shared__ std::conditional_t<DISTILL, ListTile, SoftTile> tiles[kWaves];
     __shared__ BiasShared bias;
     __shared__ unsigned long long bins[BIAS ? kWaves : 1][kBins];
     __shared__ int shifts[BIAS ? kWaves : 1][kBins];
@@ -353,13 +532,14 @@ __global__ __launch_bounds__(kBlock, DISTILL ? 3 : 4) void soft_tile_kernel(Repo
 }
 
 // ------------------------------------------------------------------------------------ longer sets
-// What a group of lanes (a wave, or a workgroup) shares of its set.
-template <int THREADS, int RUNS>
+// What a group of lanes (a wave, or a workgroup) shares of its set. ROWS: 0 without lists.
+template <int THREADS, int ROWS>
 struct SoftGroup {
     static constexpr int kGroupWaves = THREADS / kWave;
-    uint8_t slot[THREADS * RUNS * kRun];  // the entry that names a row, from 1; 0: none
-    float own[kMaxTop];
-    float factor;
+    uint8_t slot[ROWS ? ROWS : 8];  // the entry that names a row, from 1; 0: none
+    float e[kMaxTop], part[kMaxTop];
+    ListSide list;
+    float weight;
     float top[kGroupWaves];
     double sum[kGroupWaves], along[kGroupWaves];
 };
@@ -373,8 +553,8 @@ __device__ __forceinline__ void group_sync() {
 }
 
 // A set's sums from those of the lanes (each wave's relative to its own maximum), the same in every lane.
-template <bool ALONG, int THREADS, int RUNS>
-__device__ __forceinline__ SoftSums join_waves(const ReportArgs& a, SoftSums t, SoftGroup<THREADS, RUNS>& sh) {
+template <bool ALONG, int THREADS, int ROWS>
+__device__ __forceinline__ SoftSums join_waves(const ReportArgs& a, SoftSums t, SoftGroup<THREADS, ROWS>& sh) {
     if (THREADS == kWave) return t;
     const int tid = (int)threadIdx.x;
     if ((tid & (kWave - 1)) == 0) {
@@ -394,8 +574,8 @@ __device__ __forceinline__ SoftSums join_waves(const ReportArgs& a, SoftSums t, 
 }
 
 // A set's sums from those of its parts.
-template <bool ALONG, int THREADS, int RUNS>
-__device__ __forceinline__ SoftSums join_set(const ReportArgs& a, const SoftSums* parts, int n, SoftGroup<THREADS, RUNS>& sh) {
+template <bool ALONG, int THREADS, int ROWS>
+__device__ __forceinline__ SoftSums join_set(const ReportArgs& a, const SoftSums* parts, int n, SoftGroup<THREADS, ROWS>& sh) {
     SoftSums t{kLowest, 0.0, 0.0};
     for (int j = (int)threadIdx.x; j < n; j += THREADS) t.top = max2(t.top, parts[j].top);
     t.top = wave_max(t.top);
@@ -411,51 +591,80 @@ __device__ __forceinline__ SoftSums join_set(const ReportArgs& a, const SoftSums
 
 enum SoftPhase { kWholeSet, kPartSums, kPartGrads };
 
+template <bool DISTILL, int THREADS, int RUNS>
+constexpr int kListRows = DISTILL ? THREADS * RUNS * kRun : 0;
+
 // One set of more than kSetShort rows, or a part of one, by a group of THREADS lanes with RUNS runs each, in registers
-// from the load to the store.
+// from the load to the store. The first wave takes the list beside its rows; what the rest's sums add is little, and every
+// lane forms it for itself, so that a set waits for its slots and for its sums alone.
 template <bool DISTILL, int TYPE, bool MASK, bool BIAS, int THREADS, int RUNS, SoftPhase PHASE>
-__device__ __forceinline__ void soft_pass(const ReportArgs& a, const SetItem& im, int32_t index, SoftGroup<THREADS, RUNS>& sh,
-                                          const BiasShared* bias, TableSum& table, double (&tally)[3]) {
+__device__ __forceinline__ void soft_pass(const ReportArgs& a, const SetItem& im, int32_t index,
+                                          SoftGroup<THREADS, kListRows<DISTILL, THREADS, RUNS>>& sh, const BiasShared* bias,
+                                          TableSum& table, double (&tally)[3]) {
     constexpr bool EXACT = kExact<TYPE, BIAS>;
     const int tid = (int)threadIdx.x & (THREADS - 1), lane = tid & (kWave - 1);
     const int wave0 = __builtin_amdgcn_readfirstlane(tid & ~(kWave - 1));  // the wave's first thread
     const Heat heat{a.heat_hi, a.heat_lo, a.heat_low};
     const Span sp = span_of(a, im);
-    const int64_t g = im.set0, r0 = a.off[g], size = a.off[g + 1] - r0;
+    const int64_t g = im.set0;
     int32_t c = -1;
-    if (DISTILL && wave0 == 0 && lane < a.top) c = a.entry_index[g * a.top + lane];
+    uint32_t bits = 0;
+    float w = 1.0f;
+    if (DISTILL && wave0 == 0 && lane < a.top) {
+        c = a.entry_index[g * a.top + lane];
+        if (PHASE != kPartSums) bits = entry_bits(a, g * a.top + lane);
+    }
+    if (DISTILL && wave0 == 0 && PHASE != kPartSums && a.weights) w = a.weights[g];
+    const int64_t r0 = a.off[g], size = a.off[g + 1] - r0;
     RawRun<TYPE, MASK, BIAS> raw[RUNS];
 #pragma unroll
     for (int j = 0; j < RUNS; ++j) {
         const int i = kRun * (j * THREADS + tid);
         if (kRun * (j * THREADS + wave0) < sp.hi && i < sp.hi) raw[j].load(a, sp, i);
     }
-    bool on = false;
-    float z = -kInf, t = 0.0f, w = 0.0f;
     if (DISTILL) {
-        group_sync<THREADS>();  // the last set's slots have been read
 #pragma unroll
         for (int j = 0; j < RUNS; ++j) *reinterpret_cast<uint2*>(&sh.slot[kRun * (j * THREADS + tid)]) = make_uint2(0, 0);
+        bool on = c >= 0 && c < size;
+        float z = -kInf;
         if (wave0 == 0) {
-            on = c >= 0 && c < size;
-            if (PHASE != kPartSums) {
-                if (lane < a.top) t = entry_logit(a, g * a.top + lane);
-                w = (a.weights ? a.weights[g] : 1.0f) * a.scale;
-            }
             if (MASK && on) on = a.mask[r0 + c] != 0;
-            if (PHASE != kPartSums) {
-                if (on) z = one_logit<TYPE, BIAS>(a, bias, r0 + c);
-                for (int j = 0; j + 1 < a.top; ++j) {  // rows named twice: the first entry counts
+            if (PHASE != kPartSums && on) z = one_logit<TYPE, BIAS>(a, bias, r0 + c);
+        }
+        group_sync<THREADS>();
+        if (wave0 == 0) {
+            const int64_t row = r0 + c - sp.q0;
+            const bool here = on && row >= sp.lo && row < sp.hi;
+            if (here) sh.slot[row] = (uint8_t)(lane + 1);
+            wave_sync();
+            // rows named twice: the first entry counts. Of other parts' rows the slots do not tell.
+            if (PHASE != kPartSums && (PHASE == kPartGrads || __any(here && sh.slot[row] != lane + 1))) {
+                for (int j = 0; j + 1 < a.top; ++j) {
                     const int before = __builtin_amdgcn_readlane(c, j);
                     if (j < lane && before == c) on = false;
                 }
-                if (!on) z = -kInf;
+                wave_sync();
+                if (here && on) sh.slot[row] = (uint8_t)(lane + 1);
             }
         }
         group_sync<THREADS>();
-        const int64_t row = r0 + c - sp.q0;
-        if (wave0 == 0 && on && row >= sp.lo && row < sp.hi) sh.slot[row] = (uint8_t)(lane + 1);
-        group_sync<THREADS>();
+        if (wave0 == 0 && PHASE != kPartSums) {
+            if (!on) z = -kInf;
+            const float t = entry_value(a, bits);
+            ListSide l;
+            l.zmax = (float)team_max((double)(on ? fmaxf(kLowest, z) : kLowest), 6);
+            const float tmax = (float)team_max(on ? (double)t : -(double)kInf, 6);
+            const ListTerms terms(a, z, entry_term(a, on, t, tmax), l.zmax);
+            l.e = team_sum(terms.e, 6);
+            l.mass = team_sum(terms.part, 6);
+            l.lost = team_sum(terms.lost, 6);
+            sh.e[lane] = (float)terms.e;
+            sh.part[lane] = (float)terms.part;
+            if (lane == 0) {
+                sh.list = l;
+                sh.weight = w * a.scale;
+            }
+        }
     }
     float v[RUNS][kRun];
     uint32_t off[RUNS];
@@ -497,9 +706,10 @@ __device__ __forceinline__ void soft_pass(const ReportArgs& a, const SetItem& im
         if (j < live)
 #pragma unroll
             for (int k = 0; k < kRun; ++k) {
+                if (!DISTILL && PHASE == kPartGrads) continue;
                 const float d = __builtin_elementwise_maximum(v[j][k] - own.top, heat.low), e = heat_exp<EXACT>(d, heat);
                 if (PHASE != kPartGrads) sum += e;
-                if (!DISTILL && PHASE != kPartGrads) along = __builtin_fmaf(e, d, along);
+                if (!DISTILL) along = __builtin_fmaf(e, d, along);
                 if (DISTILL && PHASE != kPartSums) v[j][k] = e;
             }
     if (PHASE != kPartGrads) {
@@ -514,21 +724,12 @@ __device__ __forceinline__ void soft_pass(const ReportArgs& a, const SetItem& im
     // what the wave's exponentials are multiplied by: they are relative to its own maximum
     const double gap = (double)own.top - (double)sums.top;
     float first, slope = 0.0f, extra = 0.0f;
+    ListFactors f{0.0f, 0.0f, 0.0f, 0.0};
     int at = -kRun;  // the chosen row, as the span counts
     if (DISTILL) {
-        if (wave0 == 0) {
-            const Divergence r = diverge(a, on, z, t, sums.top, sums.sum, w, 6);
-            sh.own[lane] = r.own;
-            if (lane == 0) {
-                sh.factor = r.rest;
-                if (im.part == 0) {
-                    a.kl[g] = (float)r.kl;
-                    if (w != 0.0f) tally[0] += (double)w * (double)a.temp * (double)a.temp * r.kl;
-                }
-            }
-        }
-        group_sync<THREADS>();
-        first = sh.factor == 0.0f ? 0.0f : (float)((double)sh.factor * exp_near(gap * a.inv_temp));
+        if (THREADS == kWave) wave_sync();
+        f = list_factors<false>(a, sh.list, sums.top, sums.sum, sh.weight);
+        first = f.rest == 0.0f ? 0.0f : (float)((double)f.rest * exp_near(gap * a.inv_temp));
     } else {
         float coef = 0.0f;
         if (a.grad && sums.sum != 0.0) {
@@ -542,10 +743,10 @@ __device__ __forceinline__ void soft_pass(const ReportArgs& a, const SetItem& im
                 if (row >= sp.lo && row < sp.hi) at = (int)row;
             }
         }
-        const Slopes f = slopes_of(a, sums.sum, sums.along, coef, a.grad_entropy ? a.grad_entropy[g] : 0.0f);
+        const Slopes t = slopes_of(a, sums.sum, sums.along, coef, a.grad_entropy ? a.grad_entropy[g] : 0.0f);
         const double near = exp_near(gap * a.inv_temp);
-        slope = (float)((double)f.slope * near);
-        first = near == 0.0 ? 0.0f : (float)(near * ((double)f.first + (double)f.slope * gap));
+        slope = (float)((double)t.slope * near);
+        first = near == 0.0 ? 0.0f : (float)(near * ((double)t.first + (double)t.slope * gap));
     }
 #pragma unroll
     for (int j = 0; j < RUNS; ++j) {
@@ -566,7 +767,7 @@ __device__ __forceinline__ void soft_pass(const ReportArgs& a, const SetItem& im
 #pragma unroll
                     for (int k = 0; k < kRun; ++k) {
                         const uint32_t b = (k < 4 ? s.x : s.y) >> (8 * (k & 3)) & 0xffu;
-                        if (b) v[j][k] = sh.own[b - 1];
+                        if (b) v[j][k] = listed_grad(f.student, f.teacher, sh.e[b - 1], sh.part[b - 1]);
                     }
                 }
             }
@@ -583,13 +784,18 @@ __device__ __forceinline__ void soft_pass(const ReportArgs& a, const SetItem& im
             if (BIAS) table.add<false>(v[j], buckets[j]);
         }
     }
-    if (THREADS != kWave) __syncthreads();  // the group's sums have been read
+    if (DISTILL && tid == 0 && im.part == 0) {
+        const double kl = list_factors<true>(a, sh.list, sums.top, sums.sum, sh.weight).kl;
+        a.kl[g] = (float)kl;
+        if (sh.weight != 0.0f) tally[0] += (double)sh.weight * (double)a.temp * (double)a.temp * kl;
+    }
+    group_sync<THREADS>();  // the group's sums and slots have been read
 }
 
-// The sums of the sets' parts.
+// The sums of the sets' parts: all from `first` on, or those in `list`.
 template <bool DISTILL, int TYPE, bool MASK, bool BIAS>
 __global__ __launch_bounds__(kBlock) void soft_part_kernel(ReportArgs a, int first, const int32_t* __restrict__ list) {
-    __shared__ SoftGroup<kBlock, kWideRuns> sh;
+    __shared__ SoftGroup<kBlock, kListRows<DISTILL, kBlock, kWideRuns>> sh;
     __shared__ BiasShared bias;
     const int it = list ? list[blockIdx.x] : first + (int)blockIdx.x;
     if (BIAS) stage_bias(a, bias);
@@ -604,8 +810,8 @@ template <bool DISTILL, int TYPE, bool MASK, bool BIAS>
 __global__ __launch_bounds__(kBlock) void soft_wide_kernel(ReportArgs a, int mid_blocks, int num_parts, const int32_t* __restrict__ list,
                                                            int first_block) {
     __shared__ union {
-        SoftGroup<kWave, kWideRuns> mid[kWaves];
-        SoftGroup<kBlock, kWideRuns> whole;
+        SoftGroup<kWave, kListRows<DISTILL, kWave, kWideRuns>> mid[kWaves];
+        SoftGroup<kBlock, kListRows<DISTILL, kBlock, kWideRuns>> whole;
     } sh;
     __shared__ BiasShared bias;
     __shared__ unsigned long long bins[BIAS ? kWaves : 1][kBins];
@@ -638,32 +844,69 @@ __global__ __launch_bounds__(kBlock) void soft_wide_kernel(ReportArgs a, int mid
     leave_sums<DISTILL ? 1 : 0, BIAS>(a, first_block + (int)blockIdx.x, tally, table, bins, bad, shd);
 }
 
+// Sets of up to THREADS * 64 rows, a workgroup each: rows that would be read twice in parts are read once.
+template <bool DISTILL, int TYPE, bool MASK, int THREADS>
+__global__ __launch_bounds__(THREADS, 4) void soft_big_kernel(ReportArgs a, const SetItem* __restrict__ items, int first_block) {
+    constexpr int kBigRuns = kSetBig / (1024 * kRun);
+    __shared__ SoftGroup<THREADS, kListRows<DISTILL, THREADS, kBigRuns>> sh;
+    TableSum table;
+    double tally[3] = {0.0, 0.0, 0.0};
+    soft_pass<DISTILL, TYPE, MASK, false, THREADS, kBigRuns, kWholeSet>(a, items[blockIdx.x], 0, sh, nullptr, table, tally);
+    if (DISTILL && threadIdx.x == 0) {
+        if (a.blocks == 1)
+            a.stats[0] = (float)tally[0];
+        else
+            a.sums[first_block + (int)blockIdx.x] = tally[0];
+    }
+}
+
+// From how many sets on a workgroup to each of them beats parts.
+constexpr int kBigSets = 1024;
+
+bool takes_big(const SetLayout& s, bool bias) { return !bias && s.num_big >= kBigSets; }
+
 int tile_blocks(const SetLayout& s) { return std::min((s.num_tiles + kWaves - 1) / kWaves, kChoiceGrid); }
 
 int mid_blocks(const SetLayout& s) { return std::min((s.num_mid + kWaves - 1) / kWaves, kChoiceGrid); }
 
-int group_blocks(const SetLayout& s) { return std::min(s.num_wide, kChoiceGrid); }
+int num_parts(const SetLayout& s, bool bias) { return takes_big(s, bias) ? s.num_giant : s.num_wide - s.num_whole; }
 
-int num_parts(const SetLayout& s) { return s.num_wide - s.num_whole; }
+int group_blocks(const SetLayout& s, bool bias) { return std::min(s.num_whole + num_parts(s, bias), kChoiceGrid); }
 
-int soft_blocks(const SetLayout& s) { return tile_blocks(s) + mid_blocks(s) + group_blocks(s); }
+int soft_blocks(const SetLayout& s, bool bias) {
+    return tile_blocks(s) + mid_blocks(s) + group_blocks(s, bias) + (takes_big(s, bias) ? s.num_big : 0);
+}
 
 template <bool DISTILL, int TYPE, bool MASK, bool BIAS>
 hipError_t launch_as(const SetLayout& s, const ReportArgs& a, hipStream_t stream) {
     hipError_t e = hipSuccess;
-    const int parts = num_parts(s), first = s.num_mid + s.num_whole;
+    const bool big = takes_big(s, BIAS);
+    const int parts = num_parts(s, BIAS), first = s.num_mid + s.num_whole;
+    const int32_t* list = big ? s.giant : nullptr;
     if (parts > 0) {
-        hipLaunchKernelGGL((soft_part_kernel<DISTILL, TYPE, MASK, BIAS>), dim3(parts), dim3(kBlock), 0, stream, a, first, nullptr);
+        hipLaunchKernelGGL((soft_part_kernel<DISTILL, TYPE, MASK, BIAS>), dim3(parts), dim3(kBlock), 0, stream, a, first, list);
         if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
+    if constexpr (!BIAS) {
+        const int rest = s.num_big - s.num_half, first_block = a.blocks - s.num_big;
+        if (big && rest > 0) {
+            hipLaunchKernelGGL((soft_big_kernel<DISTILL, TYPE, MASK, 1024>), dim3(rest), dim3(1024), 0, stream, a, s.big + s.num_half,
+                               first_block + s.num_half);
+            if ((e = hipGetLastError()) != hipSuccess) return e;
+        }
+        if (big && s.num_half > 0) {
+            hipLaunchKernelGGL((soft_big_kernel<DISTILL, TYPE, MASK, 512>), dim3(s.num_half), dim3(512), 0, stream, a, s.big, first_block);
+            if ((e = hipGetLastError()) != hipSuccess) return e;
+        }
     }
     if (s.num_tiles > 0) {
         hipLaunchKernelGGL((soft_tile_kernel<DISTILL, TYPE, MASK, BIAS>), dim3(tile_blocks(s)), dim3(kBlock), 0, stream, a);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
-    const int wide = mid_blocks(s) + group_blocks(s);
+    const int wide = mid_blocks(s) + group_blocks(s, BIAS);
     if (wide > 0) {
         hipLaunchKernelGGL((soft_wide_kernel<DISTILL, TYPE, MASK, BIAS>), dim3(wide), dim3(kBlock), 0, stream, a, mid_blocks(s), parts,
-                           nullptr, tile_blocks(s));
+                           list, tile_blocks(s));
         e = hipGetLastError();
     }
     return e;

@@ -274,6 +274,19 @@ def test_distill_layouts(hip, edges, k, tail):
     check_distill(d, k, tail, 1.5 if k == 2 else 1.0, k, weighted=k != 3)
 
 
+BIG = list(np.random.RandomState(40).randint(8193, 8600, 262)) + [40_000, 3, 32_768, 70_001, 65_500, 0, 32_769, 900, 66_000]
+
+
+@pytest.mark.parametrize("dtype,masked,biased", [("f32", False, False), ("bf16", True, False), ("f16", False, True)])
+def test_many_long_sets(hip, dtype, masked, biased):
+    """So many long sets that each has a workgroup, longer ones in parts beside them; with a bias all are in parts."""
+    d = make(BIG, dtype, masked, biased, seed=41)
+    check_backward(d, 1.0 if masked else 1.3)
+    check_distill(d, 24, not masked, 1.0, 42)
+    if not biased:
+        check_report(d, 24, 1.0)
+
+
 def test_distill_many_sets(hip):
     """Thousands of lists, a few of their sets empty or without candidates."""
     d = make(EDGES["many"], "f32", True, True, seed=9)
