@@ -54,7 +54,8 @@ struct Layout {
     std::vector<SetItem> tiles, mid, whole, parts, half, big;
     std::vector<pb::TileSegment> segments;
     std::vector<int32_t> split;  // the first part of each split set, within `parts`
-    std::vector<int32_t> giant;  // the parts of sets that are not in `half` or `big`, too
+    std::vector<int32_t> giant;  // the parts of sets that are not in `half` or `big`, too, and the first of each
+    std::vector<int32_t> giant_split;
 };
 
 // The tile that is being filled.
@@ -146,6 +147,7 @@ void lay_out(const int64_t* off, int64_t num_sets, bool segments, Layout& out) {
             out.split.push_back((int32_t)out.parts.size());
             for (im.part = 0; im.part < im.parts; ++im.part) {
                 if (span > pb::kSetBig) out.giant.push_back((int32_t)out.parts.size());
+                if (span > pb::kSetBig && im.part == 0) out.giant_split.push_back((int32_t)out.parts.size());
                 im.row0 = off[g] + im.part * each;
                 im.rows = (int32_t)std::min(each, off[g + 1] - im.row0);
                 out.parts.push_back(im);
@@ -177,9 +179,11 @@ int sets_create(const int64_t* off, int64_t num_sets, bool segments, pb_sets** o
     items.insert(items.end(), lay.big.begin(), lay.big.end());
     for (int32_t& first : lay.split) first += (int32_t)(mid + whole);
     for (int32_t& part : lay.giant) part += (int32_t)(mid + whole);
-    std::vector<int32_t>& split = lay.split;  // and `giant` behind it
+    for (int32_t& part : lay.giant_split) part += (int32_t)(mid + whole);
+    std::vector<int32_t>& split = lay.split;  // and `giant`, `giant_split` behind it
     const size_t num_split = split.size();
     split.insert(split.end(), lay.giant.begin(), lay.giant.end());
+    split.insert(split.end(), lay.giant_split.begin(), lay.giant_split.end());
     const size_t b_off = round256(sizeof(int64_t) * (size_t)(num_sets + 1));
     const size_t b_items = round256(sizeof(SetItem) * items.size());
     const size_t b_split = round256(sizeof(int32_t) * split.size());
@@ -213,6 +217,7 @@ int sets_create(const int64_t* off, int64_t num_sets, bool segments, pb_sets** o
     h->s.num_half = (int32_t)half;
     h->s.giant = h->s.split + num_split;
     h->s.num_giant = (int32_t)lay.giant.size();
+    h->s.giant_split = h->s.giant + lay.giant.size();
     h->s.num_sets = num_sets;
     h->s.rows = off[num_sets];
     for (int64_t g = 0; g < num_sets; ++g) h->largest = std::max(h->largest, off[g + 1] - off[g]);

@@ -538,6 +538,7 @@ struct SetLayout {
     const int32_t* split;  // [num_split], indices of wide items
     const SetItem* big;    // [num_big], the first num_half of at most kSetHalfBig rows
     const int32_t* giant;  // [num_giant], indices of wide items
+    const int32_t* giant_split;  // [num_split - num_big], the first of each set's
     int32_t num_big;
     int32_t num_half;
     int32_t num_giant;

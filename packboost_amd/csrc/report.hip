@@ -11,9 +11,9 @@
 // a short set counts the rows that rank above it. Of longer sets a bound is found first that at least as many rows reach as
 // are listed, from the maxima of the lanes; the few rows that reach it are gathered and ranked by counting.
 #include <algorithm>
+#include <utility>
 
-#include "choice_rows.h"
-#include "report.h"
+#include "soft_rows.h"
 
 namespace pb {
 namespace {
@@ -22,6 +22,9 @@ constexpr int kCountRows = 64;    // rows of a tile's set whose rows count what 
 constexpr int kWaveList = 256;    // rows that reach the bound: room for a wave's
 constexpr int kGroupList = 512;   // and a workgroup's
 constexpr int kJoinList = kMaxTop * kMaxTop;
+constexpr int kBigSets = 1024;     // from so many long sets on a workgroup to each beats parts,
+constexpr int kFewSets = 8;        // and up to so many
+constexpr int kBoundParts = 1024;  // parts whose bound is found by counting
 
 // Orders logits as whole numbers: larger first, -0 as 0, NaN above all; 0 for what is not ranked.
 __device__ __forceinline__ uint32_t rank_of(float z) {
@@ -32,11 +35,7 @@ __device__ __forceinline__ uint32_t rank_of(float z) {
 
 __device__ __forceinline__ float rank_value(uint32_t r) { return __uint_as_float(r & 0x80000000u ? r ^ 0x80000000u : ~r); }
 
-// A row of a list: its rank, then smaller indices first. 0 for none.
-__device__ __forceinline__ unsigned long long key_of(float z, uint32_t index) {
-    return (unsigned long long)rank_of(z) << 32 | (uint32_t)~index;
-}
-
+// A row of a list is held as a key: its rank, 32 bits up, and the complement of its index. 0 for none.
 __device__ __forceinline__ float list_log_prob(const ReportArgs& a, float z, float top, double log_sum) {
     return (float)(((double)z - (double)top) * a.inv_temp - log_sum);
 }
@@ -76,17 +75,6 @@ __device__ __forceinline__ uint32_t group_count(uint32_t wave_count, RankGroup<T
     return n;
 }
 
-template <int RUNS, class F>
-__device__ __forceinline__ uint32_t wave_count(int live, F f) {
-    uint32_t n = 0;
-#pragma unroll
-    for (int j = 0; j < RUNS; ++j)
-        if (j < live)
-#pragma unroll
-            for (int k = 0; k < kRun; ++k) n += (uint32_t)__popcll(__ballot(f(j, k)));
-    return n;
-}
-
 // The largest bound, in steps of 2^16 of the ranks, that at least n of the wave's COUNT x 64 maxima reach; 0 if there are
 // fewer. So many rows reach it at least.
 template <int COUNT>
@@ -101,20 +89,30 @@ __device__ __forceinline__ uint32_t wave_bound(const uint32_t (&most)[COUNT], ui
     return t;
 }
 
+// f of 0 .. N - 1 as constants: loops within f keep the compiler from unrolling one over the runs, which lie in registers.
+template <class F, int... J>
+__device__ __forceinline__ void each_run(F f, std::integer_sequence<int, J...>) {
+    (f(std::integral_constant<int, J>{}), ...);
+}
+
+// The largest of a run, NaN left aside.
+__device__ __forceinline__ float run_max(const float (&x)[kRun]) {
+    return max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), max2(x[6], x[7]));
+}
+
 // The rows of a group's logits v (run j, row k: row kRun (j THREADS + tid) + k of the group's, from index0 on within the set)
-// that rank highest, at least a.top of them where there are so many, as keys in sh.list; returns their number.
-template <int THREADS, int LIST, int RUNS>
-__device__ __forceinline__ int gather_best(const ReportArgs& a, const float (&v)[RUNS][kRun], int live, int64_t index0,
-                                           RankGroup<THREADS, LIST>& sh) {
+// that rank highest, at least a.top of them where there are so many, as keys in sh.list; returns their number. tops: the
+// largest of the runs; `odd`: there may be NaN, which those leave aside. again(j, x): run j once more, for the rare case that
+// more rows reach the bound than there is room for.
+template <int THREADS, int LIST, int RUNS, class AGAIN>
+__device__ __forceinline__ int gather_best(const ReportArgs& a, const float (&v)[RUNS][kRun], const float (&tops)[RUNS], int live,
+                                           bool odd, int64_t index0, RankGroup<THREADS, LIST>& sh, AGAIN again) {
     const int tid = (int)threadIdx.x & (THREADS - 1), lane = tid & (kWave - 1);
     const uint32_t n = (uint32_t)a.top;
     uint32_t most[RUNS], all[1] = {0};
 #pragma unroll
     for (int j = 0; j < RUNS; ++j) {
-        float m = v[j][0];
-#pragma unroll
-        for (int k = 1; k < kRun; ++k) m = max2(m, v[j][k]);
-        most[j] = j < live ? rank_of(m) : 0;
+        most[j] = j < live ? rank_of(tops[j]) : 0;
         all[0] = max(all[0], most[j]);
     }
     uint32_t bound;
@@ -147,27 +145,39 @@ __device__ __forceinline__ int gather_best(const ReportArgs& a, const float (&v)
             for (uint32_t w = 0; w < waves; ++w) bound = max(bound, sh.bound[w]);
         }
     }
-    const auto add = [&](bool in, int j, int k, uint32_t& count) {
-        const unsigned long long m = __ballot(in);
-        if (m == 0) return;
-        uint32_t at = count;
-        if (THREADS == kWave) {
-            count += (uint32_t)__popcll(m);
-        } else {
-            if (lane == 0) at = atomicAdd(&sh.size, (uint32_t)__popcll(m));
-            at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at);
+    // the lane's rows of run j with a bit in `in`, one of each lane at a time
+    const auto add = [&](const float (&row)[kRun], int j, uint32_t in, uint32_t& count) {
+        for (unsigned long long m = __ballot(in != 0); m; m = __ballot(in != 0)) {
+            uint32_t at = count;
+            if (THREADS == kWave) {
+                count += (uint32_t)__popcll(m);
+            } else {
+                if (lane == 0) at = atomicAdd(&sh.size, (uint32_t)__popcll(m));
+                at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at);
+            }
+            at += (uint32_t)__popcll(m & ((1ull << lane) - 1ull));
+            if (in != 0 && at < (uint32_t)LIST) {
+                const int k = __ffs((int)in) - 1;
+                uint32_t x = 0;  // row[k]; a choice between the rows' places would put them in memory
+#pragma unroll
+                for (int l = 0; l < kRun; ++l) x |= __float_as_uint(row[l]) & (0u - (uint32_t)(l == k));
+                sh.list[at] = (unsigned long long)rank_of(__uint_as_float(x)) << 32 | (uint32_t)~(uint32_t)(index0 + kRun * (j * THREADS + tid) + k);
+            }
+            in &= in - 1;
         }
-        at += (uint32_t)__popcll(m & ((1ull << lane) - 1ull));
-        if (in && at < (uint32_t)LIST) sh.list[at] = key_of(v[j][k], (uint32_t)(index0 + kRun * (j * THREADS + tid) + k));
     };
     const float least = bound < 0x00800000u ? kLowest : rank_value(bound);
     uint32_t count = 0;
     wave_sync();
+    each_run([&](auto at) {
+        constexpr int j = decltype(at)::value;
+        if (j < live && (odd || __any(tops[j] >= least))) {
+            uint32_t in = 0;
 #pragma unroll
-    for (int j = 0; j < RUNS; ++j)
-        if (j < live)
-#pragma unroll
-            for (int k = 0; k < kRun; ++k) add(!(v[j][k] < least), j, k, count);
+            for (int k = 0; k < kRun; ++k) in |= v[j][k] < least ? 0u : 1u << k;
+            add(v[j], j, in, count);
+        }
+    }, std::make_integer_sequence<int, RUNS>{});
     if (THREADS != kWave) {
         __syncthreads();
         count = sh.size;
@@ -175,31 +185,48 @@ __device__ __forceinline__ int gather_best(const ReportArgs& a, const float (&v)
     wave_sync();
     if (count <= (uint32_t)LIST) return (int)count;
     // Too many rows reach the bound, of one value most often: the least rank that a.top rows reach, and of those that have
-    // it the first.
+    // it the first. The rows are read anew for each bit: held in registers, they would cost the usual path a third of
+    // its waves.
     int turn = 0;
-    uint32_t t = 0;
-    for (uint32_t bit = 1u << 31; bit != 0; bit >>= 1)
-        if (group_count(wave_count<RUNS>(live, [&](int j, int k) { return rank_of(v[j][k]) >= (t | bit); }), sh, turn) >= n) t |= bit;
-    const uint32_t above = group_count(wave_count<RUNS>(live, [&](int j, int k) { return rank_of(v[j][k]) > t; }), sh, turn);
+    const auto rows = [&](auto holds) {
+        uint32_t c = 0;
+#pragma unroll 1
+        for (int j = 0; j < live; ++j) {
+            float x[kRun];
+            again(j, x);
+#pragma unroll
+            for (int k = 0; k < kRun; ++k) c += holds(rank_of(x[k]), kRun * (j * THREADS + tid) + k) ? 1u : 0u;
+        }
+        return group_count((uint32_t)wave_sum((float)c), sh, turn);
+    };
+    // mostly the bound's high half is the rank's, too
+    const bool near = bound != 0 && rows([&](uint32_t r, int) { return r > (bound | 0xffffu); }) < n;
+    uint32_t t = near ? bound : 0;
+#pragma unroll 1
+    for (uint32_t bit = near ? 1u << 15 : 1u << 31; bit != 0; bit >>= 1)
+        if (rows([&](uint32_t r, int) { return r >= (t | bit); }) >= n) t |= bit;
+    const uint32_t above = rows([&](uint32_t r, int) { return r > t; });
     int last = RUNS * THREADS * kRun - 1;
+#pragma unroll 1
     for (int bit = RUNS * THREADS * kRun / 2; bit != 0; bit >>= 1)
-        if (above + group_count(wave_count<RUNS>(live, [&](int j, int k) {
-                                    return rank_of(v[j][k]) == t && kRun * (j * THREADS + tid) + k <= last - bit;
-                                }), sh, turn) >= n)
-            last -= bit;
+        if (above + rows([&](uint32_t r, int i) { return r == t && i <= last - bit; }) >= n) last -= bit;
     if (THREADS != kWave) {
         if (tid == 0) sh.size = 0;
         __syncthreads();
     }
     count = 0;
+#pragma unroll 1
+    for (int j = 0; j < live; ++j) {
+        float x[kRun];
+        again(j, x);
+        uint32_t in = 0;
 #pragma unroll
-    for (int j = 0; j < RUNS; ++j)
-        if (j < live)
-#pragma unroll
-            for (int k = 0; k < kRun; ++k) {
-                const uint32_t r = rank_of(v[j][k]);
-                add(r > t || (r == t && t != 0 && kRun * (j * THREADS + tid) + k <= last), j, k, count);
-            }
+        for (int k = 0; k < kRun; ++k) {
+            const uint32_t r = rank_of(x[k]);
+            in |= r > t || (r == t && t != 0 && kRun * (j * THREADS + tid) + k <= last) ? 1u << k : 0u;
+        }
+        add(x, j, in, count);
+    }
     if (THREADS != kWave) {
         __syncthreads();
         count = sh.size;
@@ -340,13 +367,17 @@ __device__ __forceinline__ void tile_lists(const ReportArgs& a, const ROWS& in, 
             const int s = r * kWave + __ffsll((long long)m) - 1;
             const uint32_t rg = sh.range[s];
             const int b = (int)(rg & 0xffffu), e = (int)(rg >> 16);
-            float v[1][kRun];
+            const auto read = [&](int, float(&x)[kRun]) {
 #pragma unroll
-            for (int k = 0; k < kRun; ++k) {
-                const uint32_t o = b + i0 + k < e ? sh.rank[b + i0 + k] : 0u;
-                v[0][k] = o ? rank_value(o) : -kInf;
-            }
-            const int n = gather_best(a, v, 1, 0, sh.group);
+                for (int k = 0; k < kRun; ++k) {
+                    const uint32_t o = b + i0 + k < e ? sh.rank[b + i0 + k] : 0u;
+                    x[k] = o ? rank_value(o) : -kInf;
+                }
+            };
+            float v[1][kRun];
+            read(0, v[0]);
+            const float tops[1] = {run_max(v[0])};
+            const int n = gather_best(a, v, tops, 1, true, 0, sh.group, read);
             rank_list<kWave>(a, sh.group.list, n, [&](int place, unsigned long long key) {
                 const bool there = key != 0;
                 put_entry(a, (int64_t)sh.set[s] * a.top + place, there ? (int32_t)~(uint32_t)key : -1,
@@ -463,39 +494,38 @@ __global__ __launch_bounds__(kBlock, 4) void report_tile_kernel(ReportArgs a) {
 template <int THREADS, int LIST>
 struct ReportGroup {
     RankGroup<THREADS, LIST> rank;
-    float top[THREADS / kWave];
-    double sum[THREADS / kWave], along[THREADS / kWave];
+    GroupSums<THREADS / kWave> sums;
 };
 
 // One set of more than kSetShort rows by a wave (THREADS 64), or a longer one or a part of it by a workgroup, its rows in
 // registers.
-template <int TYPE, bool MASK, bool BIAS, int THREADS, int LIST>
+template <int TYPE, bool MASK, bool BIAS, int THREADS, int RUNS, int LIST>
 __device__ __forceinline__ void report_pass(const ReportArgs& a, const SetItem& im, int32_t index, ReportGroup<THREADS, LIST>& sh,
                                             const BiasShared* bias) {
-    constexpr bool EXACT = TYPE == PB_F32 || BIAS;
-    const int tid = (int)threadIdx.x & (THREADS - 1), lane = tid & (kWave - 1);
+    constexpr bool EXACT = kExact<TYPE, BIAS>;
+    const int tid = (int)threadIdx.x & (THREADS - 1);
     const int wave0 = __builtin_amdgcn_readfirstlane(tid & ~(kWave - 1));  // the wave's first thread
     const Heat heat{a.heat_hi, a.heat_lo, a.heat_low};
     const Span sp = span_of(a, im);
     const int64_t g = im.set0;
-    RawRun<TYPE, MASK, BIAS> raw[kWideRuns];
+    RawRun<TYPE, MASK, BIAS> raw[RUNS];
 #pragma unroll
-    for (int j = 0; j < kWideRuns; ++j) {
+    for (int j = 0; j < RUNS; ++j) {
         const int i = kRun * (j * THREADS + tid);
         if (kRun * (j * THREADS + wave0) < sp.hi && i < sp.hi) raw[j].load(a, sp, i);
     }
     const int64_t r0 = a.off[g], size = a.off[g + 1] - r0;
     bool counts = false;
     float z = 0.0f;
-    if (a.chosen && im.parts == 1) {
+    if (a.chosen && im.parts == 1 && wave0 == 0) {
         const int32_t c = a.chosen[g];
         counts = c >= 0 && c < size;
         if (MASK && counts) counts = a.mask[r0 + c] != 0;
         if (counts) z = one_logit<TYPE, BIAS>(a, bias, r0 + c);
     }
-    float v[kWideRuns][kRun];
+    float v[RUNS][kRun], tops[RUNS];
 #pragma unroll
-    for (int j = 0; j < kWideRuns; ++j) {
+    for (int j = 0; j < RUNS; ++j) {
         const int i = kRun * (j * THREADS + tid);
 #pragma unroll
         for (int k = 0; k < kRun; ++k) v[j][k] = -kInf;
@@ -508,14 +538,14 @@ __device__ __forceinline__ void report_pass(const ReportArgs& a, const SetItem& 
     const int live = sp.hi <= kRun * wave0 ? 0 : (sp.hi - kRun * wave0 + kRun * THREADS - 1) / (kRun * THREADS);  // the wave's runs
     SoftSums t{kLowest, 0.0, 0.0};
 #pragma unroll
-    for (int j = 0; j < kWideRuns; ++j)
-        if (j < live)
-#pragma unroll
-            for (int k = 0; k < kRun; k += 2) t.top = max3(t.top, v[j][k], v[j][k + 1]);
+    for (int j = 0; j < RUNS; ++j) {
+        tops[j] = -kInf;
+        if (j < live) t.top = max2(t.top, tops[j] = run_max(v[j]));
+    }
     t.top = wave_max(t.top);
     float sum = 0.0f, along = 0.0f;
 #pragma unroll
-    for (int j = 0; j < kWideRuns; ++j)
+    for (int j = 0; j < RUNS; ++j)
         if (j < live)
 #pragma unroll
             for (int k = 0; k < kRun; ++k) {
@@ -525,21 +555,7 @@ __device__ __forceinline__ void report_pass(const ReportArgs& a, const SetItem& 
             }
     t.sum = team_sum((double)sum, 6);
     t.along = team_sum((double)along, 6);
-    if (THREADS != kWave) {
-        if (lane == 0) {
-            sh.top[tid / kWave] = t.top;
-            sh.sum[tid / kWave] = t.sum;
-            sh.along[tid / kWave] = t.along;
-        }
-        __syncthreads();
-        t = SoftSums{sh.top[0], 0.0, 0.0};
-        for (int w = 1; w < THREADS / kWave; ++w) t.top = max2(t.top, sh.top[w]);
-        for (int w = 0; w < THREADS / kWave; ++w) {
-            const double gap = (double)sh.top[w] - (double)t.top, f = exp_near(gap * a.inv_temp);
-            t.sum += sh.sum[w] * f;
-            t.along += f == 0.0 ? 0.0 : f * (sh.along[w] + sh.sum[w] * gap);
-        }
-    }
+    t = join_waves<true>(a, t, sh.sums);
     const double log_sum = log_near(t.sum);
     if (tid == 0) {
         if (im.parts == 1)
@@ -548,7 +564,14 @@ __device__ __forceinline__ void report_pass(const ReportArgs& a, const SetItem& 
             a.part_sums[index] = t;
     }
     if (a.top > 0) {
-        const int n = gather_best(a, v, live, sp.q0 - r0, sh.rank);
+        const int n = gather_best(a, v, tops, live, !(t.sum == t.sum), sp.q0 - r0, sh.rank, [&](int j, float(&x)[kRun]) {
+            const int i = kRun * (j * THREADS + tid);
+            uint32_t off;
+            Buckets buckets;
+#pragma unroll
+            for (int k = 0; k < kRun; ++k) x[k] = -kInf;
+            if (i < sp.hi) load_logits<TYPE, MASK, BIAS>(a, bias, sp, i, x, off, buckets);
+        });
         if (im.parts == 1)
             rank_list<THREADS>(a, sh.rank.list, n, [&](int place, unsigned long long key) {
                 const bool there = key != 0;
@@ -565,9 +588,11 @@ __device__ __forceinline__ void report_pass(const ReportArgs& a, const SetItem& 
         wave_sync();
 }
 
-// Workgroups [0, mid_blocks) take the sets for a wave, the others those for a workgroup and the parts, one at a time.
+// Workgroups [0, mid_blocks) take the sets for a wave, the others those for a workgroup, then the parts (all from num_mid +
+// num_whole on, or those in `list`), one at a time.
 template <int TYPE, bool MASK, bool BIAS>
-__global__ __launch_bounds__(kBlock) void report_wide_kernel(ReportArgs a, int mid_blocks) {
+__global__ __launch_bounds__(kBlock) void report_wide_kernel(ReportArgs a, int mid_blocks, int num_parts,
+                                                             const int32_t* __restrict__ list) {
     __shared__ union {
         ReportGroup<kWave, kWaveList> mid[kWaves];
         ReportGroup<kBlock, kGroupList> whole;
@@ -577,12 +602,21 @@ __global__ __launch_bounds__(kBlock) void report_wide_kernel(ReportArgs a, int m
     if ((int)blockIdx.x < mid_blocks) {
         const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), step = mid_blocks * kWaves;
         for (int it = (int)blockIdx.x * kWaves + wave; it < a.num_mid; it += step)
-            report_pass<TYPE, MASK, BIAS, kWave, kWaveList>(a, a.wide[it], it, sh.mid[wave], &bias);
+            report_pass<TYPE, MASK, BIAS, kWave, kWideRuns, kWaveList>(a, a.wide[it], it, sh.mid[wave], &bias);
     } else {
-        const int n = a.num_mid + a.num_wide;
-        for (int it = a.num_mid + (int)blockIdx.x - mid_blocks; it < n; it += (int)gridDim.x - mid_blocks)
-            report_pass<TYPE, MASK, BIAS, kBlock, kGroupList>(a, a.wide[it], it, sh.whole, &bias);
+        const int n = a.num_whole + num_parts;
+        for (int k = (int)blockIdx.x - mid_blocks; k < n; k += (int)gridDim.x - mid_blocks) {
+            const int it = list && k >= a.num_whole ? list[k - a.num_whole] : a.num_mid + k;
+            report_pass<TYPE, MASK, BIAS, kBlock, kWideRuns, kGroupList>(a, a.wide[it], it, sh.whole, &bias);
+        }
     }
+}
+
+// Sets of up to THREADS * RUNS * 8 rows, a workgroup each.
+template <int TYPE, bool MASK, int THREADS, int RUNS>
+__global__ __launch_bounds__(THREADS, 4) void report_big_kernel(ReportArgs a, const SetItem* __restrict__ items) {
+    __shared__ ReportGroup<THREADS, kGroupList> sh;
+    report_pass<TYPE, MASK, false, THREADS, RUNS, kGroupList>(a, items[blockIdx.x], 0, sh, nullptr);
 }
 
 __device__ __forceinline__ uint32_t block_count(uint32_t v, uint32_t* sh) {
@@ -600,32 +634,27 @@ __device__ __forceinline__ uint32_t block_count(uint32_t v, uint32_t* sh) {
 // reach with all of their entries and the others with fewer than d of them, 64 x 64 at most.
 template <int TYPE, bool MASK, bool BIAS>
 __global__ __launch_bounds__(kBlock) void report_join_kernel(ReportArgs a, const int32_t* __restrict__ firsts) {
-    __shared__ unsigned long long list[kJoinList];
+    constexpr int kAhead = 8;
+    __shared__ unsigned long long list[kJoinList], bound;
     __shared__ uint32_t shc[kWaves], size;
-    __shared__ float tops[kWaves];
-    __shared__ double sums[kWaves], alongs[kWaves];
+    __shared__ GroupSums<kWaves> sums;
     __shared__ BiasShared bias;
-    const int tid = (int)threadIdx.x, lane = tid & (kWave - 1);
+    const int tid = (int)threadIdx.x;
     const int32_t first = firsts[blockIdx.x];
     const SetItem im = a.wide[first];
     const int64_t g = im.set0, r0 = a.off[g];
     const int n = im.parts;
     if (BIAS) stage_bias(a, bias);
-    SoftSums t{kLowest, 0.0, 0.0};
-    for (int j = tid; j < n; j += kBlock) t.top = max2(t.top, a.part_sums[first + j].top);
-    t.top = wave_max(t.top);
-    if (lane == 0) tops[tid / kWave] = t.top;
-    if (tid == 0) size = 0;
-    __syncthreads();
-    for (int w = 0; w < kWaves; ++w) t.top = max2(t.top, tops[w]);
-    for (int j = tid; j < n; j += kBlock) {
-        const SoftSums p = a.part_sums[first + j];
-        const double gap = (double)p.top - (double)t.top, f = exp_near(gap * a.inv_temp);
-        t.sum += p.sum * f;
-        t.along += f == 0.0 ? 0.0 : f * (p.along + p.sum * gap);
+    const unsigned long long* keys = a.part_keys + (int64_t)first * a.top;
+    const int d = (a.top + n - 1) / n, want = d > 0 ? (a.top + d - 1) / d : 0;
+    const bool bounded = (int64_t)n * a.top > kBlock, few = n <= kBoundParts;
+    if (bounded && few)
+        for (int j = tid; j < n; j += kBlock) list[j] = keys[(int64_t)j * a.top + d - 1];
+    if (tid == 0) {
+        size = 0;
+        bound = 0;
     }
-    t.sum = block_sum(t.sum, sums);
-    t.along = block_sum(t.along, alongs);
+    const SoftSums t = join_set<true>(a, a.part_sums + first, n, sums);  // a barrier within
     const double log_sum = log_near(t.sum);
     if (tid == 0) {
         bool counts = false;
@@ -639,36 +668,52 @@ __global__ __launch_bounds__(kBlock) void report_join_kernel(ReportArgs a, const
         put_report(a, g, t, log_sum, counts, z);
     }
     if (a.top == 0) return;
-    const unsigned long long* keys = a.part_keys + (int64_t)first * a.top;
-    const int64_t entries = (int64_t)n * a.top;
-    unsigned long long bound = 0;
-    if (entries > kBlock) {
-        const int d = (a.top + n - 1) / n;
-        const uint32_t want = (uint32_t)((a.top + d - 1) / d);
-        for (int bit = 63; bit >= 0; --bit) {
-            const unsigned long long trial = bound | 1ull << bit;
-            uint32_t c = 0;
-            for (int j = tid; j < n; j += kBlock) c += keys[(int64_t)j * a.top + d - 1] >= trial ? 1u : 0u;
-            if (block_count(c, shc) >= want) bound = trial;
+    if (bounded) {
+        if (few) {
+            for (int j = tid; j < n; j += kBlock) {
+                const unsigned long long key = list[j];
+                int place = 0;
+                for (int i = 0; i < n; ++i) place += list[i] > key ? 1 : 0;
+                if (place == want - 1 && key != 0) bound = key;  // keys other than 0 differ
+            }
+        } else {
+            unsigned long long least = 0;
+            for (int bit = 63; bit >= 0; --bit) {
+                const unsigned long long trial = least | 1ull << bit;
+                uint32_t c = 0;
+                for (int j = tid; j < n; j += kBlock) c += keys[(int64_t)j * a.top + d - 1] >= trial ? 1u : 0u;
+                if (block_count(c, shc) >= (uint32_t)want) least = trial;
+            }
+            if (tid == 0) bound = least;
         }
+        __syncthreads();
     }
-    for (int64_t e0 = 0; e0 < entries; e0 += kBlock) {
-        const int64_t e = e0 + tid;
-        const unsigned long long key = e < entries ? keys[e] : 0ull;
-        if (key != 0 && key >= bound) {
-            const uint32_t at = atomicAdd(&size, 1u);
-            if (at < (uint32_t)kJoinList) list[at] = key;
+    // a part's entries down to the bound, kAhead asked for at a time
+    const unsigned long long least = bound;
+    __syncthreads();
+    for (int j = tid; j < n; j += kBlock) {
+        const unsigned long long* mine = keys + (int64_t)j * a.top;
+        bool more = true;
+        for (int e = 0; more && e < a.top; e += kAhead) {
+            unsigned long long key[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) key[u] = e + u < a.top ? mine[e + u] : 0ull;
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                more = more && key[u] != 0 && key[u] >= least;
+                if (more) list[atomicAdd(&size, 1u)] = key[u];
+            }
         }
     }
     __syncthreads();
-    int c = (int)min(size, (uint32_t)kJoinList);
+    int c = (int)size;
     if (c > kGroupList) {  // the a.top-th key itself, then what reaches it
-        unsigned long long least = 0;
+        unsigned long long nth = 0;
         for (int bit = 63; bit >= 0; --bit) {
-            const unsigned long long trial = least | 1ull << bit;
+            const unsigned long long trial = nth | 1ull << bit;
             uint32_t m = 0;
             for (int i = tid; i < c; i += kBlock) m += list[i] >= trial ? 1u : 0u;
-            if (block_count(m, shc) >= (uint32_t)a.top) least = trial;
+            if (block_count(m, shc) >= (uint32_t)a.top) nth = trial;
         }
         unsigned long long mine[kJoinList / kBlock];
 #pragma unroll
@@ -678,7 +723,7 @@ __global__ __launch_bounds__(kBlock) void report_join_kernel(ReportArgs a, const
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < kJoinList / kBlock; ++i)
-            if (mine[i] >= least && mine[i] != 0) list[atomicAdd(&size, 1u)] = mine[i];
+            if (mine[i] >= nth && mine[i] != 0) list[atomicAdd(&size, 1u)] = mine[i];
         __syncthreads();
         c = (int)size;
     }
@@ -693,20 +738,48 @@ int tile_blocks(const SetLayout& s) { return std::min((s.num_tiles + kWaves - 1)
 
 int mid_blocks(const SetLayout& s) { return std::min((s.num_mid + kWaves - 1) / kWaves, kChoiceGrid); }
 
+// Where long sets have a workgroup each: where there are so many that they fill the chip, and where there is one
+// kernel less for it.
+bool takes_big(const SetLayout& s, bool bias) { return !bias && s.num_big > 0 && (s.num_big >= kBigSets || s.num_big <= kFewSets); }
+
+int num_parts(const SetLayout& s, bool bias) { return takes_big(s, bias) ? s.num_giant : s.num_wide - s.num_whole; }
+
 template <int TYPE, bool MASK, bool BIAS>
 hipError_t launch_as(const SetLayout& s, const ReportArgs& a, hipStream_t stream) {
     hipError_t e = hipSuccess;
-    const int wide = mid_blocks(s) + std::min(s.num_wide, kChoiceGrid);
+    const bool big = takes_big(s, BIAS);
+    const int parts = num_parts(s, BIAS);
+    if constexpr (!BIAS) {
+        // the first kernels have the most lanes to a set, where there are few
+        const bool few = s.num_big <= kFewSets;
+        const int half = few ? 0 : s.num_half;
+        if (big && few) {
+            hipLaunchKernelGGL((report_big_kernel<TYPE, MASK, 1024, 8>), dim3(s.num_big), dim3(1024), 0, stream, a, s.big);
+            if ((e = hipGetLastError()) != hipSuccess) return e;
+        } else if (big) {
+            if (s.num_big > half) {
+                hipLaunchKernelGGL((report_big_kernel<TYPE, MASK, 1024, 8>), dim3(s.num_big - half), dim3(1024), 0, stream, a, s.big + half);
+                if ((e = hipGetLastError()) != hipSuccess) return e;
+            }
+            if (half > 0) {
+                hipLaunchKernelGGL((report_big_kernel<TYPE, MASK, 512, 8>), dim3(half), dim3(512), 0, stream, a, s.big);
+                if ((e = hipGetLastError()) != hipSuccess) return e;
+            }
+        }
+    }
+    const int wide = mid_blocks(s) + std::min(s.num_whole + parts, kChoiceGrid);
     if (wide > 0) {
-        hipLaunchKernelGGL((report_wide_kernel<TYPE, MASK, BIAS>), dim3(wide), dim3(kBlock), 0, stream, a, mid_blocks(s));
+        hipLaunchKernelGGL((report_wide_kernel<TYPE, MASK, BIAS>), dim3(wide), dim3(kBlock), 0, stream, a, mid_blocks(s), parts,
+                           big ? s.giant : nullptr);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
     if (s.num_tiles > 0) {
         hipLaunchKernelGGL((report_tile_kernel<TYPE, MASK, BIAS>), dim3(tile_blocks(s)), dim3(kBlock), 0, stream, a);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
-    if (s.num_split > 0) {
-        hipLaunchKernelGGL((report_join_kernel<TYPE, MASK, BIAS>), dim3(s.num_split), dim3(kBlock), 0, stream, a, s.split);
+    const int joins = big ? s.num_split - s.num_big : s.num_split;
+    if (joins > 0) {
+        hipLaunchKernelGGL((report_join_kernel<TYPE, MASK, BIAS>), dim3(joins), dim3(kBlock), 0, stream, a, big ? s.giant_split : s.split);
         e = hipGetLastError();
     }
     return e;

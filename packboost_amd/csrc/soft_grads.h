@@ -21,15 +21,10 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "choice_rows.h"
-#include "report.h"
+#include "soft_rows.h"
 
 namespace pb {
 namespace {
-
-// The exponentials of gradients that are rounded to 16 bits, each rounding its exponent once.
-template <int TYPE, bool BIAS>
-constexpr bool kExact = TYPE == PB_F32 || BIAS;
 
 // A teacher's value as it lies in memory, asked for but not waited for, and what it stands for.
 __device__ __forceinline__ uint32_t entry_bits(const ReportArgs& a, int64_t i) {
@@ -535,13 +530,11 @@ __global__ __launch_bounds__(kBlock, DISTILL ? 3 : 4) void soft_tile_kernel(Repo
 // What a group of lanes (a wave, or a workgroup) shares of its set. ROWS: 0 without lists.
 template <int THREADS, int ROWS>
 struct SoftGroup {
-    static constexpr int kGroupWaves = THREADS / kWave;
     uint8_t slot[ROWS ? ROWS : 8];  // the entry that names a row, from 1; 0: none
     float e[kMaxTop], part[kMaxTop];
     ListSide list;
     float weight;
-    float top[kGroupWaves];
-    double sum[kGroupWaves], along[kGroupWaves];
+    GroupSums<THREADS / kWave> sums;
 };
 
 template <int THREADS>
@@ -550,43 +543,6 @@ __device__ __forceinline__ void group_sync() {
         wave_sync();
     else
         __syncthreads();
-}
-
-// A set's sums from those of the lanes (each wave's relative to its own maximum), the same in every lane.
-template <bool ALONG, int THREADS, int ROWS>
-__device__ __forceinline__ SoftSums join_waves(const ReportArgs& a, SoftSums t, SoftGroup<THREADS, ROWS>& sh) {
-    if (THREADS == kWave) return t;
-    const int tid = (int)threadIdx.x;
-    if ((tid & (kWave - 1)) == 0) {
-        sh.top[tid / kWave] = t.top;
-        sh.sum[tid / kWave] = t.sum;
-        if (ALONG) sh.along[tid / kWave] = t.along;
-    }
-    __syncthreads();
-    SoftSums j{sh.top[0], 0.0, 0.0};
-    for (int w = 1; w < THREADS / kWave; ++w) j.top = max2(j.top, sh.top[w]);
-    for (int w = 0; w < THREADS / kWave; ++w) {
-        const double gap = (double)sh.top[w] - (double)j.top, f = exp_near(gap * a.inv_temp);
-        j.sum += sh.sum[w] * f;
-        if (ALONG) j.along += f == 0.0 ? 0.0 : f * (sh.along[w] + sh.sum[w] * gap);
-    }
-    return j;
-}
-
-// A set's sums from those of its parts.
-template <bool ALONG, int THREADS, int ROWS>
-__device__ __forceinline__ SoftSums join_set(const ReportArgs& a, const SoftSums* parts, int n, SoftGroup<THREADS, ROWS>& sh) {
-    SoftSums t{kLowest, 0.0, 0.0};
-    for (int j = (int)threadIdx.x; j < n; j += THREADS) t.top = max2(t.top, parts[j].top);
-    t.top = wave_max(t.top);
-    for (int j = (int)threadIdx.x; j < n; j += THREADS) {
-        const double gap = (double)parts[j].top - (double)t.top, f = exp_near(gap * a.inv_temp);
-        t.sum += parts[j].sum * f;
-        if (ALONG) t.along += f == 0.0 ? 0.0 : f * (parts[j].along + parts[j].sum * gap);
-    }
-    t.sum = team_sum(t.sum, 6);
-    if (ALONG) t.along = team_sum(t.along, 6);
-    return join_waves<ALONG>(a, t, sh);
 }
 
 enum SoftPhase { kWholeSet, kPartSums, kPartGrads };
@@ -690,7 +646,7 @@ __device__ __forceinline__ void soft_pass(const ReportArgs& a, const SetItem& im
     const int live = sp.hi <= kRun * wave0 ? 0 : (sp.hi - kRun * wave0 + kRun * THREADS - 1) / (kRun * THREADS);  // the wave's runs
     SoftSums own{kLowest, 0.0, 0.0}, sums;
     if (PHASE == kPartGrads) {
-        sums = join_set<!DISTILL>(a, a.part_sums + (index - im.part), im.parts, sh);
+        sums = join_set<!DISTILL>(a, a.part_sums + (index - im.part), im.parts, sh.sums);
         own.top = sums.top;
     } else {
 #pragma unroll
@@ -715,7 +671,7 @@ __device__ __forceinline__ void soft_pass(const ReportArgs& a, const SetItem& im
     if (PHASE != kPartGrads) {
         own.sum = team_sum((double)sum, 6);
         if (!DISTILL) own.along = team_sum((double)along, 6);
-        sums = join_waves<!DISTILL>(a, own, sh);
+        sums = join_waves<!DISTILL>(a, own, sh.sums);
     }
     if (PHASE == kPartSums) {
         if (tid == 0) a.part_sums[index] = sums;
