@@ -18,10 +18,11 @@
 namespace pb {
 namespace {
 
-constexpr int kCountRows = 64;    // rows of a tile's set whose rows count what ranks above them
+constexpr int kCountRows = 192;   // rows of a tile's set whose rows count what ranks above them
 constexpr int kWaveList = 256;    // rows that reach the bound: room for a wave's
 constexpr int kGroupList = 512;   // and a workgroup's
 constexpr int kJoinList = kMaxTop * kMaxTop;
+constexpr int kSharedTiles = 1024; // up to so many tiles a workgroup each
 constexpr int kBigSets = 1024;     // from so many long sets on a workgroup to each beats parts,
 constexpr int kFewSets = 8;        // and up to so many
 constexpr int kBoundParts = 1024;  // parts whose bound is found by counting
@@ -235,14 +236,34 @@ __device__ __forceinline__ int gather_best(const ReportArgs& a, const float (&v)
     return (int)count;
 }
 
+// How many of n keys are larger, eight asked for at a time.
+__device__ __forceinline__ int keys_above(const unsigned long long* list, int n, unsigned long long key) {
+    constexpr int kAhead = 8;
+    int place = 0, i = 0;
+    for (; i + kAhead <= n; i += kAhead) {
+        unsigned long long o[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) o[u] = list[i + u];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) place += o[u] > key ? 1 : 0;
+    }
+    if (i < n) {
+        unsigned long long o[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) o[u] = list[min(i + u, n - 1)];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) place += i + u < n && o[u] > key ? 1 : 0;
+    }
+    return place;
+}
+
 // f(place, key) of the first a.top of n keys, and of none (key 0) behind the last.
 template <int THREADS, class F>
 __device__ __forceinline__ void rank_list(const ReportArgs& a, const unsigned long long* list, int n, F f) {
     const int tid = (int)threadIdx.x & (THREADS - 1);
     for (int c = tid; c < n; c += THREADS) {
         const unsigned long long key = list[c];
-        int place = 0;
-        for (int i = 0; i < n; ++i) place += list[i] > key ? 1 : 0;
+        const int place = keys_above(list, n, key);
         if (place < a.top) f(place, key);
     }
     for (int c = n + tid; c < a.top; c += THREADS) f(c, 0ull);
@@ -251,141 +272,122 @@ __device__ __forceinline__ void rank_list(const ReportArgs& a, const unsigned lo
 // ------------------------------------------------------------------------------------ tiles
 struct ReportTile {
     union {
-        float x[kSetTileRows];        // logits
-        uint32_t rank[kSetTileRows];  // later: their ranks
+        float x[kSetTileRows];                // logits
+        unsigned long long key[kSetTileRows]; // later: their ranks and the complements of their places, 0 for none
     };
     float top[kSetTileSets + 4];  // per set: maximum
     union {
         uint16_t head[kSetTileRows];  // the set that starts at a row, from 1; 0: none
         float sum[kSetTileSets + 4];  // later: sum of exponentials, then its logarithm
     };
-    float along[kSetTileSets + 4];     // sum of exponentials times distances
-    uint32_t range[kSetTileSets + 4];  // first row and, 16 bits up, the row behind the last
+    union {
+        float along[kSetTileSets + 4];     // sum of exponentials times distances
+        uint32_t range[kSetTileSets + 4];  // later: first row and, 16 bits up, the row behind the last
+    };
     int32_t set[kSetTileSets + 4];
-    int32_t idle[kSetTileSets + 4];    // rows that are not ranked
-    RankGroup<kWave, kWaveList> group;
+    int32_t ranked[kSetTileSets + 4];  // rows that are ranked
+    uint8_t id[kSetTileRows];          // a row's set, from 1
+    int32_t behind, sets;              // the row behind the last set's
 };
 
-// The lists of a tile: ranks of 32 bits in LDS. A row compares itself with those of its set that lie before its lane's run,
-// in the run, and after it; what lies before belongs to the set of the run's first row, what lies after to that of its
-// last. 17 vector instructions for a row of LDS and eight of the lane's.
+// What the lists of a tile are made of, by the tile's wave: the rows' keys, and where the sets lie.
 template <class ROWS>
-__device__ __forceinline__ void tile_lists(const ReportArgs& a, const ROWS& in, const float (&x)[kRun], const int (&id)[kRun],
-                                           ReportTile& sh) {
+__device__ __forceinline__ void prepare_lists(const ROWS& in, const float (&x)[kRun], const int (&id)[kRun], ReportTile& sh) {
     const int lane = (int)threadIdx.x & (kWave - 1), i0 = kRun * lane;
-    uint32_t own[kRun];
-    int place[kRun];
 #pragma unroll
     for (int k = 0; k < kRun; ++k) {
-        own[k] = rank_of(x[k]);
-        place[k] = 0;
+        const uint32_t r = rank_of(x[k]);
+        sh.key[i0 + k] = r ? (unsigned long long)r << 32 | (uint32_t)~(uint32_t)(i0 + k) : 0ull;
     }
-    *reinterpret_cast<uint4*>(&sh.rank[i0]) = make_uint4(own[0], own[1], own[2], own[3]);
-    *reinterpret_cast<uint4*>(&sh.rank[i0 + 4]) = make_uint4(own[4], own[5], own[6], own[7]);
+    *reinterpret_cast<uint2*>(&sh.id[i0]) =
+        make_uint2((uint32_t)id[0] | (uint32_t)id[1] << 8 | (uint32_t)id[2] << 16 | (uint32_t)id[3] << 24,
+                   (uint32_t)id[4] | (uint32_t)id[5] << 8 | (uint32_t)id[6] << 16 | (uint32_t)id[7] << 24);
+    int behind = 0;
 #pragma unroll
     for (int r = 0; r < kTileRounds; ++r) {
         const int s = r * kWave + lane;
         sh.range[s] = (uint32_t)in.begin[r] | (uint32_t)in.end[r] << 16;
         sh.set[s] = in.set[r];
-        sh.idle[s] = 0;
+        sh.ranked[s] = 0;
+        behind = max(behind, in.end[r]);
     }
     if (lane < 4) sh.range[kSetTileSets + lane] = 0;
-    wave_sync();
-    uint32_t range[kRun];
-#pragma unroll
-    for (int k = 0; k < kRun; ++k) {
-        range[k] = sh.range[id[k] - 1];
-        const int i = i0 + k;
-        if (own[k] == 0 && i >= (int)(range[k] & 0xffffu) && i < (int)(range[k] >> 16)) atomicAdd(&sh.idle[id[k] - 1], 1);
+    behind = (int)wave_max((float)behind);
+    if (lane == 0) {
+        sh.behind = behind;
+        sh.sets = in.sets;
     }
-    const auto short_set = [](uint32_t r) { return (int)(r >> 16) - (int)(r & 0xffffu) <= kCountRows; };
-#pragma unroll
-    for (int k = 0; k < kRun; ++k)
-#pragma unroll
-        for (int l = k + 1; l < kRun; ++l) {
-            const bool same = id[k] == id[l], below = own[l] > own[k];
-            place[k] += same && below ? 1 : 0;
-            place[l] += same && !below ? 1 : 0;
+}
+
+// The lists of a tile, by wave `part` of `parts`. A lane takes a row and counts the larger keys of its set, 64 rows at a
+// time, and a wave waits for its longest set; sets of more than kCountRows rows are taken by a whole wave each. (A lane with
+// eight neighbouring rows took 11 us for 37 rows, where this takes XXX.)
+__device__ __forceinline__ void take_lists(const ReportArgs& a, ReportTile& sh, RankGroup<kWave, kWaveList>& group, int part, int parts) {
+    const int lane = (int)threadIdx.x & (kWave - 1), num_sets = sh.sets;
+#pragma unroll 1
+    for (int p = part * kWave; p < sh.behind; p += parts * kWave) {
+        const int i = p + lane, s = (int)sh.id[i] - 1;
+        const unsigned long long key = sh.key[i];
+        const uint32_t range = sh.range[s];
+        const int b = (int)(range & 0xffffu), n = (int)(range >> 16) - b;
+        if (key != 0 && n <= kCountRows) {
+            atomicAdd(&sh.ranked[s], 1);
+            const int place = keys_above(&sh.key[b], n, key);
+            if (place < a.top)
+                put_entry(a, (int64_t)sh.set[s] * a.top + place, i - b,
+                          list_log_prob(a, rank_value((uint32_t)(key >> 32)), sh.top[s], (double)sh.sum[s]));
         }
-    uint32_t some = 0;
-#pragma unroll
-    for (int k = 0; k < kRun; ++k) some |= own[k];
-    // rows [i, e) of LDS, four asked for at a time
-    const auto count_rows = [&](int i, int e, const uint32_t (&than)[kRun]) {
-        for (; i + 3 < e; i += 4) {
-            const uint32_t o[4] = {sh.rank[i], sh.rank[i + 1], sh.rank[i + 2], sh.rank[i + 3]};
-#pragma unroll
-            for (int l = 0; l < 4; ++l)
-#pragma unroll
-                for (int k = 0; k < kRun; ++k) place[k] += o[l] > than[k] ? 1 : 0;
-        }
-        for (; i < e; ++i) {
-            const uint32_t o = sh.rank[i];
-#pragma unroll
-            for (int k = 0; k < kRun; ++k) place[k] += o > than[k] ? 1 : 0;
-        }
-    };
-    if (some && short_set(range[0])) {  // of equal ones the rows before rank above
-        uint32_t than[kRun];
-#pragma unroll
-        for (int k = 0; k < kRun; ++k) than[k] = id[k] == id[0] && own[k] != 0 ? own[k] - 1u : ~0u;
-        count_rows((int)(range[0] & 0xffffu), min(i0, (int)(range[0] >> 16)), than);
     }
-    if (some && short_set(range[kRun - 1])) {
-        uint32_t than[kRun];
-#pragma unroll
-        for (int k = 0; k < kRun; ++k) than[k] = id[k] == id[kRun - 1] ? own[k] : ~0u;
-        count_rows(i0 + kRun, (int)(range[kRun - 1] >> 16), than);
-    }
-#pragma unroll
-    for (int k = 0; k < kRun; ++k)
-        if (own[k] != 0 && place[k] < a.top && short_set(range[k])) {
-            const int s = id[k] - 1;
-            put_entry(a, (int64_t)sh.set[s] * a.top + place[k], i0 + k - (int)(range[k] & 0xffffu),
-                      list_log_prob(a, rank_value(own[k]), sh.top[s], (double)sh.sum[s]));
-        }
-    // behind the last: lists of short sets with fewer ranked rows than entries
+    if (parts > 1)
+        __syncthreads();
+    else
+        wave_sync();
+    // behind the last: lists with fewer ranked rows than entries
     bool gaps = false;
+    unsigned long long longer[kTileRounds];
 #pragma unroll
     for (int r = 0; r < kTileRounds; ++r) {
-        const int s = r * kWave + lane, size = in.end[r] - in.begin[r];
-        gaps = gaps || (s < in.sets && size <= kCountRows && size - sh.idle[s] < a.top);
+        const int s = r * kWave + lane;
+        const uint32_t range = sh.range[s];
+        const bool counted = (int)(range >> 16) - (int)(range & 0xffffu) <= kCountRows;
+        gaps = gaps || (s < num_sets && counted && sh.ranked[s] < a.top);
+        longer[r] = __ballot(!counted);
     }
     if (__any(gaps)) {
-        const int bits = a.team_bits, entries = in.sets << bits, j = lane & ((1 << bits) - 1);
-        for (int e = lane; e < entries; e += kWave) {
+        const int bits = a.team_bits, entries = num_sets << bits, j = lane & ((1 << bits) - 1);
+#pragma unroll 4
+        for (int e = part * kWave + lane; e < entries; e += parts * kWave) {
             const int s = e >> bits;
-            const uint32_t r = sh.range[s];
-            if (j < a.top && short_set(r) && j >= (int)(r >> 16) - (int)(r & 0xffffu) - sh.idle[s])
+            const uint32_t range = sh.range[s];
+            if (j < a.top && j >= sh.ranked[s] && (int)(range >> 16) - (int)(range & 0xffffu) <= kCountRows)
                 put_entry(a, (int64_t)sh.set[s] * a.top + j, -1, -kInf);
         }
     }
-    // longer sets, one after the other
-    for (int r = 0; r < kTileRounds; ++r) {
-        const int size = r ? in.end[1] - in.begin[1] : in.end[0] - in.begin[0];
-        for (unsigned long long m = __ballot(r * kWave + lane < in.sets && size > kCountRows); m; m &= m - 1) {
+    int turn = 0;
+    for (int r = 0; r < kTileRounds; ++r)
+        for (unsigned long long m = r ? longer[1] : longer[0]; m; m &= m - 1, ++turn) {
+            if (parts > 1 && turn % parts != part) continue;
             const int s = r * kWave + __ffsll((long long)m) - 1;
-            const uint32_t rg = sh.range[s];
-            const int b = (int)(rg & 0xffffu), e = (int)(rg >> 16);
+            const uint32_t range = sh.range[s];
+            const int b = (int)(range & 0xffffu) + kRun * lane, e = (int)(range >> 16);
             const auto read = [&](int, float(&x)[kRun]) {
 #pragma unroll
                 for (int k = 0; k < kRun; ++k) {
-                    const uint32_t o = b + i0 + k < e ? sh.rank[b + i0 + k] : 0u;
-                    x[k] = o ? rank_value(o) : -kInf;
+                    const unsigned long long o = b + k < e ? sh.key[b + k] : 0ull;
+                    x[k] = o ? rank_value((uint32_t)(o >> 32)) : -kInf;
                 }
             };
             float v[1][kRun];
             read(0, v[0]);
             const float tops[1] = {run_max(v[0])};
-            const int n = gather_best(a, v, tops, 1, true, 0, sh.group, read);
-            rank_list<kWave>(a, sh.group.list, n, [&](int place, unsigned long long key) {
+            const int n = gather_best(a, v, tops, 1, true, 0, group, read);
+            rank_list<kWave>(a, group.list, n, [&](int place, unsigned long long key) {
                 const bool there = key != 0;
                 put_entry(a, (int64_t)sh.set[s] * a.top + place, there ? (int32_t)~(uint32_t)key : -1,
                           there ? list_log_prob(a, rank_value((uint32_t)(key >> 32)), sh.top[s], (double)sh.sum[s]) : -kInf);
             });
             wave_sync();
         }
-    }
 }
 
 template <int TYPE, bool MASK, bool BIAS>
@@ -469,24 +471,37 @@ __device__ __forceinline__ void report_tile(const ReportArgs& a, const TileRows<
     }
     if (a.top > 0) {
         wave_sync();
-        tile_lists(a, in, x, sets.id, sh);
+        prepare_lists(in, x, sets.id, sh);
+        wave_sync();
     }
 }
 
+// The tiles, one a wave at a time; or (`share`) one a workgroup, whose waves share the lists.
 template <int TYPE, bool MASK, bool BIAS>
-__global__ __launch_bounds__(kBlock, 4) void report_tile_kernel(ReportArgs a) {
+__global__ __launch_bounds__(kBlock, 3) void report_tile_kernel(ReportArgs a, bool share) {
     __shared__ ReportTile tiles[kWaves];
+    __shared__ RankGroup<kWave, kWaveList> groups[kWaves];
     __shared__ BiasShared bias;
     const int tid = (int)threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid & (kWave - 1);
     if (BIAS) stage_bias(a, bias);
-    const int step = (int)gridDim.x * kWaves;
-    for (int it = __builtin_amdgcn_readfirstlane((int)blockIdx.x * kWaves + wave); it < a.num_tiles; it += step) {
-        TileRows<TYPE, MASK, BIAS> in;
-        in.load(a, a.tiles[it], lane);
-        int32_t chosen[kTileRounds];
+    const int first = share ? (int)blockIdx.x : (int)blockIdx.x * kWaves + wave, step = (int)gridDim.x * (share ? 1 : kWaves);
+    ReportTile& sh = tiles[share ? 0 : wave];
+    for (int it = __builtin_amdgcn_readfirstlane(first); it < a.num_tiles; it += step) {
+        if (!share || wave == 0) {
+            TileRows<TYPE, MASK, BIAS> in;
+            in.load(a, a.tiles[it], lane);
+            int32_t chosen[kTileRounds];
 #pragma unroll
-        for (int r = 0; r < kTileRounds; ++r) chosen[r] = a.chosen && r * kWave + lane < in.sets ? a.chosen[in.set[r]] : -1;
-        report_tile<TYPE, MASK, BIAS>(a, in, chosen, tiles[wave], &bias);
+            for (int r = 0; r < kTileRounds; ++r) chosen[r] = a.chosen && r * kWave + lane < in.sets ? a.chosen[in.set[r]] : -1;
+            report_tile<TYPE, MASK, BIAS>(a, in, chosen, sh, &bias);
+        }
+        if (share) {
+            __syncthreads();
+            take_lists(a, sh, groups[wave], wave, kWaves);
+            __syncthreads();  // the lists have been taken
+        } else if (a.top > 0) {
+            take_lists(a, sh, groups[wave], 0, 1);
+        }
     }
 }
 
@@ -672,9 +687,7 @@ __global__ __launch_bounds__(kBlock) void report_join_kernel(ReportArgs a, const
         if (few) {
             for (int j = tid; j < n; j += kBlock) {
                 const unsigned long long key = list[j];
-                int place = 0;
-                for (int i = 0; i < n; ++i) place += list[i] > key ? 1 : 0;
-                if (place == want - 1 && key != 0) bound = key;  // keys other than 0 differ
+                if (keys_above(list, n, key) == want - 1 && key != 0) bound = key;  // keys other than 0 differ
             }
         } else {
             unsigned long long least = 0;
@@ -774,7 +787,9 @@ hipError_t launch_as(const SetLayout& s, const ReportArgs& a, hipStream_t stream
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
     if (s.num_tiles > 0) {
-        hipLaunchKernelGGL((report_tile_kernel<TYPE, MASK, BIAS>), dim3(tile_blocks(s)), dim3(kBlock), 0, stream, a);
+        const bool share = a.top > 0 && s.num_tiles <= kSharedTiles;
+        hipLaunchKernelGGL((report_tile_kernel<TYPE, MASK, BIAS>), dim3(share ? s.num_tiles : tile_blocks(s)), dim3(kBlock), 0, stream,
+                           a, share);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
     const int joins = big ? s.num_split - s.num_big : s.num_split;
