@@ -270,7 +270,7 @@ __device__ __forceinline__ void rank_list(const ReportArgs& a, const unsigned lo
 }
 
 // ------------------------------------------------------------------------------------ tiles
-struct ReportTile {
+struct alignas(16) ReportTile {
     union {
         float x[kSetTileRows];                // logits
         unsigned long long key[kSetTileRows]; // later: their ranks and the complements of their places, 0 for none
@@ -309,7 +309,8 @@ __device__ __forceinline__ void prepare_lists(const ROWS& in, const float (&x)[k
         sh.range[s] = (uint32_t)in.begin[r] | (uint32_t)in.end[r] << 16;
         sh.set[s] = in.set[r];
         sh.ranked[s] = 0;
-        behind = max(behind, in.end[r]);
+        // an empty set behind a longer one may lie past the tile's rows
+        behind = max(behind, in.end[r] > in.begin[r] ? in.end[r] : 0);
     }
     if (lane < 4) sh.range[kSetTileSets + lane] = 0;
     behind = (int)wave_max((float)behind);

@@ -115,7 +115,7 @@ __device__ __forceinline__ Slopes slopes_of(const ReportArgs& a, double sum, dou
 }
 
 // ------------------------------------------------------------------------------------ tiles
-struct SoftTile {
+struct alignas(16) SoftTile {
     float x[kSetTileRows];        // logits, then what listed and chosen rows have of their own
     float top[kSetTileSets + 4];  // per set: maximum
     union {
@@ -125,7 +125,7 @@ struct SoftTile {
     float slope[kSetTileSets + 4];  // entropies: sum of exponentials times distances, then slopes
 };
 
-struct ListTile : SoftTile {
+struct alignas(16) ListTile : SoftTile {
     float part[kSetTileRows];    // of listed rows: the teacher's terms
     double mass[kSetTileSets];   // with tail: their sums
     uint8_t slot[kSetTileRows];  // the entry that names a row, from 1; 0: none

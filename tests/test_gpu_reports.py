@@ -94,6 +94,18 @@ def test_report_lists(hip, edges, k):
     check_report(make(EDGES[edges], "bf16" if k & 1 else "f32", k % 3 == 0, k % 4 == 0, seed=k), k, 1.0)
 
 
+@pytest.mark.parametrize("lead", [0, 1, 5])
+def test_empty_sets_behind_full_tiles(hip, lead):
+    """A tile that is full to its last row, a longer set, and empty sets that still belong to the tile: they lie past its
+    rows. A few of each, and more tiles than workgroups share."""
+    for times in (3, 1100):
+        d = make(([500, 12] if lead == 0 else [lead, 500, 11 - lead] if lead == 1 else [lead, 490, 16]) + ([603, 0, 0, 512, 0, 13, 498, 700, 0] * times)
+                 + [2], "f32", True, False, seed=lead)
+        check_report(d, 3, 1.0)
+        check_backward(d, 1.0)
+        check_distill(d, 3, True, 1.0, lead)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("sizes", [[300, 7, 0, 3000, 1], [9000, 40], [70_001], [20, 20, 500, 2047]])
 def test_report_ties(hip, sizes, dtype):
