@@ -678,16 +678,41 @@ struct Heat {
     float hi, lo, low;
 };
 
-// exp(d / T) of d = z - m. EXACT: within 2 units; else the exponent is rounded once, which moves the result by at
-// most |d / T| 2^-24 of itself, in either direction. -inf gives 0, NaN stays NaN.
-template <bool EXACT>
+// exp(d / T) of d = z - m, within 2 units. -inf gives 0, NaN stays NaN.
 __device__ __forceinline__ float heat_exp(float distance, const Heat& h) {
     const float d = __builtin_elementwise_maximum(distance, h.low);  // a NaN is the larger one
-    const float t = d * h.hi;
-    if (!EXACT) return __builtin_amdgcn_exp2f(__builtin_fmaf(d, h.lo, t));
-    const float e = __builtin_amdgcn_exp2f(t), rest = __builtin_fmaf(d, h.lo, __builtin_fmaf(d, h.hi, -t));
+    const float t = d * h.hi, e = __builtin_amdgcn_exp2f(t);
+    const float rest = __builtin_fmaf(d, h.lo, __builtin_fmaf(d, h.hi, -t));
     return __builtin_fmaf(e * 0.693147182464599609375f, rest, e);
 }
+
+// The same for rows that share a maximum m, with less care (EXACT false): 2 to z hi - c, c = m hi rounded, in one operation
+// whose rounding moves the result by at most |d / T| 2^-24 of itself in either direction, and T counts as rounded to 2^-25.
+// What c's rounding adds to every exponent (`shift`, at most 2^-25 |m hi|) is taken back from the sums.
+// Where |m hi| is 2^31 and more, the next lower logit is 2^7 below m in the exponent and counts as nothing: there a power of
+// two in hi's place, which takes m to 2^63 or 2^64, leaves m's rows 0 and takes all others far below.
+template <bool EXACT>
+struct HeatRows {
+    float m, hi, c, shift;
+    __device__ __forceinline__ HeatRows(float top, const Heat& h) : m(top), hi(h.hi), c(0.0f), shift(0.0f) {
+        if (EXACT) return;
+        const bool far = !(__builtin_fabsf(top * h.hi) < 0x1p31f);
+        if (far) hi = __builtin_amdgcn_ldexpf(1.0f, 64 - __builtin_amdgcn_frexp_expf(top));
+        c = top * hi;
+        shift = far ? 0.0f : __builtin_fmaf(top, hi, -c);
+    }
+    // (z - m) / T in units of its own: bounded below, so that a product with the exponential is 0 where that is
+    __device__ __forceinline__ float distance(float z, const Heat& h) const {
+        return EXACT ? __builtin_elementwise_maximum(z - m, h.low)
+                     : __builtin_elementwise_maximum(__builtin_fmaf(z, hi, -c), -200.0f);
+    }
+    __device__ __forceinline__ float exp(float distance, const Heat& h) const {
+        return EXACT ? heat_exp(distance, h) : __builtin_amdgcn_exp2f(distance);
+    }
+    // what exponentials are multiplied by, and (the distances less the shift) to be in units of z
+    __device__ __forceinline__ float scale() const { return EXACT ? 1.0f : __builtin_amdgcn_exp2f(-shift); }
+    static __device__ __forceinline__ double unit(const Heat& h) { return EXACT ? 1.0 : 1.0 / (double)h.hi; }
+};
 
 // e^x in double within 2^-34 of itself: x = k log 2 + r, |r| <= log(2) / 2, and ten terms of r's series, those from
 // r^4 / 24 on in float. -inf gives 0, NaN and infinity give NaN.

@@ -270,20 +270,19 @@ __device__ __forceinline__ void rank_list(const ReportArgs& a, const unsigned lo
 }
 
 // ------------------------------------------------------------------------------------ tiles
-struct alignas(16) ReportTile {
-    union {
-        float x[kSetTileRows];                // logits
-        unsigned long long key[kSetTileRows]; // later: their ranks and the complements of their places, 0 for none
-    };
+struct alignas(16) SumTile {
+    float x[kSetTileRows];        // logits
     float top[kSetTileSets + 4];  // per set: maximum
     union {
         uint16_t head[kSetTileRows];  // the set that starts at a row, from 1; 0: none
         float sum[kSetTileSets + 4];  // later: sum of exponentials, then its logarithm
     };
-    union {
-        float along[kSetTileSets + 4];     // sum of exponentials times distances
-        uint32_t range[kSetTileSets + 4];  // later: first row and, 16 bits up, the row behind the last
-    };
+    float along[kSetTileSets + 4];  // sum of exponentials times distances
+};
+
+struct alignas(16) ReportTile : SumTile {
+    unsigned long long key[kSetTileRows];  // the rows' ranks and the complements of their places, 0 for none
+    uint32_t range[kSetTileSets + 4];      // first row and, 16 bits up, the row behind the last
     int32_t set[kSetTileSets + 4];
     int32_t ranked[kSetTileSets + 4];  // rows that are ranked
     uint8_t id[kSetTileRows];          // a row's set, from 1
@@ -322,7 +321,7 @@ __device__ __forceinline__ void prepare_lists(const ROWS& in, const float (&x)[k
 
 // The lists of a tile, by wave `part` of `parts`. A lane takes a row and counts the larger keys of its set, 64 rows at a
 // time, and a wave waits for its longest set; sets of more than kCountRows rows are taken by a whole wave each. (A lane with
-// eight neighbouring rows took 11 us for 37 rows, where this takes XXX.)
+// eight neighbouring rows took 11 us for 37 rows, where this takes 5.5 us.)
 __device__ __forceinline__ void take_lists(const ReportArgs& a, ReportTile& sh, RankGroup<kWave, kWaveList>& group, int part, int parts) {
     const int lane = (int)threadIdx.x & (kWave - 1), num_sets = sh.sets;
 #pragma unroll 1
@@ -391,9 +390,10 @@ __device__ __forceinline__ void take_lists(const ReportArgs& a, ReportTile& sh, 
         }
 }
 
-template <int TYPE, bool MASK, bool BIAS>
+template <bool LISTS, int TYPE, bool MASK, bool BIAS>
 __device__ __forceinline__ void report_tile(const ReportArgs& a, const TileRows<TYPE, MASK, BIAS>& in,
-                                            int32_t (&chosen)[kTileRounds], ReportTile& sh, const BiasShared* bias) {
+                                            int32_t (&chosen)[kTileRounds], std::conditional_t<LISTS, ReportTile, SumTile>& sh,
+                                            const BiasShared* bias) {
     const int lane = (int)threadIdx.x & (kWave - 1), i0 = kRun * lane;
     const Heat heat{a.heat_hi, a.heat_lo, a.heat_low};
     const bool alone = in.sets == 1;
@@ -432,7 +432,7 @@ __device__ __forceinline__ void report_tile(const ReportArgs& a, const TileRows<
         top = wave_max(top);
 #pragma unroll
         for (int k = 0; k < kRun; ++k) {
-            const float d = __builtin_elementwise_maximum(x[k] - top, heat.low), e = heat_exp<TYPE == PB_F32 || BIAS>(d, heat);
+            const float d = __builtin_elementwise_maximum(x[k] - top, heat.low), e = heat_exp(d, heat);
             sum += e;
             along += e * d;
         }
@@ -452,7 +452,7 @@ __device__ __forceinline__ void report_tile(const ReportArgs& a, const TileRows<
 #pragma unroll
         for (int k = 0; k < kRun; ++k) {
             const float d = __builtin_elementwise_maximum(x[k] - sh.top[sets.id[k] - 1], heat.low);
-            v[k] = heat_exp<TYPE == PB_F32 || BIAS>(d, heat);
+            v[k] = heat_exp(d, heat);
             w[k] = v[k] * d;
         }
         segment_reduce<TakeSum>(sets.seg, v, sets.id, lane, sh.sum);
@@ -470,39 +470,53 @@ __device__ __forceinline__ void report_tile(const ReportArgs& a, const TileRows<
             sh.sum[s] = (float)log_sum;
         }
     }
-    if (a.top > 0) {
+    if constexpr (LISTS) {
         wave_sync();
         prepare_lists(in, x, sets.id, sh);
         wave_sync();
     }
 }
 
-// The tiles, one a wave at a time; or (`share`) one a workgroup, whose waves share the lists.
 template <int TYPE, bool MASK, bool BIAS>
-__global__ __launch_bounds__(kBlock, 3) void report_tile_kernel(ReportArgs a, bool share) {
-    __shared__ ReportTile tiles[kWaves];
-    __shared__ RankGroup<kWave, kWaveList> groups[kWaves];
+struct ReportTileIn {
+    TileRows<TYPE, MASK, BIAS> rows;
+    int32_t chosen[kTileRounds];
+
+    __device__ __forceinline__ void load(const ReportArgs& a, const SetItem& im, int lane) {
+        rows.load(a, im, lane);
+#pragma unroll
+        for (int r = 0; r < kTileRounds; ++r) chosen[r] = a.chosen && r * kWave + lane < rows.sets ? a.chosen[rows.set[r]] : -1;
+    }
+};
+
+// The tiles, one a wave at a time, the first asked for before the bias is staged; or (`share`) one a workgroup, whose waves
+// share its lists.
+template <bool LISTS, int TYPE, bool MASK, bool BIAS>
+__global__ __launch_bounds__(kBlock, LISTS ? 3 : 4) void report_tile_kernel(ReportArgs a, bool share) {
+    __shared__ std::conditional_t<LISTS, ReportTile, SumTile> tiles[kWaves];
+    __shared__ RankGroup<kWave, LISTS ? kWaveList : 1> groups[kWaves];
     __shared__ BiasShared bias;
     const int tid = (int)threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid & (kWave - 1);
+    const bool one = LISTS && share;
+    const int step = (int)gridDim.x * (one ? 1 : kWaves);
+    auto& sh = tiles[one ? 0 : wave];
+    int it = __builtin_amdgcn_readfirstlane(one ? (int)blockIdx.x : (int)blockIdx.x * kWaves + wave);
+    ReportTileIn<TYPE, MASK, BIAS> in;
+    in.load(a, a.tiles[min(it, a.num_tiles - 1)], lane);
     if (BIAS) stage_bias(a, bias);
-    const int first = share ? (int)blockIdx.x : (int)blockIdx.x * kWaves + wave, step = (int)gridDim.x * (share ? 1 : kWaves);
-    ReportTile& sh = tiles[share ? 0 : wave];
-    for (int it = __builtin_amdgcn_readfirstlane(first); it < a.num_tiles; it += step) {
-        if (!share || wave == 0) {
-            TileRows<TYPE, MASK, BIAS> in;
-            in.load(a, a.tiles[it], lane);
-            int32_t chosen[kTileRounds];
-#pragma unroll
-            for (int r = 0; r < kTileRounds; ++r) chosen[r] = a.chosen && r * kWave + lane < in.sets ? a.chosen[in.set[r]] : -1;
-            report_tile<TYPE, MASK, BIAS>(a, in, chosen, sh, &bias);
+    while (it < a.num_tiles) {
+        if (!one || wave == 0) report_tile<LISTS, TYPE, MASK, BIAS>(a, in.rows, in.chosen, sh, &bias);
+        if constexpr (LISTS) {
+            if (one) {
+                __syncthreads();
+                take_lists(a, sh, groups[wave], wave, kWaves);
+                __syncthreads();  // the lists have been taken
+            } else {
+                take_lists(a, sh, groups[wave], 0, 1);
+            }
         }
-        if (share) {
-            __syncthreads();
-            take_lists(a, sh, groups[wave], wave, kWaves);
-            __syncthreads();  // the lists have been taken
-        } else if (a.top > 0) {
-            take_lists(a, sh, groups[wave], 0, 1);
-        }
+        it += step;
+        if (it < a.num_tiles) in.load(a, a.tiles[it], lane);
     }
 }
 
@@ -518,7 +532,6 @@ struct ReportGroup {
 template <int TYPE, bool MASK, bool BIAS, int THREADS, int RUNS, int LIST>
 __device__ __forceinline__ void report_pass(const ReportArgs& a, const SetItem& im, int32_t index, ReportGroup<THREADS, LIST>& sh,
                                             const BiasShared* bias) {
-    constexpr bool EXACT = kExact<TYPE, BIAS>;
     const int tid = (int)threadIdx.x & (THREADS - 1);
     const int wave0 = __builtin_amdgcn_readfirstlane(tid & ~(kWave - 1));  // the wave's first thread
     const Heat heat{a.heat_hi, a.heat_lo, a.heat_low};
@@ -559,18 +572,21 @@ __device__ __forceinline__ void report_pass(const ReportArgs& a, const SetItem& 
         if (j < live) t.top = max2(t.top, tops[j] = run_max(v[j]));
     }
     t.top = wave_max(t.top);
+    // sums alone: roundings of single rows in either direction leave them as they are
+    const HeatRows<false> rows(t.top, heat);
     float sum = 0.0f, along = 0.0f;
 #pragma unroll
     for (int j = 0; j < RUNS; ++j)
         if (j < live)
 #pragma unroll
             for (int k = 0; k < kRun; ++k) {
-                const float d = __builtin_elementwise_maximum(v[j][k] - t.top, heat.low), e = heat_exp<EXACT>(d, heat);
+                const float d = rows.distance(v[j][k], heat), e = rows.exp(d, heat);
                 sum += e;
                 along = __builtin_fmaf(e, d, along);
             }
-    t.sum = team_sum((double)sum, 6);
-    t.along = team_sum((double)along, 6);
+    const double all = team_sum((double)sum, 6), scale = (double)rows.scale();
+    t.sum = all * scale;
+    t.along = (team_sum((double)along, 6) - all * (double)rows.shift) * (scale * rows.unit(heat));
     t = join_waves<true>(a, t, sh.sums);
     const double log_sum = log_near(t.sum);
     if (tid == 0) {
@@ -753,8 +769,10 @@ int tile_blocks(const SetLayout& s) { return std::min((s.num_tiles + kWaves - 1)
 int mid_blocks(const SetLayout& s) { return std::min((s.num_mid + kWaves - 1) / kWaves, kChoiceGrid); }
 
 // Where long sets have a workgroup each: where there are so many that they fill the chip, and where there is one
-// kernel less for it.
-bool takes_big(const SetLayout& s, bool bias) { return !bias && s.num_big > 0 && (s.num_big >= kBigSets || s.num_big <= kFewSets); }
+// kernel less for it (all of them: larger ones bring the kernels of parts).
+bool takes_big(const SetLayout& s, bool bias) {
+    return !bias && s.num_big > 0 && (s.num_big >= kBigSets || (s.num_big <= kFewSets && s.num_giant == 0));
+}
 
 int num_parts(const SetLayout& s, bool bias) { return takes_big(s, bias) ? s.num_giant : s.num_wide - s.num_whole; }
 
@@ -789,8 +807,11 @@ hipError_t launch_as(const SetLayout& s, const ReportArgs& a, hipStream_t stream
     }
     if (s.num_tiles > 0) {
         const bool share = a.top > 0 && s.num_tiles <= kSharedTiles;
-        hipLaunchKernelGGL((report_tile_kernel<TYPE, MASK, BIAS>), dim3(share ? s.num_tiles : tile_blocks(s)), dim3(kBlock), 0, stream,
-                           a, share);
+        const dim3 grid(share ? s.num_tiles : tile_blocks(s));
+        if (a.top > 0)
+            hipLaunchKernelGGL((report_tile_kernel<true, TYPE, MASK, BIAS>), grid, dim3(kBlock), 0, stream, a, share);
+        else
+            hipLaunchKernelGGL((report_tile_kernel<false, TYPE, MASK, BIAS>), grid, dim3(kBlock), 0, stream, a, false);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
     const int joins = big ? s.num_split - s.num_big : s.num_split;

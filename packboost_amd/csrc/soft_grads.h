@@ -326,8 +326,8 @@ __device__ __forceinline__ void weigh_listed(const ReportArgs& a, const ListWalk
                 const int row = on ? r.begin + e.c[u] : 0;
                 on = on && sh.slot[row] == walk.entry(group, u, lane) + 1;
                 const float z = on ? sh.x[row] : -kInf, t = on ? entry_value(a, e.t[u]) : -kInf;
-                const float student = heat_exp<true>(z - l.zmax, heat);
-                const float part = !a.tail ? heat_exp<true>(t - most, heat) : on ? sh.part[row] : 0.0f;
+                const float student = heat_exp(z - l.zmax, heat);
+                const float part = !a.tail ? heat_exp(t - most, heat) : on ? sh.part[row] : 0.0f;
                 if (on) {
                     sh.x[row] = student;
                     sh.part[row] = part;
@@ -415,7 +415,7 @@ __device__ __forceinline__ void soft_tile(const ReportArgs& a, SoftTileIn<DISTIL
 #pragma unroll
         for (int k = 0; k < kRun; ++k) {
             d[k] = __builtin_elementwise_maximum(x[k] - top, heat.low);
-            sum += v[k] = heat_exp<kExact<TYPE, BIAS>>(d[k], heat);
+            sum += v[k] = heat_exp(d[k], heat);
             along += v[k] * d[k];
         }
         sum = wave_sum(sum);
@@ -432,7 +432,7 @@ __device__ __forceinline__ void soft_tile(const ReportArgs& a, SoftTileIn<DISTIL
 #pragma unroll
         for (int k = 0; k < kRun; ++k) {
             d[k] = __builtin_elementwise_maximum(x[k] - sh.top[sets.id[k] - 1], heat.low);
-            v[k] = heat_exp<kExact<TYPE, BIAS>>(d[k], heat);
+            v[k] = heat_exp(d[k], heat);
         }
         segment_reduce<TakeSum>(sets.seg, v, sets.id, lane, sh.first);
         if (!DISTILL) {
@@ -656,6 +656,7 @@ __device__ __forceinline__ void soft_pass(const ReportArgs& a, const SetItem& im
                 for (int k = 0; k < kRun; k += 2) own.top = max3(own.top, v[j][k], v[j][k + 1]);
         own.top = wave_max(own.top);
     }
+    const HeatRows<EXACT> rows(own.top, heat);
     float sum = 0.0f, along = 0.0f;
 #pragma unroll
     for (int j = 0; j < RUNS; ++j)
@@ -663,14 +664,17 @@ __device__ __forceinline__ void soft_pass(const ReportArgs& a, const SetItem& im
 #pragma unroll
             for (int k = 0; k < kRun; ++k) {
                 if (!DISTILL && PHASE == kPartGrads) continue;
-                const float d = __builtin_elementwise_maximum(v[j][k] - own.top, heat.low), e = heat_exp<EXACT>(d, heat);
+                // without the sum along, -inf needs no bound
+                const float d = DISTILL && !EXACT ? __builtin_fmaf(v[j][k], rows.hi, -rows.c) : rows.distance(v[j][k], heat);
+                const float e = rows.exp(d, heat);
                 if (PHASE != kPartGrads) sum += e;
                 if (!DISTILL) along = __builtin_fmaf(e, d, along);
                 if (DISTILL && PHASE != kPartSums) v[j][k] = e;
             }
     if (PHASE != kPartGrads) {
-        own.sum = team_sum((double)sum, 6);
-        if (!DISTILL) own.along = team_sum((double)along, 6);
+        const double all = team_sum((double)sum, 6), scale = (double)rows.scale();
+        own.sum = all * scale;
+        if (!DISTILL) own.along = (team_sum((double)along, 6) - all * (double)rows.shift) * (scale * rows.unit(heat));
         sums = join_waves<!DISTILL>(a, own, sh.sums);
     }
     if (PHASE == kPartSums) {
@@ -685,7 +689,7 @@ __device__ __forceinline__ void soft_pass(const ReportArgs& a, const SetItem& im
     if (DISTILL) {
         if (THREADS == kWave) wave_sync();
         f = list_factors<false>(a, sh.list, sums.top, sums.sum, sh.weight);
-        first = f.rest == 0.0f ? 0.0f : (float)((double)f.rest * exp_near(gap * a.inv_temp));
+        first = f.rest == 0.0f ? 0.0f : (float)((double)f.rest * exp_near(gap * a.inv_temp) * (double)rows.scale());
     } else {
         float coef = 0.0f;
         if (a.grad && sums.sum != 0.0) {
@@ -700,9 +704,10 @@ __device__ __forceinline__ void soft_pass(const ReportArgs& a, const SetItem& im
             }
         }
         const Slopes t = slopes_of(a, sums.sum, sums.along, coef, a.grad_entropy ? a.grad_entropy[g] : 0.0f);
-        const double near = exp_near(gap * a.inv_temp);
-        slope = (float)((double)t.slope * near);
-        first = near == 0.0 ? 0.0f : (float)(near * ((double)t.first + (double)t.slope * gap));
+        const double near = exp_near(gap * a.inv_temp) * (double)rows.scale();
+        const double step = rows.unit(heat);
+        slope = (float)((double)t.slope * near * step);
+        first = near == 0.0 ? 0.0f : (float)(near * ((double)t.first + (double)t.slope * (gap - (double)rows.shift * step)));
     }
 #pragma unroll
     for (int j = 0; j < RUNS; ++j) {
@@ -713,8 +718,8 @@ __device__ __forceinline__ void soft_pass(const ReportArgs& a, const SetItem& im
                 if (DISTILL) {
                     v[j][k] = first == 0.0f ? 0.0f : first * v[j][k];
                 } else {
-                    const float d = __builtin_elementwise_maximum(v[j][k] - own.top, heat.low);
-                    v[j][k] = heat_exp<EXACT>(d, heat) * __builtin_fmaf(slope, d, first);
+                    const float d = rows.distance(v[j][k], heat);
+                    v[j][k] = rows.exp(d, heat) * __builtin_fmaf(slope, d, first);
                 }
             }
             if (DISTILL && i < sp.hi) {

@@ -148,6 +148,57 @@ def test_report_of_what_is_not_finite(hip, sizes):
     assert np.isnan(step[0]) and step[1] == 0 and step[2] == -np.inf and np.isnan(step[3])
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("size,temperature", [(24.0, 2.0**-20), (24.0, 2.0**-15), (-1.5 * 2**30, 1.0), (1.5 * 2**100, 2.0**20),
+                                              (-1.5 * 2**100, 2.0**-20), (2.0**31, 1.0)])
+def test_large_logits_over_the_temperature(hip, size, temperature, dtype):
+    """Sets' rows are z or lie below it by |z| 2^-6 and more, which over the temperature is 10^4 and more: a set is the
+    uniform distribution over its best rows. The exponents' common rounding, up to S = 2^-24 |z / T| in lanes' sums of 64
+    rows and more each, leaves an entropy within 130 * 2^-24 S as long as S < 2^7, and nothing beyond."""
+    from packboost_amd import ChoiceSets, choice_report, choice_report_backward, distillation_loss
+
+    sizes = [3, 300, 1, 1500, 7000, 31_000, 60_000, 140_000]
+    sets = ChoiceSets(offsets_of(sizes), device=DEV)
+    r = np.random.default_rng(5)
+    step = r.integers(0, 4, sum(sizes)) / 64.0
+    off = np.concatenate([[0], np.cumsum(sizes)])
+    step[off[:-1]] = 0.0
+    z = size * (1.0 + step * (1 if size < 0 else -1))
+    x = torch.from_numpy(z).to(DEV).to({"f32": torch.float32, "bf16": torch.bfloat16}[dtype])
+    assert np.array_equal(x.double().cpu().numpy(), z)
+    best = np.add.reduceat((step == 0).astype(np.float64), off[:-1])
+    chosen = torch.zeros(len(sizes), dtype=torch.int32, device=DEV)
+    rep = choice_report(x, sets, chosen=chosen, temperature=temperature)
+    shift = abs(size) / temperature * 2.0**-24
+    tol = 2.0**-20 + (130 * 2.0**-24 * shift if shift < 2**8 else 0.0)
+    assert np.all(np.abs(rep.entropy.double().cpu().numpy() - np.log(best)) <= tol)
+    assert np.all(np.abs(rep.log_probs.double().cpu().numpy() + np.log(best)) <= tol)
+    lse = rep.lse.double().cpu().numpy()
+    assert np.all(np.abs(lse - size / temperature - np.log(best)) <= 2.0**-22 * abs(size / temperature))
+    ones = torch.ones(len(sizes), device=DEV)
+    p = np.where(step == 0, 1.0 / np.repeat(best, sizes), 0.0)
+    at = np.zeros(len(z))
+    at[off[:-1]] = 1.0
+    half = 2.0**-8 if dtype == "bf16" else 0.0
+    gs, _ = choice_report_backward(ones, None, x, sets, chosen=chosen, temperature=temperature)
+    want = (at - p) / temperature
+    assert np.all(np.abs(gs.double().cpu().numpy() - want) <= (tol + half) * (at + p) / temperature)
+    # the entropy's gradient is p (log p + H) / T, and log p + H is 0 but for the roundings of both
+    gs, _ = choice_report_backward(None, ones, x, sets, temperature=temperature)
+    assert np.all(np.abs(gs.double().cpu().numpy()) <= 2 * tol * p / temperature)
+    # a teacher that names the first row, and one other
+    index = torch.zeros((len(sizes), 2), dtype=torch.int32, device=DEV)
+    index[:, 1] = -1
+    value = torch.zeros((len(sizes), 2), device=DEV)
+    for tail in (False, True):
+        loss, gs, _, _ = distillation_loss(x, sets, index, value if not tail else value - 1.0 / 1024, tail=tail,
+                                           temperature=temperature)
+        if not tail:
+            assert abs(float(loss) / temperature**2 - np.log(best).sum()) <= len(sizes) * tol
+            assert np.all(np.abs(gs.double().cpu().numpy() / temperature**2 + want) <= (tol + half) * (at + p) / temperature)
+        assert torch.isfinite(gs).all()
+
+
 def check_backward(d, temperature, which="both"):
     from packboost_amd import choice_report_backward
 
