@@ -51,7 +51,7 @@ int32_t team_of(int64_t rows, int64_t sets, int64_t largest) {
 }
 
 struct Layout {
-    std::vector<SetItem> tiles, mid, whole, parts, half, big;
+    std::vector<SetItem> tiles, mid, whole, parts, half, big, shorts;
     std::vector<pb::TileSegment> segments;
     std::vector<int32_t> split;  // the first part of each split set, within `parts`
     std::vector<int32_t> giant;  // the parts of sets that are not in `half` or `big`, too, and the first of each
@@ -115,21 +115,26 @@ class TileFill {
     int64_t total_ = 0, largest_ = 0;
 };
 
+SetItem whole_set(const int64_t* off, int64_t g) {
+    SetItem im{};
+    im.row0 = off[g];
+    im.rows = (int32_t)std::min<int64_t>(off[g + 1] - off[g], pb::kSetWideRows);
+    im.set0 = (int32_t)g;
+    im.sets = im.parts = 1;
+    return im;
+}
+
 void lay_out(const int64_t* off, int64_t num_sets, bool segments, Layout& out) {
     TileFill tiles(out, segments);
     for (int64_t g = 0; g < num_sets; ++g) {
         const int64_t size = off[g + 1] - off[g];
         if (size <= pb::kSetShort) {
             tiles.add(off[g], size, g);
+            if ((int)out.shorts.size() <= pb::kSetFewShorts) out.shorts.push_back(whole_set(off, g));
             continue;
         }
         tiles.interrupt();
-        SetItem im{};
-        im.row0 = off[g];
-        im.rows = (int32_t)std::min<int64_t>(size, pb::kSetWideRows);
-        im.set0 = (int32_t)g;
-        im.sets = 1;
-        im.parts = 1;
+        SetItem im = whole_set(off, g);
         if ((off[g] & 7) + size <= pb::kSetMidRows) {
             out.mid.push_back(im);
         } else if ((off[g] & 7) + size <= pb::kSetWideRows) {
@@ -155,6 +160,7 @@ void lay_out(const int64_t* off, int64_t num_sets, bool segments, Layout& out) {
         }
     }
     tiles.flush();
+    if ((int)out.shorts.size() > pb::kSetFewShorts || out.mid.size() + out.whole.size() + out.parts.size() == 0) out.shorts.clear();
 }
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
@@ -177,6 +183,8 @@ int sets_create(const int64_t* off, int64_t num_sets, bool segments, pb_sets** o
     const size_t wide_end = items.size(), half = lay.half.size();
     items.insert(items.end(), lay.half.begin(), lay.half.end());
     items.insert(items.end(), lay.big.begin(), lay.big.end());
+    const size_t big_end = items.size();
+    items.insert(items.end(), lay.shorts.begin(), lay.shorts.end());
     for (int32_t& first : lay.split) first += (int32_t)(mid + whole);
     for (int32_t& part : lay.giant) part += (int32_t)(mid + whole);
     for (int32_t& part : lay.giant_split) part += (int32_t)(mid + whole);
@@ -213,7 +221,9 @@ int sets_create(const int64_t* off, int64_t num_sets, bool segments, pb_sets** o
     h->s.num_whole = (int32_t)whole;
     h->s.num_split = (int32_t)num_split;
     h->s.big = h->s.tiles + wide_end;
-    h->s.num_big = (int32_t)(items.size() - wide_end);
+    h->s.num_big = (int32_t)(big_end - wide_end);
+    h->s.shorts = h->s.tiles + big_end;
+    h->s.num_shorts = (int32_t)lay.shorts.size();
     h->s.num_half = (int32_t)half;
     h->s.giant = h->s.split + num_split;
     h->s.num_giant = (int32_t)lay.giant.size();

@@ -512,6 +512,8 @@ constexpr int kSetWideRows = 8192;
 // parts of the others.
 constexpr int kSetHalfBig = 32768;
 constexpr int kSetBig = 65536;
+// Short sets beside longer ones: up to so many are listed one by one, too (`shorts`), for the waves that take the mid sets.
+constexpr int kSetFewShorts = 256;
 struct SetItem {
     int64_t row0;
     int32_t rows;
@@ -539,9 +541,11 @@ struct SetLayout {
     const SetItem* big;    // [num_big], the first num_half of at most kSetHalfBig rows
     const int32_t* giant;  // [num_giant], indices of wide items
     const int32_t* giant_split;  // [num_split - num_big], the first of each set's
+    const SetItem* shorts;  // [num_shorts]: the short sets one by one, where a few of them lie beside longer ones; else none
     int32_t num_big;
     int32_t num_half;
     int32_t num_giant;
+    int32_t num_shorts;
     int32_t num_tiles;
     int32_t num_mid;
     int32_t num_wide;

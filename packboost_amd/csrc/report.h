@@ -17,6 +17,8 @@ struct ReportArgs : ChoiceArgs {
     float temp;
     float heat_hi, heat_lo, heat_low;  // log2(e) / T in two parts; see Heat
     int32_t top;                       // entries of each set's list
+    int32_t num_shorts;                // sets that waves take behind the mid ones, instead of tiles
+    const SetItem* shorts;
     int32_t team_bits;                 // 1 << team_bits lanes take it
     SoftSums* part_sums;               // of the parts of split sets, by wide item
     unsigned long long* part_keys;     // [top] of each, best first

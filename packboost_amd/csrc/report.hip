@@ -492,7 +492,7 @@ struct ReportTileIn {
 // The tiles, one a wave at a time, the first asked for before the bias is staged; or (`share`) one a workgroup, whose waves
 // share its lists.
 template <bool LISTS, int TYPE, bool MASK, bool BIAS>
-__global__ __launch_bounds__(kBlock, LISTS ? 3 : 4) void report_tile_kernel(ReportArgs a, bool share) {
+__global__ __launch_bounds__(kBlock, LISTS ? 3 : 5) void report_tile_kernel(ReportArgs a, bool share) {
     __shared__ std::conditional_t<LISTS, ReportTile, SumTile> tiles[kWaves];
     __shared__ RankGroup<kWave, LISTS ? kWaveList : 1> groups[kWaves];
     __shared__ BiasShared bias;
@@ -623,7 +623,7 @@ __device__ __forceinline__ void report_pass(const ReportArgs& a, const SetItem& 
 // Workgroups [0, mid_blocks) take the sets for a wave, the others those for a workgroup, then the parts (all from num_mid +
 // num_whole on, or those in `list`), one at a time.
 template <int TYPE, bool MASK, bool BIAS>
-__global__ __launch_bounds__(kBlock) void report_wide_kernel(ReportArgs a, int mid_blocks, int num_parts,
+__global__ __launch_bounds__(kBlock, BIAS ? 3 : MASK || TYPE == PB_F16 ? 4 : 5) void report_wide_kernel(ReportArgs a, int mid_blocks, int num_parts,
                                                              const int32_t* __restrict__ list) {
     __shared__ union {
         ReportGroup<kWave, kWaveList> mid[kWaves];
@@ -633,8 +633,8 @@ __global__ __launch_bounds__(kBlock) void report_wide_kernel(ReportArgs a, int m
     if (BIAS) stage_bias(a, bias);
     if ((int)blockIdx.x < mid_blocks) {
         const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), step = mid_blocks * kWaves;
-        for (int it = (int)blockIdx.x * kWaves + wave; it < a.num_mid; it += step)
-            report_pass<TYPE, MASK, BIAS, kWave, kWideRuns, kWaveList>(a, a.wide[it], it, sh.mid[wave], &bias);
+        for (int it = (int)blockIdx.x * kWaves + wave; it < a.num_mid + a.num_shorts; it += step)
+            report_pass<TYPE, MASK, BIAS, kWave, kWideRuns, kWaveList>(a, wave_item(a, it), it, sh.mid[wave], &bias);
     } else {
         const int n = a.num_whole + num_parts;
         for (int k = (int)blockIdx.x - mid_blocks; k < n; k += (int)gridDim.x - mid_blocks) {
@@ -764,9 +764,9 @@ __global__ __launch_bounds__(kBlock) void report_join_kernel(ReportArgs a, const
     });
 }
 
-int tile_blocks(const SetLayout& s) { return std::min((s.num_tiles + kWaves - 1) / kWaves, kChoiceGrid); }
+int tile_blocks(const SetLayout& s) { return s.num_shorts > 0 ? 0 : std::min((s.num_tiles + kWaves - 1) / kWaves, kChoiceGrid); }
 
-int mid_blocks(const SetLayout& s) { return std::min((s.num_mid + kWaves - 1) / kWaves, kChoiceGrid); }
+int mid_blocks(const SetLayout& s) { return std::min((s.num_mid + s.num_shorts + kWaves - 1) / kWaves, kChoiceGrid); }
 
 // Where long sets have a workgroup each: where there are so many that they fill the chip, and where there is one
 // kernel less for it (all of them: larger ones bring the kernels of parts).
@@ -805,7 +805,7 @@ hipError_t launch_as(const SetLayout& s, const ReportArgs& a, hipStream_t stream
                            big ? s.giant : nullptr);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
-    if (s.num_tiles > 0) {
+    if (tile_blocks(s) > 0) {
         const bool share = a.top > 0 && s.num_tiles <= kSharedTiles;
         const dim3 grid(share ? s.num_tiles : tile_blocks(s));
         if (a.top > 0)
@@ -840,6 +840,8 @@ hipError_t launch_report(const SetLayout& s, ReportArgs a, int32_t type, char* w
     a.wide = s.wide;
     a.segments = s.segments;
     a.num_tiles = s.num_tiles;
+    a.shorts = s.shorts;
+    a.num_shorts = s.num_shorts;
     a.num_wide = s.num_wide;
     a.num_mid = s.num_mid;
     a.num_whole = s.num_whole;

@@ -22,6 +22,8 @@ hipError_t launch_soft_grads(bool distill, const SetLayout& s, ReportArgs a, int
     a.wide = s.wide;
     a.segments = s.segments;
     a.num_tiles = s.num_tiles;
+    a.shorts = s.shorts;
+    a.num_shorts = s.num_shorts;
     a.num_wide = s.num_wide;
     a.num_mid = s.num_mid;
     a.num_whole = s.num_whole;

@@ -447,6 +447,7 @@ __device__ __forceinline__ void soft_tile(const ReportArgs& a, SoftTileIn<DISTIL
         weigh_listed(a, walk, all, sh, lane, tally);
         wave_sync();
         float e[kRun], part[kRun];
+        slots = *reinterpret_cast<const uint2*>(&sh.slot[i0]);  // again: two registers less meanwhile
         const bool any = (slots.x | slots.y) != 0;
         if (any) {
             read_run(&sh.x[i0], e);
@@ -768,7 +769,7 @@ __global__ __launch_bounds__(kBlock) void soft_part_kernel(ReportArgs a, int fir
 // The longer sets: workgroups [0, mid_blocks) take those for a wave, the others those for a workgroup, then the parts (all
 // from num_mid + num_whole on, or those in `list`), one at a time.
 template <bool DISTILL, int TYPE, bool MASK, bool BIAS>
-__global__ __launch_bounds__(kBlock) void soft_wide_kernel(ReportArgs a, int mid_blocks, int num_parts, const int32_t* __restrict__ list,
+__global__ __launch_bounds__(kBlock, BIAS ? 2 : MASK ? 3 : DISTILL || TYPE != PB_F32 ? 4 : 5) void soft_wide_kernel(ReportArgs a, int mid_blocks, int num_parts, const int32_t* __restrict__ list,
                                                            int first_block) {
     __shared__ union {
         SoftGroup<kWave, kListRows<DISTILL, kWave, kWideRuns>> mid[kWaves];
@@ -789,8 +790,8 @@ __global__ __launch_bounds__(kBlock) void soft_wide_kernel(ReportArgs a, int mid
     double tally[3] = {0.0, 0.0, 0.0};
     if ((int)blockIdx.x < mid_blocks) {
         const int step = mid_blocks * kWaves;
-        for (int it = __builtin_amdgcn_readfirstlane((int)blockIdx.x * kWaves + wave); it < a.num_mid; it += step)
-            soft_pass<DISTILL, TYPE, MASK, BIAS, kWave, kWideRuns, kWholeSet>(a, a.wide[it], it, sh.mid[wave], &bias, table, tally);
+        for (int it = __builtin_amdgcn_readfirstlane((int)blockIdx.x * kWaves + wave); it < a.num_mid + a.num_shorts; it += step)
+            soft_pass<DISTILL, TYPE, MASK, BIAS, kWave, kWideRuns, kWholeSet>(a, wave_item(a, it), it, sh.mid[wave], &bias, table, tally);
     } else {
         const int n = a.num_whole + num_parts;
         for (int k = (int)blockIdx.x - mid_blocks; k < n; k += (int)gridDim.x - mid_blocks) {
@@ -826,9 +827,9 @@ constexpr int kBigSets = 1024;
 
 bool takes_big(const SetLayout& s, bool bias) { return !bias && s.num_big >= kBigSets; }
 
-int tile_blocks(const SetLayout& s) { return std::min((s.num_tiles + kWaves - 1) / kWaves, kChoiceGrid); }
+int tile_blocks(const SetLayout& s) { return s.num_shorts > 0 ? 0 : std::min((s.num_tiles + kWaves - 1) / kWaves, kChoiceGrid); }
 
-int mid_blocks(const SetLayout& s) { return std::min((s.num_mid + kWaves - 1) / kWaves, kChoiceGrid); }
+int mid_blocks(const SetLayout& s) { return std::min((s.num_mid + s.num_shorts + kWaves - 1) / kWaves, kChoiceGrid); }
 
 int num_parts(const SetLayout& s, bool bias) { return takes_big(s, bias) ? s.num_giant : s.num_wide - s.num_whole; }
 
@@ -860,7 +861,7 @@ hipError_t launch_as(const SetLayout& s, const ReportArgs& a, hipStream_t stream
             if ((e = hipGetLastError()) != hipSuccess) return e;
         }
     }
-    if (s.num_tiles > 0) {
+    if (tile_blocks(s) > 0) {
         hipLaunchKernelGGL((soft_tile_kernel<DISTILL, TYPE, MASK, BIAS>), dim3(tile_blocks(s)), dim3(kBlock), 0, stream, a);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }

@@ -148,6 +148,20 @@ def test_report_of_what_is_not_finite(hip, sizes):
     assert np.isnan(step[0]) and step[1] == 0 and step[2] == -np.inf and np.isnan(step[3])
 
 
+@pytest.mark.parametrize("dtype,masked,biased", [("f32", True, True), ("bf16", False, False), ("f16", True, False)])
+@pytest.mark.parametrize("few", [1, 255, 256, 257])
+def test_few_short_sets_beside_longer_ones(hip, few, dtype, masked, biased):
+    """Up to 256 short sets are taken by the waves of the longer ones, more by tiles; empty ones, single rows and the
+    largest that are short are among them."""
+    r = np.random.default_rng(few)
+    short = ([0, 1, 504, 505 - 1, 2, 0] + r.integers(0, 120, 300).tolist())[:few] if few > 1 else [5]
+    sizes = short[: few // 2] + [700, 20_000] + short[few // 2:] + [9000, 2500]
+    d = make(sizes, dtype, masked, biased, seed=few)
+    check_report(d, 6, 1.0)
+    check_backward(d, 1.3)
+    check_distill(d, 6, few % 2 == 0, 1.0, few)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("size,temperature", [(24.0, 2.0**-20), (24.0, 2.0**-15), (-1.5 * 2**30, 1.0), (1.5 * 2**100, 2.0**20),
                                               (-1.5 * 2**100, 2.0**-20), (2.0**31, 1.0)])
