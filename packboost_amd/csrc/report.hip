@@ -666,7 +666,7 @@ __device__ __forceinline__ uint32_t block_count(uint32_t v, uint32_t* sh) {
 // reach with all of their entries and the others with fewer than d of them, 64 x 64 at most.
 template <int TYPE, bool MASK, bool BIAS>
 __global__ __launch_bounds__(kBlock) void report_join_kernel(ReportArgs a, const int32_t* __restrict__ firsts) {
-    constexpr int kAhead = 8;
+    constexpr int kAhead = 8, kHeld = 8;
     __shared__ unsigned long long list[kJoinList], bound;
     __shared__ uint32_t shc[kWaves], size;
     __shared__ GroupSums<kWaves> sums;
@@ -680,23 +680,29 @@ __global__ __launch_bounds__(kBlock) void report_join_kernel(ReportArgs a, const
     const unsigned long long* keys = a.part_keys + (int64_t)first * a.top;
     const int d = (a.top + n - 1) / n, want = d > 0 ? (a.top + d - 1) / d : 0;
     const bool bounded = (int64_t)n * a.top > kBlock, few = n <= kBoundParts;
+    // up to 2048 entries are all asked for at once, before it is known which of them count
+    const bool held = (int64_t)n * a.top <= kHeld * kBlock;
+    unsigned long long own[kHeld];
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u) own[u] = held && u * kBlock + tid < n * a.top ? keys[u * kBlock + tid] : 0ull;
     if (bounded && few)
         for (int j = tid; j < n; j += kBlock) list[j] = keys[(int64_t)j * a.top + d - 1];
     if (tid == 0) {
         size = 0;
         bound = 0;
     }
+    bool counts = false;
+    float z = 0.0f;
+    if (tid == 0 && a.chosen) {
+        const int32_t c = a.chosen[g];
+        counts = c >= 0 && c < a.off[g + 1] - r0;
+        if (MASK && counts) counts = a.mask[r0 + c] != 0;
+        if (!BIAS && counts) z = one_logit<TYPE, BIAS>(a, &bias, r0 + c);
+    }
     const SoftSums t = join_set<true>(a, a.part_sums + first, n, sums);  // a barrier within
     const double log_sum = log_near(t.sum);
     if (tid == 0) {
-        bool counts = false;
-        float z = 0.0f;
-        if (a.chosen) {
-            const int32_t c = a.chosen[g];
-            counts = c >= 0 && c < a.off[g + 1] - r0;
-            if (MASK && counts) counts = a.mask[r0 + c] != 0;
-            if (counts) z = one_logit<TYPE, BIAS>(a, &bias, r0 + c);
-        }
+        if (BIAS && counts) z = one_logit<TYPE, BIAS>(a, &bias, r0 + (int64_t)a.chosen[g]);
         put_report(a, g, t, log_sum, counts, z);
     }
     if (a.top == 0) return;
@@ -721,7 +727,11 @@ __global__ __launch_bounds__(kBlock) void report_join_kernel(ReportArgs a, const
     // a part's entries down to the bound, kAhead asked for at a time
     const unsigned long long least = bound;
     __syncthreads();
-    for (int j = tid; j < n; j += kBlock) {
+    if (held)
+#pragma unroll
+        for (int u = 0; u < kHeld; ++u)
+            if (own[u] != 0 && own[u] >= least) list[atomicAdd(&size, 1u)] = own[u];
+    for (int j = held ? n : tid; j < n; j += kBlock) {
         const unsigned long long* mine = keys + (int64_t)j * a.top;
         bool more = true;
         for (int e = 0; more && e < a.top; e += kAhead) {
