@@ -18,14 +18,23 @@
 namespace pb {
 namespace {
 
-constexpr int kCountRows = 192;   // rows of a tile's set whose rows count what ranks above them
-constexpr int kWaveList = 256;    // rows that reach the bound: room for a wave's
-constexpr int kGroupList = 512;   // and a workgroup's
+// Rows of a tile's set whose rows count what ranks above them; of a longer one the wave finds a bound. 1M rows in sets of
+// one size, counted / by a bound: 40 rows 20 / 52 us, 64 20 / 27, 80 27 / 23, 96 30 / 20, 192 37 / 12, 384 58 / 9. With sizes
+// about 12.5 on average, where the few longer ones hold up their tiles, 64 costs 11 us and 192 costs 10.
+constexpr int kCountRows = 80;
+constexpr int kWaveList = 256;   // rows that reach the bound: room for a wave's
+constexpr int kGroupList = 512;  // and a workgroup's
 constexpr int kJoinList = kMaxTop * kMaxTop;
-constexpr int kSharedTiles = 1024; // up to so many tiles a workgroup each
-constexpr int kBigSets = 1024;     // from so many long sets on a workgroup to each beats parts,
-constexpr int kFewSets = 8;        // and up to so many
-constexpr int kBoundParts = 1024;  // parts whose bound is found by counting
+// Up to so many tiles have a workgroup each, whose waves share the lists, else a wave each: 64 tiles of 21 sets 7 / 11 us,
+// 512 7.8 / 11.4, 1024 13.7 / 11.7, 4096 38 / 25.
+constexpr int kSharedTiles = 512;
+// Long sets have a workgroup each where nothing else is there for the kernel of parts (4 sets of 30 thousand 16-bit rows
+// 9 us, in parts 12; 256 sets 11 and 15; 2048 sets 45 and 68), and beside others from so many on: parts add 27 us to what
+// that kernel takes for 1024 sets, as much as a launch of their own.
+constexpr int kBigSets = 1024;
+constexpr int kOneLaunch = 256;  // as many of mixed lengths as fit beside each other go in one launch
+// Parts whose bound is found by counting, not bit by bit: 256 parts 20 / 48 us, 1024 85 / 87, 2048 276 / 140.
+constexpr int kBoundParts = 1024;
 
 // Orders logits as whole numbers: larger first, -0 as 0, NaN above all; 0 for what is not ranked.
 __device__ __forceinline__ uint32_t rank_of(float z) {
@@ -778,10 +787,9 @@ int tile_blocks(const SetLayout& s) { return s.num_shorts > 0 ? 0 : std::min((s.
 
 int mid_blocks(const SetLayout& s) { return std::min((s.num_mid + s.num_shorts + kWaves - 1) / kWaves, kChoiceGrid); }
 
-// Where long sets have a workgroup each: where there are so many that they fill the chip, and where there is one
-// kernel less for it (all of them: larger ones bring the kernels of parts).
 bool takes_big(const SetLayout& s, bool bias) {
-    return !bias && s.num_big > 0 && (s.num_big >= kBigSets || (s.num_big <= kFewSets && s.num_giant == 0));
+    const bool alone = s.num_mid + s.num_shorts + s.num_whole + s.num_giant == 0;
+    return !bias && s.num_big > 0 && (alone || s.num_big >= kBigSets);
 }
 
 int num_parts(const SetLayout& s, bool bias) { return takes_big(s, bias) ? s.num_giant : s.num_wide - s.num_whole; }
@@ -792,21 +800,14 @@ hipError_t launch_as(const SetLayout& s, const ReportArgs& a, hipStream_t stream
     const bool big = takes_big(s, BIAS);
     const int parts = num_parts(s, BIAS);
     if constexpr (!BIAS) {
-        // the first kernels have the most lanes to a set, where there are few
-        const bool few = s.num_big <= kFewSets;
-        const int half = few ? 0 : s.num_half;
-        if (big && few) {
-            hipLaunchKernelGGL((report_big_kernel<TYPE, MASK, 1024, 8>), dim3(s.num_big), dim3(1024), 0, stream, a, s.big);
+        const int half = s.num_half < s.num_big && s.num_big <= kOneLaunch ? 0 : s.num_half;
+        if (big && s.num_big > half) {
+            hipLaunchKernelGGL((report_big_kernel<TYPE, MASK, 1024, 8>), dim3(s.num_big - half), dim3(1024), 0, stream, a, s.big + half);
             if ((e = hipGetLastError()) != hipSuccess) return e;
-        } else if (big) {
-            if (s.num_big > half) {
-                hipLaunchKernelGGL((report_big_kernel<TYPE, MASK, 1024, 8>), dim3(s.num_big - half), dim3(1024), 0, stream, a, s.big + half);
-                if ((e = hipGetLastError()) != hipSuccess) return e;
-            }
-            if (half > 0) {
-                hipLaunchKernelGGL((report_big_kernel<TYPE, MASK, 512, 8>), dim3(half), dim3(512), 0, stream, a, s.big);
-                if ((e = hipGetLastError()) != hipSuccess) return e;
-            }
+        }
+        if (big && half > 0) {
+            hipLaunchKernelGGL((report_big_kernel<TYPE, MASK, 512, 8>), dim3(half), dim3(512), 0, stream, a, s.big);
+            if ((e = hipGetLastError()) != hipSuccess) return e;
         }
     }
     const int wide = mid_blocks(s) + std::min(s.num_whole + parts, kChoiceGrid);

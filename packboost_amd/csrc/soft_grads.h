@@ -822,10 +822,16 @@ __global__ __launch_bounds__(THREADS, 4) void soft_big_kernel(ReportArgs a, cons
     }
 }
 
-// From how many sets on a workgroup to each of them beats parts.
-constexpr int kBigSets = 1024;
+// Long sets have a workgroup each where nothing else is there for the kernels of parts (bfloat16 sets of 30 thousand rows,
+// with a teacher / without: 16 sets 10.7 / 8.2 us, in parts 14.3 / 8.9; 256 14 / 11 and 22 / 17; 2048 58 / 55 and 100 / 80),
+// and beside others from so many on: 512 take 21 / 18 us, and add 28 / 23 in parts; 256 add about as much as they take.
+constexpr int kBigSets = 512;
+constexpr int kOneLaunch = 256;  // as many of mixed lengths as fit beside each other go in one launch
 
-bool takes_big(const SetLayout& s, bool bias) { return !bias && s.num_big >= kBigSets; }
+bool takes_big(const SetLayout& s, bool bias) {
+    const bool alone = s.num_mid + s.num_shorts + s.num_whole + s.num_giant == 0;
+    return !bias && s.num_big > 0 && (alone || s.num_big >= kBigSets);
+}
 
 int tile_blocks(const SetLayout& s) { return s.num_shorts > 0 ? 0 : std::min((s.num_tiles + kWaves - 1) / kWaves, kChoiceGrid); }
 
@@ -850,14 +856,14 @@ hipError_t launch_as(const SetLayout& s, const ReportArgs& a, hipStream_t stream
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
     if constexpr (!BIAS) {
-        const int rest = s.num_big - s.num_half, first_block = a.blocks - s.num_big;
-        if (big && rest > 0) {
-            hipLaunchKernelGGL((soft_big_kernel<DISTILL, TYPE, MASK, 1024>), dim3(rest), dim3(1024), 0, stream, a, s.big + s.num_half,
-                               first_block + s.num_half);
+        const int half = s.num_half < s.num_big && s.num_big <= kOneLaunch ? 0 : s.num_half, first_block = a.blocks - s.num_big;
+        if (big && s.num_big > half) {
+            hipLaunchKernelGGL((soft_big_kernel<DISTILL, TYPE, MASK, 1024>), dim3(s.num_big - half), dim3(1024), 0, stream, a, s.big + half,
+                               first_block + half);
             if ((e = hipGetLastError()) != hipSuccess) return e;
         }
-        if (big && s.num_half > 0) {
-            hipLaunchKernelGGL((soft_big_kernel<DISTILL, TYPE, MASK, 512>), dim3(s.num_half), dim3(512), 0, stream, a, s.big, first_block);
+        if (big && half > 0) {
+            hipLaunchKernelGGL((soft_big_kernel<DISTILL, TYPE, MASK, 512>), dim3(half), dim3(512), 0, stream, a, s.big, first_block);
             if ((e = hipGetLastError()) != hipSuccess) return e;
         }
     }
