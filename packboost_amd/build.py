@@ -55,7 +55,8 @@ NO_SCRATCH = re.compile(r"hist_era_kernel|seg_score_kernel|des_score|kcuts_kerne
 # Kernels that must not spill vector registers: the choice operators'. (The policy's wide_kernel with a bias has
 # 36 bytes of scratch reserved, for kernel arguments that end in lanes of a vector register; nothing in it is
 # read or written.)
-NO_SPILLS = re.compile(r"\d(?:(?:report_|soft_)?(?:tile|wide|part|big|join)|part_grads|part_far|split_steps)_kernel")
+NO_SPILLS = re.compile(r"\d(?:(?:report_|soft_)?(?:tile|wide|part)|part_grads|part_far|split_steps|report_join|"
+                       r"(?:report|soft)_big)_kernel")
 
 
 def spilling_kernels(remarks: str) -> list[str]:

@@ -499,7 +499,9 @@ struct ReportTileIn {
 };
 
 // The tiles, one a wave at a time, the first asked for before the bias is staged; or (`share`) one a workgroup, whose waves
-// share its lists.
+// share its lists. Bound by the chain of a tile (loads, scans, lists) and by instructions: 100 thousand masked sets of 24
+// rows with a bias 10.3 us (683 vector instructions a wave; 12.1 at 4 waves a SIMD), 16 thousand of 12 with lists of 8 12.3,
+// one of 37 rows 6.
 template <bool LISTS, int TYPE, bool MASK, bool BIAS>
 __global__ __launch_bounds__(kBlock, LISTS ? 3 : 5) void report_tile_kernel(ReportArgs a, bool share) {
     __shared__ std::conditional_t<LISTS, ReportTile, SumTile> tiles[kWaves];
@@ -630,7 +632,9 @@ __device__ __forceinline__ void report_pass(const ReportArgs& a, const SetItem& 
 }
 
 // Workgroups [0, mid_blocks) take the sets for a wave, the others those for a workgroup, then the parts (all from num_mid +
-// num_whole on, or those in `list`), one at a time.
+// num_whole on, or those in `list`), one at a time. 30M bfloat16 rows of 17 thousand sets in 30 us (33 at 4 waves a SIMD, which
+// is what masks, a bias and float16 have registers for): vector instructions are issued in two thirds of the time. Parts
+// with lists of 64 12 us for 20 MB, a chain of a workgroup: rows, sums, bound, list.
 template <int TYPE, bool MASK, bool BIAS>
 __global__ __launch_bounds__(kBlock, BIAS ? 3 : MASK || TYPE == PB_F16 ? 4 : 5) void report_wide_kernel(ReportArgs a, int mid_blocks, int num_parts,
                                                              const int32_t* __restrict__ list) {
@@ -653,7 +657,9 @@ __global__ __launch_bounds__(kBlock, BIAS ? 3 : MASK || TYPE == PB_F16 ? 4 : 5) 
     }
 }
 
-// Sets of up to THREADS * RUNS * 8 rows, a workgroup each.
+// Sets of up to THREADS * RUNS * 8 rows, a workgroup each. Bound by instructions: 4096 sets of 32 thousand bfloat16 rows with
+// lists of 8 in 88 us (3.0 TB/s), 1156 vector instructions a wave of 64 rows a lane, 78 % of the time. One such set: 10.8 us
+// (11.2 with 1024 lanes).
 template <int TYPE, bool MASK, int THREADS, int RUNS>
 __global__ __launch_bounds__(THREADS, 4) void report_big_kernel(ReportArgs a, const SetItem* __restrict__ items) {
     __shared__ ReportGroup<THREADS, kGroupList> sh;
@@ -672,7 +678,8 @@ __device__ __forceinline__ uint32_t block_count(uint32_t v, uint32_t* sh) {
 
 // The sets in parts, a workgroup each: sums and lists from those of the parts. With d = top / parts, rounded up, entry d of
 // a part says that d of its rows rank as high: the bound is the (top / d)-th largest of these, which at most top / d parts
-// reach with all of their entries and the others with fewer than d of them, 64 x 64 at most.
+// reach with all of their entries and the others with fewer than d of them, 64 x 64 at most. A chain of loads and counts:
+// 22 sets in 600 parts with lists of 64 take 10 us (13 with the entries asked for after the bound), without lists 4.5.
 template <int TYPE, bool MASK, bool BIAS>
 __global__ __launch_bounds__(kBlock) void report_join_kernel(ReportArgs a, const int32_t* __restrict__ firsts) {
     constexpr int kAhead = 8, kHeld = 8;

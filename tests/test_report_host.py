@@ -55,3 +55,14 @@ def test_distillation_objective_checks():
                 dict(teacher_index=np.zeros((2, 65), int), teacher_logits=np.zeros((2, 65))), dict(mask=np.ones(4, bool))):
         with pytest.raises(ValueError):
             DistillationObjective([0, 4, 9], **{**dict(teacher_index=index, teacher_logits=logits), **bad})
+
+
+def test_build_refuses_spills_of_the_report_kernels():
+    from packboost_amd.build import spilling_kernels
+
+    names = ["_ZN2pb12_GLOBAL__N_118report_tile_kernelILb1E", "_ZN2pb12_GLOBAL__N_116soft_wide_kernelILb1E",
+             "_ZN2pb12_GLOBAL__N_118report_join_kernelILi0E", "_ZN2pb12_GLOBAL__N_115soft_big_kernelILb1E"]
+    remarks = lambda spill: "\n".join(f"x.hip:1:0: remark:     {v} [-Rpass-analysis=kernel-resource-usage]" for n in names for v in
+                                      (f"Function Name: {n}", "ScratchSize [bytes/lane]: 0", f"VGPRs Spill: {spill}"))
+    assert spilling_kernels(remarks(0)) == []
+    assert spilling_kernels(remarks(2)) == names
