@@ -7,7 +7,8 @@
 // are not ranked.
 //
 // Rows are laid out and read as choice.hip has them, each once: tiles of short sets by a wave, longer sets by a wave or a
-// workgroup that holds them in registers, what is longer still in parts that a second kernel joins. In a tile, a row of
+// workgroup that holds them in registers (of up to 65536 rows where that pays, see kBigSets), what is longer still in parts
+// that a second kernel joins. In a tile, a row of
 // a short set counts the rows that rank above it. Of longer sets a bound is found first that at least as many rows reach as
 // are listed, from the maxima of the lanes; the few rows that reach it are gathered and ranked by counting.
 #include <algorithm>

@@ -14,7 +14,8 @@
 // teacher's entries or the student have no probability are left out.
 //
 // Rows are laid out, read and written as choice.hip has them: tiles of short sets by a wave, longer sets by a wave or a
-// workgroup that holds them in registers, what is longer still in parts that are read twice. A set's list is taken by as many
+// workgroup that holds them in registers (of up to 65536 rows where that pays, see kBigSets), what is longer still in parts
+// that are read twice. A set's list is taken by as many
 // lanes as it has entries, rounded up to a power of 2; a byte a row in LDS says which entry names it.
 #pragma once
 

@@ -618,6 +618,50 @@ def test_replayed_and_beside_each_other(hip):
                 assert torch.equal(x, y)
 
 
+@pytest.mark.parametrize("dtype,masked", [("f32", True), ("bf16", False)])
+@pytest.mark.parametrize("sizes", [[9000], [33_000], [65_530, 9001], [9000, 33_000] * 130, [0] * 4100 + [12_000, 40_000, 3]])
+def test_long_sets_alone(hip, sizes, dtype, masked):
+    """Sets of more than 8192 and at most 65536 rows with nothing else for the kernels of parts: one workgroup each, in
+    one launch and in two, and beside tiles."""
+    d = make(sizes, dtype, masked, False, seed=len(sizes))
+    check_report(d, 9, 0.8)
+    check_backward(d, 1.0)
+    check_distill(d, 9, masked, 1.0, 3)
+
+
+def test_long_sets_replayed_on_two_streams(hip):
+    """Captured and eager calls at once, on layouts of one workgroup to a set and of few short sets beside longer ones."""
+    from packboost_amd import choice_report, choice_report_backward, distillation_loss
+
+    for sizes in ([30_000, 64_000, 9000], [7, 0, 30_000, 700, 5, 9000]):
+        d = make(sizes, "bf16", False, False, seed=30)
+        index, value = (t.to(DEV) for t in (lambda p: (torch.from_numpy(p[0]), p[1]))(teacher_of(d, 5, False, 1.0, 31)))
+        g = torch.linspace(-1, 1, len(sizes), device=DEV)
+
+        def calls(z):
+            rep = choice_report(z, d["sets"], chosen=d["chosen"], top=5)
+            gs, _ = choice_report_backward(g, g, z, d["sets"], chosen=d["chosen"])
+            return [*rep, gs, *(v for v in distillation_loss(z, d["sets"], index, value) if v is not None)]
+
+        z, other = d["scores"].clone(), d["scores"] * 0.5
+        want_other = calls(other)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = calls(z)
+        side = torch.cuda.Stream()
+        for k in range(4):
+            z.copy_(d["scores"] * (1.0 + 0.5 * k))
+            want = calls(z)
+            torch.cuda.synchronize()
+            graph.replay()
+            with torch.cuda.stream(side):
+                got_other = calls(other)
+            torch.cuda.synchronize()
+            for x, y in [*zip(held, want), *zip(got_other, want_other)]:
+                assert torch.equal(x, y)
+
+
 def test_teacher_to_student(hip):
     """The run together: a report of the teacher's scores is what the student is distilled from; a student with the
     teacher's own scores has no divergence and no gradient."""
