@@ -633,7 +633,7 @@ int pb_policy_loss(const pb_sets* sets, const pb_choice_scores* scores, const pb
  * largest logit by their index within the set, and their log p; equal logits (as float32, the bias added) by index, NaN above
  * all. Rows left out and rows of logit -inf are not listed; behind the last row stand -1 and -inf. Sets of more than
  * 2^31 - 1 rows have no lists (PB_ERR_UNSUPPORTED). The workspace has pb_choice_report_work_bytes (-1: bad argument). */
-int64_t pb_choice_report_work_bytes(const pb_sets* sets, int32_t top);
+int64_t pb_choice_report_work_bytes(const pb_sets* sets, int32_t top, int32_t num_buckets);
 int pb_choice_report(const pb_sets* sets, const pb_choice_scores* scores, const int32_t* chosen_dev, float temperature,
                      int32_t top, float* log_probs_dev, float* entropy_dev, float* lse_dev, int32_t* top_index_dev,
                      float* top_log_probs_dev, void* work_dev, int64_t work_bytes, void* stream);

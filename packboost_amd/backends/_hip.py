@@ -199,7 +199,7 @@ _SIGNATURES = {
     "pb_choice_log_probs_backward": (ctypes.c_int, [_VP, ctypes.POINTER(PbChoiceScores)] + [_VP] * 6 + [_I64, _VP]),
     "pb_policy_loss": (ctypes.c_int, [_VP, ctypes.POINTER(PbChoiceScores), ctypes.POINTER(PbPolicyTerms)] + [_VP] * 6 +
                        [_I64, _VP]),
-    "pb_choice_report_work_bytes": (_I64, [_VP, _I32]),
+    "pb_choice_report_work_bytes": (_I64, [_VP, _I32, _I32]),
     "pb_choice_report": (ctypes.c_int, [_VP, ctypes.POINTER(PbChoiceScores), _VP, _F32, _I32] + [_VP] * 6 + [_I64, _VP]),
     "pb_choice_report_backward": (ctypes.c_int, [_VP, ctypes.POINTER(PbChoiceScores), _VP, _F32] + [_VP] * 5 + [_I64, _VP]),
     "pb_distillation_loss": (ctypes.c_int, [_VP, ctypes.POINTER(PbChoiceScores), ctypes.POINTER(PbTeacher)] + [_VP] * 5 +

@@ -150,11 +150,11 @@ class ChoiceSets(_Handle):
             n = self._work[op, num_buckets] = int(_hip.load().pb_choice_work_bytes(self._open(), op, num_buckets))
         return (_empty(n, self.device, torch.uint8), n) if n else (None, 0)
 
-
-    def _report_workspace(self, top: int) -> tuple[torch.Tensor | None, int]:
-        n = self._work.get((-1, top))
+    def _report_workspace(self, top: int, num_buckets: int) -> tuple[torch.Tensor | None, int]:
+        key = -1, top, num_buckets
+        n = self._work.get(key)
         if n is None:
-            n = self._work[-1, top] = int(_hip.load().pb_choice_report_work_bytes(self._open(), top))
+            n = self._work[key] = int(_hip.load().pb_choice_report_work_bytes(self._open(), top, num_buckets))
         return (_empty(n, self.device, torch.uint8), n) if n else (None, 0)
 
 
@@ -464,7 +464,7 @@ def choice_report(scores: torch.Tensor, sets: ChoiceSets, *, chosen: torch.Tenso
         entropy, lse = _empty(g, dev), _empty(g, dev)
         index = torch.empty((g, top), dtype=torch.int32, device=dev) if top else None
         best = torch.empty((g, top), dtype=torch.float32, device=dev) if top else None
-        work, size = sets._report_workspace(top)
+        work, size = sets._report_workspace(top, c.num_buckets)
         _hip.check(_hip.load().pb_choice_report(
             sets._open(), c, _hip.ptr(chosen), temperature, top, _hip.ptr(lp), entropy.data_ptr(), lse.data_ptr(),
             _hip.ptr(index), _hip.ptr(best), _hip.ptr(work), size, _hip.stream_ptr()), "pb_choice_report")

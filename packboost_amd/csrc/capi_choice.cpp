@@ -424,8 +424,9 @@ int64_t pb_choice_work_bytes(const pb_sets* s, int32_t op, int32_t num_buckets) 
     return work_need(s, op, num_buckets);
 }
 
-int64_t pb_choice_report_work_bytes(const pb_sets* s, int32_t top) {
-    return !s || top < 0 || top > pb::kMaxTop ? -1 : pb::report_work_bytes(s->s, top);
+int64_t pb_choice_report_work_bytes(const pb_sets* s, int32_t top, int32_t num_buckets) {
+    if (!s || top < 0 || top > pb::kMaxTop || num_buckets < 0 || num_buckets > pb::kMaxBuckets) return -1;
+    return pb::report_work_bytes(s->s, top, num_buckets > 0);
 }
 
 int pb_choice_log_probs(const pb_sets* s, const pb_choice_scores* in, const int32_t* chosen_dev, float* log_probs_dev,
@@ -501,7 +502,7 @@ int pb_choice_report(const pb_sets* s, const pb_choice_scores* in, const int32_t
     if (rc == PB_OK) rc = report_args(who, temperature, top, a);
     if (rc == PB_OK && top > 0 && s->largest > INT32_MAX)
         rc = pb::api_fail(PB_ERR_UNSUPPORTED, "pb_choice_report: lists name rows of sets of at most 2^31 - 1 rows");
-    if (rc == PB_OK) rc = scores_args(who, s, in, work_dev, work_bytes, pb::report_work_bytes(s->s, top), a);
+    if (rc == PB_OK) rc = scores_args(who, s, in, work_dev, work_bytes, pb::report_work_bytes(s->s, top, in->num_buckets > 0), a);
     if (rc != PB_OK || s->s.num_sets == 0) return rc;
     if (!entropy_dev || !lse_dev || (chosen_dev && !log_probs_dev) || (top > 0 && (!top_index_dev || !top_log_probs_dev)))
         return pb::api_fail(PB_ERR_INVALID, "pb_choice_report: null output");

@@ -33,7 +33,7 @@ struct ReportArgs : ChoiceArgs {
     bool tail;
     float* kl;
 };
-int64_t report_work_bytes(const SetLayout& s, int32_t top);
+int64_t report_work_bytes(const SetLayout& s, int32_t top, bool bias);
 hipError_t launch_report(const SetLayout& s, ReportArgs a, int32_t type, char* work, hipStream_t stream);
 // distill: the loss's gradient, else that of the log-probabilities and entropies; `sums` are in the workspace
 int64_t soft_grads_work_bytes(const SetLayout& s, bool distill, int32_t num_buckets);

@@ -847,11 +847,13 @@ hipError_t launch_typed(const SetLayout& s, const ReportArgs& a, hipStream_t str
     return a.table ? launch_as<TYPE, false, true>(s, a, stream) : launch_as<TYPE, false, false>(s, a, stream);
 }
 
-int64_t part_items(const SetLayout& s) { return s.num_wide > s.num_whole ? s.num_mid + s.num_wide : 0; }
+int64_t part_items(const SetLayout& s, bool bias) { return num_parts(s, bias) > 0 ? s.num_mid + s.num_wide : 0; }
 
 }  // namespace
 
-int64_t report_work_bytes(const SetLayout& s, int32_t top) { return part_items(s) * ((int64_t)sizeof(SoftSums) + 8 * top); }
+int64_t report_work_bytes(const SetLayout& s, int32_t top, bool bias) {
+    return part_items(s, bias) * ((int64_t)sizeof(SoftSums) + 8 * top);
+}
 
 hipError_t launch_report(const SetLayout& s, ReportArgs a, int32_t type, char* work, hipStream_t stream) {
     a.off = s.off;
@@ -866,7 +868,7 @@ hipError_t launch_report(const SetLayout& s, ReportArgs a, int32_t type, char* w
     a.num_whole = s.num_whole;
     a.rows = s.rows;
     a.part_sums = reinterpret_cast<SoftSums*>(work);
-    a.part_keys = reinterpret_cast<unsigned long long*>(work + sizeof(SoftSums) * part_items(s));
+    a.part_keys = reinterpret_cast<unsigned long long*>(work + sizeof(SoftSums) * part_items(s, a.num_buckets > 0));
     a.team_bits = 0;
     while (1 << a.team_bits < a.top) ++a.team_bits;
     const auto at = [](const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; };

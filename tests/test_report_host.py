@@ -19,7 +19,7 @@ def test_report_entry_points_refuse():
 
     lib = _hip.load()
     c, t = _hip.PbChoiceScores(), _hip.PbTeacher()
-    assert lib.pb_choice_report_work_bytes(None, 1) == -1
+    assert lib.pb_choice_report_work_bytes(None, 1, 0) == -1
     for op in (_hip.PB_REPORT_BACKWARD, _hip.PB_DISTILL):
         assert lib.pb_choice_work_bytes(None, op, 0) == -1
     assert lib.pb_choice_report(None, c, None, 1.0, 0, None, None, None, None, None, None, 0, None) == -1
