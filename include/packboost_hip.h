@@ -665,7 +665,8 @@ typedef struct {
  * are divided by their sum and rho is 0.
  *   kl_dev float32 [num_sets] = sum of q (log q - log p) + rho (log rho - log pi),
  *   loss_dev[0] = scale T^2 * sum of w kl.
- * Sets in which the teacher's entries or the student have no probability are left out (kl 0, no gradient); sets of weight
+ * Sets in which the teacher's entries or the student have no probability (with tail, log-probabilities whose exponentials
+ * are 0 in double, below -745) are left out (kl 0, no gradient); sets of weight
  * 0 count for nothing, also where their divergence is infinite. The gradients are the loss's, laid out as in
  * pb_choice_log_probs_backward. */
 int pb_distillation_loss(const pb_sets* sets, const pb_choice_scores* scores, const pb_teacher* teacher, float* loss_dev,

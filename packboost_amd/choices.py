@@ -529,7 +529,8 @@ def distillation_loss(scores: torch.Tensor, sets: ChoiceSets, teacher_index: tor
         kl = sum q (log q - log p) + rho (log rho - log pi);  loss = scale * T^2 * sum of w * kl
 
     over the sets. weights (w, default 1) are float32 per set; a set of weight 0 counts for nothing, also where its
-    divergence is infinite. A set in which the teacher's entries or the student have no probability is left out."""
+    divergence is infinite. A set in which the teacher's entries or the student have no probability is left out; a
+    log-probability whose exponential is 0 in 64 bits (below -745) has none."""
     c, keep = _scores(scores, sets, mask, bias)
     dev, g = sets.device, sets.num_sets
     index = _list_of("teacher_index", teacher_index, sets, torch.int32)

@@ -42,13 +42,27 @@ __device__ __forceinline__ double inverse(double d) {
     return __builtin_fma(__builtin_fma(-d, r, 1.0), r, r);
 }
 
-// What a set's list says without the rows that are not listed: zmax the largest listed logit, E = sum of e = exp((z - zmax) / T),
-// mass = sum of part = exp(t), t the teacher's value (over T and less its largest, without tail), and lost = sum of
-// part (t - (z - zmax) / T). In double: a divergence is what large terms leave where student and teacher are close.
+// What a set's list says without the rows that are not listed: zmax the largest listed logit, e the sum of the listed rows'
+// exp((z - zmax) / T), most the teacher's largest value (0 where that is -inf), mass the sum of the terms exp(t - most) (over
+// T without tail), lost that of the terms times ((t - most) - (z - zmax) / T), and left, with tail, the sum of exp(t) itself, as far
+// as it matters (see list_share), else mass. Terms over the largest are neither too small nor too large for what is divided by
+// their sum, wherever the values lie. mass and lost are sums, in double, of the same terms, so that a term's rounding moves a
+// divergence by its share of log (q / p) alone. In tiles the terms of e, and the sums over the rest, are float32, and
+// the teacher's terms have a float32's digits.
 struct ListSide {
-    float zmax;
-    double e, mass, lost;
+    float zmax, most;
+    double e, mass, left, lost;
 };
+
+// exp(t) of a log-probability. From 1 on the list leaves nothing to the rest, by however much.
+__device__ __forceinline__ double list_share(double t) { return exp_near(t > 1.0 ? 1.0 : t); }
+
+// e^x as a float's digits with a double's exponent: a term that is nothing beside the others counts where the student is as
+// far off. Within 2^-22 of itself; -inf gives 0, NaN stays NaN.
+__device__ __forceinline__ double list_exp(double x) {
+    const double t = (x < -800.0 ? -800.0 : x) * 1.4426950408889634, k = __builtin_rint(t);
+    return ldexp((double)__builtin_amdgcn_exp2f((float)(t - k)), (int)k);
+}
 
 // An entry's terms; z is -inf and t -inf where it does not count.
 struct ListTerms {
@@ -61,9 +75,9 @@ struct ListTerms {
     }
 };
 
-// The teacher's value as the terms take it, `most` the largest of the set's.
-__device__ __forceinline__ double entry_term(const ReportArgs& a, bool on, float t, float most) {
-    return !on ? -(double)kInf : a.tail ? (double)t : ((double)t - (most > -kInf ? (double)most : 0.0)) * a.inv_temp;
+// The teacher's value as the terms take it.
+__device__ __forceinline__ double entry_term(const ReportArgs& a, float t, float most) {
+    return ((double)t - (double)most) * (a.tail ? 1.0 : a.inv_temp);
 }
 
 // What the rows' terms are multiplied by: a listed row's gradient is student e - teacher part, another's rest times its
@@ -81,12 +95,12 @@ __device__ __forceinline__ ListFactors list_factors(const ReportArgs& a, const L
     const double less = exp_near(up == 0.0 ? gap : -up);  // of the two sides' exponentials one is 1
     const double ours = up == 0.0 ? 1.0 : less, theirs = up == 0.0 ? less : 1.0;
     const double total = l.e * ours + (has_rest ? rest_sum * theirs : 0.0);
-    if (l.mass == 0.0 || total == 0.0) return ListFactors{0.0f, 0.0f, 0.0f, 0.0};
-    const bool open = a.tail && has_rest && l.mass < 1.0;
-    const double wt = (double)w * (double)a.temp, per_total = inverse(total), rho = 1.0 - l.mass;
-    const double per = inverse(open ? rest_sum : l.mass);
-    ListFactors f{(float)(wt * ours * per_total), (float)(open ? wt : wt * per),
-                  has_rest ? (float)(wt * (theirs * per_total - (open ? rho * per : 0.0))) : 0.0f, 0.0};
+    if (l.left == 0.0 || total == 0.0) return ListFactors{0.0f, 0.0f, 0.0f, 0.0};
+    const bool open = a.tail && has_rest && l.left < 1.0;
+    const double wt = (double)w * (double)a.temp, per_total = inverse(total), per = inverse(l.mass);
+    const double share = open ? l.left : 1.0, rho = 1.0 - l.left;  // the list's sum of q; the rest's, where it is open
+    ListFactors f{(float)(wt * ours * per_total), (float)(wt * share * per),
+                  has_rest ? (float)(wt * (theirs * per_total - (open ? rho * inverse(rest_sum) : 0.0))) : 0.0f, 0.0};
     if (w == 0.0f) f.student = f.teacher = f.rest = 0.0f;
     if (KL) {  // one logarithm after the other: beside each other they take the registers of the rows
         __builtin_amdgcn_sched_barrier(0);
@@ -94,15 +108,15 @@ __device__ __forceinline__ ListFactors list_factors(const ReportArgs& a, const L
         __builtin_amdgcn_sched_barrier(0);
         const double log_left = log_near(open ? rho : l.mass);
         __builtin_amdgcn_sched_barrier(0);
-        f.kl = open ? l.lost + l.mass * log_total + rho * (log_left - (gap + log_near(rest_sum) - log_total))
-                    : l.lost * per - log_left + log_total;
+        f.kl = share * (l.lost * per + (open ? (double)l.most : -log_left) + log_total);
+        if (open) f.kl += rho * (log_left - (gap + log_near(rest_sum) - log_total));
     }
     return f;
 }
 
 // A listed row's gradient. A set that counts for nothing has factors of 0, whatever its terms.
 __device__ __forceinline__ float listed_grad(float student, float teacher, float e, float part) {
-    return teacher == 0.0f ? 0.0f : student * e - teacher * part;
+    return student == 0.0f && teacher == 0.0f ? 0.0f : student * e - teacher * part;
 }
 
 // A row's gradient is its exponential times (first + slope (z - m)), from a set's sums.
@@ -128,7 +142,7 @@ struct alignas(16) SoftTile {
 
 struct alignas(16) ListTile : SoftTile {
     float part[kSetTileRows];    // of listed rows: the teacher's terms
-    double mass[kSetTileSets];   // with tail: their sums
+    double left[kSetTileSets];   // with tail: the lists' sums of exp(t)
     uint8_t slot[kSetTileRows];  // the entry that names a row, from 1; 0: none
     float other[kSetTileSets + 4];  // slope and other: the list's largest logit and teacher's value, then factors
 };
@@ -225,9 +239,9 @@ struct RoundSet {
     }
 };
 
-// Marks the rows that a tile's lists name, and leaves each list's largest logit and teacher's value. With tail also the
-// teacher's terms, in double: 1 less their sum may be small. (All terms here or all in weigh_listed, where the rows'
-// exponentials lie in registers, would take one wave a SIMD.)
+// Marks the rows that a tile's lists name, and leaves each list's largest logit and teacher's value. With tail also its sum
+// of exp(t), in double: 1 less that may be small. (All sums here or all in weigh_listed, where the rows' exponentials
+// lie in registers, would take one wave a SIMD.)
 template <bool MASK, class IN>
 __device__ __forceinline__ void mark_listed(const ReportArgs& a, const ListWalk& walk, IN& all, ListTile& sh, int lane) {
     const auto& in = all.rows;
@@ -235,7 +249,7 @@ __device__ __forceinline__ void mark_listed(const ReportArgs& a, const ListWalk&
     for (int round = 0; round < walk.rounds; ++round) {
         const RoundSet r(walk, in, round, lane);
         float zmax = kLowest, tmax = -kInf;
-        double mass = 0.0;
+        double left = 0.0;
 #pragma unroll 1
         for (int group = 0; group < walk.groups; ++group) {
             const int index = round * walk.groups + group;
@@ -286,20 +300,16 @@ __device__ __forceinline__ void mark_listed(const ReportArgs& a, const ListWalk&
             }
             if (a.tail) {
 #pragma unroll
-                for (int u = 0; u < kGroup; ++u) {
-                    const double part = on[u] ? exp_near((double)entry_value(a, e.t[u])) : 0.0;
-                    mass += part;
-                    if (on[u]) sh.part[r.begin + e.c[u]] = (float)part;
-                }
+                for (int u = 0; u < kGroup; ++u) left += on[u] ? list_share((double)entry_value(a, e.t[u])) : 0.0;
             }
         }
         zmax = (float)team_max((double)zmax, walk.bits);
         tmax = (float)team_max((double)tmax, walk.bits);
-        if (a.tail) mass = team_sum(mass, walk.bits);
+        if (a.tail) left = team_sum(left, walk.bits);
         if (r.first) {
             sh.slope[r.s] = zmax;
             sh.other[r.s] = tmax;
-            sh.mass[r.s] = mass;
+            sh.left[r.s] = left;
         }
     }
 }
@@ -315,7 +325,7 @@ __device__ __forceinline__ void weigh_listed(const ReportArgs& a, const ListWalk
         const RoundSet r(walk, in, round, lane);
         const float w = __shfl(round ? all.weight[1] : all.weight[0], lane >> walk.bits) * a.scale, tmax = sh.other[r.s];
         const float most = tmax > -kInf ? tmax : 0.0f;
-        ListSide l{sh.slope[r.s], 0.0, 0.0, 0.0};
+        ListSide l{sh.slope[r.s], most, 0.0, 0.0, 0.0, 0.0};
 #pragma unroll 1
         for (int group = 0; group < walk.groups; ++group) {
             const int index = round * walk.groups + group;
@@ -328,20 +338,21 @@ __device__ __forceinline__ void weigh_listed(const ReportArgs& a, const ListWalk
                 on = on && sh.slot[row] == walk.entry(group, u, lane) + 1;
                 const float z = on ? sh.x[row] : -kInf, t = on ? entry_value(a, e.t[u]) : -kInf;
                 const float student = heat_exp(z - l.zmax, heat);
-                const float part = !a.tail ? heat_exp(t - most, heat) : on ? sh.part[row] : 0.0f;
+                const double term = entry_term(a, t, most), part = list_exp(term);
                 if (on) {
                     sh.x[row] = student;
-                    sh.part[row] = part;
+                    sh.part[row] = (float)part;
                 }
-                const double x = ((double)z - (double)l.zmax) * a.inv_temp, given = a.tail ? (double)t : ((double)t - (double)most) * a.inv_temp;
+                const double x = ((double)z - (double)l.zmax) * a.inv_temp;
                 l.e += (double)student;
-                l.mass += (double)part;
-                l.lost += part == 0.0f ? 0.0 : (double)part * (given - x);
+                l.mass += part;
+                l.lost += part == 0.0 ? 0.0 : part * (term - x);
             }
         }
         l.e = team_sum(l.e, walk.bits);
-        l.mass = a.tail ? sh.mass[min(r.s, kSetTileSets - 1)] : team_sum(l.mass, walk.bits);
+        l.mass = team_sum(l.mass, walk.bits);
         l.lost = team_sum(l.lost, walk.bits);
+        l.left = a.tail ? sh.left[min(r.s, kSetTileSets - 1)] : l.mass;
         const ListFactors f = list_factors<true>(a, l, r.size > 0 ? sh.top[r.s] : kLowest, r.size > 0 ? (double)sh.first[r.s] : 0.0, w);
         wave_sync();
         if (r.first) {
@@ -611,13 +622,15 @@ __device__ __forceinline__ void soft_pass(const ReportArgs& a, const SetItem& im
         group_sync<THREADS>();
         if (wave0 == 0 && PHASE != kPartSums) {
             if (!on) z = -kInf;
-            const float t = entry_value(a, bits);
+            const float t = on ? entry_value(a, bits) : -kInf;
             ListSide l;
             l.zmax = (float)team_max((double)(on ? fmaxf(kLowest, z) : kLowest), 6);
-            const float tmax = (float)team_max(on ? (double)t : -(double)kInf, 6);
-            const ListTerms terms(a, z, entry_term(a, on, t, tmax), l.zmax);
+            const float tmax = (float)team_max((double)t, 6);
+            l.most = tmax > -kInf ? tmax : 0.0f;
+            const ListTerms terms(a, z, entry_term(a, t, l.most), l.zmax);
             l.e = team_sum(terms.e, 6);
             l.mass = team_sum(terms.part, 6);
+            l.left = a.tail ? l.mass * list_share((double)l.most) : l.mass;
             l.lost = team_sum(terms.lost, 6);
             sh.e[lane] = (float)terms.e;
             sh.part[lane] = (float)terms.part;
