@@ -106,7 +106,9 @@ class PreferenceObjective(Objective):
 
 
 class _Choices(Objective):
-    """Sets of rows, with one choice each where `chosen` is given, a mask and a learned position bias."""
+    """Sets of rows with a mask and a learned position bias, and one choice each (`chosen`) where `_chooses`."""
+
+    _chooses = True
 
     def __init__(self, offsets, chosen=None, *, mask=None, positions=None, buckets: PositionBuckets | None = None,
                  bias_rate: float = 0.1) -> None:
@@ -114,7 +116,7 @@ class _Choices(Objective):
         if self._off.size == 0 or self._off[0] != 0 or np.any(self._off[1:] < self._off[:-1]):
             raise ValueError("offsets must start at 0 and not decrease")
         self._g, self._n = self._off.size - 1, int(self._off[-1])
-        self._chosen = None if chosen is None else _indices("chosen", chosen, self._g)
+        self._chosen = _indices("chosen", chosen, self._g) if self._chooses else None
         self._mask = None if mask is None else _array("mask", mask, self._n, bool)
         self._positions = None if positions is None else _indices("positions", positions, self._n)
         if buckets is not None and positions is None:
@@ -213,6 +215,8 @@ class DistillationObjective(_Choices):
     offsets, mask, positions: as ChoiceSets and choice_log_probs take them; teacher_index, teacher_logits [sets, k]
     (top_index and top_log_probs of a choice_report of the teacher's scores at this temperature, with tail=True, or logits);
     weights: per set."""
+
+    _chooses = False
 
     def __init__(self, offsets, teacher_index, teacher_logits, *, tail: bool = False, weights=None, mask=None,
                  positions=None, buckets=None, bias_rate: float = 0.1, temperature: float = 1.0) -> None:

@@ -57,6 +57,18 @@ def test_distillation_objective_checks():
             DistillationObjective([0, 4, 9], **{**dict(teacher_index=index, teacher_logits=logits), **bad})
 
 
+def test_objectives_on_choices_need_them():
+    """Sets whose choices are None: refused where the objective is made, as any other wrong `chosen`; a distillation has none."""
+    from packboost_amd import ChoicePreferenceObjective, DistillationObjective, PolicyObjective
+
+    off, one = [0, 4, 9], np.ones(2)
+    with pytest.raises(ValueError, match="chosen"):
+        PolicyObjective(off, None, one, one)
+    with pytest.raises(ValueError, match="chosen"):
+        ChoicePreferenceObjective(off, None, [0, 1, 2], [0], [1])
+    DistillationObjective(off, np.zeros((2, 3), int), np.zeros((2, 3)))
+
+
 def test_build_refuses_spills_of_the_report_kernels():
     from packboost_amd.build import spilling_kernels
 
