@@ -56,7 +56,8 @@ __device__ __forceinline__ void put_report(const ReportArgs& a, int64_t g, const
     const bool none = t.sum == 0.0;
     const double m = none ? 0.0 : (double)t.top;
     a.lse_out[g] = (float)(m * a.inv_temp + log_sum);
-    a.entropy[g] = none ? 0.0f : (float)(log_sum - t.along * a.inv_temp / t.sum);
+    const double h = log_sum - t.along * a.inv_temp / t.sum;
+    a.entropy[g] = none || h < 0.0 ? 0.0f : (float)h;  // roundings may leave less than 0; NaN is kept
     if (a.chosen) a.log_probs[g] = counts && !none ? (float)(((double)z - m) * a.inv_temp - log_sum) : 0.0f;
 }
 

@@ -711,3 +711,28 @@ def test_distillation_objective(hip):
     # sets at other places of the table are summed over other lanes
     assert np.all(np.abs(grad.cpu().numpy() - want.grad_scores.cpu().numpy()[perm]) <= 100 * U)
     obj.release()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("size", [3, 300, 700, 5000, 9000, 70_000])
+def test_entropy_is_not_negative(hip, size, dtype):
+    """Sets of one row with probability, by its score's or by the mask's word, and of one row far above the others: the
+    entropy is 0 within its roundings, and never below."""
+    from packboost_amd import ChoiceSets, choice_report
+
+    r = np.random.default_rng(size)
+    many = 64
+    z = np.full((many, size), -np.inf)
+    at = r.integers(0, size, many)
+    z[np.arange(many), at] = 3 * r.standard_normal(many)
+    sets = ChoiceSets(np.arange(many + 1) * size)
+    for kind in ("lone", "masked", "far"):
+        if kind == "far":
+            z = np.where(np.isneginf(z), z[np.arange(many), at][:, None] - 30.0, z)
+        x = torch.from_numpy(z if kind != "masked" else np.where(np.isneginf(z), 1.0, z)).to(DEV)
+        mask = torch.from_numpy(~np.isneginf(z).reshape(-1)).to(DEV) if kind == "masked" else None
+        x = x.to({"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}[dtype]).reshape(-1)
+        for temperature in (1.0, 0.3):
+            h = choice_report(x, sets, mask=mask, temperature=temperature).entropy
+            # log(1) and u / s of one term are within 4 units of 0; e^-30 of 70 thousand others is 1e-8 times 30 at most
+            assert float(h.min()) >= 0 and float(h.max()) <= 2.0**-21 + (3e-7 if kind == "far" else 0.0)
