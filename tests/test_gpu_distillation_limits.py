@@ -15,7 +15,9 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_choices import DEV, TYPES, U, offsets_of
+from test_gpu_choice_layouts import EDGES
+from test_gpu_choices import DEV, LAYOUTS, TYPES, U, make, offsets_of
+from test_gpu_reports import check_distill, teacher_of
 
 pytestmark = pytest.mark.gpu
 
@@ -263,3 +265,15 @@ def test_faint_entry_of_a_row_far_below(hip, below, pad, tail):
         if tail:
             want[2:] -= (1.0 - q.sum()) * p[2:] / pi
         assert np.all(np.abs(grad[:4] - want) <= 2.0**-18) and not grad[4:].any()
+
+
+@pytest.mark.parametrize("dtype,masked,biased", [("f32", True, True), ("bf16", False, False), ("f16", True, False), ("f32", False, False)])
+@pytest.mark.parametrize("layout", list(LAYOUTS) + list(EDGES))
+def test_lists_at_any_level(hip, layout, dtype, masked, biased):
+    """Every layout, each set's values moved to a level of its own: next to nothing, their own, or far more than 1."""
+    d = make({**EDGES, **LAYOUTS}[layout], dtype, masked, biased, seed=50)
+    for k in (3, 64 if masked else 20):
+        index, value = teacher_of(d, k, True, 1.5, 51)
+        level = np.random.default_rng(52).choice([0.0, 0.0, -5.0, -60.0, -90.0, -200.0, -600.0, 5.0, 100.0], (len(d["size"]), 1))
+        value = (value.double() + torch.from_numpy(level)).float()
+        check_distill(d, k, True, 1.5, 53, lists=(index, value))
