@@ -171,7 +171,8 @@ __device__ __forceinline__ uint32_t outside(const Span& s, int i) {
 // Whether a run goes in accesses of 16 bytes: the addresses are aligned (a.vec) and all its rows lie in the
 // table. Else it goes row by row, in a rolled loop, within [lo, hi). That is what a table whose rows start off a
 // 16-byte boundary, or whose scores have a stride, costs the whole call (us, aligned / one row off / stride 2: steps of
-// 100k sets 28 / 44 / 52; policy of 480k sets 28 / 38 / 40; 4096 sets of 32000 bfloat16 scores 154 / 509 / 707).
+// 100k sets 28 / 44 / 52; policy of 480k sets 28 / 38 / 40; 4096 sets of 32000 bfloat16 scores 154 / 509 / 707; with a
+// teacher of 8, 100k sets of 24 27 / 33 / 34 and the 4096 sets 112 / 404 / 433; their report without lists 57 / 203 / 297).
 __device__ __forceinline__ bool whole_run(const ChoiceArgs& a, const Span& s, int i) { return a.vec && i + kRun <= s.end; }
 
 __device__ __forceinline__ void put_row(float (&x)[kRun], int k, float v) {

@@ -10,7 +10,8 @@
 // workgroup that holds them in registers (of up to 65536 rows where that pays, see kBigSets), what is longer still in parts
 // that a second kernel joins. In a tile, a row of
 // a short set counts the rows that rank above it. Of longer sets a bound is found first that at least as many rows reach as
-// are listed, from the maxima of the lanes; the few rows that reach it are gathered and ranked by counting.
+// are listed, from the maxima of the lanes; the rows that reach it, few where they lie in no order, are gathered and
+// ranked by counting.
 #include <algorithm>
 #include <utility>
 
@@ -196,9 +197,10 @@ __device__ __forceinline__ int gather_best(const ReportArgs& a, const float (&v)
     }
     wave_sync();
     if (count <= (uint32_t)LIST) return (int)count;
-    // Too many rows reach the bound, of one value most often: the least rank that a.top rows reach, and of those that have
-    // it the first. The rows are read anew for each bit: held in registers, they would cost the usual path a third of
-    // its waves.
+    // Too many rows reach the bound, where many are of one value, or rise or fall along a workgroup's set, where the wave at
+    // the lower end gives a low bound: the least rank that a.top rows reach, and of those that have it the first. The rows are read
+    // anew for each bit: held in registers, they would cost the usual path a third of its waves. 4096 sets of 32 thousand
+    // bfloat16 rows with lists of 8 take 2520 us here, 87 in any order (2000 sets of 6000 float32 rows 218 and 18).
     int turn = 0;
     const auto rows = [&](auto holds) {
         uint32_t c = 0;

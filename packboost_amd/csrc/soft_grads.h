@@ -512,7 +512,7 @@ __device__ __forceinline__ void soft_tile(const ReportArgs& a, SoftTileIn<DISTIL
 
 // The tiles, one a wave at a time. Bound by instructions and by a tile's chain of loads, scans and sums at 3 or 4 waves a SIMD:
 // 100 thousand masked sets of 24 rows with a bias 20 us (1175 vector instructions a tile, issued in 70 % of the time that
-// four waves give them), with a teacher's lists of 8 38 us (2067, a third of them the lists' doubles).
+// four waves give them), with a teacher's lists of 8 39 us (2125, a third of them the lists' doubles).
 template <bool DISTILL, int TYPE, bool MASK, bool BIAS>
 __global__ __launch_bounds__(kBlock, DISTILL ? 3 : 4) void soft_tile_kernel(ReportArgs a) {
     __shared__ std::conditional_t<DISTILL, ListTile, SoftTile> tiles[kWaves];
